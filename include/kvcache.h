@@ -390,6 +390,97 @@ int kvc_paged_attention_fp8_planned(kvc_dltensor* out, kvc_dltensor* exp_sums, k
  * (decode(code) * scale), uint8 -> uint8 rescales, float -> float scales. */
 int kvc_convert_fp8(kvc_dltensor* dst, const kvc_dltensor* src, float scale, int fp8_format, void* stream);
 
+/* ---- sliding window with sinks ----------------------------------------------
+ * Attention in which the query at position i of a sequence sees position j <= i
+ * when j < sink_size (the sequence's first tokens, which stay visible) or
+ * j > i - window_size (the window, the query's own position included):
+ *   out = sum_j e^{s_j - m} v_j / (sum_j e^{s_j - m} + 1e-6)   (decode)
+ *   out = sum_j e^{s_j - m} v_j / sum_j e^{s_j - m}            (prefill)
+ * with s_j = scale * q.k_j and m the largest of them.  No counterpart in the
+ * reference, whose make_mask has a window for prefill only
+ * (memory_pool.py:240-270).  window_size is positive; window_size >= the
+ * context gives the unwindowed attention.  Block-table entries of blocks that no
+ * query sees are not read (a server may have freed those blocks), and the values
+ * in positions that no query of a sequence sees never matter.
+ *
+ * kvc_paged_attention_window: one new token per sequence, arguments and edge
+ * rules of kvc_paged_attention_v1 (paged layout, every dtype pair, head size and
+ * block size of that call) or, with 4-D / 3-D caches, of
+ * kvc_paged_attention_flash (float16/bfloat16, head size 64/128, up to 16 query
+ * heads per KV head).  One launch and no workspace: the seen tokens of a
+ * (sequence, KV head) pair are split over a thread-block cluster, which joins
+ * its softmax states through distributed shared memory.
+ *
+ * kvc_paged_prefill_window: the new tokens of a ragged batch, arguments, layouts
+ * and index rules of kvc_paged_prefill. */
+int kvc_paged_attention_window(kvc_dltensor* out, const kvc_dltensor* query, const kvc_dltensor* key_cache,
+                               const kvc_dltensor* value_cache, const kvc_dltensor* block_tables,
+                               const kvc_dltensor* context_lens, int num_kv_heads, float scale, int block_size,
+                               int max_seq_len, int window_size, int sink_size, void* stream);
+int kvc_paged_prefill_window(kvc_dltensor* out, const kvc_dltensor* query, const kvc_dltensor* key_cache,
+                             const kvc_dltensor* value_cache, const kvc_dltensor* block_tables,
+                             const kvc_dltensor* qo_indptr, const kvc_dltensor* kv_lens, int num_kv_heads, float scale,
+                             int block_size, int max_q_len, int window_size, int sink_size, void* stream);
+
+/* ---- step tables --------------------------------------------------------------
+ * The index arrays of a step, built on the device from the requests' lengths in
+ * one launch (the reference builds them on the host, model_runner.py:190-258).
+ * Request b has prefix_lens[b] cached tokens in the blocks block_tables[b][0 ..
+ * ceil(prefix_lens[b] / block_size) - 1] and brings new_lens[b] new ones.  The
+ * blocks these need are taken from free_blocks, in request order, and written to
+ * block_tables in place (entries of other columns stay as they are).
+ *   block_tables  int32 [num_seqs, max_blocks], updated
+ *   kv_lens       int32 [num_seqs]      prefix_lens + new_lens
+ *   qo_indptr     int32 [num_seqs + 1]  exclusive sum of new_lens, then their total
+ *   positions     int32 [N]  position of every new token in its sequence
+ *   slot_mapping  int32/int64 [N]  block * block_size + offset of every new token
+ *   blocks_used   int32 [1]  entries of free_blocks taken
+ *   prefix_lens, new_lens  int32 [num_seqs];  free_blocks  int32 [any]
+ * N may exceed the total (the capacity of a captured step): the rows past it get
+ * position -1 and slot -1, which the appends and kvc_qk_norm_rope skip.
+ * KVC_STATUS_INDEX_OOB is set, and the affected slots are -1, when the total
+ * exceeds N, the free list or a table row is too short (entries past the free
+ * list are written as -1), a table entry that a new token falls into is
+ * negative, a length is negative (read as 0, with its request's other length)
+ * or an int32 slot overflows. */
+int kvc_step_tables(kvc_dltensor* block_tables, kvc_dltensor* kv_lens, kvc_dltensor* qo_indptr,
+                    kvc_dltensor* positions, kvc_dltensor* slot_mapping, kvc_dltensor* blocks_used,
+                    const kvc_dltensor* prefix_lens, const kvc_dltensor* new_lens, const kvc_dltensor* free_blocks,
+                    int block_size, void* stream);
+
+/* ---- rotary position and per-head norm ----------------------------------------
+ * kvc_rotary_table writes cos_sin (float32 [positions, R], R even, at most 256):
+ * row p is cos(p f_i) * factor, i < R / 2, then sin(p f_i) * factor, the angles
+ * formed in 64 bits.  inv_freq: R / 2 host doubles f_i (with any scaling for long
+ * contexts already applied); factor scales the rotated part (1 for most rules).
+ *
+ * kvc_qk_norm_rope: for every token and head of q [T, num_heads, D] and k [T,
+ * num_kv_heads, D] (float32/float16/bfloat16, any token and head strides, D up to
+ * 512; q_out / k_out may be q / k themselves):
+ *   y = x * weight / sqrt(mean(x^2) + eps)  over the D elements, weight
+ *       [D] float32 or the input's dtype; a NULL weight leaves that tensor unnormed
+ *   the first R elements of y rotated by the token's row of cos_sin, in pairs
+ *       (i, i + R/2), or (2i, 2i + 1) with interleaved != 0; the rest pass.
+ * Computed in float32, rounded once.  positions int32/int64 [>= T]: a negative one
+ * skips the token's rows (padding), one past cos_sin skips them and sets
+ * KVC_STATUS_INDEX_OOB.
+ *
+ * kvc_qk_norm_rope_append: the same, with the keys stored to the cache instead
+ * of k_out and v [T, num_kv_heads, D] stored beside them, as kvc_reshape_and_cache
+ * (5-D key_cache) or kvc_reshape_and_cache_flash (4-D / 3-D) would: one launch
+ * instead of two, and the rotated keys never go through memory.  A token with a
+ * negative slot stores neither K nor V (its q rows are still written); one with a
+ * skipped position stores V only. */
+int kvc_rotary_table(kvc_dltensor* cos_sin, const double* inv_freq, double factor, void* stream);
+int kvc_qk_norm_rope(kvc_dltensor* q_out, kvc_dltensor* k_out, const kvc_dltensor* q, const kvc_dltensor* k,
+                     const kvc_dltensor* positions, const kvc_dltensor* cos_sin, const kvc_dltensor* q_weight,
+                     const kvc_dltensor* k_weight, float eps, int interleaved, void* stream);
+int kvc_qk_norm_rope_append(kvc_dltensor* q_out, kvc_dltensor* key_cache, kvc_dltensor* value_cache,
+                            const kvc_dltensor* q, const kvc_dltensor* k, const kvc_dltensor* v,
+                            const kvc_dltensor* positions, const kvc_dltensor* cos_sin, const kvc_dltensor* q_weight,
+                            const kvc_dltensor* k_weight, float eps, int interleaved, const kvc_dltensor* slot_mapping,
+                            void* stream);
+
 /* ---- device attributes (paged_attention/mlx_device.cpp) -------------------- */
 /* mlx_device.cpp:16-20: max shared memory per block (opt-in) of `device`. */
 int kvc_get_max_shared_memory_per_block_device_attribute(int device, int64_t* out);

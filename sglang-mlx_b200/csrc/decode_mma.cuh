@@ -368,13 +368,15 @@ struct GroupState {
 // sequences (the shared-prefix kernel), `end_lo` / `end_hi` further end the
 // scores of this lane's rows r and r + 8; `end` still bounds the V data.
 // `beg_lo` / `beg_hi` start them (sliding-window prefill); tokens before a
-// row's start are masked like tokens past its end.
-template <typename T, typename Geo, int D, bool SPLIT_P = true>
+// row's start are masked like tokens past its end.  WINDOW: the first `sinks`
+// tokens stay visible whatever the starts say, and V of the other tokens before
+// `v_beg` (which no row sees) is zeroed like V past the end.
+template <typename T, typename Geo, int D, bool SPLIT_P = true, bool WINDOW = false>
 __device__ __forceinline__ void mma_group(GroupState<D>& gs, const uint32_t (&qa)[D / 16][4], uint32_t kst,
                                           uint32_t vst, int tok0, int end, uint32_t pmask, int ctx, float qk_scale,
                                           bool alibi, float slope_lo, float slope_hi, int lane,
                                           int end_lo = 2147483647, int end_hi = 2147483647, int beg_lo = 0,
-                                          int beg_hi = 0) {
+                                          int beg_hi = 0, int sinks = 0, int v_beg = 0) {
   using namespace mma_detail;
   constexpr int GT = Geo::GT, BOX = Geo::BOX, VBS = Geo::VBS;
   constexpr uint32_t VSW_MASK = Geo::VSWZ ? (uint32_t)(Geo::VSWZ / 16 - 1) : 0u;
@@ -427,8 +429,9 @@ __device__ __forceinline__ void mma_group(GroupState<D>& gs, const uint32_t (&qa
       }
       if (tail) {
         const bool ok = (tok0 + t < end) && ((pmask >> (t / Geo::MBS)) & 1u);
-        x_lo = (ok && tok0 + t < end_lo && tok0 + t >= beg_lo) ? x_lo : -INFINITY;
-        x_hi = (ok && tok0 + t < end_hi && tok0 + t >= beg_hi) ? x_hi : -INFINITY;
+        const bool sink = WINDOW && tok0 + t < sinks;
+        x_lo = (ok && tok0 + t < end_lo && (tok0 + t >= beg_lo || sink)) ? x_lo : -INFINITY;
+        x_hi = (ok && tok0 + t < end_hi && (tok0 + t >= beg_hi || sink)) ? x_hi : -INFINITY;
       }
       sacc[j][e] = x_lo;
       sacc[j][2 + e] = x_hi;
@@ -498,6 +501,12 @@ __device__ __forceinline__ void mma_group(GroupState<D>& gs, const uint32_t (&qa
       ok_lo1 = (t_lo + 1 < end) && ((pmask >> ((tl + 1) / Geo::MBS)) & 1u);
       ok_hi0 = (t_lo + 8 < end) && ((pmask >> ((tl + 8) / Geo::MBS)) & 1u);
       ok_hi1 = (t_lo + 9 < end) && ((pmask >> ((tl + 9) / Geo::MBS)) & 1u);
+      if constexpr (WINDOW) {
+        ok_lo0 = ok_lo0 && (t_lo >= v_beg || t_lo < sinks);
+        ok_lo1 = ok_lo1 && (t_lo + 1 >= v_beg || t_lo + 1 < sinks);
+        ok_hi0 = ok_hi0 && (t_lo + 8 >= v_beg || t_lo + 8 < sinks);
+        ok_hi1 = ok_hi1 && (t_lo + 9 >= v_beg || t_lo + 9 < sinks);
+      }
     }
 #pragma unroll
     for (int nt = 0; nt < NT; nt += 2) {
@@ -1314,34 +1323,6 @@ __global__ void __launch_bounds__(NW * 32)
 // ramp overlaps another's streaming.  KVC_MMA_CONFIG="<warps>x<stages>"
 // overrides the default for tuning runs.
 
-static bool mma_disabled_by_env() {
-  const char* v = getenv("KVC_DECODE_KERNEL");
-  return v && (v[0] == 'g' || v[0] == 'G');  // "generic"
-}
-
-static bool mma_supported(const DecodeArgs& a) {
-  if (a.cache_type == ElemType::U8) {  // one-byte caches have no other kernel
-    const int G = a.num_heads / a.num_kv_heads;
-    return (a.q_type == ElemType::F16 || a.q_type == ElemType::BF16) && (a.head_size == 64 || a.head_size == 128) &&
-           (a.block_size == 8 || a.block_size == 16 || a.block_size == 32) && G >= 1 && G <= 16 && !a.flash &&
-           (a.num_partitions == 1 || a.partition_size % 32 == 0) && (reinterpret_cast<uintptr_t>(a.q) & 3u) == 0 &&
-           (a.q_seq_stride & 1) == 0 && (a.q_head_stride & 1) == 0;
-  }
-  if (mma_disabled_by_env()) return false;
-  if (a.q_type != a.cache_type) return false;
-  if (a.q_type != ElemType::F16 && a.q_type != ElemType::BF16) return false;
-  if (!(a.head_size == 64 || a.head_size == 128)) return false;
-  if (!a.flash && a.block_size != 8 && a.block_size != 16 && a.block_size != 32) return false;
-  const int G = a.num_heads / a.num_kv_heads;
-  if (G < 1 || G > 16) return false;
-  if (a.num_partitions > 1 && a.partition_size % 32 != 0) return false;
-  if (a.flash) return (reinterpret_cast<uintptr_t>(a.q) & 3u) == 0 && (a.q_seq_stride & 1) == 0 &&
-                      (a.q_head_stride & 1) == 0;
-  // q rows are read as 4-byte pairs
-  if ((reinterpret_cast<uintptr_t>(a.q) & 3u) || (a.q_seq_stride & 1) || (a.q_head_stride & 1)) return false;
-  return true;
-}
-
 // ---- tensor maps ---------------------------------------------------------------
 // cuTensorMapEncodeTiled is a driver entry point; it is looked up through the
 // runtime so the library needs no link against libcuda.
@@ -1551,19 +1532,6 @@ static cudaError_t launch_mma_nw(const DecodeParams& p, cudaStream_t stream) {
   return e != cudaSuccess ? e : cudaGetLastError();
 }
 
-// Variant id = warps * 1000 + stages * 100 + group tokens, + 100000 for tiled
-// tensor copies ("<warps>x<stages>x<group>t"), + 200000 for bulk K with the
-// swizzled whole-page V ("<warps>x<stages>x<group>s").
-static int mma_variant() {
-  const char* v = getenv("KVC_MMA_CONFIG");
-  if (!v) return 0;
-  int w = 0, s = 0, g = 32;
-  char t = 0;
-  const int n = sscanf(v, "%dx%dx%d%c", &w, &s, &g, &t);
-  if (n < 2) return 0;
-  return (t == 't' ? 100000 : (t == 's' ? 200000 : 0)) + w * 1000 + s * 100 + g;
-}
-
 // SMs of the current device (cached per device; any racing writer stores the same value).
 static int decode_sm_count() {
   static std::atomic<int> sms[64];
@@ -1575,162 +1543,6 @@ static int decode_sm_count() {
     if (dev >= 0 && dev < 64) sms[dev] = n;
   }
   return n;
-}
-
-template <typename T, int D, int BS>
-static cudaError_t launch_mma_typed(const DecodeParams& p, cudaStream_t stream) {
-  const int v = mma_variant();
-  const int g = v % 100;
-  const bool part_ok = p.num_partitions == 1 || (g > 0 && p.partition_size % g == 0);
-  if (D == 128 && v && part_ok) {
-    cudaError_t e = cudaErrorNotSupported;
-    switch (v) {
-      case 2332: e = launch_mma_nw<T, D, BS, 2, 3, 32>(p, stream); break;
-      case 2232: e = launch_mma_nw<T, D, BS, 2, 2, 32>(p, stream); break;
-      case 4316: if constexpr (BS <= 16) e = launch_mma_nw<T, D, BS, 4, 3, 16>(p, stream); break;
-      case 1316: if constexpr (BS <= 16) e = launch_mma_nw<T, D, BS, 1, 3, 16>(p, stream); break;
-      case 1416: if constexpr (BS <= 16) e = launch_mma_nw<T, D, BS, 1, 4, 16>(p, stream); break;
-      case 2316: if constexpr (BS <= 16) e = launch_mma_nw<T, D, BS, 2, 3, 16>(p, stream); break;
-      case 6216: if constexpr (BS <= 16) e = launch_mma_nw<T, D, BS, 6, 2, 16>(p, stream); break;
-      case 8216: if constexpr (BS <= 16) e = launch_mma_nw<T, D, BS, 8, 2, 16>(p, stream); break;
-      case 6316: if constexpr (BS <= 16) e = launch_mma_nw<T, D, BS, 6, 3, 16>(p, stream); break;
-      case 8316: if constexpr (BS <= 16) e = launch_mma_nw<T, D, BS, 8, 3, 16>(p, stream); break;
-      case 10216: if constexpr (BS <= 16) e = launch_mma_nw<T, D, BS, 10, 2, 16>(p, stream); break;
-      case 12216: if constexpr (BS <= 16) e = launch_mma_nw<T, D, BS, 12, 2, 16>(p, stream); break;
-      case 104316: e = launch_mma_nw<T, D, BS, 4, 3, 16, kTiles>(p, stream); break;
-      case 102232: e = launch_mma_nw<T, D, BS, 2, 2, 32, kTiles>(p, stream); break;
-      case 204316: if constexpr (BS <= 16) e = launch_mma_nw<T, D, BS, 4, 3, 16, kSwizzledV>(p, stream); break;
-      case 202232: e = launch_mma_nw<T, D, BS, 2, 2, 32, kSwizzledV>(p, stream); break;
-      case 203232: e = launch_mma_nw<T, D, BS, 3, 2, 32, kSwizzledV>(p, stream); break;
-      case 202332: e = launch_mma_nw<T, D, BS, 2, 3, 32, kSwizzledV>(p, stream); break;
-      default: break;
-    }
-    if (e != cudaErrorNotSupported) return e;
-  }
-  // The tail partitions of a shared-prefix decode (short, at most 256 tokens):
-  // 2 warps x 3 stages, so each warp streams more of its partition before the
-  // CTA's merge (config 4: 57.8 us against 62.2 us with 4 warps).
-  if constexpr (BS <= 16) {
-    if (p.part_offset > 0 && p.partition_size <= 256 && p.partition_size % 16 == 0)
-      return launch_mma_nw<T, D, BS, 2, 3, 16>(p, stream);
-  }
-  // Defaults from sweeps on B200: 16-token groups, 4 warps x 3 stages (96 KB,
-  // two CTAs and 8 warps per SM; 6 x 2 at D = 128, below) with whole-page 1-D bulk copies where the
-  // block size allows (98% of copy bandwidth on config 2, against 81% for
-  // 32-token groups).  32-token blocks: 32-token groups, 2 warps x 2 stages
-  // (64 KB, three CTAs per SM), K by bulk copy and V through the 128-byte
-  // swizzled tensor map (config 3: 77.7% against 73.9% with the 4-way bank
-  // conflicts of unswizzled 64-byte V rows; config 5: 91% against 89%).
-  // Tiled 16-token boxes of 32-token pages measured slower: such a box is
-  // hundreds of 16-32 byte rows.  If no tensor map can be encoded for the
-  // cache, plain bulk copies are used.
-  if constexpr (BS <= 16) {
-    // One rank's share of a head-sharded batch: a planned decode with at most
-    // two (sequence, KV head) pairs per SM whose partitions hold whole
-    // sequences runs on 10 warps x 2 stages (160 KB, one CTA per SM), so the
-    // longest sequences, which end the launch, stream on more warps (256
-    // sequences of U[512, 4096] tokens, one KV head: 1.71 ms per 32-layer step
-    // against 1.89 with 4 warps and 2048-token partitions; 8 warps 1.74, 12
-    // warps 1.71; with more pairs per SM the 4-warp CTAs are faster).
-    if (D == 128 && p.plan_items && p.part_offset == 0 && p.partition_size >= 4096 && p.partition_size % 16 == 0 &&
-        p.max_seq_len <= p.partition_size + 2 * BS &&
-        (int64_t)p.num_seqs * p.num_kv_heads <= 2 * (int64_t)decode_sm_count())
-      return launch_mma_nw<T, D, BS, 10, 2, 16>(p, stream);
-    // Otherwise, at D = 128, 6 warps x 2 stages (96 KB, two CTAs and 12 warps
-    // per SM).  Config 2 per 32-layer step against 4 warps x 3 stages: planned
-    // at 2 / 4 / 8 KV heads per GPU 3.02 / 6.15 / 12.06 ms against 3.12 / 6.33 /
-    // 12.62; single pass (v1) 12.22 against 13.11; split-K (v2) 15.29 against
-    // 15.61.
-    if (p.num_partitions == 1 || p.partition_size % 16 == 0) {
-      if constexpr (D == 128) return launch_mma_nw<T, D, BS, 6, 2, 16>(p, stream);
-      return launch_mma_nw<T, D, BS, 4, 3, 16>(p, stream);
-    }
-  } else {
-    cudaError_t e = launch_mma_nw<T, D, BS, 2, 2, 32, kSwizzledV>(p, stream);
-    if (e != cudaErrorNotSupported) return e;
-  }
-  return launch_mma_nw<T, D, BS, 2, 2, 32>(p, stream);
-}
-
-// One-byte caches: 16-token groups, 4 warps x 4 stages of 4 KB (three CTAs per
-// SM) for blocks of up to 16 tokens; 32-token groups, 4 warps x 3 stages of
-// 8 KB for 32-token blocks.
-template <typename T, int D, int MODE>
-static cudaError_t launch_mma_fp8(const DecodeParams& p, int block_size, cudaStream_t stream) {
-  if (block_size == 8) return launch_mma_nw<T, D, 8, 4, 4, 16, MODE>(p, stream);
-  if (block_size == 16) return launch_mma_nw<T, D, 16, 4, 4, 16, MODE>(p, stream);
-  return launch_mma_nw<T, D, 32, 4, 3, 32, MODE>(p, stream);
-}
-
-template <typename T>
-static cudaError_t launch_mma_t(const DecodeParams& p, const DecodeArgs& a, cudaStream_t stream) {
-  if (a.cache_type == ElemType::U8) {
-    const bool e5m2 = a.fp8_format == 1 || a.fp8_format == 3;  // the -sat formats decode alike
-    if (a.head_size == 128)
-      return e5m2 ? launch_mma_fp8<T, 128, kFp8E5M2>(p, a.block_size, stream)
-                  : launch_mma_fp8<T, 128, kFp8E4M3>(p, a.block_size, stream);
-    return e5m2 ? launch_mma_fp8<T, 64, kFp8E5M2>(p, a.block_size, stream)
-                : launch_mma_fp8<T, 64, kFp8E4M3>(p, a.block_size, stream);
-  }
-  if (a.flash) {
-    // token-major caches: 16-token groups, 6 warps x 2 stages for D = 128 and
-    // 4 warps x 3 stages for D = 64 (two CTAs per SM); the block size is read
-    // at run time.
-    // KVC_FLASH_COPY=bulk selects per-row bulk copies (tuning runs).
-    // KVC_FLASH_COPY=cpasync keeps the per-lane row copies where tensor copies apply (tuning runs).
-    // KVC_FLASH_COPY=gather reads dense rows in any order by tensor gathers (below).
-    const char* fc = getenv("KVC_FLASH_COPY");
-    if (fc && fc[0] == 'b') {
-      if (a.head_size == 128) return launch_mma_nw<T, 128, 16, 4, 3, 16, kFlashBulk>(p, stream);
-      return launch_mma_nw<T, 64, 16, 4, 3, 16, kFlashBulk>(p, stream);
-    }
-    // blocks of 16k consecutive token rows: a tensor copy per (16-token group, head, 64 dims)
-    const bool rows_ok = a.block_size % 16 == 0 && a.k_block_stride == (int64_t)a.block_size * a.k_tok_stride &&
-                         a.v_block_stride == (int64_t)a.block_size * a.v_tok_stride &&
-                         a.num_blocks * (int64_t)a.block_size < (int64_t)1 << 31 && !(fc && fc[0] == 'c');
-    // D = 128: 6 warps x 2 stages (two CTAs and 12 warps per SM; config 2 on
-    // the pool: page tables 12.67 against 13.54 ms per step with 4 x 3, slot
-    // lists 15.67 against 16.66)
-    const bool six = a.head_size == 128;
-    if (rows_ok) {
-      cudaError_t e = six ? launch_mma_nw<T, 128, 16, 6, 2, 16, kFlashTma>(p, stream)
-                    : a.head_size == 128 ? launch_mma_nw<T, 128, 16, 4, 3, 16, kFlashTma>(p, stream)
-                                         : launch_mma_nw<T, 64, 16, 4, 3, 16, kFlashTma>(p, stream);
-      if (e != cudaErrorNotSupported) return e;
-    }
-    // KVC_FLASH_COPY=gather: dense token rows in any order (the pool's slot
-    // lists) by 4-row tensor gathers.  Not the default: on config 2's slot-list
-    // pool they measured 0.661 of the copy peak against 0.708 for the per-lane
-    // row copies (16 gather requests per 16-token group and head, against 4
-    // tensor copies for blocks of consecutive rows).
-    // (block size 1, the pool's [slots, H, D]: a block is one row and carries no token stride)
-    const int64_t D = a.head_size, H = a.num_kv_heads, rbs = a.block_size;
-    const int64_t ktok = rbs == 1 ? H * D : a.k_tok_stride, vtok = rbs == 1 ? H * D : a.v_tok_stride;
-    const bool dense = a.k_head_stride == D && ktok == H * D && a.k_block_stride == rbs * H * D &&
-                       a.v_head_stride == D && vtok == H * D && a.v_block_stride == rbs * H * D &&
-                       a.num_blocks * rbs * H < (int64_t)1 << 31 && fc && fc[0] == 'g';
-    if (dense) {
-      cudaError_t e = a.head_size == 128 ? launch_mma_nw<T, 128, 16, 4, 3, 16, kFlashGather>(p, stream)
-                                         : launch_mma_nw<T, 64, 16, 4, 3, 16, kFlashGather>(p, stream);
-      if (e != cudaErrorNotSupported) return e;
-    }
-    if (six) return launch_mma_nw<T, 128, 16, 6, 2, 16, kFlash>(p, stream);
-    if (a.head_size == 128) return launch_mma_nw<T, 128, 16, 4, 3, 16, kFlash>(p, stream);
-    return launch_mma_nw<T, 64, 16, 4, 3, 16, kFlash>(p, stream);
-  }
-  if (a.head_size == 128) {
-    if (a.block_size == 8) return launch_mma_typed<T, 128, 8>(p, stream);
-    if (a.block_size == 16) return launch_mma_typed<T, 128, 16>(p, stream);
-    return launch_mma_typed<T, 128, 32>(p, stream);
-  }
-  if (a.block_size == 8) return launch_mma_typed<T, 64, 8>(p, stream);
-  if (a.block_size == 16) return launch_mma_typed<T, 64, 16>(p, stream);
-  return launch_mma_typed<T, 64, 32>(p, stream);
-}
-
-static cudaError_t launch_mma(const DecodeParams& p, const DecodeArgs& a, cudaStream_t stream) {
-  if (a.q_type == ElemType::BF16) return launch_mma_t<__nv_bfloat16>(p, a, stream);
-  return launch_mma_t<__half>(p, a, stream);
 }
 
 }  // namespace kvc

@@ -67,7 +67,8 @@ bool parse(const kvc_dltensor* t, const char* name, View* v) {
       set_error(std::string(name) + ": negative extent");
       return false;
     }
-    v->strides[i] = t->strides ? t->strides[i] : expect;
+    // (the stride of an extent of 1 moves nothing; producers may leave any value there)
+    v->strides[i] = t->strides && v->shape[i] != 1 ? t->strides[i] : expect;
     expect *= v->shape[i];
   }
   v->data = static_cast<char*>(t->data) + t->byte_offset;
@@ -440,12 +441,15 @@ int kvc_get_status(int device, uint32_t* flags, int clear) {
   DeviceGuard g(device);
   if (!g.ok()) return fail(KVC_ECUDA, "cudaSetDevice failed");
   cudaError_t e1 = cudaSuccess, e2 = cudaSuccess;
-  cudaError_t e3 = cudaSuccess;
-  unsigned int f =
-      kvc_cache_ops_status(clear, &e1) | kvc_decode_status(clear, &e2) | kvc_block_ops_status(clear, &e3);
+  cudaError_t e3 = cudaSuccess, e4 = cudaSuccess, e5 = cudaSuccess;
+  unsigned int f = kvc_cache_ops_status(clear, &e1) | kvc_decode_status(clear, &e2) |
+                   kvc_block_ops_status(clear, &e3) | kvc_layer_ops_status(clear, &e4) |
+                   kvc_window_status(clear, &e5);
   if (e1 != cudaSuccess) return cuda_fail(e1, "kvc_get_status");
   if (e2 != cudaSuccess) return cuda_fail(e2, "kvc_get_status");
   if (e3 != cudaSuccess) return cuda_fail(e3, "kvc_get_status");
+  if (e4 != cudaSuccess) return cuda_fail(e4, "kvc_get_status");
+  if (e5 != cudaSuccess) return cuda_fail(e5, "kvc_get_status");
   *flags = f;
   return KVC_OK;
 }
@@ -645,10 +649,10 @@ int kvc_paged_attention_cascade(kvc_dltensor* out, kvc_dltensor* exp_sums, kvc_d
 // create_attention_mask (memory_pool.py:240-270), reading the cache in place
 // instead of the update_and_fetch gather + SDPA of the reference
 // (memory_pool.py:205-234, model_runner.py:190-258).
-int kvc_paged_prefill(kvc_dltensor* out, const kvc_dltensor* query, const kvc_dltensor* key_cache,
-                      const kvc_dltensor* value_cache, const kvc_dltensor* block_tables,
-                      const kvc_dltensor* qo_indptr, const kvc_dltensor* kv_lens, int num_kv_heads, float scale,
-                      int block_size, int max_q_len, int window_size, void* stream) {
+static int prepare_prefill(kvc_dltensor* out, const kvc_dltensor* query, const kvc_dltensor* key_cache,
+                           const kvc_dltensor* value_cache, const kvc_dltensor* block_tables,
+                           const kvc_dltensor* qo_indptr, const kvc_dltensor* kv_lens, int num_kv_heads, float scale,
+                           int block_size, int max_q_len, int window_size, PrefillArgs* args, int* device) {
   View q, kc, vc, bt, qi, kl, o;
   if (!parse(query, "query", &q) || !parse(key_cache, "key_cache", &kc) ||
       !parse(value_cache, "value_cache", &vc) || !parse(block_tables, "block_tables", &bt) ||
@@ -706,9 +710,8 @@ int kvc_paged_prefill(kvc_dltensor* out, const kvc_dltensor* query, const kvc_dl
   if (!aligned16(kc.data) || !aligned16(vc.data) || (kc.stride(0) * cs) % 16 || (vc.stride(0) * cs) % 16 ||
       (kc.stride(hd) * cs) % 16 || (vc.stride(hd) * cs) % 16 || (k_tok * cs) % 16 || (v_tok * cs) % 16)
     return fail(KVC_EINVAL, "key_cache/value_cache pages and rows must start on 16-byte boundaries");
-  int device_of_call = -1;
-  if (int rc = check_all_cuda({&q, &kc, &vc, &bt, &qi, &kl, &o}, &device_of_call)) return rc;
-  PrefillArgs a;
+  if (int rc = check_all_cuda({&q, &kc, &vc, &bt, &qi, &kl, &o}, device)) return rc;
+  PrefillArgs& a = *args;
   memset(&a, 0, sizeof(a));
   a.out = o.data;
   a.q = q.data;
@@ -741,6 +744,18 @@ int kvc_paged_prefill(kvc_dltensor* out, const kvc_dltensor* query, const kvc_dl
   a.q_type = q.dtype;
   a.head_size = (int)D;
   a.token_major = !paged;
+  return KVC_OK;
+}
+
+int kvc_paged_prefill(kvc_dltensor* out, const kvc_dltensor* query, const kvc_dltensor* key_cache,
+                      const kvc_dltensor* value_cache, const kvc_dltensor* block_tables,
+                      const kvc_dltensor* qo_indptr, const kvc_dltensor* kv_lens, int num_kv_heads, float scale,
+                      int block_size, int max_q_len, int window_size, void* stream) {
+  PrefillArgs a;
+  int device_of_call = -1;
+  if (int rc = prepare_prefill(out, query, key_cache, value_cache, block_tables, qo_indptr, kv_lens, num_kv_heads,
+                               scale, block_size, max_q_len, window_size, &a, &device_of_call))
+    return rc;
   if (a.num_seqs == 0 || a.num_tokens == 0 || max_q_len == 0) return KVC_OK;
   if (a.num_seqs > 65535) return fail(KVC_EINVAL, "at most 65535 sequences per call");
   DeviceGuard g(device_of_call);
@@ -1105,6 +1120,294 @@ int kvc_gather_kv(kvc_dltensor* k_out, kvc_dltensor* v_out, const kvc_dltensor* 
   if (!g.ok()) return fail(KVC_ECUDA, "cudaSetDevice failed");
   cudaError_t e = launch_gather_kv(a, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e, "gather_kv launch");
+  return KVC_OK;
+}
+
+// ---- sliding window with sinks (window.cu) ----------------------------------------
+
+static int check_window(int window_size, int sink_size) {
+  if (window_size <= 0) return fail(KVC_EINVAL, "window_size must be positive");
+  if (sink_size < 0) return fail(KVC_EINVAL, "sink_size must be non-negative");
+  return KVC_OK;
+}
+
+int kvc_paged_attention_window(kvc_dltensor* out, const kvc_dltensor* query, const kvc_dltensor* key_cache,
+                               const kvc_dltensor* value_cache, const kvc_dltensor* block_tables,
+                               const kvc_dltensor* context_lens, int num_kv_heads, float scale, int block_size,
+                               int max_seq_len, int window_size, int sink_size, void* stream) {
+  if (int rc = check_window(window_size, sink_size)) return rc;
+  DecodeArgs a;
+  int device = -1;
+  const bool paged = key_cache != nullptr && key_cache->ndim == 5;
+  const int rc = paged ? prepare_decode(out, query, key_cache, value_cache, block_tables, context_lens, num_kv_heads,
+                                        scale, block_size, max_seq_len, nullptr, &a, &device)
+                       : prepare_flash(out, query, key_cache, value_cache, block_tables, context_lens, num_kv_heads,
+                                       scale, block_size, max_seq_len, nullptr, &a, &device);
+  if (rc) return rc;
+  if (a.num_seqs == 0) return KVC_OK;
+  DeviceGuard g(device);
+  if (!g.ok()) return fail(KVC_ECUDA, "cudaSetDevice failed");
+  WindowArgs w = {window_size, sink_size};
+  cudaError_t e = launch_window_decode(a, w, static_cast<cudaStream_t>(stream));
+  if (e == cudaErrorMisalignedAddress)
+    return fail(KVC_EINVAL, "key_cache/value_cache rows, blocks and heads must start on 16-byte boundaries");
+  if (e == cudaErrorNotSupported)
+    return fail(KVC_EUNSUPPORTED, "paged_attention_window over token-major caches needs query rows on 4-byte boundaries");
+  if (e != cudaSuccess) return cuda_fail(e, "paged_attention_window launch");
+  return KVC_OK;
+}
+
+int kvc_paged_prefill_window(kvc_dltensor* out, const kvc_dltensor* query, const kvc_dltensor* key_cache,
+                             const kvc_dltensor* value_cache, const kvc_dltensor* block_tables,
+                             const kvc_dltensor* qo_indptr, const kvc_dltensor* kv_lens, int num_kv_heads, float scale,
+                             int block_size, int max_q_len, int window_size, int sink_size, void* stream) {
+  if (int rc = check_window(window_size, sink_size)) return rc;
+  PrefillArgs a;
+  int device = -1;
+  if (int rc = prepare_prefill(out, query, key_cache, value_cache, block_tables, qo_indptr, kv_lens, num_kv_heads,
+                               scale, block_size, max_q_len, window_size, &a, &device))
+    return rc;
+  a.sinks = sink_size;
+  if (a.num_seqs == 0 || a.num_tokens == 0 || max_q_len == 0) return KVC_OK;
+  if (a.num_seqs > 65535) return fail(KVC_EINVAL, "at most 65535 sequences per call");
+  DeviceGuard g(device);
+  if (!g.ok()) return fail(KVC_ECUDA, "cudaSetDevice failed");
+  cudaError_t e = launch_window_prefill(a, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "paged_prefill_window launch");
+  return KVC_OK;
+}
+
+// ---- step tables, rotary positions (layer_ops.cu) ----------------------------------
+
+int kvc_step_tables(kvc_dltensor* block_tables, kvc_dltensor* kv_lens, kvc_dltensor* qo_indptr,
+                    kvc_dltensor* positions, kvc_dltensor* slot_mapping, kvc_dltensor* blocks_used,
+                    const kvc_dltensor* prefix_lens, const kvc_dltensor* new_lens, const kvc_dltensor* free_blocks,
+                    int block_size, void* stream) {
+  View bt, kl, qi, po, sm, us, pl, nl, fb;
+  if (!parse(block_tables, "block_tables", &bt) || !parse(kv_lens, "kv_lens", &kl) ||
+      !parse(qo_indptr, "qo_indptr", &qi) || !parse(positions, "positions", &po) ||
+      !parse(slot_mapping, "slot_mapping", &sm) || !parse(blocks_used, "blocks_used", &us) ||
+      !parse(prefix_lens, "prefix_lens", &pl) || !parse(new_lens, "new_lens", &nl) ||
+      !parse(free_blocks, "free_blocks", &fb))
+    return KVC_EINVAL;
+  if (bt.ndim != 2) return fail(KVC_EINVAL, "block_tables must be 2D");
+  const View* ones[] = {&kl, &qi, &po, &sm, &us, &pl, &nl, &fb};
+  for (const View* v : ones)
+    if (v->ndim != 1 || (v->shape[0] > 1 && v->stride(0) != 1))
+      return fail(KVC_EINVAL, "kv_lens, qo_indptr, positions, slot_mapping, blocks_used, prefix_lens, new_lens and "
+                              "free_blocks must be contiguous 1-D arrays");
+  const int64_t B = pl.shape[0];
+  if (nl.shape[0] != B || bt.shape[0] != B || kl.shape[0] != B || qi.shape[0] != B + 1 || us.shape[0] != 1)
+    return fail(KVC_EINVAL, "prefix_lens, new_lens, kv_lens and block_tables must have num_seqs rows, qo_indptr "
+                            "num_seqs + 1 and blocks_used one");
+  if (po.shape[0] != sm.shape[0]) return fail(KVC_EINVAL, "positions and slot_mapping must have the same length");
+  if (block_size <= 0) return fail(KVC_EINVAL, "block_size must be positive");
+  if (bt.dtype != ElemType::I32 || kl.dtype != ElemType::I32 || qi.dtype != ElemType::I32 ||
+      po.dtype != ElemType::I32 || us.dtype != ElemType::I32 || pl.dtype != ElemType::I32 ||
+      nl.dtype != ElemType::I32 || fb.dtype != ElemType::I32)
+    return fail(KVC_EINVAL, "block_tables, kv_lens, qo_indptr, positions, blocks_used, prefix_lens, new_lens and "
+                            "free_blocks must be int32");
+  if (sm.dtype != ElemType::I32 && sm.dtype != ElemType::I64)
+    return fail(KVC_EINVAL, "slot_mapping must be int32 or int64");
+  if (bt.shape[1] > 1 && bt.stride(1) != 1) return fail(KVC_EINVAL, "block_tables rows must be contiguous");
+  if (B > 1 && bt.stride(0) < bt.shape[1]) return fail(KVC_EINVAL, "block_tables rows must not overlap");
+  if (B > 0x7fffffffll - 2048) return fail(KVC_EINVAL, "too many sequences");
+  int device = -1;
+  if (int rc = check_all_cuda({&bt, &kl, &qi, &po, &sm, &us, &pl, &nl, &fb}, &device)) return rc;
+  StepTablesArgs a;
+  memset(&a, 0, sizeof(a));
+  a.tables = reinterpret_cast<int32_t*>(bt.data);
+  a.table_stride = bt.stride(0);
+  a.table_len = bt.shape[1];
+  a.prefix_lens = reinterpret_cast<const int32_t*>(pl.data);
+  a.new_lens = reinterpret_cast<const int32_t*>(nl.data);
+  a.free_blocks = reinterpret_cast<const int32_t*>(fb.data);
+  a.num_free = fb.shape[0];
+  a.kv_lens = reinterpret_cast<int32_t*>(kl.data);
+  a.qo_indptr = reinterpret_cast<int32_t*>(qi.data);
+  a.positions = reinterpret_cast<int32_t*>(po.data);
+  a.slots = sm.data;
+  a.slots_i64 = sm.dtype == ElemType::I64;
+  a.blocks_used = reinterpret_cast<int32_t*>(us.data);
+  a.num_seqs = (int)B;
+  a.block_size = block_size;
+  a.num_tokens = po.shape[0];
+  DeviceGuard g(device);
+  if (!g.ok()) return fail(KVC_ECUDA, "cudaSetDevice failed");
+  cudaError_t e = launch_step_tables(a, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "step_tables launch");
+  return KVC_OK;
+}
+
+int kvc_rotary_table(kvc_dltensor* cos_sin, const double* inv_freq, double factor, void* stream) {
+  View t;
+  if (!parse(cos_sin, "cos_sin", &t)) return KVC_EINVAL;
+  if (t.ndim != 2 || t.shape[1] <= 0 || t.shape[1] % 2 || t.shape[1] > 2 * kMaxRotaryHalf)
+    return fail(KVC_EINVAL, "cos_sin must have shape [positions, rotary_dim] with an even rotary_dim of at most " +
+                                std::to_string(2 * kMaxRotaryHalf));
+  if (t.dtype != ElemType::F32) return fail(KVC_EINVAL, "cos_sin must be float32");
+  if (t.stride(1) != 1) return fail(KVC_EINVAL, "cos_sin rows must be contiguous");
+  if (inv_freq == nullptr) return fail(KVC_EINVAL, "inv_freq is null");
+  int device = -1;
+  if (int rc = check_all_cuda({&t}, &device)) return rc;
+  RotaryTableArgs a;
+  memset(&a, 0, sizeof(a));
+  a.table = reinterpret_cast<float*>(t.data);
+  a.rows = t.shape[0];
+  a.stride = t.stride(0);
+  a.half = (int)(t.shape[1] / 2);
+  a.factor = factor;
+  for (int i = 0; i < a.half; ++i) {
+    if (!std::isfinite(inv_freq[i])) return fail(KVC_EINVAL, "inv_freq must be finite");
+    a.inv_freq[i] = inv_freq[i];
+  }
+  DeviceGuard g(device);
+  if (!g.ok()) return fail(KVC_ECUDA, "cudaSetDevice failed");
+  cudaError_t e = launch_rotary_table(a, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "rotary_table launch");
+  return KVC_OK;
+}
+
+// What both forms of the norm and rotation check: q, k, positions, the table,
+// the weights and q_out.
+static int prepare_rope(kvc_dltensor* q_out, const kvc_dltensor* q, const kvc_dltensor* k,
+                        const kvc_dltensor* positions, const kvc_dltensor* cos_sin, const kvc_dltensor* q_weight,
+                        const kvc_dltensor* k_weight, float eps, int interleaved, RopeArgs* a, int* device) {
+  View qv, kv, qo, po, cs, qw, kw;
+  if (!parse(q, "q", &qv) || !parse(k, "k", &kv) || !parse(q_out, "q_out", &qo) ||
+      !parse(positions, "positions", &po) || !parse(cos_sin, "cos_sin", &cs))
+    return KVC_EINVAL;
+  if ((q_weight && !parse(q_weight, "q_weight", &qw)) || (k_weight && !parse(k_weight, "k_weight", &kw)))
+    return KVC_EINVAL;
+  if (qv.ndim != 3 || kv.ndim != 3 || qv.shape[0] != kv.shape[0] || qv.shape[2] != kv.shape[2])
+    return fail(KVC_EINVAL, "q must have shape [num_tokens, num_heads, head_size] and k [num_tokens, num_kv_heads, "
+                            "head_size]");
+  const int64_t T = qv.shape[0], D = qv.shape[2];
+  if (qv.shape[1] <= 0 || kv.shape[1] <= 0 || D <= 0 || D > 512)
+    return fail(KVC_EINVAL, "head counts must be positive and head_size between 1 and 512");
+  if (qv.shape[1] > 1 << 20 || kv.shape[1] > 1 << 20) return fail(KVC_EINVAL, "unsupported head count");
+  if (!is_float(qv.dtype) || kv.dtype != qv.dtype)
+    return fail(KVC_EINVAL, std::string("q and k must share float32, float16 or bfloat16 (got ") +
+                                elem_name(qv.dtype) + "/" + elem_name(kv.dtype) + ")");
+  if (qo.ndim != 3 || qo.shape[0] != T || qo.shape[1] != qv.shape[1] || qo.shape[2] != D || qo.dtype != qv.dtype)
+    return fail(KVC_EINVAL, "q_out must have the shape and dtype of q");
+  if (D > 1 && (qv.stride(2) != 1 || kv.stride(2) != 1 || qo.stride(2) != 1))
+    return fail(KVC_EINVAL, "q/k/q_out head_size dimension must be contiguous");
+  if (po.ndim != 1 || po.shape[0] < T || (po.shape[0] > 1 && po.stride(0) != 1))
+    return fail(KVC_EINVAL, "positions must be a contiguous array of at least num_tokens entries");
+  if (po.dtype != ElemType::I32 && po.dtype != ElemType::I64)
+    return fail(KVC_EINVAL, "positions must be int32 or int64");
+  if (cs.ndim != 2 || cs.shape[1] <= 0 || cs.shape[1] % 2 || cs.shape[1] > D)
+    return fail(KVC_EINVAL, "cos_sin must have shape [positions, rotary_dim] with an even rotary_dim of at most "
+                            "head_size");
+  if (cs.dtype != ElemType::F32 || cs.stride(1) != 1)
+    return fail(KVC_EINVAL, "cos_sin must be float32 with contiguous rows");
+  for (const View* w : {q_weight ? &qw : nullptr, k_weight ? &kw : nullptr}) {
+    if (!w) continue;
+    if (w->ndim != 1 || w->shape[0] != D || (D > 1 && w->stride(0) != 1))
+      return fail(KVC_EINVAL, "q_weight/k_weight must be contiguous arrays of head_size entries");
+    if (w->dtype != ElemType::F32 && w->dtype != qv.dtype)
+      return fail(KVC_EINVAL, "q_weight/k_weight must be float32 or of q's dtype");
+  }
+  if (q_weight && k_weight && qw.dtype != kw.dtype) return fail(KVC_EINVAL, "q_weight and k_weight must share a dtype");
+  if ((q_weight || k_weight) && !(eps >= 0.f && std::isfinite(eps)))
+    return fail(KVC_EINVAL, "eps must be finite and non-negative");
+  if (int rc = check_all_cuda({&qv, &kv, &qo, &po, &cs, q_weight ? &qw : nullptr, k_weight ? &kw : nullptr}, device))
+    return rc;
+  memset(a, 0, sizeof(*a));
+  a->q = qv.data;
+  a->k = kv.data;
+  a->q_out = qo.data;
+  a->positions = po.data;
+  a->table = reinterpret_cast<const float*>(cs.data);
+  a->q_weight = q_weight ? qw.data : nullptr;
+  a->k_weight = k_weight ? kw.data : nullptr;
+  a->type = a->cache_type = qv.dtype;
+  a->weight_type = q_weight ? qw.dtype : (k_weight ? kw.dtype : qv.dtype);
+  a->pos_i64 = po.dtype == ElemType::I64;
+  a->interleaved = interleaved != 0;
+  a->eps = eps;
+  a->num_heads = (int)qv.shape[1];
+  a->num_kv_heads = (int)kv.shape[1];
+  a->head_size = (int)D;
+  a->rot = (int)cs.shape[1];
+  a->num_tokens = T;
+  a->table_rows = cs.shape[0];
+  a->table_stride = cs.stride(0);
+  a->q_tok = qv.stride(0);
+  a->q_head = qv.stride(1);
+  a->k_tok = kv.stride(0);
+  a->k_head = kv.stride(1);
+  a->qo_tok = qo.stride(0);
+  a->qo_head = qo.stride(1);
+  return KVC_OK;
+}
+
+int kvc_qk_norm_rope(kvc_dltensor* q_out, kvc_dltensor* k_out, const kvc_dltensor* q, const kvc_dltensor* k,
+                     const kvc_dltensor* positions, const kvc_dltensor* cos_sin, const kvc_dltensor* q_weight,
+                     const kvc_dltensor* k_weight, float eps, int interleaved, void* stream) {
+  RopeArgs a;
+  int device = -1;
+  if (int rc = prepare_rope(q_out, q, k, positions, cos_sin, q_weight, k_weight, eps, interleaved, &a, &device))
+    return rc;
+  View ko;
+  if (!parse(k_out, "k_out", &ko)) return KVC_EINVAL;
+  if (ko.ndim != 3 || ko.shape[0] != a.num_tokens || ko.shape[1] != a.num_kv_heads || ko.shape[2] != a.head_size ||
+      ko.dtype != a.type)
+    return fail(KVC_EINVAL, "k_out must have the shape and dtype of k");
+  if (a.head_size > 1 && ko.stride(2) != 1) return fail(KVC_EINVAL, "k_out head_size dimension must be contiguous");
+  int dev2 = -1;
+  if (int rc = check_all_cuda({&ko}, &dev2)) return rc;
+  if (dev2 != device) return fail(KVC_EINVAL, "all tensors must live on the same CUDA device");
+  a.k_out = ko.data;
+  a.ko_tok = ko.stride(0);
+  a.ko_head = ko.stride(1);
+  if (a.num_tokens == 0) return KVC_OK;
+  DeviceGuard g(device);
+  if (!g.ok()) return fail(KVC_ECUDA, "cudaSetDevice failed");
+  cudaError_t e = launch_qk_norm_rope(a, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "qk_norm_rope launch");
+  return KVC_OK;
+}
+
+int kvc_qk_norm_rope_append(kvc_dltensor* q_out, kvc_dltensor* key_cache, kvc_dltensor* value_cache,
+                            const kvc_dltensor* q, const kvc_dltensor* k, const kvc_dltensor* v,
+                            const kvc_dltensor* positions, const kvc_dltensor* cos_sin, const kvc_dltensor* q_weight,
+                            const kvc_dltensor* k_weight, float eps, int interleaved, const kvc_dltensor* slot_mapping,
+                            void* stream) {
+  RopeArgs a;
+  int device = -1;
+  if (int rc = prepare_rope(q_out, q, k, positions, cos_sin, q_weight, k_weight, eps, interleaved, &a, &device))
+    return rc;
+  const bool paged = key_cache != nullptr && key_cache->ndim == 5;
+  ReshapeArgs r;
+  int dev2 = device;
+  if (int rc = prepare_reshape(k, v, key_cache, value_cache, slot_mapping, !paged, &r, &dev2)) return rc;
+  if (dev2 != device) return fail(KVC_EINVAL, "all tensors must live on the same CUDA device");
+  if (r.slot_type == ElemType::U32) return fail(KVC_EINVAL, "slot_mapping must be int32 or int64");
+  if (r.num_tokens != a.num_tokens) return fail(KVC_EINVAL, "q, k and v must hold the same tokens");
+  a.v = r.value;
+  a.v_tok = r.value_tok_stride;
+  a.v_head = r.value_head_stride;
+  a.k_cache = r.key_cache;
+  a.v_cache = r.value_cache;
+  a.slots = r.slots;
+  a.slots_i64 = r.slot_type == ElemType::I64;
+  a.cache_type = r.cache_type;
+  a.paged = paged;
+  a.block_size = r.block_size;
+  a.num_blocks = r.num_blocks;
+  a.kc_block = r.kc_block_stride;
+  a.kc_head = r.kc_head_stride;
+  a.kc_tok = paged ? 0 : r.kc_tok_stride;
+  a.vc_block = r.vc_block_stride;
+  a.vc_head = r.vc_head_stride;
+  a.vc_tok = paged ? 0 : r.vc_tok_stride;
+  if (a.num_tokens == 0) return KVC_OK;
+  DeviceGuard g(device);
+  if (!g.ok()) return fail(KVC_ECUDA, "cudaSetDevice failed");
+  cudaError_t e = launch_qk_norm_rope(a, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "qk_norm_rope_append launch");
   return KVC_OK;
 }
 

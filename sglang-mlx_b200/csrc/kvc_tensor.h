@@ -156,7 +156,61 @@ struct PrefillArgs {
   float* part_sum;
   float* part_out;
   int64_t part_seq_stride, part_head_stride, part_out_seq_stride, part_out_head_stride, part_out_part_stride;
+  int sinks;         // window form (window.cu): first tokens of a sequence that stay visible
   int single_issue;  // tcgen05 kernel: the producer's lane 0 issues every copy of a tile (tuning; default: spread)
+};
+
+// Step tables (layer_ops.cu): requests' lengths -> block tables, offsets,
+// positions and slots of a step's new tokens.
+struct StepTablesArgs {
+  int32_t* tables;  // [num_seqs][table_len], rows table_stride apart; new blocks are written in place
+  int64_t table_stride, table_len;
+  const int32_t* prefix_lens;
+  const int32_t* new_lens;
+  const int32_t* free_blocks;
+  int64_t num_free;
+  int32_t* kv_lens;
+  int32_t* qo_indptr;
+  int32_t* positions;
+  void* slots;
+  bool slots_i64;
+  int32_t* blocks_used;
+  int num_seqs, block_size;
+  int64_t num_tokens;  // rows of positions / slots
+};
+
+constexpr int kMaxRotaryHalf = 128;
+struct RotaryTableArgs {
+  float* table;
+  int64_t rows, stride;
+  int half;
+  double factor;
+  double inv_freq[kMaxRotaryHalf];
+};
+
+// Per-head norm and rotary position, and (k_cache set) the append of K and V.
+// Strides in elements.
+struct RopeArgs {
+  const void* q;
+  const void* k;
+  const void* v;  // append only
+  void* q_out;
+  void* k_out;  // without append
+  const void* positions;
+  const float* table;  // [table_rows][rot]: cosines, then sines
+  const void* q_weight;  // [head_size] or nullptr (no norm)
+  const void* k_weight;
+  void* k_cache;
+  void* v_cache;
+  const void* slots;
+  ElemType type, cache_type, weight_type;
+  bool pos_i64, slots_i64, interleaved;
+  bool paged;  // append: the [nb, H, D/x, bs, x] / [nb, H, D, bs] layout, else token-major rows
+  float eps;
+  int num_heads, num_kv_heads, head_size, rot, block_size;
+  int64_t num_tokens, table_rows, table_stride, num_blocks;
+  int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head, qo_tok, qo_head, ko_tok, ko_head;
+  int64_t kc_block, kc_head, kc_tok, vc_block, vc_head, vc_tok;
 };
 
 struct ReshapeArgs {
@@ -230,6 +284,15 @@ cudaError_t launch_convert_fp8(ElemType src_type, ElemType dst_type, const void*
                                int64_t n, int fmt, cudaStream_t stream);
 cudaError_t launch_reshape_and_cache_flash(const ReshapeArgs& a, cudaStream_t stream);
 cudaError_t launch_gather_kv(const GatherArgs& a, cudaStream_t stream);
+cudaError_t launch_step_tables(const StepTablesArgs& a, cudaStream_t stream);
+cudaError_t launch_rotary_table(const RotaryTableArgs& a, cudaStream_t stream);
+cudaError_t launch_qk_norm_rope(const RopeArgs& a, cudaStream_t stream);
+// Sliding window with sinks over the paged cache (window.cu): decode and extend.
+struct WindowArgs {
+  int window, sinks;
+};
+cudaError_t launch_window_decode(const DecodeArgs& a, const WindowArgs& w, cudaStream_t stream);
+cudaError_t launch_window_prefill(const PrefillArgs& a, cudaStream_t stream);
 
 }  // namespace kvc
 
@@ -237,3 +300,5 @@ cudaError_t launch_gather_kv(const GatherArgs& a, cudaStream_t stream);
 unsigned int kvc_cache_ops_status(int clear, cudaError_t* err);
 unsigned int kvc_decode_status(int clear, cudaError_t* err);
 unsigned int kvc_block_ops_status(int clear, cudaError_t* err);
+unsigned int kvc_layer_ops_status(int clear, cudaError_t* err);
+unsigned int kvc_window_status(int clear, cudaError_t* err);

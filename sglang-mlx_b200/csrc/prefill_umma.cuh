@@ -166,15 +166,16 @@ struct UmmaSched {
   unsigned next, done;
 };
 constexpr int kUmmaSchedSlots = 4096, kUmmaSchedCaptured = 1024;
-__device__ UmmaSched g_umma_sched[kUmmaSchedSlots];
+static __device__ UmmaSched g_umma_sched[kUmmaSchedSlots];
 
 struct UmmaItem {
   int64_t q0, rows, R0;
-  int y, kvh, prefix, kv_beg, kv_end, ntiles;
+  int y, kvh, prefix, kv_beg, kv_end, ntiles;  // (window form: virtual key positions, prefix less the gap)
+  Seen seen;                                   // window form only
   bool bad, skip, first_tile;
 };
 
-template <bool CASCADE>
+template <bool CASCADE, bool WINDOW = false>
 __device__ __forceinline__ UmmaItem umma_item(const PrefillArgs& p, int idx, int tiles_x, int ny) {
   constexpr int KT = kUmmaTile;
   UmmaItem it;
@@ -211,9 +212,15 @@ __device__ __forceinline__ UmmaItem umma_item(const PrefillArgs& p, int idx, int
     it.prefix = it.bad ? 0 : (int)(kvl - ql);
     const int64_t R_last = (it.R0 + kUmmaRows < it.rows ? it.R0 + kUmmaRows : it.rows) - 1;
     const int t_first = (int)(it.R0 / G), t_last = (int)(R_last / G);
-    it.kv_end = it.bad ? 0 : it.prefix + t_last + 1;
-    int kb = p.window > 0 ? it.prefix + t_first + 1 - p.window : 0;
-    it.kv_beg = kb > 0 ? kb / KT * KT : 0;
+    if constexpr (WINDOW) {
+      it.seen = seen_range(it.prefix + t_first, it.prefix + t_last, p.window, p.sinks, p.block_size);
+      it.prefix -= it.seen.jump;
+      it.kv_end = it.bad ? 0 : it.seen.end;
+    } else {
+      it.kv_end = it.bad ? 0 : it.prefix + t_last + 1;
+      int kb = p.window > 0 ? it.prefix + t_first + 1 - p.window : 0;
+      it.kv_beg = kb > 0 ? kb / KT * KT : 0;
+    }
   }
   it.ntiles = it.kv_end > it.kv_beg ? (it.kv_end - it.kv_beg + KT - 1) / KT : 0;
   it.skip = false;
@@ -230,7 +237,12 @@ __device__ __forceinline__ UmmaItem umma_item(const PrefillArgs& p, int idx, int
 // tiles_x x ny x num_kv_heads items) until none is left, keeping TMEM, its
 // barriers and its ring across them (every barrier phase below counts this
 // CTA's tiles or items).
-template <typename T, int D, int BS, bool GK, bool CASCADE = false>
+// WINDOW: prefill / extend under a sliding window whose first p.sinks tokens stay
+// visible.  An item's keys are its sink blocks and its window's blocks, numbered
+// without the gap (struct Seen): the tiles are filled page by page, so the few
+// sink tokens share a tile with the window's first pages, and a tile starts at
+// the window's first block, not at a multiple of 128 tokens.
+template <typename T, int D, int BS, bool GK, bool CASCADE = false, bool WINDOW = false>
 __global__ void __launch_bounds__(kUmmaThreads, 1)
     prefill_umma_kernel(const PrefillArgs p, const __grid_constant__ TmaMaps maps, int tiles_x, int ny, int slot) {
   using namespace mma_detail;
@@ -284,10 +296,10 @@ __global__ void __launch_bounds__(kUmmaThreads, 1)
       asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&maps.v)) : "memory");
       if (GK) asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&maps.k)) : "memory");
     }
-    it0 = umma_item<CASCADE>(p, blockIdx.x, tiles_x, ny);
+    it0 = umma_item<CASCADE, WINDOW>(p, blockIdx.x, tiles_x, ny);
     const uint32_t* t0row = p.block_tables + (CASCADE ? (int64_t)0 : (int64_t)it0.y * p.table_stride);
     if (!it0.skip && lane < PAGES && it0.ntiles > 0 && it0.kv_beg + lane * BS < it0.kv_end)
-      first_id = __ldg(t0row + (it0.kv_beg + lane * BS) / BS);
+      first_id = __ldg(t0row + (WINDOW ? it0.seen.real_block(lane) : (it0.kv_beg + lane * BS) / BS));
   }
 
   if (threadIdx.x == 0) {
@@ -355,7 +367,7 @@ __global__ void __launch_bounds__(kUmmaThreads, 1)
     UmmaSched* sched = &g_umma_sched[slot];
     for (int idx = blockIdx.x; idx < n_items && !stop;) {
       const bool first = idx == (int)blockIdx.x;  // (claimed items are all past the grid)
-      const UmmaItem it = first ? it0 : umma_item<CASCADE>(p, idx, tiles_x, ny);
+      const UmmaItem it = first ? it0 : umma_item<CASCADE, WINDOW>(p, idx, tiles_x, ny);
       if (!CASCADE && it.bad && it.first_tile && it.kvh == 0 && lane == 0)
         set_status(&g_decode_status, KVC_STATUS_INDEX_OOB);
       // the next item is claimed once this one's loads are issued
@@ -394,7 +406,8 @@ __global__ void __launch_bounds__(kUmmaThreads, 1)
       auto load_id = [&](int j) -> uint32_t {
         uint32_t id = 0xffffffffu;
         const int tok = kv_beg + j * KT + lane * BS;
-        if (lane < PAGES && j < ntiles && tok < kv_end) id = __ldg(table + tok / BS);
+        if (lane < PAGES && j < ntiles && tok < kv_end)
+          id = __ldg(table + (WINDOW ? it.seen.real_block(tok / BS) : tok / BS));
         return id;
       };
       uint32_t id = first ? first_id : load_id(0);
@@ -542,7 +555,7 @@ __global__ void __launch_bounds__(kUmmaThreads, 1)
         mbar_arrive(&item_empty[sl]);
         ++nread;
         if (idx >= n_items) break;
-        const UmmaItem it = umma_item<CASCADE>(p, idx, tiles_x, ny);
+        const UmmaItem it = umma_item<CASCADE, WINDOW>(p, idx, tiles_x, ny);
         if (it.skip || it.ntiles == 0) continue;  // (no Q is handed over for an item without keys)
         if (abort_now() || !umma::wait(q_ready, (uint32_t)(nit & 1))) {
           ok = false;
@@ -661,6 +674,7 @@ __global__ void __launch_bounds__(kUmmaThreads, 1)
     struct RowItem {
       int64_t q0;
       int y, kvh, kv_beg, kv_end, ntiles;
+      int v_beg;               // window form: the item's first window position (virtual)
       int t, g, end_r, beg_r;  // t: the new token (prefill) or the sequence (cascade) of the row
       bool in_tile;            // a row (else padding of the last tile)
     };
@@ -682,7 +696,7 @@ __global__ void __launch_bounds__(kUmmaThreads, 1)
         if (lane == 0) mbar_arrive(&item_empty[sl]);
         ++nread;
         if (idx >= n_items) return false;
-        const UmmaItem it = umma_item<CASCADE>(p, idx, tiles_x, ny);
+        const UmmaItem it = umma_item<CASCADE, WINDOW>(p, idx, tiles_x, ny);
         if (it.skip) continue;
         ri.q0 = it.q0;
         ri.y = it.y;
@@ -690,6 +704,7 @@ __global__ void __launch_bounds__(kUmmaThreads, 1)
         ri.kv_beg = it.kv_beg;
         ri.kv_end = it.kv_end;
         ri.ntiles = it.ntiles;
+        if constexpr (WINDOW) ri.v_beg = it.seen.beg;
         bool on;  // a row that sees keys
         const int64_t R = it.R0 + r;
         ri.in_tile = R < it.rows;
@@ -801,7 +816,8 @@ __global__ void __launch_bounds__(kUmmaThreads, 1)
 #pragma unroll
           for (int c = 0; c < HK; ++c) {
             const int tok = t0 + c;
-            const bool vis = tok >= beg_r && tok < end_r && ((pm >> ((half * HK + c) / BS)) & 1u);
+            const bool vis = (tok >= beg_r || (WINDOW && tok < p.sinks)) && tok < end_r &&
+                             ((pm >> ((half * HK + c) / BS)) & 1u);
             x[c] = vis ? x[c] * qk_scale : -INFINITY;
             mx = fmaxf(mx, x[c]);
           }
@@ -887,6 +903,24 @@ __global__ void __launch_bounds__(kUmmaThreads, 1)
                 const int ch = tk / 8;
                 const int phys = BS == 32 ? (ch ^ ((d >> 1) & 3)) : (ch ^ ((d >> 2) & 1));
                 *reinterpret_cast<uint16_t*>(vpage + d * BS * 2 + phys * 16 + (tk % 8) * 2) = 0;
+              }
+            }
+            fence_proxy_async();
+          }
+        }
+        // window form: V of the tokens between the sinks and the first row's window
+        // start, which share their pages with seen ones, becomes 0 for the same reason
+        if constexpr (WINDOW) {
+          const int u0 = p.sinks > tile0 ? p.sinks : tile0;
+          const int u1 = cur.v_beg < tile0 + KT ? cur.v_beg : tile0 + KT;
+          if (half == 0 && u0 < u1) {
+            const int d = r;
+            if (d < D) {
+              uint8_t* vst = ring + (size_t)st * UG::STAGE + PAGES * PAGE;
+              for (int tk = u0 - tile0; tk < u1 - tile0; ++tk) {
+                const int ch = (tk % BS) / 8;
+                const int phys = BS == 32 ? (ch ^ ((d >> 1) & 3)) : (ch ^ ((d >> 2) & 1));
+                *reinterpret_cast<uint16_t*>(vst + (tk / BS) * PAGE + d * BS * 2 + phys * 16 + (tk % 8) * 2) = 0;
               }
             }
             fence_proxy_async();
@@ -1033,246 +1067,6 @@ static int umma_sched_slot(cudaStream_t stream) {
     return kUmmaSchedSlots - kUmmaSchedCaptured +
            (int)(next_captured.fetch_add(1u, std::memory_order_relaxed) % (unsigned)kUmmaSchedCaptured);
   return (int)(next.fetch_add(1u, std::memory_order_relaxed) % (unsigned)(kUmmaSchedSlots - kUmmaSchedCaptured));
-}
-
-// the two-tile form of the gathered-K kernel (prefill_umma_pair.cuh)
-static bool pair_enabled();
-template <typename T, int D, int BS, bool CASCADE>
-static cudaError_t launch_pair(const PrefillArgs& a, const TmaMaps& maps, int64_t tiles, int ny, cudaStream_t stream);
-
-template <typename T, int D, int BS, bool GK>
-static cudaError_t launch_prefill_umma(const PrefillArgs& a, cudaStream_t stream) {
-  using UG = UmmaGeom<D, BS>;
-  DecodeParams dp;
-  memset(&dp, 0, sizeof(dp));
-  dp.k_cache = a.k_cache;
-  dp.v_cache = a.v_cache;
-  dp.num_blocks = a.num_blocks;
-  dp.num_kv_heads = a.num_kv_heads;
-  dp.k_head_stride = a.k_head_stride;
-  dp.k_block_stride = a.k_block_stride;
-  dp.v_head_stride = a.v_head_stride;
-  dp.v_block_stride = a.v_block_stride;
-  TmaMaps maps;
-  memset(&maps, 0, sizeof(maps));
-  // the kTiles maps: V as [nb][H][D][BS] pages, one whole page per box, bs*2-byte swizzle
-  if (!make_tensor_maps(dp, std::is_same<T, __nv_bfloat16>::value ? ElemType::BF16 : ElemType::F16, D, BS, BS, BS * 2,
-                        kTiles, &maps))
-    return cudaErrorNotSupported;
-  if (GK && !make_k_gather_map(a, D, BS, &maps.k)) return cudaErrorNotSupported;
-  if constexpr (GK) {
-    if (pair_enabled()) {
-      const int G2 = a.num_heads / a.num_kv_heads;
-      const int64_t tiles2 = ((int64_t)a.max_q_len * G2 + kUmmaRows - 1) / kUmmaRows;
-      if (tiles2 <= 0 || a.num_seqs <= 0) return cudaSuccess;
-      const cudaError_t e = launch_pair<T, D, BS, false>(a, maps, tiles2, (int)a.num_seqs, stream);
-      if (e != cudaErrorNotSupported) return e;
-    }
-  }
-  auto kern = prefill_umma_kernel<T, D, BS, GK>;
-  static std::atomic<bool> configured[64];  // per device; setting the attribute twice is harmless
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev >= 0 && dev < 64 && !configured[dev]) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, UG::SMEM);
-    if (e != cudaSuccess) return e;
-    configured[dev] = true;
-  }
-  const int G = a.num_heads / a.num_kv_heads;
-  const int64_t tiles = ((int64_t)a.max_q_len * G + kUmmaRows - 1) / kUmmaRows;
-  if (tiles <= 0 || a.num_seqs <= 0) return cudaSuccess;
-  const int64_t items = tiles * a.num_seqs * a.num_kv_heads;
-  if (items > 0x7fffffffll - 1024) return cudaErrorInvalidValue;
-  const int ctas = umma_persistent_ctas(dev, items);
-  const int slot = umma_sched_slot(stream);  // (runtime queries stay outside the launch statement)
-  PrefillArgs aa = a;
-  aa.single_issue = umma_single_issue();
-  kern<<<ctas, kUmmaThreads, UG::SMEM, stream>>>(aa, maps, (int)tiles, (int)a.num_seqs, slot);
-  count_launch();
-  return cudaGetLastError();
-}
-
-// The tcgen05 kernel serves the paged layout with block size 16 or 32 (pages
-// tile a 128-token S tile; V rows of 32 or 64 bytes match a swizzle mode).
-static bool prefill_umma_supported(const PrefillArgs& a) {
-  if (a.token_major || !(a.block_size == 16 || a.block_size == 32) || !(a.head_size == 64 || a.head_size == 128))
-    return false;
-  // rows are stored as 16-byte vectors
-  if ((reinterpret_cast<uintptr_t>(a.out) & 15u) || (a.out_tok_stride & 7) || (a.out_head_stride & 7)) return false;
-  const char* v = getenv("KVC_PREFILL_KERNEL");
-  return !(v && (v[0] == 'm' || v[0] == 'M'));  // "mma": the mma.sync kernel
-}
-
-static cudaError_t launch_prefill_umma_any(const PrefillArgs& a, cudaStream_t stream) {
-  const bool bf = a.q_type == ElemType::BF16;
-  const int64_t D = a.head_size, BS = a.block_size;
-  // the 4-row gathers need K rows uniformly strided: the dense paged layout
-  const bool dense = a.k_head_stride == D * BS && a.k_block_stride == (int64_t)a.num_kv_heads * D * BS &&
-                     a.num_blocks * a.num_kv_heads * (D / 8) < 0x7fffffffll;  // (row indices are 32-bit)
-  if (a.head_size == 128) {
-    if (a.block_size == 32) {
-      if (dense)
-        return bf ? launch_prefill_umma<__nv_bfloat16, 128, 32, true>(a, stream)
-                  : launch_prefill_umma<__half, 128, 32, true>(a, stream);
-      return bf ? launch_prefill_umma<__nv_bfloat16, 128, 32, false>(a, stream)
-                : launch_prefill_umma<__half, 128, 32, false>(a, stream);
-    }
-    if (dense)
-      return bf ? launch_prefill_umma<__nv_bfloat16, 128, 16, true>(a, stream)
-                : launch_prefill_umma<__half, 128, 16, true>(a, stream);
-    return bf ? launch_prefill_umma<__nv_bfloat16, 128, 16, false>(a, stream)
-              : launch_prefill_umma<__half, 128, 16, false>(a, stream);
-  }
-  if (a.block_size == 32) {
-    if (dense)
-      return bf ? launch_prefill_umma<__nv_bfloat16, 64, 32, true>(a, stream)
-                : launch_prefill_umma<__half, 64, 32, true>(a, stream);
-    return bf ? launch_prefill_umma<__nv_bfloat16, 64, 32, false>(a, stream)
-              : launch_prefill_umma<__half, 64, 32, false>(a, stream);
-  }
-  if (dense)
-    return bf ? launch_prefill_umma<__nv_bfloat16, 64, 16, true>(a, stream)
-              : launch_prefill_umma<__half, 64, 16, true>(a, stream);
-  return bf ? launch_prefill_umma<__nv_bfloat16, 64, 16, false>(a, stream)
-            : launch_prefill_umma<__half, 64, 16, false>(a, stream);
-}
-
-// ---- shared-prefix (cascade) decode through the tcgen05 kernel ----
-template <typename T, int D, int BS, bool GK>
-static cudaError_t launch_cascade_umma(const PrefillArgs& a, int prefix_parts, cudaStream_t stream) {
-  using UG = UmmaGeom<D, BS>;
-  DecodeParams dp;
-  memset(&dp, 0, sizeof(dp));
-  dp.k_cache = a.k_cache;
-  dp.v_cache = a.v_cache;
-  dp.num_blocks = a.num_blocks;
-  dp.num_kv_heads = a.num_kv_heads;
-  dp.k_head_stride = a.k_head_stride;
-  dp.k_block_stride = a.k_block_stride;
-  dp.v_head_stride = a.v_head_stride;
-  dp.v_block_stride = a.v_block_stride;
-  TmaMaps maps;
-  memset(&maps, 0, sizeof(maps));
-  if (!make_tensor_maps(dp, std::is_same<T, __nv_bfloat16>::value ? ElemType::BF16 : ElemType::F16, D, BS, BS, BS * 2,
-                        kTiles, &maps))
-    return cudaErrorNotSupported;
-  if (GK && !make_k_gather_map(a, D, BS, &maps.k)) return cudaErrorNotSupported;
-  if constexpr (GK) {
-    if (pair_enabled()) {
-      const int G2 = a.num_heads / a.num_kv_heads;
-      const cudaError_t e = launch_pair<T, D, BS, true>(
-          a, maps, ((int64_t)a.num_seqs * G2 + kUmmaRows - 1) / kUmmaRows, prefix_parts, stream);
-      if (e != cudaErrorNotSupported) return e;
-    }
-  }
-  auto kern = prefill_umma_kernel<T, D, BS, GK, true>;
-  static std::atomic<bool> configured[64];  // per device; setting the attribute twice is harmless
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev >= 0 && dev < 64 && !configured[dev]) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, UG::SMEM);
-    if (e != cudaSuccess) return e;
-    configured[dev] = true;
-  }
-  const int G = a.num_heads / a.num_kv_heads;
-  const int64_t tiles = ((int64_t)a.num_seqs * G + kUmmaRows - 1) / kUmmaRows;
-  const int64_t items = tiles * prefix_parts * a.num_kv_heads;
-  if (items <= 0) return cudaSuccess;
-  if (items > 0x7fffffffll - 1024) return cudaErrorInvalidValue;
-  const int ctas = umma_persistent_ctas(dev, items);
-  const int slot = umma_sched_slot(stream);
-  PrefillArgs aa = a;
-  aa.single_issue = umma_single_issue();
-  // a programmatic dependent of the kernel before it (see the kernel's start)
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)ctas);
-  cfg.blockDim = dim3(kUmmaThreads);
-  cfg.dynamicSmemBytes = UG::SMEM;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, aa, maps, (int)tiles, prefix_parts, slot);
-  count_launch();
-  return e != cudaSuccess ? e : cudaGetLastError();
-}
-
-// The prefix of a shared-prefix decode on the tensor cores' own pipeline when
-// the cache suits the gathered-K tcgen05 kernel (dense paged layout, block size
-// 16 or 32, head size 64 / 128, prefix and chunks in whole blocks, partial
-// buffers of 16-byte rows);
-// cudaErrorNotSupported otherwise (the caller then runs the mma.sync prefix
-// kernel).
-static cudaError_t launch_cascade_prefix_umma(const DecodeParams& p, const DecodeArgs& da, cudaStream_t stream) {
-  const int D = da.head_size, BS = da.block_size;
-  // Only the gathered-K form (dense K): with per-page S chains (N = 16 for
-  // block size 16, 64 products per tile) the single-lane product issue set the
-  // pace and config 4 measured 69.0 us against 65.9 us for the mma.sync prefix
-  // kernel.
-  if (!(BS == 16 || BS == 32) || !(D == 64 || D == 128)) return cudaErrorNotSupported;
-  if (!(p.k_head_stride == (int64_t)D * BS && p.k_block_stride == (int64_t)p.num_kv_heads * D * BS))
-    return cudaErrorNotSupported;
-  if ((reinterpret_cast<uintptr_t>(p.part_out) & 15u) || (p.part_out_seq_stride & 3) || (p.part_out_head_stride & 3) ||
-      (p.part_out_part_stride & 3) || (p.prefix_len % BS) || (p.prefix_part_size % BS))
-    return cudaErrorNotSupported;
-  const char* v = getenv("KVC_PREFILL_KERNEL");
-  if (v && (v[0] == 'm' || v[0] == 'M')) return cudaErrorNotSupported;
-  PrefillArgs a;
-  memset(&a, 0, sizeof(a));
-  a.q = p.q;
-  a.k_cache = p.k_cache;
-  a.v_cache = p.v_cache;
-  a.block_tables = p.block_tables;
-  a.num_seqs = p.num_seqs;
-  a.num_heads = p.num_heads;
-  a.num_kv_heads = p.num_kv_heads;
-  a.block_size = BS;
-  a.num_blocks = p.num_blocks;
-  a.table_stride = p.table_stride;
-  a.q_tok_stride = p.q_seq_stride;
-  a.q_head_stride = p.q_head_stride;
-  a.k_block_stride = p.k_block_stride;
-  a.k_head_stride = p.k_head_stride;
-  a.v_block_stride = p.v_block_stride;
-  a.v_head_stride = p.v_head_stride;
-  a.scale = p.scale;
-  a.q_type = da.q_type;
-  a.head_size = D;
-  a.context_lens = p.context_lens;
-  a.max_seq_len = p.max_seq_len;
-  a.prefix_len = p.prefix_len;
-  a.prefix_part_size = p.prefix_part_size;
-  a.part_max = p.part_max;
-  a.part_sum = p.part_sum;
-  a.part_out = p.part_out;
-  a.part_seq_stride = p.part_seq_stride;
-  a.part_head_stride = p.part_head_stride;
-  a.part_out_seq_stride = p.part_out_seq_stride;
-  a.part_out_head_stride = p.part_out_head_stride;
-  a.part_out_part_stride = p.part_out_part_stride;
-  const bool bf = a.q_type == ElemType::BF16;
-  const bool dense = a.k_head_stride == (int64_t)D * BS && a.k_block_stride == (int64_t)a.num_kv_heads * D * BS &&
-                     a.num_blocks * a.num_kv_heads * (D / 8) < 0x7fffffffll;
-  const int parts = p.prefix_parts;
-  if (!dense) return cudaErrorNotSupported;
-  if (D == 128)
-    return BS == 32 ? (bf ? launch_cascade_umma<__nv_bfloat16, 128, 32, true>(a, parts, stream)
-                          : launch_cascade_umma<__half, 128, 32, true>(a, parts, stream))
-                    : (bf ? launch_cascade_umma<__nv_bfloat16, 128, 16, true>(a, parts, stream)
-                          : launch_cascade_umma<__half, 128, 16, true>(a, parts, stream));
-  return BS == 32 ? (bf ? launch_cascade_umma<__nv_bfloat16, 64, 32, true>(a, parts, stream)
-                        : launch_cascade_umma<__half, 64, 32, true>(a, parts, stream))
-                  : (bf ? launch_cascade_umma<__nv_bfloat16, 64, 16, true>(a, parts, stream)
-                        : launch_cascade_umma<__half, 64, 16, true>(a, parts, stream));
-}
-
-cudaError_t launch_paged_prefill(const PrefillArgs& a, cudaStream_t stream) {
-  if (a.num_seqs <= 0 || a.max_q_len <= 0) return cudaSuccess;
-  if (a.num_seqs > 65535 || a.num_kv_heads > 65535) return cudaErrorInvalidValue;
-  if (prefill_umma_supported(a)) return launch_prefill_umma_any(a, stream);
-  return launch_prefill_mma_any(a, stream);
 }
 
 }  // namespace kvc

@@ -1,0 +1,788 @@
+// window.cu — attention over a sliding window with a few first tokens that stay
+// visible (sinks), on the paged and token-major caches, for sm_100a: one new
+// token per sequence (decode, below) and the new tokens of a ragged batch
+// (extend: the prefill kernels in their WINDOW form).
+//
+// The query at position i of a sequence sees position j <= i when j < sinks or
+// j > i - window:
+//   out = sum_j e^{s_j - m} v_j / (sum_j e^{s_j - m} + 1e-6),  s_j = scale q.k_j
+// with m the largest s_j; a sequence of length 0 or past max_seq_len gives zeros.
+#include "decode_common.cuh"
+#include "decode_mma.cuh"
+#include "prefill.cuh"
+#include "prefill_umma.cuh"
+
+namespace kvc {
+
+// ---------------------------------------------------------------------------
+// Decode.  What a sequence sees is at most window + sinks tokens (and the rest
+// of their blocks), whatever its length, so instead of partitions of the
+// context with partials in device memory and a second kernel, the seen blocks of
+// one (sequence, KV head) go to the CTAs of one thread-block cluster in equal
+// runs, and the cluster joins its softmax states through distributed shared
+// memory: CTA r owns a slice of the output elements, every CTA stores its
+// (max, sum) and its unnormalised values of that slice into r's shared memory,
+// and after one cluster barrier each CTA finishes its own slice.  One launch, no
+// workspace, a fixed order of summation.
+// ---------------------------------------------------------------------------
+constexpr int kMaxCluster = 16;
+
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t n;
+  asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(n));
+  return n;
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t n;
+  asm volatile("mov.u32 %0, %%cluster_ctaid.x;" : "=r"(n));
+  return n;
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+// Stores into the shared memory of CTA `rank` of the cluster, at this CTA's address `dst`.
+__device__ __forceinline__ void store_remote(const float* dst, uint32_t rank, float v) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
+               : "=r"(a)
+               : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(dst))), "r"(rank));
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(a), "f"(v) : "memory");
+}
+
+// The exchange area of one CTA: [C][nh] (max, sum) pairs, then [C][S] values of
+// its slice of the nh * D elements, S = ceil(nh * D / C).
+__host__ __device__ constexpr int exchange_floats(int nh, int D) {
+  return kMaxCluster * nh * 2 + nh * D + kMaxCluster;
+}
+
+// Joins the CTA states of a cluster.  state(g, &M, &L): the CTA's max (natural
+// log units) and sum of row g; value(i): its unnormalised element i = g * D + d.
+// Every thread of every CTA of the cluster calls it; each CTA has arrived once
+// on the cluster barrier before (its shared memory is live).
+template <typename T, typename FState, typename FValue>
+__device__ __forceinline__ void cluster_join(const DecodeParams& p, int seq, int h0, int nh, int D, int C, int rank,
+                                             float* xch, FState state, FValue value) {
+  T* out = reinterpret_cast<T*>(p.out) + (int64_t)seq * p.out_seq_stride + (int64_t)h0 * p.out_head_stride;
+  if (C == 1) {
+    for (int i = threadIdx.x; i < nh * D; i += blockDim.x) {
+      const int g = i / D, d = i - g * D;
+      float M, L;
+      state(g, &M, &L);
+      out[(int64_t)g * p.out_head_stride + d] = from_float<T>(value(i) / (L + 1e-6f));
+    }
+    return;
+  }
+  const int S = (nh * D + C - 1) / C;
+  float* ml = xch;                          // [C][nh][2]
+  float* val = xch + kMaxCluster * nh * 2;  // [C][S]
+  cluster_wait();  // every CTA of the cluster runs: its exchange area may be written
+  for (int i = threadIdx.x; i < nh * C; i += blockDim.x) {
+    const int r = i / nh, g = i - r * nh;
+    float M, L;
+    state(g, &M, &L);
+    store_remote(ml + (rank * nh + g) * 2, (uint32_t)r, M);
+    store_remote(ml + (rank * nh + g) * 2 + 1, (uint32_t)r, L);
+  }
+  for (int i = threadIdx.x; i < nh * D; i += blockDim.x) {
+    const int r = i / S;
+    store_remote(val + rank * S + (i - r * S), (uint32_t)r, value(i));
+  }
+  cluster_arrive();
+  cluster_wait();
+  for (int j = threadIdx.x; j < S && rank * S + j < nh * D; j += blockDim.x) {
+    const int i = rank * S + j, g = i / D, d = i - g * D;
+    float M = -INFINITY;
+    for (int c = 0; c < C; ++c) M = fmaxf(M, ml[(c * nh + g) * 2]);
+    float L = 0.f, A = 0.f;
+    for (int c = 0; c < C; ++c) {
+      const float m = ml[(c * nh + g) * 2];
+      const float w = m == -INFINITY ? 0.f : expf(m - M);
+      L += w * ml[(c * nh + g) * 2 + 1];
+      A += w * val[c * S + j];
+    }
+    out[(int64_t)g * p.out_head_stride + d] = from_float<T>(A / (L + 1e-6f));
+  }
+}
+
+// Tensor-core form: the G <= 16 query heads of a KV head are the rows of the
+// decode's m16n8k16 tile (mma_group, decode_mma.cuh); each warp streams every
+// NW-th group of GT tokens of the CTA's run through its own ring of STAGES
+// stages, as paged_decode_mma_kernel does.  MODE: kBulk (whole pages), kSwizzledV
+// (32-token pages), kFlashTma (token rows in blocks of 16k), kFlash (token rows).
+template <int D, int BS, int NW, int STAGES, int GT, int MODE>
+struct WindowGeom {
+  using Geo = MmaGeom<D, BS, NW, STAGES, GT, MODE>;
+  static constexpr int XCH_OFF = (Geo::SMEM + 15) / 16 * 16;
+  static constexpr int SMEM = XCH_OFF + exchange_floats(16, D) * 4;
+};
+
+template <typename T, int D, int BS, int NW, int STAGES, int GTOK, int MODE>
+__global__ void __launch_bounds__(NW * 32)
+    window_decode_kernel(const DecodeParams p, const WindowArgs wa, const __grid_constant__ TmaMaps tm) {
+  using namespace mma_detail;
+  using WG = WindowGeom<D, BS, NW, STAGES, GTOK, MODE>;
+  using Geo = typename WG::Geo;
+  constexpr int GT = Geo::GT, NBOX = Geo::NBOX, BOX = Geo::BOX, VBS = Geo::VBS;
+  constexpr int KS = D / 16, NT = D / 8;
+  extern __shared__ __align__(128) uint8_t smem[];
+
+  const int C = (int)cluster_size(), rank = (int)cluster_rank();
+  const int kvh = blockIdx.x / C, seq = blockIdx.y;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int r = lane >> 2, q4 = lane & 3;
+  const int G = p.num_heads / p.num_kv_heads, h0 = kvh * G;
+  grid_dependents_launch();
+  const uint32_t ctx = p.context_lens[seq];
+  if (ctx == 0 || ctx > (uint32_t)p.max_seq_len) {  // (the same for the whole cluster)
+    grid_dependency_wait();
+    if (rank == 0) write_zero_heads<T>(p, seq, h0, G, D);
+    return;
+  }
+  if (C > 1) cluster_arrive();
+  const int rbs = Geo::TROWS || Geo::FLASH ? p.block_size : BS;
+  const Seen seen = seen_range((int)ctx - 1, (int)ctx - 1, wa.window, wa.sinks, rbs);
+  // this CTA's run of groups
+  const int all = (seen.end + GT - 1) / GT, per = (all + C - 1) / C;
+  const int begin = rank * per * GT;
+  const int end = begin + per * GT < seen.end ? begin + per * GT : seen.end;
+  const int ngroups = end > begin ? (end - begin + GT - 1) / GT : 0;
+  const int n_mine = warp < ngroups ? (ngroups - warp + NW - 1) / NW : 0;
+
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Geo::BAR_OFF) + warp * STAGES;
+  uint32_t* masks = reinterpret_cast<uint32_t*>(smem + Geo::MASK_OFF) + warp * STAGES;
+  constexpr int IDC = Geo::IDC, IDV = IDC * GT / 32;
+  uint32_t* ids = reinterpret_cast<uint32_t*>(smem + Geo::IDS_OFF) + warp * 2 * IDC * GT;
+  uint8_t* ring_base = smem;
+  if constexpr (Geo::ALIGN > 0) {
+    constexpr uint32_t A = (uint32_t)Geo::ALIGN;
+    ring_base += (A - (smem_u32(smem) & (A - 1u))) & (A - 1u);
+  }
+  uint8_t* ring = ring_base + (size_t)warp * STAGES * Geo::STAGE;
+  if (lane == 0) {
+    for (int s = 0; s < STAGES; ++s) mbar_init(&bars[s], Geo::CP_ASYNC ? 32 : 1);
+    mbar_fence_init();
+  }
+  __syncwarp();
+
+  const T* kbase = reinterpret_cast<const T*>(p.k_cache) + (int64_t)kvh * p.k_head_stride;
+  const T* vbase = reinterpret_cast<const T*>(p.v_cache) + (int64_t)kvh * p.v_head_stride;
+  const uint32_t* table = p.block_tables + (int64_t)seq * p.table_stride;
+  const int tbs = p.block_size;
+  const bool tok_blocks = tbs == 1, group_blocks = (tbs & 15) == 0;
+
+  // block ids: lane i holds box i's of group k (paged, tensor rows); token rows
+  // keep chunks of IDC groups, an id per token, loaded a chunk ahead
+  auto load_block = [&](int k) -> uint32_t {
+    uint32_t b = 0xffffffffu;
+    if constexpr (!Geo::TOKIDS) {
+      const int tok = begin + (warp + k * NW) * GT + lane * VBS;
+      if (lane < NBOX && k < n_mine && tok < end) b = __ldg(table + seen.real_block(tok / rbs));
+    }
+    return b;
+  };
+  auto load_ids = [&](int c, uint32_t (&v)[IDV]) {
+#pragma unroll
+    for (int i = 0; i < IDV; ++i) {
+      const int j = lane + 32 * i, kg = c * IDC + j / GT;
+      const int tt = begin + (warp + kg * NW) * GT + j % GT;
+      v[i] = kg < n_mine && tt < end ? __ldg(table + seen.real_block(tok_blocks ? tt : tt / tbs)) : 0xffffffffu;
+    }
+  };
+  auto store_ids = [&](int c, const uint32_t (&v)[IDV]) {
+#pragma unroll
+    for (int i = 0; i < IDV; ++i) ids[(c & 1) * IDC * GT + lane + 32 * i] = v[i];
+    __syncwarp();
+  };
+  auto issue = [&](int k, int s, uint32_t blk) {
+    const int t0 = begin + (warp + k * NW) * GT;
+    uint8_t* st = ring + (size_t)s * Geo::STAGE;
+    if constexpr (Geo::FLASH) {
+      constexpr int CPR = Geo::ROWB / 16, RPP = 32 / CPR, RPL = GT / RPP;
+      const uint32_t* cid = ids + ((k / IDC) & 1) * IDC * GT + (k % IDC) * GT;
+      const bool in_ctx = lane < GT && t0 + lane < end;
+      const bool ok = in_ctx && (int64_t)cid[lane < GT ? lane : 0] < p.num_blocks;
+      if (in_ctx && !ok) set_status(&g_decode_status, KVC_STATUS_BLOCK_OOB);
+      const uint32_t mask = __ballot_sync(0xffffffffu, ok);
+      if (lane == 0) masks[s] = mask;
+      if (mask) {  // (a set bit means num_blocks > 0: block 0 is mapped for the masked rows)
+        const int in0 = tok_blocks ? 0 : (group_blocks ? t0 % tbs : 0);
+        const int col = lane % CPR, r0 = (lane / CPR) * RPL;
+        uint32_t rid[RPL];
+#pragma unroll
+        for (int i = 0; i < RPL; i += 4) {
+          const uint4 v4 = *reinterpret_cast<const uint4*>(cid + r0 + i);
+          rid[i] = v4.x;
+          rid[i + 1] = v4.y;
+          rid[i + 2] = v4.z;
+          rid[i + 3] = v4.w;
+        }
+#pragma unroll
+        for (int i = 0; i < RPL; ++i) {
+          const int row = r0 + i;
+          const bool on = (mask >> row) & 1u;
+          const int64_t b = on ? rid[i] : 0;
+          const int64_t in_blk = tok_blocks ? 0 : (group_blocks ? in0 + row : (t0 + row) % tbs);
+          cp_async16_zfill(st + row * BOX + col * 16, kbase + col * 8 + b * p.k_block_stride + in_blk * p.k_tok_stride,
+                           on ? 16u : 0u);
+          cp_async16_zfill(st + (NBOX + row) * BOX + col * 16,
+                           vbase + col * 8 + b * p.v_block_stride + in_blk * p.v_tok_stride, on ? 16u : 0u);
+        }
+      }
+      cp_async_arrive(&bars[s]);
+    } else {
+      uint32_t bid[NBOX];
+#pragma unroll
+      for (int i = 0; i < NBOX; ++i) bid[i] = __shfl_sync(0xffffffffu, blk, i);
+      if (lane == 0) {
+        uint32_t mask = 0, bytes = 0;
+#pragma unroll
+        for (int i = 0; i < NBOX; ++i) {
+          if (t0 + i * VBS < end) {
+            if ((int64_t)bid[i] < p.num_blocks) {
+              mask |= 1u << i;
+              bytes += 2 * BOX;
+            } else {
+              set_status(&g_decode_status, KVC_STATUS_BLOCK_OOB);
+            }
+          }
+        }
+        masks[s] = mask;
+        if (bytes) mbar_arrive_expect_tx(&bars[s], bytes);
+        else mbar_arrive(&bars[s]);
+#pragma unroll
+        for (int i = 0; i < NBOX; ++i) {
+          if (!(mask & (1u << i))) continue;
+          if constexpr (Geo::TROWS) {
+            const int row = (int)bid[i] * rbs + t0 % rbs;  // (rows are below 2^31: the host checked)
+#pragma unroll
+            for (int h = 0; h < D / 64; ++h) {
+              tma_load_3d(st + i * BOX + h * GT * 128, &tm.k, 64 * h, kvh, row, &bars[s]);
+              tma_load_3d(st + (NBOX + i) * BOX + h * GT * 128, &tm.v, 64 * h, kvh, row, &bars[s]);
+            }
+          } else {
+            bulk_g2s(st + i * BOX, kbase + (int64_t)bid[i] * p.k_block_stride, BOX, &bars[s]);
+            if constexpr (MODE == kSwizzledV)
+              tma_load_4d(st + (NBOX + i) * BOX, &tm.v, 0, 0, kvh, (int)bid[i], &bars[s]);
+            else
+              bulk_g2s(st + (NBOX + i) * BOX, vbase + (int64_t)bid[i] * p.v_block_stride, BOX, &bars[s]);
+          }
+        }
+      }
+    }
+  };
+
+  // the first groups' ids and the query rows are on their way before the wait
+  // for the kernel before this one (tables, lengths and queries are written by
+  // none of this library's kernels that let their dependents start early)
+  uint32_t first_blk[STAGES], ids_next[IDV];
+#pragma unroll
+  for (int s = 0; s < STAGES; ++s) first_blk[s] = load_block(s);
+  if constexpr (Geo::TOKIDS) {
+    uint32_t first[IDV];
+    load_ids(0, first);
+    load_ids(1, ids_next);
+    store_ids(0, first);
+  }
+  uint32_t qa[KS][4];
+  const T* qp = reinterpret_cast<const T*>(p.q) + (int64_t)seq * p.q_seq_stride;
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) {
+    const int d0 = ks * 16 + 2 * q4;
+    qa[ks][0] = qa[ks][1] = qa[ks][2] = qa[ks][3] = 0u;
+    if (r < G) {
+      const T* row = qp + (int64_t)(h0 + r) * p.q_head_stride;
+      qa[ks][0] = *reinterpret_cast<const uint32_t*>(row + d0);
+      qa[ks][2] = *reinterpret_cast<const uint32_t*>(row + d0 + 8);
+    }
+    if (r + 8 < G) {
+      const T* row = qp + (int64_t)(h0 + r + 8) * p.q_head_stride;
+      qa[ks][1] = *reinterpret_cast<const uint32_t*>(row + d0);
+      qa[ks][3] = *reinterpret_cast<const uint32_t*>(row + d0 + 8);
+    }
+  }
+  const float qk_scale = p.scale * kLog2e;
+  grid_dependency_wait();
+#pragma unroll
+  for (int s = 0; s < STAGES; ++s)
+    if (s < n_mine) issue(s, s, first_blk[s]);
+
+  GroupState<D> gs;
+  gs.reset();
+  int k_fail = -1;
+  for (int k = 0; k < n_mine; ++k) {
+    const int s = k % STAGES;
+    if constexpr (Geo::TOKIDS) {
+      if (k % IDC == 0 && k + STAGES < n_mine) {
+        store_ids(k / IDC + 1, ids_next);
+        load_ids(k / IDC + 2, ids_next);
+      }
+    }
+    const uint32_t next_blk = load_block(k + STAGES);
+    if (!mbar_wait_bounded(&bars[s], (uint32_t)((k / STAGES) & 1))) {
+      k_fail = k;
+      break;
+    }
+    const uint8_t* st = ring + (size_t)s * Geo::STAGE;
+    mma_group<T, Geo, D, true, true>(gs, qa, smem_u32(st), smem_u32(st + NBOX * BOX), begin + (warp + k * NW) * GT, end,
+                                     masks[s], 0, qk_scale, false, 0.f, 0.f, lane, 2147483647, 2147483647, seen.beg,
+                                     seen.beg, wa.sinks, seen.beg);
+    __syncwarp();
+    if (k + STAGES < n_mine) {
+      fence_proxy_async();
+      issue(k + STAGES, s, next_blk);
+    }
+  }
+  if (k_fail >= 0) {  // the copies in flight land (or time out) before the ring is reused
+    if (lane == 0) set_status(&g_decode_status, KVC_STATUS_WAIT_TIMEOUT);
+    for (int kk = k_fail; kk < n_mine && kk < k_fail + STAGES; ++kk)
+      mbar_wait_bounded(&bars[kk % STAGES], (uint32_t)((kk / STAGES) & 1));
+  }
+
+  // ---- the warps' states, then the cluster's
+  const float l_lo = gs.quad_sum_lo(), l_hi = gs.quad_sum_hi();
+  __syncthreads();  // every warp is done with its ring
+  float* red_o = reinterpret_cast<float*>(smem);  // [NW][16][D]
+  float* red_ml = red_o + NW * 16 * D;            // [NW][16][2]
+  {
+    float* ow = red_o + (size_t)warp * 16 * D;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int d = 8 * nt + 2 * q4;
+      *reinterpret_cast<float2*>(ow + r * D + d) = make_float2(gs.o[nt][0], gs.o[nt][1]);
+      *reinterpret_cast<float2*>(ow + (r + 8) * D + d) = make_float2(gs.o[nt][2], gs.o[nt][3]);
+    }
+    if (q4 == 0) {
+      red_ml[(warp * 16 + r) * 2] = gs.m_lo;
+      red_ml[(warp * 16 + r) * 2 + 1] = l_lo;
+      red_ml[(warp * 16 + r + 8) * 2] = gs.m_hi;
+      red_ml[(warp * 16 + r + 8) * 2 + 1] = l_hi;
+    }
+  }
+  __syncthreads();
+  auto top = [&](int g) -> float {  // log2 units
+    float M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) M = fmaxf(M, red_ml[(w * 16 + g) * 2]);
+    return M;
+  };
+  auto weight = [&](int w, int g, float M) -> float {
+    const float m = red_ml[(w * 16 + g) * 2];
+    return m == -INFINITY ? 0.f : fast_exp2(m - M);
+  };
+  auto state = [&](int g, float* M, float* L) {
+    const float m = top(g);
+    float l = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) l += weight(w, g, m) * red_ml[(w * 16 + g) * 2 + 1];
+    *M = m * kLn2;
+    *L = l;
+  };
+  auto value = [&](int i) -> float {
+    const int g = i / D;
+    const float m = top(g);
+    float a = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) a += weight(w, g, m) * red_o[(size_t)w * 16 * D + i];
+    return a;
+  };
+  cluster_join<T>(p, seq, h0, G, D, C, rank, reinterpret_cast<float*>(smem + WG::XCH_OFF), state, value);
+}
+
+// CUDA-core form, for every other pair of types, head size and group: the
+// generic decode's page walk (4 warps, fp32 math, up to 8 heads of a KV group to
+// a CTA) over the cluster's share of the seen blocks.
+constexpr int kWinWarps = 4, kWinGC = 8;
+
+template <typename Q_T, typename CACHE_T, int D>
+__global__ void __launch_bounds__(kWinWarps * 32) window_decode_any_kernel(const DecodeParams p, const WindowArgs wa) {
+  constexpr int X = 16 / sizeof(CACHE_T), NCHUNK = D / X, DPL = (D + 31) / 32, GC = kWinGC;
+  __shared__ float qs[GC][D];
+  __shared__ float ps[kWinWarps][GC][32];
+  __shared__ float red_ml[kWinWarps][GC][2];
+  __shared__ float red_o[kWinWarps][GC * D];
+  extern __shared__ __align__(16) float xch[];
+  const int C = (int)cluster_size(), rank = (int)cluster_rank();
+  const int G = p.num_heads / p.num_kv_heads, per_kv = (G + GC - 1) / GC;
+  const int cx = blockIdx.x / C, kvh = cx / per_kv, hc = cx - kvh * per_kv;
+  const int h0 = kvh * G + hc * GC, nh = min(GC, G - hc * GC), seq = blockIdx.y;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, bs = p.block_size;
+  grid_dependents_launch();
+  grid_dependency_wait();
+  const uint32_t ctx = p.context_lens[seq];
+  if (ctx == 0 || ctx > (uint32_t)p.max_seq_len) {
+    if (rank == 0) write_zero_heads<Q_T>(p, seq, h0, nh, D);
+    return;
+  }
+  if (C > 1) cluster_arrive();
+  const Seen seen = seen_range((int)ctx - 1, (int)ctx - 1, wa.window, wa.sinks, bs);
+  const int pages = (seen.end + bs - 1) / bs, per = (pages + C - 1) / C;
+  const int page0 = rank * per, page1 = min(pages, page0 + per);
+
+  const Q_T* q = reinterpret_cast<const Q_T*>(p.q);
+  for (int i = threadIdx.x; i < GC * D; i += blockDim.x) {
+    const int g = i / D, d = i - g * D;
+    qs[g][d] = g < nh ? to_float(q[(int64_t)seq * p.q_seq_stride + (int64_t)(h0 + g) * p.q_head_stride + d]) : 0.f;
+  }
+  __syncthreads();
+  float m[GC], l[GC], o[GC][DPL];
+#pragma unroll
+  for (int g = 0; g < GC; ++g) {
+    m[g] = -INFINITY;
+    l[g] = 0.f;
+#pragma unroll
+    for (int i = 0; i < DPL; ++i) o[g][i] = 0.f;
+  }
+  const CACHE_T* kcache = reinterpret_cast<const CACHE_T*>(p.k_cache);
+  const CACHE_T* vcache = reinterpret_cast<const CACHE_T*>(p.v_cache);
+  const uint32_t* table = p.block_tables + (int64_t)seq * p.table_stride;
+  const int tpl = 32 / bs, t = lane % bs, sub = lane / bs;
+  auto visible = [&](int v) { return v < seen.end && (v >= seen.beg || v < wa.sinks); };
+
+  for (int pg = page0 + warp; pg < page1; pg += kWinWarps) {
+    const int64_t blk = (int64_t)table[seen.real_block(pg)];
+    if (blk >= p.num_blocks) {
+      if (lane == 0) set_status(&g_decode_status, KVC_STATUS_BLOCK_OOB);
+      continue;
+    }
+    const CACHE_T* kp = kcache + blk * p.k_block_stride + (int64_t)kvh * p.k_head_stride;
+    float acc[GC];
+#pragma unroll
+    for (int g = 0; g < GC; ++g) acc[g] = 0.f;
+    for (int c = sub; c < NCHUNK; c += tpl) {
+      const uint4 raw = *reinterpret_cast<const uint4*>(kp + ((int64_t)c * bs + t) * X);
+      const CACHE_T* kv = reinterpret_cast<const CACHE_T*>(&raw);
+#pragma unroll
+      for (int e = 0; e < X; ++e) {
+        const float kf = to_float(kv[e]);
+#pragma unroll
+        for (int g = 0; g < GC; ++g) acc[g] += qs[g][c * X + e] * kf;
+      }
+    }
+    for (int off = bs; off < 32; off <<= 1) {
+#pragma unroll
+      for (int g = 0; g < GC; ++g) acc[g] += __shfl_xor_sync(0xffffffffu, acc[g], off);
+    }
+    const bool on = visible(pg * bs + t);
+#pragma unroll
+    for (int g = 0; g < GC; ++g) {
+      const float s = on ? acc[g] * p.scale : -INFINITY;
+      float pm = s;
+      for (int off = 1; off < bs; off <<= 1) pm = fmaxf(pm, __shfl_xor_sync(0xffffffffu, pm, off));
+      const float mn = fmaxf(m[g], pm);
+      const float ref = mn == -INFINITY ? 0.f : mn;  // (a page none of whose tokens is seen)
+      const float alpha = m[g] == -INFINITY ? 0.f : expf(m[g] - ref);
+      const float e = on ? expf(s - ref) : 0.f;
+      float es = e;
+      for (int off = 1; off < bs; off <<= 1) es += __shfl_xor_sync(0xffffffffu, es, off);
+      l[g] = l[g] * alpha + es;
+      m[g] = mn;
+#pragma unroll
+      for (int i = 0; i < DPL; ++i) o[g][i] *= alpha;
+      if (sub == 0) ps[warp][g][t] = e;
+    }
+    __syncwarp();
+    // tokens nobody sees are skipped: their slots may hold anything, and 0 * NaN would poison the sum
+    const CACHE_T* vp = vcache + blk * p.v_block_stride + (int64_t)kvh * p.v_head_stride;
+#pragma unroll
+    for (int i = 0; i < DPL; ++i) {
+      const int d = lane + 32 * i;
+      if (d < D) {
+        const CACHE_T* row = vp + (int64_t)d * bs;
+        for (int t0 = 0; t0 < bs; t0 += X) {
+          const uint4 raw = *reinterpret_cast<const uint4*>(row + t0);
+          const CACHE_T* vv = reinterpret_cast<const CACHE_T*>(&raw);
+#pragma unroll
+          for (int e = 0; e < X; ++e) {
+            const float vf = visible(pg * bs + t0 + e) ? to_float(vv[e]) : 0.f;
+#pragma unroll
+            for (int g = 0; g < GC; ++g) o[g][i] += ps[warp][g][t0 + e] * vf;
+          }
+        }
+      }
+    }
+    __syncwarp();
+  }
+
+  if (lane == 0) {
+#pragma unroll
+    for (int g = 0; g < GC; ++g) {
+      red_ml[warp][g][0] = m[g];
+      red_ml[warp][g][1] = l[g];
+    }
+  }
+#pragma unroll
+  for (int g = 0; g < GC; ++g)
+#pragma unroll
+    for (int i = 0; i < DPL; ++i)
+      if (lane + 32 * i < D) red_o[warp][g * D + lane + 32 * i] = o[g][i];
+  __syncthreads();
+  auto top = [&](int g) -> float {
+    float M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWinWarps; ++w) M = fmaxf(M, red_ml[w][g][0]);
+    return M;
+  };
+  auto weight = [&](int w, int g, float M) -> float {
+    return red_ml[w][g][0] == -INFINITY ? 0.f : expf(red_ml[w][g][0] - M);
+  };
+  auto state = [&](int g, float* M, float* L) {
+    *M = top(g);
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWinWarps; ++w) s += weight(w, g, *M) * red_ml[w][g][1];
+    *L = s;
+  };
+  auto value = [&](int i) -> float {
+    const int g = i / D;
+    const float M = top(g);
+    float a = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWinWarps; ++w) a += weight(w, g, M) * red_o[w][i];
+    return a;
+  };
+  cluster_join<Q_T>(p, seq, h0, nh, D, C, rank, xch, state, value);
+}
+
+// ---- launches -------------------------------------------------------------------
+// CTAs to a cluster: the smallest power of two (at most 16) that brings the
+// launch to one CTA per SM, while a CTA keeps at least `least` tokens of the
+// longest run a sequence can see.
+static int window_cluster(const DecodeParams& p, const WindowArgs& w, int units, int least) {
+  const int64_t sinks = (w.sinks + (int64_t)p.block_size - 1) / p.block_size * p.block_size;
+  int64_t seen = sinks + w.window + p.block_size;
+  if (seen > p.max_seq_len) seen = p.max_seq_len;
+  int c = 1;
+  while (c < kMaxCluster && (int64_t)units * p.num_seqs * c < decode_sm_count() && seen >= (int64_t)least * 2 * c) c *= 2;
+  return c;
+}
+
+template <typename K, typename... Args>
+static cudaError_t launch_clustered(K kern, int smem, int cluster, unsigned units, unsigned seqs, int threads,
+                                    std::atomic<bool>* configured, cudaStream_t stream, Args... args) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !configured[dev]) {  // setting the attributes twice is harmless
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return e;
+    if (dev >= 0 && dev < 64) configured[dev] = true;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(units * (unsigned)cluster, seqs);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
+  count_launch();
+  return e != cudaSuccess ? e : cudaGetLastError();
+}
+
+template <typename T, int D, int BS, int NW, int STAGES, int GT, int MODE>
+static cudaError_t launch_window_nw(const DecodeParams& p, const WindowArgs& w, cudaStream_t stream) {
+  using WG = WindowGeom<D, BS, NW, STAGES, GT, MODE>;
+  TmaMaps maps;
+  memset(&maps, 0, sizeof(maps));
+  if (MODE == kSwizzledV || MODE == kFlashTma) {
+    const ElemType et = std::is_same<T, __nv_bfloat16>::value ? ElemType::BF16 : ElemType::F16;
+    if (!make_tensor_maps(p, et, D, BS, WG::Geo::VBS, WG::Geo::VSWZ, MODE, &maps)) return cudaErrorNotSupported;
+  }
+  static std::atomic<bool> configured[64];
+  return launch_clustered(window_decode_kernel<T, D, BS, NW, STAGES, GT, MODE>, WG::SMEM,
+                          window_cluster(p, w, p.num_kv_heads, NW * GT), (unsigned)p.num_kv_heads,
+                          (unsigned)p.num_seqs, NW * 32, configured, stream, p, w, maps);
+}
+
+template <typename T, int D>
+static cudaError_t launch_window_mma(const DecodeParams& p, const DecodeArgs& a, const WindowArgs& w,
+                                     cudaStream_t stream) {
+  constexpr int NW = D == 128 ? 6 : 4, ST = D == 128 ? 2 : 3;  // as the decode (decode_mma.cuh)
+  if (a.flash) {
+    const bool rows_ok = a.block_size % 16 == 0 && a.k_block_stride == (int64_t)a.block_size * a.k_tok_stride &&
+                         a.v_block_stride == (int64_t)a.block_size * a.v_tok_stride &&
+                         a.num_blocks * (int64_t)a.block_size < (int64_t)1 << 31;
+    if (rows_ok) {
+      const cudaError_t e = launch_window_nw<T, D, 16, NW, ST, 16, kFlashTma>(p, w, stream);
+      if (e != cudaErrorNotSupported) return e;
+    }
+    return launch_window_nw<T, D, 16, NW, ST, 16, kFlash>(p, w, stream);
+  }
+  if (a.block_size == 8) return launch_window_nw<T, D, 8, NW, ST, 16, kBulk>(p, w, stream);
+  if (a.block_size == 16) return launch_window_nw<T, D, 16, NW, ST, 16, kBulk>(p, w, stream);
+  const cudaError_t e = launch_window_nw<T, D, 32, 2, 2, 32, kSwizzledV>(p, w, stream);
+  if (e != cudaErrorNotSupported) return e;
+  return launch_window_nw<T, D, 32, 2, 2, 32, kBulk>(p, w, stream);
+}
+
+template <typename Q_T, typename CACHE_T, int D>
+static cudaError_t launch_window_any(const DecodeParams& p, const WindowArgs& w, cudaStream_t stream) {
+  const int G = p.num_heads / p.num_kv_heads;
+  const int units = p.num_kv_heads * ((G + kWinGC - 1) / kWinGC);
+  static std::atomic<bool> configured[64];
+  return launch_clustered(window_decode_any_kernel<Q_T, CACHE_T, D>, exchange_floats(kWinGC, D) * 4,
+                          window_cluster(p, w, units, kWinWarps * p.block_size), (unsigned)units, (unsigned)p.num_seqs,
+                          kWinWarps * 32, configured, stream, p, w);
+}
+
+template <typename Q_T, typename CACHE_T>
+static cudaError_t launch_window_any_d(const DecodeParams& p, const WindowArgs& w, int D, cudaStream_t stream) {
+  switch (D) {
+    case 32: return launch_window_any<Q_T, CACHE_T, 32>(p, w, stream);
+    case 64: return launch_window_any<Q_T, CACHE_T, 64>(p, w, stream);
+    case 80: return launch_window_any<Q_T, CACHE_T, 80>(p, w, stream);
+    case 96: return launch_window_any<Q_T, CACHE_T, 96>(p, w, stream);
+    case 112: return launch_window_any<Q_T, CACHE_T, 112>(p, w, stream);
+    case 120: return launch_window_any<Q_T, CACHE_T, 120>(p, w, stream);
+    case 128: return launch_window_any<Q_T, CACHE_T, 128>(p, w, stream);
+    case 192: return launch_window_any<Q_T, CACHE_T, 192>(p, w, stream);
+    case 256: return launch_window_any<Q_T, CACHE_T, 256>(p, w, stream);
+    default: return cudaErrorInvalidValue;
+  }
+}
+
+cudaError_t launch_window_decode(const DecodeArgs& a, const WindowArgs& w, cudaStream_t stream) {
+  if (a.num_seqs > 65535) return cudaErrorInvalidValue;
+  const int cs = elem_size(a.cache_type);
+  auto al = [](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15u) == 0; };
+  if (!al(a.k_cache) || !al(a.v_cache) || (a.k_block_stride * cs) % 16 || (a.k_head_stride * cs) % 16 ||
+      (a.v_block_stride * cs) % 16 || (a.v_head_stride * cs) % 16 || (a.k_tok_stride * cs) % 16 ||
+      (a.v_tok_stride * cs) % 16)
+    return cudaErrorMisalignedAddress;
+  DecodeParams p;
+  memset(&p, 0, sizeof(p));
+  p.out = a.out;
+  p.q = a.q;
+  p.k_cache = a.k_cache;
+  p.v_cache = a.v_cache;
+  p.block_tables = a.block_tables;
+  p.context_lens = a.context_lens;
+  p.num_seqs = a.num_seqs;
+  p.num_heads = a.num_heads;
+  p.num_kv_heads = a.num_kv_heads;
+  p.block_size = a.block_size;
+  p.max_seq_len = a.max_seq_len;
+  p.num_partitions = 1;
+  p.num_blocks = a.num_blocks;
+  p.q_seq_stride = a.q_seq_stride;
+  p.q_head_stride = a.q_head_stride;
+  p.out_seq_stride = a.out_seq_stride;
+  p.out_head_stride = a.out_head_stride;
+  p.k_block_stride = a.k_block_stride;
+  p.k_head_stride = a.k_head_stride;
+  p.v_block_stride = a.v_block_stride;
+  p.v_head_stride = a.v_head_stride;
+  p.k_tok_stride = a.k_tok_stride;
+  p.v_tok_stride = a.v_tok_stride;
+  p.table_stride = a.table_stride;
+  p.scale = a.scale;
+  // tensor cores: 16-bit query and cache of one type, head size 64 / 128, up to
+  // 16 query heads to a KV head, query rows read as pairs of elements
+  const bool mma = a.q_type == a.cache_type && a.q_type != ElemType::F32 && (a.head_size == 64 || a.head_size == 128) &&
+                   a.num_heads / a.num_kv_heads <= 16 && (reinterpret_cast<uintptr_t>(a.q) & 3u) == 0 &&
+                   ((a.q_seq_stride | a.q_head_stride) & 1) == 0;
+  if (mma) {
+    if (a.q_type == ElemType::BF16)
+      return a.head_size == 128 ? launch_window_mma<__nv_bfloat16, 128>(p, a, w, stream)
+                                : launch_window_mma<__nv_bfloat16, 64>(p, a, w, stream);
+    return a.head_size == 128 ? launch_window_mma<__half, 128>(p, a, w, stream)
+                              : launch_window_mma<__half, 64>(p, a, w, stream);
+  }
+  if (a.flash) return cudaErrorNotSupported;  // no CUDA-core kernel for token-major caches
+  const int D = a.head_size;
+  if (a.q_type == ElemType::F32) {
+    if (a.cache_type == ElemType::F32) return launch_window_any_d<float, float>(p, w, D, stream);
+    if (a.cache_type == ElemType::F16) return launch_window_any_d<float, __half>(p, w, D, stream);
+    return launch_window_any_d<float, __nv_bfloat16>(p, w, D, stream);
+  }
+  if (a.q_type == ElemType::F16) return launch_window_any_d<__half, __half>(p, w, D, stream);
+  return launch_window_any_d<__nv_bfloat16, __nv_bfloat16>(p, w, D, stream);
+}
+
+// ---------------------------------------------------------------------------
+// Extend: the prefill kernels in their WINDOW form; which one serves a call goes
+// by the same rule as the causal prefill (attention_dispatch.cuh).
+// ---------------------------------------------------------------------------
+template <typename T, int D, int BS, bool GK>
+static cudaError_t launch_window_umma(const PrefillArgs& a, cudaStream_t stream) {
+  using UG = UmmaGeom<D, BS>;
+  DecodeParams dp;
+  memset(&dp, 0, sizeof(dp));
+  dp.k_cache = a.k_cache;
+  dp.v_cache = a.v_cache;
+  dp.num_blocks = a.num_blocks;
+  dp.num_kv_heads = a.num_kv_heads;
+  dp.k_head_stride = a.k_head_stride;
+  dp.k_block_stride = a.k_block_stride;
+  dp.v_head_stride = a.v_head_stride;
+  dp.v_block_stride = a.v_block_stride;
+  TmaMaps maps;
+  memset(&maps, 0, sizeof(maps));
+  if (!make_tensor_maps(dp, std::is_same<T, __nv_bfloat16>::value ? ElemType::BF16 : ElemType::F16, D, BS, BS, BS * 2,
+                        kTiles, &maps))
+    return cudaErrorNotSupported;
+  if (GK && !make_k_gather_map(a, D, BS, &maps.k)) return cudaErrorNotSupported;
+  auto kern = prefill_umma_kernel<T, D, BS, GK, false, true>;
+  static std::atomic<bool> configured[64];  // per device; setting the attribute twice is harmless
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 0 && dev < 64 && !configured[dev]) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, UG::SMEM);
+    if (e != cudaSuccess) return e;
+    configured[dev] = true;
+  }
+  const int G = a.num_heads / a.num_kv_heads;
+  const int64_t tiles = ((int64_t)a.max_q_len * G + kUmmaRows - 1) / kUmmaRows;
+  const int64_t items = tiles * a.num_seqs * a.num_kv_heads;
+  if (items > 0x7fffffffll - 1024) return cudaErrorInvalidValue;
+  const int ctas = umma_persistent_ctas(dev, items);
+  const int slot = umma_sched_slot(stream);
+  PrefillArgs aa = a;
+  aa.single_issue = umma_single_issue();
+  kern<<<ctas, kUmmaThreads, UG::SMEM, stream>>>(aa, maps, (int)tiles, (int)a.num_seqs, slot);
+  count_launch();
+  return cudaGetLastError();
+}
+
+template <typename T, int D>
+static cudaError_t launch_window_prefill_t(const PrefillArgs& a, cudaStream_t stream) {
+  const bool rows16 = (reinterpret_cast<uintptr_t>(a.out) & 15u) == 0 && ((a.out_tok_stride | a.out_head_stride) & 7) == 0;
+  if (!a.token_major && (a.block_size == 16 || a.block_size == 32) && rows16) {
+    const int64_t BS = a.block_size;
+    const bool dense = a.k_head_stride == D * BS && a.k_block_stride == (int64_t)a.num_kv_heads * D * BS &&
+                       a.num_blocks * a.num_kv_heads * (D / 8) < 0x7fffffffll;  // (row indices are 32-bit)
+    cudaError_t e;
+    if (BS == 32) e = dense ? launch_window_umma<T, D, 32, true>(a, stream) : launch_window_umma<T, D, 32, false>(a, stream);
+    else e = dense ? launch_window_umma<T, D, 16, true>(a, stream) : launch_window_umma<T, D, 16, false>(a, stream);
+    if (e != cudaErrorNotSupported) return e;
+  }
+  return launch_prefill_layout<T, D, true>(a, a.token_major, stream);
+}
+
+cudaError_t launch_window_prefill(const PrefillArgs& a, cudaStream_t stream) {
+  if (a.num_seqs <= 0 || a.max_q_len <= 0) return cudaSuccess;
+  if (a.num_seqs > 65535 || a.num_kv_heads > 65535) return cudaErrorInvalidValue;
+  if (a.q_type == ElemType::BF16)
+    return a.head_size == 128 ? launch_window_prefill_t<__nv_bfloat16, 128>(a, stream)
+                              : launch_window_prefill_t<__nv_bfloat16, 64>(a, stream);
+  return a.head_size == 128 ? launch_window_prefill_t<__half, 128>(a, stream)
+                            : launch_window_prefill_t<__half, 64>(a, stream);
+}
+
+}  // namespace kvc
+
+unsigned int kvc_window_status(int clear, cudaError_t* err) {
+  unsigned int v = 0;
+  *err = cudaMemcpyFromSymbol(&v, kvc::g_decode_status, sizeof(v));
+  if (*err == cudaSuccess && clear) {
+    const unsigned int zero = 0;
+    *err = cudaMemcpyToSymbol(kvc::g_decode_status, &zero, sizeof(zero));
+  }
+  return v;
+}

@@ -84,6 +84,12 @@ SIGNATURES: dict[str, tuple] = {
     ),
     "kvc_convert_fp8": (_i, [_p, _p, _f, _i, _p]),
     "kvc_swap_blocks": (_i, [_p, _p, _p, _p]),
+    "kvc_paged_attention_window": (_i, [_p, _p, _p, _p, _p, _p, _i, _f, _i, _i, _i, _i, _p]),
+    "kvc_paged_prefill_window": (_i, [_p, _p, _p, _p, _p, _p, _p, _i, _f, _i, _i, _i, _i, _p]),
+    "kvc_step_tables": (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _p]),
+    "kvc_rotary_table": (_i, [_p, ctypes.POINTER(ctypes.c_double), ctypes.c_double, _p]),
+    "kvc_qk_norm_rope": (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _f, _i, _p]),
+    "kvc_qk_norm_rope_append": (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _f, _i, _p, _p]),
     "kvc_get_max_shared_memory_per_block_device_attribute": (
         _i,
         [_i, ctypes.POINTER(ctypes.c_int64)],

@@ -100,6 +100,76 @@ class _ForeignView:
         return self.managed.dl_tensor
 
 
+# DLPack's C exchange API (the public struct `DLPackExchangeAPI` of DLPack 1.x,
+# a capsule on the producer's type): its dltensor_from_py_object_no_sync fills a
+# DLTensor in one C call, without a capsule, where __dlpack__ takes microseconds.
+class _ExchangeAPI(ctypes.Structure):
+    _fields_ = [
+        ("major", ctypes.c_uint32),
+        ("minor", ctypes.c_uint32),
+        ("prev_api", ctypes.c_void_p),
+        ("managed_tensor_allocator", ctypes.c_void_p),
+        ("managed_tensor_from_py_object_no_sync", ctypes.c_void_p),
+        ("managed_tensor_to_py_object_no_sync", ctypes.c_void_p),
+        ("dltensor_from_py_object_no_sync", ctypes.c_void_p),
+        ("current_work_stream", ctypes.c_void_p),
+    ]
+
+
+_FROM_OBJECT = ctypes.PYFUNCTYPE(ctypes.c_int, ctypes.py_object, ctypes.c_void_p)
+_WORK_STREAM = ctypes.PYFUNCTYPE(ctypes.c_int, ctypes.c_int, ctypes.c_int32, ctypes.POINTER(ctypes.c_void_p))
+_exchange: dict = {}  # producer type -> (from_py_object, current_work_stream) or None
+
+
+def _exchange_api(cls):
+    """The exchange functions of a producer type, or None (looked up once per type)."""
+    if cls in _exchange:
+        return _exchange[cls]
+    found = None
+    cap = getattr(cls, "__dlpack_c_exchange_api__", None)
+    if cap is not None and _pyapi.PyCapsule_IsValid(cap, b"dlpack_exchange_api"):
+        api = _ExchangeAPI.from_address(_pyapi.PyCapsule_GetPointer(cap, b"dlpack_exchange_api"))
+        if api.major == 1 and api.dltensor_from_py_object_no_sync and api.current_work_stream:
+            found = (_FROM_OBJECT(api.dltensor_from_py_object_no_sync), _WORK_STREAM(api.current_work_stream))
+    _exchange[cls] = found
+    return found
+
+
+def call_tensors(objs, names, stream):
+    """DLTensor pointers for one call: a list of ctypes references (None for
+    None) and what to keep alive until the call returns.
+
+    Producers with the C exchange API are read through it.  That API does no
+    stream synchronisation, so without an explicit `stream` (the call then runs
+    on the legacy default stream) it is used only while the producer's current
+    stream is that one; otherwise `__dlpack__` makes the default stream wait for
+    the producer's, as it does for every other call here.
+    """
+    refs, keep = [], []
+    checked = stream is not None
+    for obj, name in zip(objs, names):
+        if obj is None:
+            refs.append(None)
+            continue
+        api = _exchange_api(type(obj))
+        if api is not None:
+            t = DLTensor()
+            ref = ctypes.byref(t)
+            if api[0](obj, ctypes.addressof(t)) == 0:
+                if not checked:
+                    cur = ctypes.c_void_p()
+                    checked = (t.device.device_type == KDL_CUDA
+                               and api[1](KDL_CUDA, t.device.device_id, ctypes.byref(cur)) == 0 and not cur.value)
+                if checked:
+                    refs.append(ref)
+                    keep.append(t)
+                    continue
+        ptr, k = as_dltensor(obj, name)
+        refs.append(ptr)
+        keep.append(k)
+    return refs, keep
+
+
 def as_dltensor(obj, name: str = "tensor"):
     """Returns (ctypes pointer to a DLTensor, keepalive) for `obj`."""
     from .device_array import DeviceArray, HostBuffer

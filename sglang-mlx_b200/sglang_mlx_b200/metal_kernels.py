@@ -16,12 +16,13 @@ from __future__ import annotations
 
 import ctypes
 import math
+from typing import NamedTuple
 
 import numpy as np
 
 from . import _lib, dtypes
 from .device_array import DeviceArray, HostBuffer, _stream, asarray
-from .dlpack import DLTensor, as_dltensor, describe
+from .dlpack import DLTensor, as_dltensor, call_tensors, describe
 
 _L = _lib.lib
 
@@ -502,6 +503,228 @@ def paged_attention_append(query, key, value, key_cache, value_cache, slot_mappi
     return out
 
 
+def paged_attention_window(query, key_cache, value_cache, block_tables, context_lens, num_kv_heads: int, scale: float,
+                           block_size: int, max_seq_len: int, window_size: int, sink_size: int = 0, *, out=None,
+                           stream=None):
+    """Decode over a sliding window: the new token of each sequence (position
+    context_len - 1) sees the last `window_size` tokens, itself included, and the
+    first `sink_size` tokens of its sequence, which stay visible.
+
+    Arguments and result of paged_attention_v1 (every dtype pair, head size and
+    block size of that call), or, with token-major caches ([num_blocks,
+    block_size, kv_heads, D], or a token pool [slots, kv_heads, D] with block_size
+    1), of paged_attention_flash.  Table entries of blocks that no token sees are
+    not read, so their blocks may have been freed.  One launch, no workspace."""
+    query, key_cache, value_cache = _dev(query), _dev(key_cache), _dev(value_cache)
+    block_tables, context_lens = _dev(block_tables), _dev(context_lens)
+    if out is None:
+        out = _out_like_query(query)
+    t, keep = call_tensors((out, query, key_cache, value_cache, block_tables, context_lens),
+                           ("out", "query", "key_cache", "value_cache", "block_tables", "context_lens"), stream)
+    rc = _L.kvc_paged_attention_window(t[0], t[1], t[2], t[3], t[4], t[5], int(num_kv_heads), float(scale),
+                                       int(block_size), int(max_seq_len), int(window_size), int(sink_size),
+                                       _stream(stream))
+    _lib.check(rc)
+    return out
+
+
+def paged_prefill_window(query, key_cache, value_cache, block_tables, qo_indptr, kv_lens, num_kv_heads: int,
+                         scale: float, block_size: int, window_size: int, sink_size: int = 0, *,
+                         max_q_len: int | None = None, out=None, stream=None):
+    """Prefill / extend attention over a sliding window with sinks: as
+    paged_prefill_attention, where the new token at position i sees position j <= i
+    when j < sink_size or j > i - window_size.  Table entries of blocks that no
+    new token of their sequence sees are not read."""
+    if max_q_len is None:
+        if isinstance(qo_indptr, (np.ndarray, list, tuple)):
+            ind = np.asarray(qo_indptr, dtype=np.int64)
+            max_q_len = int(np.max(np.diff(ind))) if ind.size > 1 else 0
+        else:
+            max_q_len = describe(query)[0][0]
+    query, key_cache, value_cache = _dev(query), _dev(key_cache), _dev(value_cache)
+    block_tables, qo_indptr, kv_lens = _dev(block_tables), _dev(qo_indptr), _dev(kv_lens)
+    if out is None:
+        out = _out_like_query(query)
+    t, keep = call_tensors((out, query, key_cache, value_cache, block_tables, qo_indptr, kv_lens),
+                           ("out", "query", "key_cache", "value_cache", "block_tables", "qo_indptr", "kv_lens"), stream)
+    rc = _L.kvc_paged_prefill_window(t[0], t[1], t[2], t[3], t[4], t[5], t[6], int(num_kv_heads), float(scale),
+                                     int(block_size), int(max(0, max_q_len)), int(window_size), int(sink_size),
+                                     _stream(stream))
+    _lib.check(rc)
+    return out
+
+
+class StepTables(NamedTuple):
+    """What build_step_tables writes (the block tables are updated in place)."""
+
+    block_tables: object
+    kv_lens: object
+    qo_indptr: object
+    positions: object
+    slot_mapping: object
+    blocks_used: object
+
+
+def build_step_tables(block_tables, prefix_lens, new_lens, free_blocks, block_size: int, num_tokens: int | None = None,
+                      *, kv_lens=None, qo_indptr=None, positions=None, slot_mapping=None, blocks_used=None,
+                      stream=None) -> StepTables:
+    """The index arrays of a step, built on the GPU from the requests' lengths.
+
+    Request b has prefix_lens[b] cached tokens and brings new_lens[b] new ones;
+    the blocks these need come off free_blocks in request order and are written to
+    block_tables[b] in place.  Returns the tables, kv_lens [B], qo_indptr [B + 1],
+    positions [N] and slot_mapping [N] of the new tokens, and the number of free
+    blocks taken [1] (int32; slots int64).  N = num_tokens, which may exceed the
+    step's tokens: the rows past them get -1.  Host lengths (a list or NumPy
+    array) give N themselves.  Preallocated outputs may be passed instead.
+
+    Args:
+        block_tables: [B, max_blocks] int32 device array
+        prefix_lens, new_lens: [B] int32
+        free_blocks: [any] int32 block ids
+    """
+    if num_tokens is None and positions is None:
+        if not isinstance(new_lens, (np.ndarray, list, tuple)):
+            raise ValueError("num_tokens is needed when new_lens is a device array")
+        num_tokens = int(np.sum(np.asarray(new_lens, dtype=np.int64)))
+    prefix_lens, new_lens, free_blocks = (
+        _dev(np.asarray(a, dtype=np.int32) if isinstance(a, (list, tuple)) else a)
+        for a in (prefix_lens, new_lens, free_blocks))
+    if kv_lens is None or qo_indptr is None or positions is None or slot_mapping is None or blocks_used is None:
+        shape, _, _, _, dev = describe(block_tables)
+        n = num_tokens if num_tokens is not None else describe(positions)[0][0]
+        kv_lens = DeviceArray.empty((shape[0],), dtypes.int32, dev) if kv_lens is None else kv_lens
+        qo_indptr = DeviceArray.empty((shape[0] + 1,), dtypes.int32, dev) if qo_indptr is None else qo_indptr
+        positions = DeviceArray.empty((n,), dtypes.int32, dev) if positions is None else positions
+        slot_mapping = DeviceArray.empty((n,), dtypes.int64, dev) if slot_mapping is None else slot_mapping
+        blocks_used = DeviceArray.empty((1,), dtypes.int32, dev) if blocks_used is None else blocks_used
+    t, keep = call_tensors((block_tables, kv_lens, qo_indptr, positions, slot_mapping, blocks_used, prefix_lens,
+                            new_lens, free_blocks),
+                           ("block_tables", "kv_lens", "qo_indptr", "positions", "slot_mapping", "blocks_used",
+                            "prefix_lens", "new_lens", "free_blocks"), stream)
+    _lib.check(_L.kvc_step_tables(*t, int(block_size), _stream(stream)))
+    return StepTables(block_tables, kv_lens, qo_indptr, positions, slot_mapping, blocks_used)
+
+
+def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: dict | None = None):
+    """(inverse frequencies [rotary_dim / 2] float64, factor of the rotated part).
+
+    scaling: None, or a dict with "type" and its parameters:
+      "linear"  every frequency divided by `factor` (position interpolation)
+      "ntk"     the base raised so that the lowest frequency is divided by `factor`:
+                base * factor^(d / (d - 2)), d = rotary_dim
+      "bands"   frequencies by wavelength: as they are below
+                original_max_position / high_freq_factor, divided by `factor` above
+                original_max_position / low_freq_factor, blended between
+      "yarn"    dims that turn more than beta_fast times over
+                original_max_position keep their frequency, those that turn less
+                than beta_slow times are divided by `factor`, a linear ramp over the
+                dim index between; the rotated part is scaled by attention_factor
+                (default 0.1 ln(factor) + 1)
+    """
+    if rotary_dim <= 0 or rotary_dim % 2:
+        raise ValueError("rotary_dim must be positive and even")
+    if not base > 0:
+        raise ValueError("base must be positive")
+    d = float(rotary_dim)
+    i = np.arange(0, rotary_dim, 2, dtype=np.float64)
+    freq = float(base) ** (-i / d)
+    if scaling is None:
+        return freq, 1.0
+    kind, f = scaling.get("type"), float(scaling.get("factor", 1.0))
+    if not f > 0:
+        raise ValueError("scaling factor must be positive")
+    if kind == "linear":
+        return freq / f, 1.0
+    if kind == "ntk":
+        if rotary_dim == 2:
+            return freq, 1.0
+        return (float(base) * f ** (d / (d - 2.0))) ** (-i / d), 1.0
+    if kind == "bands":
+        orig = float(scaling["original_max_position"])
+        low, high = float(scaling.get("low_freq_factor", 1.0)), float(scaling.get("high_freq_factor", 4.0))
+        if not high > low > 0:
+            raise ValueError("high_freq_factor must exceed low_freq_factor, both positive")
+        turns = orig * freq / (2.0 * math.pi)  # over the original context
+        keep = np.clip((turns - low) / (high - low), 0.0, 1.0)
+        return freq * (keep + (1.0 - keep) / f), 1.0
+    if kind == "yarn":
+        orig = float(scaling["original_max_position"])
+        fast, slow = float(scaling.get("beta_fast", 32.0)), float(scaling.get("beta_slow", 1.0))
+
+        def dim_of(turns):  # the (real) pair index whose frequency turns that often over the original context
+            return d * math.log(orig / (turns * 2.0 * math.pi)) / (2.0 * math.log(float(base)))
+
+        lo, hi = max(math.floor(dim_of(fast)), 0), min(math.ceil(dim_of(slow)), rotary_dim - 1)
+        ramp = np.clip((i / 2.0 - lo) / max(hi - lo, 1e-3), 0.0, 1.0)
+        att = scaling.get("attention_factor")
+        return freq * (1.0 - ramp) + freq / f * ramp, float(att) if att is not None else (
+            0.1 * math.log(f) + 1.0 if f > 1.0 else 1.0)
+    raise ValueError("scaling type must be 'linear', 'ntk', 'bands' or 'yarn'")
+
+
+def rotary_table(max_position: int, rotary_dim: int, base: float = 10000.0, *, scaling: dict | None = None, out=None,
+                 device: int | None = None, stream=None):
+    """The cosines and sines of every position, [max_position, rotary_dim] float32
+    (row p: cos of p * f_i, then sin), written on the GPU with the angles in 64
+    bits.  `scaling`: see rotary_frequencies.  Made once per model."""
+    if max_position <= 0:
+        raise ValueError("max_position must be positive")
+    freq, factor = rotary_frequencies(rotary_dim, base, scaling)
+    if out is None:
+        out = DeviceArray.empty((int(max_position), int(rotary_dim)), dtypes.float32, device)
+    freq = np.ascontiguousarray(freq, dtype=np.float64)
+    t, keep = call_tensors((out,), ("out",), stream)
+    _lib.check(_L.kvc_rotary_table(t[0], freq.ctypes.data_as(ctypes.POINTER(ctypes.c_double)), float(factor),
+                                   _stream(stream)))
+    return out
+
+
+def qk_norm_rope(q, k, positions, cos_sin, *, q_weight=None, k_weight=None, eps: float = 1e-6,
+                 interleaved: bool = False, q_out=None, k_out=None, stream=None):
+    """Per-head RMS norm of queries and keys (where a weight [D] is given) and the
+    rotary position, in one pass; returns (q_out, k_out).
+
+    Args:
+        q: [T, num_heads, D], k: [T, num_kv_heads, D]; any token and head strides
+            (slices of a fused projection), float32 / float16 / bfloat16
+        positions: [T] int32/int64; a negative one skips the token
+        cos_sin: [positions, rotary_dim] float32 (rotary_table); the first
+            rotary_dim elements of a head are rotated, the rest pass
+        interleaved: pairs (2i, 2i + 1) instead of (i, i + rotary_dim / 2)
+        q_out, k_out: outputs; q and k themselves rotate in place
+    """
+    q, k, positions, cos_sin = _dev(q), _dev(k), _dev(positions), _dev(cos_sin)
+    q_weight, k_weight = _dev(q_weight), _dev(k_weight)
+    if q_out is None:
+        q_out = _out_like_query(q)
+    if k_out is None:
+        k_out = _out_like_query(k)
+    t, keep = call_tensors((q_out, k_out, q, k, positions, cos_sin, q_weight, k_weight),
+                           ("q_out", "k_out", "q", "k", "positions", "cos_sin", "q_weight", "k_weight"), stream)
+    _lib.check(_L.kvc_qk_norm_rope(*t, float(eps), int(bool(interleaved)), _stream(stream)))
+    return q_out, k_out
+
+
+def qk_norm_rope_append(q, k, v, positions, cos_sin, key_cache, value_cache, slot_mapping, *, q_weight=None,
+                        k_weight=None, eps: float = 1e-6, interleaved: bool = False, q_out=None, stream=None):
+    """qk_norm_rope with the append: the rotated keys and the values go to the
+    caches at slot_mapping, as reshape_and_cache (paged caches) or
+    reshape_and_cache_flash (token-major caches) would store them, in the same
+    launch.  Returns (q_out, key_cache, value_cache); the caches are updated in
+    place.  q_out may be q."""
+    q, k, v, positions, cos_sin = _dev(q), _dev(k), _dev(v), _dev(positions), _dev(cos_sin)
+    q_weight, k_weight, slot_mapping = _dev(q_weight), _dev(k_weight), _dev(slot_mapping)
+    if q_out is None:
+        q_out = _out_like_query(q)
+    t, keep = call_tensors((q_out, key_cache, value_cache, q, k, v, positions, cos_sin, q_weight, k_weight,
+                            slot_mapping),
+                           ("q_out", "key_cache", "value_cache", "q", "k", "v", "positions", "cos_sin", "q_weight",
+                            "k_weight", "slot_mapping"), stream)
+    _lib.check(_L.kvc_qk_norm_rope_append(*t[:10], float(eps), int(bool(interleaved)), t[10], _stream(stream)))
+    return q_out, key_cache, value_cache
+
+
 def reshape_and_cache(key, value, key_cache, value_cache, slot_mapping, *, stream=None):
     """Scatter-write new KV tokens into the paged cache (metal_kernels.py:64-74).
 
@@ -695,6 +918,14 @@ __all__ = [
     "gather_kv",
     "copy_blocks",
     "swap_blocks",
+    "paged_attention_window",
+    "paged_prefill_window",
+    "StepTables",
+    "build_step_tables",
+    "rotary_frequencies",
+    "rotary_table",
+    "qk_norm_rope",
+    "qk_norm_rope_append",
     "splitk_workspace",
     "use_split_k",
     "get_max_shared_memory_per_block_device_attribute",

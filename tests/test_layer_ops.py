@@ -1,0 +1,422 @@
+"""Step tables, rotary tables, and the per-head norm with the rotary position
+(alone and with the append), against plain NumPy in float64 / integers."""
+
+import ctypes
+import math
+
+import numpy as np
+import pytest
+
+from oracle import kv_oracle
+from sglang_mlx_b200 import _lib, dlpack, dtypes
+from sglang_mlx_b200 import metal_kernels as mk
+from sglang_mlx_b200.device_array import DeviceArray, Stream
+
+# ---- step tables ----------------------------------------------------------------
+
+
+def plain_tables(tables, prefix, new, free, bs, capacity):
+    t = tables.copy()
+    at, slots, pos, indptr = 0, [], [], [0]
+    for b, (p, n) in enumerate(zip(prefix, new)):
+        first, last = -(-p // bs), -(-(p + n) // bs)
+        t[b, first:last] = free[at:at + last - first]
+        at += last - first
+        for i in range(p, p + n):
+            pos.append(i)
+            slots.append(int(t[b, i // bs]) * bs + i % bs)
+        indptr.append(indptr[-1] + n)
+    pad = capacity - len(pos)
+    return t, np.asarray(prefix) + new, indptr, pos + [-1] * pad, slots + [-1] * pad, at
+
+
+def run_tables(tables, prefix, new, free, bs, capacity, slot_dtype="int64"):
+    dev = lambda a, dt="int32": DeviceArray.from_numpy(np.asarray(a), dtype=dt)  # noqa: E731
+    bt = dev(tables)
+    out = mk.build_step_tables(bt, dev(np.asarray(prefix, np.int32)), dev(np.asarray(new, np.int32)),
+                               dev(np.asarray(free, np.int32)), bs, capacity,
+                               slot_mapping=DeviceArray.zeros((capacity,), slot_dtype))
+    return [np.asarray(x.to_numpy()) for x in out]
+
+
+def tables_case(seed, B, bs, longest, most_new):
+    rng = np.random.default_rng(seed)
+    prefix = rng.integers(0, longest + 1, B)
+    new = rng.integers(0, most_new + 1, B)
+    need, have = -(-(prefix + new) // bs), -(-prefix // bs)
+    blocks = rng.permutation(int(need.sum()) + 4)
+    tables = np.full((B, int(need.max(initial=0)) + 2), -7, np.int64)
+    at = 0
+    for b in range(B):
+        tables[b, :have[b]] = blocks[at:at + have[b]]
+        at += have[b]
+    return tables, prefix, new, blocks[at:]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,bs,longest,most_new,extra", [
+    (1, 16, 0, 1, 0), (1, 16, 100, 1, 3), (3, 8, 40, 50, 5), (64, 16, 4096, 1, 0), (65, 32, 50, 9, 1),
+    (300, 1, 20, 6, 2), (1023, 16, 100, 3, 0), (1024, 16, 100, 3, 7), (1025, 7, 100, 3, 1), (4000, 16, 60, 5, 0),
+    (5, 16, 10, 40000, 11), (2, 48, 0, 0, 4)])
+@pytest.mark.parametrize("slot_dtype", ["int32", "int64"])
+def test_step_tables(gpu, B, bs, longest, most_new, extra, slot_dtype):
+    case = tables_case(B * 31 + bs, B, bs, longest, most_new)
+    capacity = int(case[2].sum()) + extra
+    want = plain_tables(*case, bs, capacity)
+    got = run_tables(*case, bs, capacity, slot_dtype)
+    for g, w in zip(got, want):
+        np.testing.assert_array_equal(g.reshape(-1), np.asarray(w).reshape(-1))
+    assert _lib.get_status(0, clear=True) == 0
+
+
+@pytest.mark.gpu
+def test_step_tables_no_requests(gpu):
+    got = run_tables(np.zeros((0, 4), np.int32), [], [], [1, 2], 16, 3)
+    assert got[2].tolist() == [0] and got[3].tolist() == [-1] * 3 and got[4].tolist() == [-1] * 3
+    assert got[5].tolist() == [0] and _lib.get_status(0, clear=True) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("what", ["free", "table", "capacity", "negative", "hole", "slot32"])
+def test_step_tables_flags_what_does_not_fit(gpu, what):
+    tables, prefix, new, free, bs, cap, sd = np.full((2, 4), -1, np.int64), [5, 0], [20, 30], [9, 8, 7], 16, 50, "int64"
+    tables[0, 0] = 3
+    if what == "free":  # needs 1 + 2 blocks, one is free
+        free = [9]
+        want = [-1] * 50
+        want[:20] = [3 * 16 + i for i in range(5, 16)] + [9 * 16 + i for i in range(9)]
+    elif what == "table":
+        new = [20, 70]
+        cap, free = 90, [9, 8, 7, 6, 5, 4]
+        want = [3 * 16 + i for i in range(5, 16)] + [9 * 16 + i for i in range(9)]
+        want += [b * 16 + i for b in (8, 7, 6, 5) for i in range(16)] + [-1] * 6
+    elif what == "capacity":
+        cap = 45
+        want = ([3 * 16 + i for i in range(5, 16)] + [9 * 16 + i for i in range(9)] + [8 * 16 + i for i in range(16)] +
+                [7 * 16 + i for i in range(14)])[:45]
+    elif what == "negative":
+        new = [-4, 30]
+        want = [9 * 16 + i for i in range(16)] + [8 * 16 + i for i in range(14)] + [-1] * 20
+    elif what == "hole":  # the block that the cached tokens end in is not in the table
+        tables[0, 0] = -1
+        want = [-1] * 11 + [9 * 16 + i for i in range(9)] + [8 * 16 + i for i in range(16)] + [7 * 16 + i for i in range(14)]
+    else:
+        sd, free = "int32", [1 << 27, 8, 7]  # block 2^27 of 16 tokens: past int32
+        want = [3 * 16 + i for i in range(5, 16)] + [-1] * 9 + [8 * 16 + i for i in range(16)] + [7 * 16 + i for i in range(14)]
+    got = run_tables(tables, prefix, new, free, bs, cap, sd)
+    assert got[4].tolist() == want
+    assert _lib.get_status(0, clear=True) == _lib.STATUS_INDEX_OOB
+
+
+# ---- rotary frequencies and tables ------------------------------------------------
+
+
+def test_rotary_frequencies():
+    f, a = mk.rotary_frequencies(8, 10000.0)
+    np.testing.assert_allclose(f, [1.0, 0.1, 0.01, 0.001], rtol=1e-14)
+    assert a == 1.0
+    np.testing.assert_allclose(mk.rotary_frequencies(8, 10000.0, {"type": "linear", "factor": 4.0})[0],
+                               np.array([1.0, 0.1, 0.01, 0.001]) / 4, rtol=1e-14)
+    # ntk: the highest frequency keeps, the lowest is divided by the factor
+    n = mk.rotary_frequencies(128, 10000.0, {"type": "ntk", "factor": 8.0})[0]
+    g = mk.rotary_frequencies(128, 10000.0)[0]
+    assert n[0] == 1.0 and abs(n[-1] * 8.0 / g[-1] - 1) < 1e-12
+    # bands: short wavelengths keep, long ones are divided, between them monotone
+    b = mk.rotary_frequencies(128, 500000.0, {"type": "bands", "factor": 8.0, "original_max_position": 8192})[0]
+    g = mk.rotary_frequencies(128, 500000.0)[0]
+    turns = 8192 * g / (2 * math.pi)
+    np.testing.assert_allclose(b[turns >= 4], g[turns >= 4], rtol=1e-14)
+    np.testing.assert_allclose(b[turns <= 1], g[turns <= 1] / 8, rtol=1e-14)
+    assert (np.diff(b) < 0).all()
+    # yarn: as they are up to beta_fast turns, divided below beta_slow turns, the factor of the rotated part
+    y, a = mk.rotary_frequencies(128, 10000.0, {"type": "yarn", "factor": 4.0, "original_max_position": 4096})
+    g = mk.rotary_frequencies(128, 10000.0)[0]
+    turns = 4096 * g / (2 * math.pi)
+    np.testing.assert_allclose(y[turns > 33], g[turns > 33], rtol=1e-14)
+    np.testing.assert_allclose(y[turns < 0.9], g[turns < 0.9] / 4, rtol=1e-14)
+    assert abs(a - (0.1 * math.log(4.0) + 1.0)) < 1e-15
+
+
+@pytest.mark.parametrize("kw", [dict(rotary_dim=7), dict(rotary_dim=0), dict(rotary_dim=8, base=0.0),
+                                dict(rotary_dim=8, scaling={"type": "other"}),
+                                dict(rotary_dim=8, scaling={"type": "linear", "factor": 0.0}),
+                                dict(rotary_dim=8, scaling={"type": "bands", "factor": 2.0, "original_max_position": 64,
+                                                            "low_freq_factor": 4.0, "high_freq_factor": 1.0})])
+def test_rotary_frequencies_refusals(kw):
+    with pytest.raises(ValueError):
+        mk.rotary_frequencies(**kw)
+
+
+def table64(positions, rot, base=10000.0, scaling=None):
+    f, a = mk.rotary_frequencies(rot, base, scaling)
+    ang = np.asarray(positions, np.float64)[:, None] * f
+    return np.concatenate([np.cos(ang), np.sin(ang)], 1) * a
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rot,rows,scaling", [(2, 5, None), (64, 70000, None), (128, 4097, {"type": "yarn", "factor": 8.0,
+                                               "original_max_position": 4096}), (256, 33, {"type": "ntk", "factor": 2.0})])
+def test_rotary_table(gpu, rot, rows, scaling):
+    t = mk.rotary_table(rows, rot, scaling=scaling).to_numpy()
+    # one rounding to float32 of values up to 1.21: at most 2^-24 * 2 (and the 64-bit sine's own error)
+    assert np.abs(t - table64(np.arange(rows), rot, scaling=scaling)).max() <= 1.2e-7
+
+
+# ---- norm and rotation --------------------------------------------------------------
+
+
+def plain_rope(x, w, cs, rot, interleaved, eps):
+    x = x.astype(np.float64)
+    if w is not None:
+        x = x / np.sqrt((x * x).mean(-1, keepdims=True) + eps) * w.astype(np.float64)
+    half = rot // 2
+    c, s = cs[:, None, :half].astype(np.float64), cs[:, None, half:].astype(np.float64)
+    out = x.copy()
+    if interleaved:
+        a, b = x[..., 0:rot:2], x[..., 1:rot:2]
+        out[..., 0:rot:2], out[..., 1:rot:2] = a * c - b * s, b * c + a * s
+    else:
+        a, b = x[..., :half], x[..., half:rot]
+        out[..., :half], out[..., half:rot] = a * c - b * s, b * c + a * s
+    return out
+
+
+# half a step of the output's type (2^-9, 2^-12, 2^-25 of the value), doubled for a value whose 32-bit
+# error moves it across a rounding boundary, and the 32-bit arithmetic's own error on values up to about 8
+TOL = {"bfloat16": (1e-5, 2.0 ** -8), "float16": (1e-5, 2.0 ** -11), "float32": (1e-5, 2.0 ** -20)}
+
+
+def close(got, want, dtype):
+    atol, rtol = TOL[dtype]
+    bad = np.abs(got - want) - (atol + rtol * np.abs(want))
+    assert np.isfinite(got).all() and bad.max() <= 0, f"{dtype}: {np.abs(got - want).max():.3g}"
+
+
+class Rope:
+    def __init__(self, seed, dtype, T, hq, hkv, d, rot, norm, wdtype=None, fused=True, rows=5000, poison=False):
+        rng = np.random.default_rng(seed)
+        rnd = lambda *s: kv_oracle.round_to(rng.standard_normal(s).astype(np.float32), dtype)  # noqa: E731
+        self.dtype, self.d, self.rot, self.hq, self.hkv, self.T = dtype, d, rot, hq, hkv, T
+        wide = rnd(T, hq + 2 * hkv, d)
+        self.q, self.k, self.v = wide[:, :hq], wide[:, hq:hq + hkv], wide[:, hq + hkv:]
+        if fused:
+            dev = DeviceArray.from_numpy(wide, dtype=dtype)
+            self.dq, self.dk, self.dv = dev[:, :hq], dev[:, hq:hq + hkv], dev[:, hq + hkv:]
+        else:
+            self.dq, self.dk, self.dv = (DeviceArray.from_numpy(np.ascontiguousarray(a), dtype=dtype)
+                                         for a in (self.q, self.k, self.v))
+        self.pos = rng.integers(0, rows, T)
+        self.table = mk.rotary_table(rows, rot)
+        self.cs = self.table.to_numpy()[self.pos]
+        wdtype = wdtype or dtype
+        self.qw = kv_oracle.round_to((1 + 0.2 * rng.standard_normal(d)).astype(np.float32), wdtype) if norm else None
+        self.kw = kv_oracle.round_to((1 + 0.2 * rng.standard_normal(d)).astype(np.float32), wdtype) if norm else None
+        self.w = dict(q_weight=DeviceArray.from_numpy(self.qw, dtype=wdtype),
+                      k_weight=DeviceArray.from_numpy(self.kw, dtype=wdtype)) if norm else {}
+
+    def want(self, interleaved, eps=1e-6):
+        return (plain_rope(self.q, self.qw, self.cs, self.rot, interleaved, eps),
+                plain_rope(self.k, self.kw, self.cs, self.rot, interleaved, eps))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("d,rot", [(128, 128), (128, 64), (64, 64), (64, 2), (80, 80), (80, 40), (96, 96), (256, 256),
+                                   (256, 64), (120, 24), (10, 6), (7, 4), (512, 128), (32, 16)])
+def test_qk_norm_rope_head_sizes(gpu, d, rot, dtype, interleaved):
+    for norm in (False, True):
+        c = Rope(d + rot, dtype, 9, 5, 2, d, rot, norm)
+        q, k = mk.qk_norm_rope(c.dq, c.dk, c.pos.astype(np.int64), c.table, interleaved=interleaved, **c.w)
+        for g, w in zip((q, k), c.want(interleaved)):
+            close(g.to_numpy(), w, dtype)
+    assert _lib.get_status(0, clear=True) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,hq,hkv", [(1, 1, 1), (1, 32, 8), (2, 28, 4), (700, 32, 8), (33, 64, 8), (1500, 3, 1)])
+@pytest.mark.parametrize("fused", [False, True])
+def test_qk_norm_rope_shapes(gpu, T, hq, hkv, fused):
+    c = Rope(T, "bfloat16", T, hq, hkv, 128, 128, True, "float32", fused)
+    q, k = mk.qk_norm_rope(c.dq, c.dk, c.pos.astype(np.int32), c.table, eps=1e-5, **c.w)
+    for g, w in zip((q, k), c.want(False, 1e-5)):
+        close(g.to_numpy(), w, "bfloat16")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d,rot", [(128, 128), (10, 10)])
+def test_qk_norm_rope_in_place_one_weight_and_padding(gpu, d, rot):
+    c = Rope(5, "bfloat16", 40, 6, 2, d, rot, True, fused=False)
+    pos = c.pos.copy()
+    pos[3], pos[17], pos[39] = -1, 5000, -9  # padding, past the table, padding
+    want_q, _ = c.want(True)
+    want_k = plain_rope(c.k, None, c.cs, rot, True, 0.0)
+    want_q[[3, 17, 39]], want_k[[3, 17, 39]] = c.q[[3, 17, 39]], c.k[[3, 17, 39]]
+    s = Stream()
+    mk.synchronize()
+    mk.qk_norm_rope(c.dq, c.dk, DeviceArray.from_numpy(pos.astype(np.int32)), c.table, q_weight=c.w["q_weight"],
+                    interleaved=True, q_out=c.dq, k_out=c.dk, stream=s)
+    s.synchronize()
+    close(c.dq.to_numpy(), want_q, "bfloat16")
+    close(c.dk.to_numpy(), want_k, "bfloat16")
+    assert _lib.get_status(0, clear=True) == _lib.STATUS_INDEX_OOB
+
+
+@pytest.mark.gpu
+def test_qk_norm_rope_zero_rows_and_unrotated_infinities(gpu):
+    """A row of zeros stays zero; elements past the rotated part pass as they are."""
+    c = Rope(6, "float16", 3, 2, 1, 128, 64, True, fused=False)
+    x = np.zeros((3, 2, 128), np.float32)
+    q, _ = mk.qk_norm_rope(DeviceArray.from_numpy(x, dtype="float16"), c.dk, c.pos.astype(np.int32), c.table, **c.w)
+    assert not q.to_numpy().any()
+    x[1, 0, 70:75] = [np.inf, -np.inf, 3.0, np.nan, 1.0]
+    q, _ = mk.qk_norm_rope(DeviceArray.from_numpy(x, dtype="float16"), c.dk, c.pos.astype(np.int32), c.table)
+    np.testing.assert_array_equal(q.to_numpy(), x)
+
+
+# ---- with the append ------------------------------------------------------------------
+
+
+def cache_shapes(layout, blocks, bs, hkv, d, dtype):
+    x = 16 // dtypes.itemsize(dtype)
+    return {"paged": ((blocks, hkv, d // x, bs, x), (blocks, hkv, d, bs)), "flash": ((blocks, bs, hkv, d),) * 2,
+            "pool": ((blocks * bs, hkv, d),) * 2}[layout]
+
+
+def place(layout, kc, vc, slots, k, v, bs):
+    for t, s in enumerate(slots):
+        if s < 0 or s >= kc.shape[0] * (1 if layout == "pool" else bs):
+            continue
+        if layout == "paged":
+            kc[s // bs, :, :, s % bs, :] = k[t].reshape(k.shape[1], -1, kc.shape[-1])
+            vc[s // bs, :, :, s % bs] = v[t]
+        elif layout == "flash":
+            kc[s // bs, s % bs], vc[s // bs, s % bs] = k[t], v[t]
+        else:
+            kc[s], vc[s] = k[t], v[t]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("layout,bs", [("paged", 8), ("paged", 16), ("paged", 32), ("flash", 16), ("flash", 5),
+                                       ("pool", 1)])
+@pytest.mark.parametrize("dtype,cache,d,rot,T", [
+    ("bfloat16", "bfloat16", 128, 128, 50), ("bfloat16", "bfloat16", 128, 64, 1), ("float16", "float16", 64, 64, 1333),
+    ("float16", "float16", 80, 40, 20), ("float32", "float32", 96, 96, 1100), ("float32", "float16", 128, 128, 30),
+    ("float32", "bfloat16", 64, 64, 30), ("bfloat16", "bfloat16", 256, 256, 1025), ("float16", "float16", 120, 24, 9)])
+def test_append(gpu, layout, bs, dtype, cache, d, rot, T):
+    if layout != "paged" and cache != dtype:
+        pytest.skip("token-major caches take their own dtype (refused, see below)")
+    c = Rope(T + d, dtype, T, 4, 3, d, rot, T % 2 == 0)
+    rng = np.random.default_rng(T)
+    blocks = -(-T // bs) * 2 + 2
+    # runs of consecutive slots and scattered ones, some padding, one past the cache
+    slots = np.concatenate([np.arange(T // 2) + 3, rng.permutation(np.arange(T // 2 + 3, blocks * bs))[:T - T // 2]])
+    flagged = 0
+    if T > 8:
+        slots[4] = -1
+        slots[7] = blocks * bs + 5
+        flagged = _lib.STATUS_SLOT_OOB
+    ks, vs = cache_shapes(layout, blocks, bs, 3, d, cache)
+    kc0 = kv_oracle.round_to(rng.standard_normal(ks).astype(np.float32), cache)
+    vc0 = kv_oracle.round_to(rng.standard_normal(vs).astype(np.float32), cache)
+    kc, vc = DeviceArray.from_numpy(kc0, dtype=cache), DeviceArray.from_numpy(vc0, dtype=cache)
+    for idt in (np.int32, np.int64):
+        q, _, _ = mk.qk_norm_rope_append(c.dq, c.dk, c.dv, c.pos.astype(idt), c.table, kc, vc, slots.astype(idt),
+                                         interleaved=d == 64, **c.w)
+        want_q, want_k = c.want(d == 64)
+        close(q.to_numpy(), want_q, dtype)
+        kw, vw = kc0.astype(np.float64), vc0.astype(np.float64)
+        place(layout, kw, vw, slots, want_k, kv_oracle.round_to(c.v, cache), bs)
+        close(kc.to_numpy(), kw, cache)
+        np.testing.assert_array_equal(vc.to_numpy(), vw.astype(np.float32))
+        assert _lib.get_status(0, clear=True) == flagged
+
+
+@pytest.mark.gpu
+def test_append_skipped_position_keeps_the_value(gpu):
+    c = Rope(9, "bfloat16", 4, 4, 2, 128, 128, False)
+    pos = np.array([5, -1, 7, 9], np.int32)
+    ks, vs = cache_shapes("paged", 4, 16, 2, 128, "bfloat16")
+    kc, vc = DeviceArray.zeros(ks, "bfloat16"), DeviceArray.zeros(vs, "bfloat16")
+    mk.qk_norm_rope_append(c.dq, c.dk, c.dv, pos, c.table, kc, vc, np.array([0, 17, 33, 50], np.int64))
+    assert not kc.to_numpy()[1].any()
+    np.testing.assert_array_equal(vc.to_numpy()[1, :, :, 1], c.v[1])
+    assert _lib.get_status(0, clear=True) == 0
+
+
+# ---- refusals ---------------------------------------------------------------------------
+
+
+def _fake(shape, dtype="float16", strides=None):
+    if strides is None:
+        acc, st = 1, []
+        for s in reversed(shape):
+            st.append(acc)
+            acc *= s
+        strides = tuple(reversed(st))
+    t, keep = dlpack.make_dltensor(0x10000, shape, strides, dtype, 0)
+    _fake.keep.append(keep)
+    return ctypes.pointer(t)
+
+
+_fake.keep = []
+
+
+def _rope_rc(q=(3, 4, 64), k=(3, 2, 64), pos=(3,), posd="int32", cs=(10, 64), csd="float32", w=(64,), wd="float16",
+             qo=None, ko=None, eps=1e-6, kd="float16", qst=None):
+    return _lib.lib.kvc_qk_norm_rope(_fake(qo or q), _fake(ko or k), _fake(q, strides=qst), _fake(k, kd),
+                                     _fake(pos, posd), _fake(cs, csd), _fake(w, wd), None, eps, 0, None)
+
+
+@pytest.mark.parametrize("kw,text", [
+    (dict(k=(2, 2, 64)), "q must have shape"), (dict(kd="float32"), "must share"), (dict(pos=(2,)), "positions must be"),
+    (dict(posd="uint32"), "positions must be int32 or int64"), (dict(cs=(10, 65)), "even rotary_dim"),
+    (dict(cs=(10, 66)), "even rotary_dim"), (dict(csd="float16"), "cos_sin must be float32"),
+    (dict(w=(32,)), "head_size entries"), (dict(wd="bfloat16"), "float32 or of q's dtype"),
+    (dict(qo=(3, 4, 32)), "q_out must have"), (dict(ko=(3, 4, 64)), "k_out must have"), (dict(eps=-1.0), "eps must be"),
+    (dict(eps=float("nan")), "eps must be"), (dict(qst=(256, 64, 2)), "must be contiguous"),
+    (dict(q=(3, 4, 514), k=(3, 2, 514), cs=(10, 64), w=(514,)), "between 1 and 512")])
+def test_rope_refusals(kw, text):
+    assert _rope_rc(**kw) == 1
+    assert text in _lib.last_error()
+
+
+def test_append_refusals():
+    def rc(kc=(5, 2, 8, 16, 8), vc=(5, 2, 64, 16), slots=(3,), sd="int64", v=(3, 2, 64), cd="float16", qd="float16"):
+        return _lib.lib.kvc_qk_norm_rope_append(
+            _fake((3, 4, 64), qd), _fake(kc, cd), _fake(vc, cd), _fake((3, 4, 64), qd), _fake((3, 2, 64), qd), _fake(v, qd),
+            _fake((3,), "int32"), _fake((10, 64), "float32"), None, None, 1e-6, 0, _fake(slots, sd), None)
+
+    for kw, text in ((dict(slots=(2,)), "slot_mapping must have shape"), (dict(sd="uint32"), "int32 or int64"),
+                     (dict(v=(3, 4, 64)), "key and value must both"), (dict(kc=(5, 3, 8, 16, 8)), "KV-head count"),
+                     (dict(cd="bfloat16"), "Unsupported dtype combination"),
+                     (dict(kc=(5, 16, 2, 64), vc=(5, 16, 2, 64), qd="float32"), "dtypes to match")):
+        assert rc(**kw) == 1
+        assert text in _lib.last_error()
+
+
+def test_step_tables_refusals():
+    def rc(bt=(2, 4), kl=(2,), qi=(3,), po=(9,), sm=(9,), us=(1,), pl=(2,), nl=(2,), smd="int64", fd="int32", bs=16):
+        return _lib.lib.kvc_step_tables(_fake(bt, "int32"), _fake(kl, "int32"), _fake(qi, "int32"), _fake(po, "int32"),
+                                        _fake(sm, smd), _fake(us, "int32"), _fake(pl, "int32"), _fake(nl, "int32"),
+                                        _fake((7,), fd), bs, None)
+
+    for kw, text in ((dict(bt=(2,)), "block_tables must be 2D"), (dict(nl=(3,)), "num_seqs rows"),
+                     (dict(qi=(2,)), "num_seqs + 1"), (dict(sm=(8,)), "same length"), (dict(bs=0), "block_size must be"),
+                     (dict(smd="uint32"), "slot_mapping must be"), (dict(fd="int64"), "must be int32"),
+                     (dict(kl=(2, 1)), "contiguous 1-D")):
+        assert rc(**kw) == 1
+        assert text in _lib.last_error()
+    with pytest.raises(ValueError, match="num_tokens is needed"):
+        mk.build_step_tables(None, None, object(), None, 16)
+
+
+def test_rotary_table_refusals():
+    f = (ctypes.c_double * 32)(*([1.0] * 32))
+    for t, text in (((_fake((4, 65), "float32")), "even rotary_dim"), (_fake((4, 258), "float32"), "even rotary_dim"),
+                    (_fake((4, 64)), "must be float32")):
+        assert _lib.lib.kvc_rotary_table(t, f, 1.0, None) == 1 and text in _lib.last_error()
+    f[3] = math.inf
+    assert _lib.lib.kvc_rotary_table(_fake((4, 64), "float32"), f, 1.0, None) == 1 and "finite" in _lib.last_error()
+    with pytest.raises(ValueError):
+        mk.rotary_table(0, 64)

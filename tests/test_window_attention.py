@@ -1,0 +1,324 @@
+"""Sliding-window attention with sinks (paged_attention_window,
+paged_prefill_window) against the formula in float64: the query at position i
+sees j <= i with j < sink_size or j > i - window_size."""
+
+import ctypes
+
+import numpy as np
+import pytest
+
+from helpers import assert_close, tolerance
+from oracle import kv_oracle
+from sglang_mlx_b200 import _lib, dlpack
+from sglang_mlx_b200 import metal_kernels as mk
+from sglang_mlx_b200.device_array import DeviceArray, Stream
+
+NAN = float("nan")
+
+
+def visible(i, window, sinks):
+    j = np.arange(i + 1)
+    return j[(j < sinks) | (j > i - window)]
+
+
+def attend(q, K, V, i, window, sinks, scale, G, eps):
+    """One query token [H, D] at position i over K, V [len, Hkv, D], float64."""
+    j = visible(i, window, sinks)
+    out = np.zeros(q.shape, np.float64)
+    for h in range(q.shape[0]):
+        s = K[j, h // G] @ q[h] * scale
+        e = np.exp(s - s.max())
+        out[h] = e @ V[j, h // G] / (e.sum() + eps)
+    return out
+
+
+class Case:
+    """A ragged batch in a paged ("paged"), flash ("flash") or pool ("pool") cache."""
+
+    def __init__(self, seed, dtype, lens, hq, hkv, d, bs, layout="paged", new=None, cache_dtype=None, spare=5):
+        rng = np.random.default_rng(seed)
+        self.lens, self.bs, self.layout, self.G = np.asarray(lens, np.int64), bs, layout, hq // hkv
+        self.new = np.ones(len(lens), np.int64) if new is None else np.asarray(new, np.int64)
+        self.dtype, self.cache_dtype = dtype, cache_dtype or dtype
+        rows = int(self.new.sum())
+        rnd = lambda shape, dt: kv_oracle.round_to(rng.standard_normal(shape).astype(np.float32), dt)  # noqa: E731
+        self.q = rnd((rows, hq, d), dtype)
+        need = -(-self.lens // bs)
+        self.blocks = int(need.sum()) + spare
+        perm = rng.permutation(self.blocks)
+        width = int(max(1, need.max())) + 1
+        self.tables = np.full((len(lens), width), -1, np.int64)
+        at = 0
+        for b, n in enumerate(need):
+            self.tables[b, :n] = perm[at:at + n]
+            at += n
+        self.K = [rnd((int(n), hkv, d), self.cache_dtype) for n in self.lens]
+        self.V = [rnd((int(n), hkv, d), self.cache_dtype) for n in self.lens]
+        # what is not the cache of any sequence (the rest of last blocks, spare blocks) is NaN
+        self.k_rows = np.full((self.blocks * bs, hkv, d), NAN, np.float32)
+        self.v_rows = np.full((self.blocks * bs, hkv, d), NAN, np.float32)
+        for b, n in enumerate(self.lens):
+            t = np.arange(int(n))
+            slot = self.tables[b, t // bs] * bs + t % bs
+            self.k_rows[slot], self.v_rows[slot] = self.K[b], self.V[b]
+        self.scale = d ** -0.5
+        self.hkv, self.d = hkv, d
+        self.indptr = np.concatenate([[0], np.cumsum(self.new)]).astype(np.int32)
+
+    def poison(self, window, sinks):
+        """NaN into every cached token that no query sees, -1 into table entries of blocks without a seen token."""
+        for b, n in enumerate(self.lens):
+            seen = np.zeros(int(n), bool)
+            for i in range(int(n - self.new[b]), int(n)):
+                seen[visible(i, window, sinks)] = True
+            t = np.nonzero(~seen)[0]
+            slot = self.tables[b, t // self.bs] * self.bs + t % self.bs
+            self.k_rows[slot] = self.v_rows[slot] = NAN
+            for blk in range(-(-int(n) // self.bs)):
+                if not seen[blk * self.bs:(blk + 1) * self.bs].any():
+                    self.tables[b, blk] = -1
+
+    def upload(self):
+        hkv, d, bs, nb = self.hkv, self.d, self.bs, self.blocks
+        kr, vr = self.k_rows.reshape(nb, bs, hkv, d), self.v_rows.reshape(nb, bs, hkv, d)
+        if self.layout == "paged":
+            x = 16 // (4 if self.cache_dtype == "float32" else 2)
+            kr = kr.reshape(nb, bs, hkv, d // x, x).transpose(0, 2, 3, 1, 4)
+            vr = vr.transpose(0, 2, 3, 1)
+        elif self.layout == "pool":
+            kr, vr = kr.reshape(nb * bs, hkv, d), vr.reshape(nb * bs, hkv, d)
+        kc = DeviceArray.from_numpy(np.ascontiguousarray(kr), dtype=self.cache_dtype)
+        vc = DeviceArray.from_numpy(np.ascontiguousarray(vr), dtype=self.cache_dtype)
+        q = DeviceArray.from_numpy(self.q, dtype=self.dtype)
+        return q, kc, vc, DeviceArray.from_numpy(self.tables.astype(np.int32)), DeviceArray.from_numpy(
+            self.lens.astype(np.int32))
+
+    @property
+    def max_seq_len(self):
+        return self.tables.shape[1] * self.bs
+
+    def reference(self, window, sinks, eps):
+        out = np.zeros(self.q.shape, np.float64)
+        for b, n in enumerate(self.lens):
+            K, V = self.K[b].astype(np.float64), self.V[b].astype(np.float64)
+            for t in range(int(self.new[b])):
+                i = int(n - self.new[b]) + t
+                if i < 0 or n == 0:
+                    continue
+                r = int(self.indptr[b]) + t
+                out[r] = attend(self.q[r].astype(np.float64), K, V, i, window, sinks, self.scale, self.G, eps)
+        return out
+
+    def decode(self, window, sinks, **kw):
+        q, kc, vc, tables, lens = self.upload()
+        return mk.paged_attention_window(q, kc, vc, tables, lens, self.hkv, self.scale, self.bs, self.max_seq_len,
+                                         window, sinks, **kw).to_numpy()
+
+    def extend(self, window, sinks, **kw):
+        q, kc, vc, tables, lens = self.upload()
+        return mk.paged_prefill_window(q, kc, vc, tables, self.indptr, lens, self.hkv, self.scale, self.bs, window,
+                                       sinks, **kw).to_numpy()
+
+
+LENS = [1, 2, 15, 16, 17, 33, 100, 257, 700, 1500]
+WINDOWS = [(1, 0), (1, 1), (7, 0), (16, 4), (33, 17), (128, 64), (500, 3), (5000, 4)]
+
+
+def check_decode(c, window, sinks, what=""):
+    ref = c.reference(window, sinks, 1e-6)
+    c.poison(window, sinks)
+    got = c.decode(window, sinks)
+    assert_close(got, ref, *tolerance(c.dtype), f"{what} window {window} sinks {sinks}")
+    assert _lib.get_status(0, clear=True) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("window,sinks", WINDOWS)
+@pytest.mark.parametrize("layout,bs,d", [("paged", 8, 128), ("paged", 16, 128), ("paged", 32, 128), ("paged", 16, 64),
+                                         ("paged", 32, 64), ("flash", 16, 128), ("flash", 32, 64), ("flash", 5, 128),
+                                         ("flash", 24, 64), ("pool", 1, 128), ("pool", 1, 64)])
+def test_decode_layouts(gpu, layout, bs, d, window, sinks):
+    c = Case(11, "bfloat16", LENS, 8, 2, d, bs, layout)
+    check_decode(c, window, sinks, f"{layout} {bs} {d}")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hq,hkv", [(1, 1), (5, 1), (16, 1), (28, 4), (8, 8), (40, 2)])
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+def test_decode_head_groups(gpu, hq, hkv, dtype):
+    check_decode(Case(12, dtype, [1, 40, 333], hq, hkv, 128, 16), 100, 4, f"{hq}/{hkv}")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [32, 64, 80, 96, 112, 120, 128, 192, 256])
+@pytest.mark.parametrize("dtype,cache", [("float32", "float32"), ("float32", "float16"), ("float32", "bfloat16"),
+                                         ("float16", "float16"), ("bfloat16", "bfloat16")])
+def test_decode_types_and_head_sizes(gpu, d, dtype, cache):
+    check_decode(Case(13, dtype, [3, 70, 300], 6, 2, d, 8 if d == 120 else 16, cache_dtype=cache), 65, 9)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,window", [(1, 64), (1, 4096), (3, 1024), (40, 300)])
+def test_decode_one_or_few_sequences(gpu, n, window):
+    """Few (sequence, KV head) pairs: the seen tokens are split over a cluster."""
+    rng = np.random.default_rng(n)
+    check_decode(Case(14, "bfloat16", rng.integers(1, 9000, n), 8, 1, 128, 16), window, 4)
+    check_decode(Case(15, "float32", rng.integers(1, 3000, n), 8, 1, 64, 32), window, 4)
+
+
+@pytest.mark.gpu
+def test_decode_zero_and_overlong_sequences(gpu):
+    c = Case(16, "float16", [0, 5, 64, 0], 4, 2, 64, 16)
+    ref = c.reference(8, 2, 1e-6)
+    q, kc, vc, tables, lens = c.upload()
+    out = mk.paged_attention_window(q, kc, vc, tables, lens, 2, c.scale, 16, 63, 8, 2).to_numpy()
+    ref[2] = 0  # 64 tokens, past max_seq_len 63
+    assert_close(out, ref, *tolerance("float16"))
+    c32 = Case(16, "float32", [0, 5, 64, 0], 4, 2, 64, 16)
+    q, kc, vc, tables, lens = c32.upload()
+    out = mk.paged_attention_window(q, kc, vc, tables, lens, 2, c32.scale, 16, 63, 8, 2).to_numpy()
+    ref = c32.reference(8, 2, 1e-6)
+    ref[2] = 0
+    assert_close(out, ref, *tolerance("float32"))
+
+
+@pytest.mark.gpu
+def test_decode_window_past_the_context_is_the_plain_decode(gpu):
+    c = Case(17, "bfloat16", [7, 90, 600], 8, 2, 128, 16)
+    q, kc, vc, tables, lens = c.upload()
+    a = mk.paged_attention_window(q, kc, vc, tables, lens, 2, c.scale, 16, c.max_seq_len, 10000, 0).to_numpy()
+    b = mk.paged_attention_v1(q, kc, vc, tables, lens, 2, c.scale, 16, c.max_seq_len).to_numpy()
+    assert_close(a, b, 1e-6, 2.0 ** -7)  # two roundings of nearly the same value: one bfloat16 step
+
+
+@pytest.mark.gpu
+def test_decode_is_deterministic_and_strided(gpu):
+    """The same bits every time; query and output rows may be slices of wider rows."""
+    c = Case(18, "bfloat16", [9, 130, 1000], 8, 2, 128, 16)
+    q, kc, vc, tables, lens = c.upload()
+    wide = np.zeros((3, 12, 128), np.float32)
+    wide[:, 2:10] = c.q
+    qs = DeviceArray.from_numpy(wide, dtype="bfloat16")[:, 2:10]
+    outw = DeviceArray.zeros((3, 11, 128), "bfloat16")
+    args = (kc, vc, tables, lens, 2, c.scale, 16, c.max_seq_len, 100, 4)
+    first = mk.paged_attention_window(q, *args).to_numpy(raw=True)
+    for _ in range(3):
+        np.testing.assert_array_equal(mk.paged_attention_window(q, *args).to_numpy(raw=True), first)
+    s = Stream()
+    mk.synchronize()
+    mk.paged_attention_window(qs, *args, out=outw[:, 1:9], stream=s)
+    s.synchronize()
+    got = outw.to_numpy(raw=True)
+    np.testing.assert_array_equal(got[:, 1:9], first)
+    assert not got[:, :1].any() and not got[:, 9:].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_decode_large_scores_and_infinite_unseen(gpu, sign):
+    """Scores of +-1000 stay finite; infinities in unseen places do not matter."""
+    c = Case(19, "float16", [300], 4, 1, 128, 16)
+    c.q[:] = sign * 30.0
+    c.K[0][:] = np.abs(c.K[0])
+    c.k_rows[:] = np.inf
+    t = np.arange(300)
+    slot = c.tables[0, t // 16] * 16 + t % 16
+    c.k_rows[slot] = c.K[0]
+    check_decode(c, 50, 3)
+
+
+@pytest.mark.gpu
+def test_decode_bad_block_is_skipped_and_flagged(gpu):
+    c = Case(20, "bfloat16", [200], 8, 2, 128, 16)
+    q, kc, vc, _, lens = c.upload()
+    t = c.tables.copy()
+    t[0, 11] = c.blocks + 7  # tokens 176 .. 191, inside the window
+    out = mk.paged_attention_window(q, kc, vc, DeviceArray.from_numpy(t.astype(np.int32)), lens, 2, c.scale, 16,
+                                    c.max_seq_len, 40, 2).to_numpy()
+    assert np.isfinite(out).all()
+    assert _lib.get_status(0, clear=True) == _lib.STATUS_BLOCK_OOB
+
+
+# ---- extend ---------------------------------------------------------------------
+
+
+def check_extend(c, window, sinks, what=""):
+    ref = c.reference(window, sinks, 0.0)
+    c.poison(window, sinks)
+    got = c.extend(window, sinks)
+    assert_close(got, ref, *tolerance(c.dtype), f"{what} window {window} sinks {sinks}")
+    assert _lib.get_status(0, clear=True) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("window,sinks", WINDOWS)
+@pytest.mark.parametrize("layout,bs,d", [("paged", 8, 128), ("paged", 16, 128), ("paged", 32, 128), ("paged", 16, 64),
+                                         ("paged", 32, 64), ("flash", 16, 128), ("flash", 5, 64), ("pool", 1, 128)])
+def test_extend_layouts(gpu, layout, bs, d, window, sinks):
+    c = Case(31, "bfloat16", [1, 40, 130, 300, 555], 4, 2, d, bs, layout, new=[1, 40, 33, 1, 150])
+    check_extend(c, window, sinks, f"{layout} {bs} {d}")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hq,hkv,dtype", [(28, 4, "float16"), (8, 8, "float16"), (16, 1, "bfloat16"), (5, 1, "bfloat16")])
+def test_extend_head_groups(gpu, hq, hkv, dtype):
+    check_extend(Case(32, dtype, [77, 400], hq, hkv, 128, 16, new=[77, 90]), 100, 4)
+
+
+@pytest.mark.gpu
+def test_extend_many_sequences_and_a_long_prefix(gpu):
+    rng = np.random.default_rng(33)
+    new = rng.integers(0, 30, 60)
+    lens = new + rng.integers(0, 200, 60)
+    lens[7] = new[7] + 5000
+    check_extend(Case(33, "bfloat16", lens, 4, 1, 64, 32, new=new), 64, 20)
+
+
+@pytest.mark.gpu
+def test_extend_of_one_token(gpu):
+    check_extend(Case(34, "float16", [5, 64, 700], 8, 2, 64, 16), 90, 4)
+
+
+# ---- refusals -------------------------------------------------------------------
+
+
+def _fake(shape, dtype="float16"):
+    acc, st = 1, []
+    for s in reversed(shape):
+        st.append(acc)
+        acc *= s
+    t, keep = dlpack.make_dltensor(0x10000, shape, tuple(reversed(st)), dtype, 0)
+    _fake.keep.append(keep)
+    return ctypes.pointer(t)
+
+
+_fake.keep = []
+
+
+def _decode_rc(q=(2, 8, 64), kc=(20, 4, 8, 16, 8), vc=(20, 4, 64, 16), w=8, s=0, qd="float16", msl=64, bs=16):
+    return _lib.lib.kvc_paged_attention_window(_fake(q, qd), _fake(q, qd), _fake(kc), _fake(vc), _fake((2, 4), "int32"),
+                                               _fake((2,), "int32"), 4, 0.125, bs, msl, w, s, None)
+
+
+@pytest.mark.parametrize("kw,rc,text", [
+    (dict(w=0), 1, "window_size must be positive"),
+    (dict(w=-3), 1, "window_size must be positive"),
+    (dict(s=-1), 1, "sink_size must be non-negative"),
+    (dict(msl=65), 1, "max_seq_len exceeds block table capacity"),
+    (dict(qd="int32"), 1, "Unsupported dtype combination"),
+    (dict(kc=(20, 4, 8, 8, 8)), 1, "cache block dimensions"),
+    (dict(kc=(20, 16, 4, 64), vc=(20, 16, 4, 64), qd="float32"), 4, "float16/bfloat16"),
+    (dict(kc=(20, 16), vc=(20, 16)), 1, "key_cache/value_cache must be"),
+])
+def test_decode_refusals(kw, rc, text):
+    assert _decode_rc(**kw) == rc
+    assert text in _lib.last_error()
+
+
+@pytest.mark.parametrize("w,s,text", [(0, 0, "window_size must be positive"), (4, -1, "sink_size must be")])
+def test_extend_refusals(w, s, text):
+    q = (6, 8, 64)
+    rc = _lib.lib.kvc_paged_prefill_window(_fake(q), _fake(q), _fake((20, 4, 8, 16, 8)), _fake((20, 4, 64, 16)),
+                                           _fake((2, 4), "int32"), _fake((3,), "int32"), _fake((2,), "int32"), 4, 0.125,
+                                           16, 3, w, s, None)
+    assert rc == 1 and text in _lib.last_error()
