@@ -26,6 +26,25 @@ from .dlpack import DLTensor, as_dltensor, call_tensors, describe
 
 _L = _lib.lib
 
+# The step operators' calls without ctypes (csrc/calls.cpp): each returns the
+# library's status code, or -1 when an argument needs the general path below.
+try:
+    from . import _calls
+except ImportError:  # built without the interpreter's headers
+    _calls = None
+else:
+    _calls.bind(DeviceArray, {n: ctypes.cast(getattr(_L, n), ctypes.c_void_p).value for n in (
+        "kvc_paged_attention_window", "kvc_paged_prefill_window", "kvc_step_tables", "kvc_qk_norm_rope",
+        "kvc_qk_norm_rope_append")})
+
+
+def _done(rc: int) -> bool:
+    """True when a direct call ran (its errors raised); False for the general path."""
+    if rc > 0:
+        _lib.check(rc)
+    return rc == 0
+
+
 DEFAULT_PARTITION_SIZE = 512
 
 
@@ -515,6 +534,10 @@ def paged_attention_window(query, key_cache, value_cache, block_tables, context_
     block_size, kv_heads, D], or a token pool [slots, kv_heads, D] with block_size
     1), of paged_attention_flash.  Table entries of blocks that no token sees are
     not read, so their blocks may have been freed.  One launch, no workspace."""
+    if _calls is not None and out is not None and _done(_calls.paged_attention_window(
+            out, query, key_cache, value_cache, block_tables, context_lens, num_kv_heads, scale, block_size,
+            max_seq_len, window_size, sink_size, stream)):
+        return out
     query, key_cache, value_cache = _dev(query), _dev(key_cache), _dev(value_cache)
     block_tables, context_lens = _dev(block_tables), _dev(context_lens)
     if out is None:
@@ -535,6 +558,10 @@ def paged_prefill_window(query, key_cache, value_cache, block_tables, qo_indptr,
     paged_prefill_attention, where the new token at position i sees position j <= i
     when j < sink_size or j > i - window_size.  Table entries of blocks that no
     new token of their sequence sees are not read."""
+    if _calls is not None and out is not None and max_q_len is not None and _done(_calls.paged_prefill_window(
+            out, query, key_cache, value_cache, block_tables, qo_indptr, kv_lens, num_kv_heads, scale, block_size,
+            max_q_len, window_size, sink_size, stream)):
+        return out
     if max_q_len is None:
         if isinstance(qo_indptr, (np.ndarray, list, tuple)):
             ind = np.asarray(qo_indptr, dtype=np.int64)
@@ -583,6 +610,11 @@ def build_step_tables(block_tables, prefix_lens, new_lens, free_blocks, block_si
         prefix_lens, new_lens: [B] int32
         free_blocks: [any] int32 block ids
     """
+    if (_calls is not None and kv_lens is not None and qo_indptr is not None and positions is not None
+            and slot_mapping is not None and blocks_used is not None and _done(_calls.step_tables(
+                block_tables, kv_lens, qo_indptr, positions, slot_mapping, blocks_used, prefix_lens, new_lens,
+                free_blocks, block_size, stream))):
+        return StepTables(block_tables, kv_lens, qo_indptr, positions, slot_mapping, blocks_used)
     if num_tokens is None and positions is None:
         if not isinstance(new_lens, (np.ndarray, list, tuple)):
             raise ValueError("num_tokens is needed when new_lens is a device array")
@@ -694,6 +726,9 @@ def qk_norm_rope(q, k, positions, cos_sin, *, q_weight=None, k_weight=None, eps:
         interleaved: pairs (2i, 2i + 1) instead of (i, i + rotary_dim / 2)
         q_out, k_out: outputs; q and k themselves rotate in place
     """
+    if _calls is not None and q_out is not None and k_out is not None and _done(_calls.qk_norm_rope(
+            q_out, k_out, q, k, positions, cos_sin, q_weight, k_weight, eps, 1 if interleaved else 0, stream)):
+        return q_out, k_out
     q, k, positions, cos_sin = _dev(q), _dev(k), _dev(positions), _dev(cos_sin)
     q_weight, k_weight = _dev(q_weight), _dev(k_weight)
     if q_out is None:
@@ -713,6 +748,10 @@ def qk_norm_rope_append(q, k, v, positions, cos_sin, key_cache, value_cache, slo
     reshape_and_cache_flash (token-major caches) would store them, in the same
     launch.  Returns (q_out, key_cache, value_cache); the caches are updated in
     place.  q_out may be q."""
+    if _calls is not None and q_out is not None and _done(_calls.qk_norm_rope_append(
+            q_out, key_cache, value_cache, q, k, v, positions, cos_sin, q_weight, k_weight, slot_mapping, eps,
+            1 if interleaved else 0, stream)):
+        return q_out, key_cache, value_cache
     q, k, v, positions, cos_sin = _dev(q), _dev(k), _dev(v), _dev(positions), _dev(cos_sin)
     q_weight, k_weight, slot_mapping = _dev(q_weight), _dev(k_weight), _dev(slot_mapping)
     if q_out is None:
