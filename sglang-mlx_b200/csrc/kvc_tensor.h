@@ -205,6 +205,7 @@ struct RopeArgs {
   const void* slots;
   ElemType type, cache_type, weight_type;
   bool pos_i64, slots_i64, interleaved;
+  bool v_wide;  // append: 16-byte runs of value_cache rows are aligned (set by the launcher)
   bool paged;  // append: the [nb, H, D/x, bs, x] / [nb, H, D, bs] layout, else token-major rows
   float eps;
   int num_heads, num_kv_heads, head_size, rot, block_size;

@@ -7,12 +7,38 @@
 #include <stdint.h>
 
 #include <atomic>
+#include <type_traits>
 
 #include "kvc_common.cuh"
 
 namespace kvc {
 
 __device__ unsigned int g_layer_ops_status = 0;
+
+// Every kernel here is a programmatic dependent of the kernel before it on the
+// stream: its launch overlaps that kernel's end, and it waits for it before it
+// reads or writes anything.  None lets its own dependents start early: the decode
+// kernels read queries, tables and lengths, which are written here, before they
+// wait.
+__device__ __forceinline__ void wait_for_prior() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <typename... P, typename... A>
+static cudaError_t launch_dependent(void (*kern)(P...), dim3 grid, int threads, size_t smem, cudaStream_t stream,
+                                    A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
+  count_launch();
+  return e != cudaSuccess ? e : cudaGetLastError();
+}
 
 // SMs of the current device (cached per device; any racing writer stores the same value).
 static int sm_count() {
@@ -77,6 +103,7 @@ __global__ void __launch_bounds__(kTablesThreads) step_tables_kernel(StepTablesA
   const bool last_chunk = blockIdx.y == gridDim.y - 1;
   const uint32_t bs = (uint32_t)p.block_size;
   bool bad = false;
+  wait_for_prior();
   // request b's cached tokens, new tokens and new blocks (lengths below zero, or
   // past 2^31 - 1 together, are input errors: flagged, read as zero)
   auto request = [&](int b, uint32_t* pre, uint32_t* fresh, uint32_t* blocks) {
@@ -263,9 +290,7 @@ cudaError_t launch_step_tables(const StepTablesArgs& a, cudaStream_t stream) {
   const int64_t most = 2 * (int64_t)sm_count() / chunks;
   if (slices > most) slices = most;
   if (slices < 1) slices = 1;
-  step_tables_kernel<<<dim3((unsigned)slices, (unsigned)chunks), kTablesThreads, 0, stream>>>(a);
-  count_launch();
-  return cudaGetLastError();
+  return launch_dependent(step_tables_kernel, dim3((unsigned)slices, (unsigned)chunks), kTablesThreads, 0, stream, a);
 }
 
 // ---------------------------------------------------------------------------
@@ -275,6 +300,7 @@ cudaError_t launch_step_tables(const StepTablesArgs& a, cudaStream_t stream) {
 // Written once per model; the division of work is of no weight.
 // ---------------------------------------------------------------------------
 __global__ void __launch_bounds__(256) rotary_table_kernel(RotaryTableArgs p) {
+  wait_for_prior();
   const int64_t total = p.rows * p.half;
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
     const int64_t row = i / p.half;
@@ -292,9 +318,7 @@ cudaError_t launch_rotary_table(const RotaryTableArgs& a, cudaStream_t stream) {
   int64_t ctas = (total + 255) / 256;
   const int64_t most = 8 * (int64_t)sm_count();
   if (ctas > most) ctas = most;
-  rotary_table_kernel<<<(unsigned)ctas, 256, 0, stream>>>(a);
-  count_launch();
-  return cudaGetLastError();
+  return launch_dependent(rotary_table_kernel, dim3((unsigned)ctas), 256, 0, stream, a);
 }
 
 // ---------------------------------------------------------------------------
@@ -306,39 +330,81 @@ cudaError_t launch_rotary_table(const RotaryTableArgs& a, cudaStream_t stream) {
 //   (a, b) -> (a c_i - b s_i, b c_i + a s_i)
 // in 32 bits, rounded once to the output's type.
 // ---------------------------------------------------------------------------
-template <typename T, int VEC>
-struct Vec {  // VEC consecutive elements as the widest loads and stores up to 16 bytes
-  static constexpr int BYTES = VEC * (int)sizeof(T);
-  static_assert(BYTES % 8 == 0, "whole 8-byte words");
-  T e[VEC];
-  __device__ __forceinline__ void load(const T* src) {
-    if constexpr (BYTES == 8) {
-      *reinterpret_cast<uint2*>(e) = *reinterpret_cast<const uint2*>(src);
+// Two fp32 lanes per instruction (the f32x2 arithmetic of sm_100), rounded as two
+// scalar operations are.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n.reg .b64 ra, rb, rd;\nmov.b64 ra, {%2, %3};\nmov.b64 rb, {%4, %5};\nmul.rn.f32x2 rd, ra, rb;\n"
+      "mov.b64 {%0, %1}, rd;\n}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n.reg .b64 ra, rb, rc, rd;\nmov.b64 ra, {%2, %3};\nmov.b64 rb, {%4, %5};\nmov.b64 rc, {%6, %7};\n"
+      "fma.rn.f32x2 rd, ra, rb, rc;\nmov.b64 {%0, %1}, rd;\n}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+
+__device__ __forceinline__ float2 pair_to_float(uint32_t w, __nv_bfloat16*) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+__device__ __forceinline__ float2 pair_to_float(uint32_t w, __half*) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+__device__ __forceinline__ uint32_t pair_from_float(float2 x, __nv_bfloat16*) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(x.x, x.y);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t pair_from_float(float2 x, __half*) {
+  const __half2 v = __floats2half2_rn(x.x, x.y);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+template <typename T>
+struct Quad {  // four consecutive elements, one load or store (8 or 16 bytes)
+  using Word = typename std::conditional<sizeof(T) == 2, uint2, uint4>::type;
+  Word w;
+  __device__ __forceinline__ void load(const T* src) { w = *reinterpret_cast<const Word*>(src); }
+  __device__ __forceinline__ void store(T* dst) const { *reinterpret_cast<Word*>(dst) = w; }
+  __device__ __forceinline__ void get(float2& x, float2& y) const {
+    if constexpr (sizeof(T) == 2) {
+      x = pair_to_float(w.x, (T*)nullptr);
+      y = pair_to_float(w.y, (T*)nullptr);
     } else {
-#pragma unroll
-      for (int i = 0; i < BYTES / 16; ++i) reinterpret_cast<uint4*>(e)[i] = reinterpret_cast<const uint4*>(src)[i];
+      x = make_float2(__uint_as_float(w.x), __uint_as_float(w.y));
+      y = make_float2(__uint_as_float(w.z), __uint_as_float(w.w));
     }
   }
-  __device__ __forceinline__ void store(T* dst) const {
-    if constexpr (BYTES == 8) {
-      *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(e);
+  __device__ __forceinline__ void put(float2 x, float2 y) {
+    if constexpr (sizeof(T) == 2) {
+      w.x = pair_from_float(x, (T*)nullptr);
+      w.y = pair_from_float(y, (T*)nullptr);
     } else {
-#pragma unroll
-      for (int i = 0; i < BYTES / 16; ++i) reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(e)[i];
+      w = make_uint4(__float_as_uint(x.x), __float_as_uint(x.y), __float_as_uint(y.x), __float_as_uint(y.y));
     }
   }
 };
 
-// The token's table row and cache place; false: its rows are skipped (a negative
-// position or slot is padding, one past the table or the cache is flagged).
 __device__ __forceinline__ int64_t load_index(const void* a, bool i64, int64_t i) {
   return i64 ? reinterpret_cast<const int64_t*>(a)[i] : (int64_t)reinterpret_cast<const int32_t*>(a)[i];
 }
 
+// The cache place of a slot; false: the token's rows are skipped (a negative
+// slot is padding, one past the cache is flagged).
 __device__ __forceinline__ bool token_place(const RopeArgs& p, int64_t slot, bool flag, int64_t* blk, int* off) {
   if (slot < 0) return false;
-  *blk = slot / p.block_size;
-  *off = (int)(slot - *blk * p.block_size);
+  if (slot <= 0xffffffffll) {  // (a 64-bit division costs a hundred instructions)
+    const uint32_t s = (uint32_t)slot, b = s / (uint32_t)p.block_size;
+    *blk = b;
+    *off = (int)(s - b * (uint32_t)p.block_size);
+  } else {
+    *blk = slot / p.block_size;
+    *off = (int)(slot - *blk * p.block_size);
+  }
   if (*blk >= p.num_blocks) {
     if (flag) set_status(&g_layer_ops_status, KVC_STATUS_SLOT_OOB);
     return false;
@@ -346,201 +412,318 @@ __device__ __forceinline__ bool token_place(const RopeArgs& p, int64_t slot, boo
   return true;
 }
 
-// How a launch divides a token's rows: chunks of U passes of the warp, each over
-// 32 >> lpr_shift rows; first the q heads, then the k heads, then (append) the v
-// heads.  CTAs from `row_ctas` on move V through shared-memory tiles instead.
+// How a launch divides a token's rows.  A group is the 32 >> lpr_shift rows that a
+// warp holds at a time; a token's groups are its q heads', then its k heads', then
+// (append) its v heads', and a warp takes `span` of one token's groups.  CTAs from
+// `row_ctas` on move V through shared-memory tiles instead.
 struct RopePlan {
-  int lpr_shift, q_chunks, k_chunks, v_chunks;
-  unsigned row_ctas;
+  int lpr_shift, q_groups, k_groups, v_groups, span;
+  unsigned warps_per_token, row_ctas;
+  float inv_d;
 };
 constexpr int kRopeWarps = 8;
 constexpr int kVTile = 32;  // tokens of a V tile
 
-// V of kVTile tokens and one head into [block][head][dim][offset]: rows in, then
-// lane = token, so tokens at consecutive offsets of a block make one run.
-template <typename T, int VEC>
-__device__ __forceinline__ void store_v_tile(const RopeArgs& p, int64_t tile, unsigned char* smem) {
-  constexpr int PAD = sizeof(T) == 2 ? 2 : 1;  // an odd number of words to a row
+// V of kVTile tokens and one head into [block][head][dim][offset].  The rows are
+// staged in shared memory (16 bytes of padding: 8 rows cover all banks).  16-bit
+// elements: a transposed matrix load whose matrix i takes tokens 8q + 2i, 8q + 2i
+// + 1 for q = 0..3 leaves lane (dim, q) the tokens 8q .. 8q + 7 of its dim in
+// order, so 8 tokens that lie in one block at consecutive offsets from a multiple
+// of 8 on are one 16-byte store.  Tokens that do not, and 32-bit elements, go
+// one by one, lane = token.
+template <typename T>
+__device__ __forceinline__ void store_v_tile(const RopeArgs& p, unsigned tile, unsigned char* smem) {
   __shared__ int64_t s_dst[kVTile];
-  const int64_t t0 = tile / p.num_kv_heads * kVTile;
-  const int h = (int)(tile % p.num_kv_heads), D = p.head_size, stride = D + PAD;
+  __shared__ uint32_t s_runs;  // bit q: tokens 8q .. 8q + 7 make such a run
+  const unsigned tt = tile / (unsigned)p.num_kv_heads;
+  const int64_t t0 = (int64_t)tt * kVTile;
+  const int h = (int)(tile - tt * (unsigned)p.num_kv_heads), D = p.head_size;
+  const int stride = D + 16 / (int)sizeof(T);
   T* rows = reinterpret_cast<T*>(smem);
   const int ntok = (int)(p.num_tokens - t0 < kVTile ? p.num_tokens - t0 : kVTile);
   if (threadIdx.x < kVTile) {
+    const int lane = threadIdx.x;
     int64_t blk = 0;
     int off = 0;
-    const bool on = (int)threadIdx.x < ntok &&
-                    token_place(p, load_index(p.slots, p.slots_i64, t0 + threadIdx.x), h == 0, &blk, &off);
-    s_dst[threadIdx.x] = on ? blk * p.vc_block + (int64_t)h * p.vc_head + off : -1;
-  }
-  const T* v = reinterpret_cast<const T*>(p.v) + (int64_t)h * p.v_head;
-  const int nvec = D / VEC;
-  for (int i = threadIdx.x; i < ntok * nvec; i += kRopeWarps * 32) {
-    const int t = i / nvec, d = (i - t * nvec) * VEC;
-    Vec<T, VEC> x;
-    x.load(v + (t0 + t) * p.v_tok + d);
-    constexpr int W = VEC * (int)sizeof(T) / 4;
+    const bool on = lane < ntok && token_place(p, load_index(p.slots, p.slots_i64, t0 + lane), h == 0, &blk, &off);
+    const int64_t dst = on ? blk * p.vc_block + (int64_t)h * p.vc_head + off : -1;
+    s_dst[lane] = dst;
+    const int64_t lead = __shfl_sync(0xffffffffu, dst, lane & ~7);
+    const int lead_off = __shfl_sync(0xffffffffu, off, lane & ~7);
+    const bool run = on && lead >= 0 && lead_off % 8 == 0 && off == lead_off + (lane & 7) && dst == lead + (lane & 7);
+    const uint32_t m = __ballot_sync(0xffffffffu, run);
+    uint32_t runs = 0;
 #pragma unroll
-    for (int e = 0; e < W; ++e)
-      reinterpret_cast<uint32_t*>(rows + t * stride + d)[e] = reinterpret_cast<const uint32_t*>(x.e)[e];
+    for (int q = 0; q < 4; ++q) runs |= ((m >> (8 * q)) & 0xffu) == 0xffu ? 1u << q : 0u;
+    if (lane == 0) s_runs = runs;
+  }
+  const T* v = reinterpret_cast<const T*>(p.v) + (int64_t)h * p.v_head + t0 * p.v_tok;
+  const int nq = D / 4;
+  for (int i = threadIdx.x; i < kVTile * nq; i += kRopeWarps * 32) {
+    const int t = i / nq, d = (i - t * nq) * 4;
+    Quad<T> x;
+    x.w = typename Quad<T>::Word{};
+    if (t < ntok) x.load(v + t * p.v_tok + d);
+    x.store(rows + t * stride + d);
   }
   __syncthreads();
   T* vc = reinterpret_cast<T*>(p.v_cache);
-  for (int i = threadIdx.x; i < kVTile * D; i += kRopeWarps * 32) {
-    const int t = i % kVTile, d = i / kVTile;
-    const int64_t dst = s_dst[t];
-    if (dst >= 0) vc[dst + (int64_t)d * p.block_size] = rows[t * stride + d];
+  // (16-byte stores need 16-byte pages: block sizes of 8, 16 and 32 tokens in aligned caches)
+  const bool wide = sizeof(T) == 2 && p.v_wide;
+  const uint32_t runs = wide ? s_runs : 0u;
+  if constexpr (sizeof(T) == 2) {
+    if (runs) {
+      const int lane = threadIdx.x & 31, q = lane & 3;
+      // lane l gives row l % 8 of matrix l / 8: token 8 (row / 2) + 2 matrix + row % 2
+      const int row = lane & 7, tok = 8 * (row >> 1) + 2 * (lane >> 3) + (row & 1);
+      const uint32_t base = static_cast<uint32_t>(__cvta_generic_to_shared(rows + tok * stride));
+      const int64_t dst = s_dst[8 * q];
+      for (int d = (threadIdx.x >> 5) * 8; d < D; d += kRopeWarps * 8) {
+        uint4 x;
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                     : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
+                     : "r"(base + (uint32_t)d * 2u));
+        if ((runs >> q) & 1u) *reinterpret_cast<uint4*>(vc + dst + (int64_t)(d + (lane >> 2)) * p.block_size) = x;
+      }
+    }
+  }
+  if (runs == 0xfu) return;
+  const int t = threadIdx.x % kVTile;
+  const int64_t dst = s_dst[t];
+  if (dst < 0 || ((runs >> (t >> 3)) & 1u)) return;
+  for (int d = threadIdx.x / kVTile; d < D; d += kRopeWarps * 32 / kVTile)
+    vc[dst + (int64_t)d * p.block_size] = rows[t * stride + d];
+}
+
+// A lane holds 8 elements of a row as two quads: in the half layout quads a and
+// a + half of the rotated part, so that its pairs are its own and share four
+// cosines and sines; otherwise 8 neighbours.  The elements past the rotated part
+// are 8 neighbours to a lane in both layouts.
+struct RopeLane {
+  int sub, lpr, rpw;  // row of the warp's group, lanes to a row, rows to a group
+  int da, db;         // first elements of the two quads
+  bool on, rotated;
+};
+
+// A lane's ring of quad pairs in shared memory, filled by its own asynchronous
+// copies and read by itself alone: no barrier, and what is in flight costs no
+// registers (with 16 bytes to a lane and group, 32 warps to an SM and 5 groups
+// ahead, 80 KB to an SM; loads into registers reached 4.1 TB/s at 8192 tokens,
+// the ring 4.9).  Quad e of place i of lane l lies at (i * 2 + e) * 32 + l.
+constexpr int kRopeStages = 6;
+
+template <typename T>
+__device__ __forceinline__ void quad_async(Quad<T>* dst, const T* src) {
+  const uint32_t d = static_cast<uint32_t>(__cvta_generic_to_shared(dst));
+  if constexpr (sizeof(T) == 2) asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(d), "l"(src) : "memory");
+  else asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(src) : "memory");
+}
+__device__ __forceinline__ void quads_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void quads_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// Rows of groups [g0, g1) of one tensor (heads of one token); STAGES > 1: through
+// the ring, STAGES 1: loads into registers.  `oa`, `ob`: where the two quads of a
+// row go.  Arithmetic in pairs: what bounds the kernel next to memory is issue
+// slots (about 60 instructions to a lane's 8 elements; 160 with scalar arithmetic
+// and 64-bit index arithmetic, which ran at 3.2 TB/s).
+template <typename T, bool INTER, int STAGES>
+__device__ __forceinline__ void rope_rows(const RopeLane& ln, Quad<T>* ring, const T* src, int s_head, T* dst, int d_head,
+                                          int oa, int ob, int heads, int g0, int g1, const void* weight, bool w_f32,
+                                          float eps, float inv_d, float4 c, float4 s) {
+  const float2 cc[4] = {INTER ? make_float2(c.x, c.x) : make_float2(c.x, c.y),
+                        INTER ? make_float2(c.y, c.y) : make_float2(c.z, c.w), make_float2(c.z, c.z),
+                        make_float2(c.w, c.w)};
+  const float2 sn[4] = {INTER ? make_float2(-s.x, s.x) : make_float2(s.x, s.y),
+                        INTER ? make_float2(-s.y, s.y) : make_float2(s.z, s.w), make_float2(-s.z, s.z),
+                        make_float2(-s.w, s.w)};
+  float2 wt[4];
+  if (weight && ln.on) {
+    if (w_f32) {
+      const float* w = reinterpret_cast<const float*>(weight);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        wt[i] = make_float2(__ldg(w + ln.da + 2 * i), __ldg(w + ln.da + 2 * i + 1));
+        wt[2 + i] = make_float2(__ldg(w + ln.db + 2 * i), __ldg(w + ln.db + 2 * i + 1));
+      }
+    } else {
+      const T* w = reinterpret_cast<const T*>(weight);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        wt[i] = make_float2(to_float(w[ln.da + 2 * i]), to_float(w[ln.da + 2 * i + 1]));
+        wt[2 + i] = make_float2(to_float(w[ln.db + 2 * i]), to_float(w[ln.db + 2 * i + 1]));
+      }
+    }
+  }
+  int h = g0 * ln.rpw + ln.sub;
+  const int h_end = ln.on ? (g1 * ln.rpw < heads ? g1 * ln.rpw : heads) : 0;
+  const T* row = src + (int64_t)h * s_head;
+  T* out = dst + (int64_t)h * d_head;
+  const int64_t s_step = (int64_t)ln.rpw * s_head, d_step = (int64_t)ln.rpw * d_head;
+  int h_in = h, stage_in = 0, stage = 0;  // (ring) the next row to be asked for, and where it goes
+  auto ask = [&]() {
+    if (h_in < h_end) {
+      quad_async(ring + stage_in * 64, row + ln.da);
+      quad_async(ring + stage_in * 64 + 32, row + ln.db);
+    }
+    quads_commit();
+    row += s_step;
+    h_in += ln.rpw;
+    stage_in = stage_in + 1 == STAGES ? 0 : stage_in + 1;
+  };
+  if constexpr (STAGES > 1) {
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) ask();
+  }
+  for (int g = g0; g < g1; ++g) {
+    Quad<T> a, b;
+    a.w = b.w = typename Quad<T>::Word{};
+    if constexpr (STAGES > 1) {
+      ask();
+      quads_wait<STAGES - 1>();
+      if (h < h_end) {
+        a = ring[stage * 64];
+        b = ring[stage * 64 + 32];
+      }
+      stage = stage + 1 == STAGES ? 0 : stage + 1;
+    } else {
+      if (h < h_end) {
+        a.load(row + ln.da);
+        b.load(row + ln.db);
+      }
+      row += s_step;
+    }
+    float2 y[4];
+    a.get(y[0], y[1]);
+    b.get(y[2], y[3]);
+    if (weight) {
+      float2 q = mul2(y[0], y[0]);
+#pragma unroll
+      for (int i = 1; i < 4; ++i) q = fma2(y[i], y[i], q);
+      float ss = q.x + q.y;
+      for (int o = 1; o < ln.lpr; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      const float inv = rsqrtf(fmaf(ss, inv_d, eps));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i] = mul2(y[i], mul2(make_float2(inv, inv), wt[i]));
+    }
+    if (ln.rotated) {
+      if constexpr (INTER) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = fma2(make_float2(y[i].y, y[i].x), sn[i], mul2(y[i], cc[i]));
+      } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float2 va = y[i], vb = y[2 + i];
+          y[i] = fma2(vb, make_float2(-sn[i].x, -sn[i].y), mul2(va, cc[i]));
+          y[2 + i] = fma2(va, sn[i], mul2(vb, cc[i]));
+        }
+      }
+    }
+    if (h < h_end) {
+      a.put(y[0], y[1]);
+      b.put(y[2], y[3]);
+      a.store(out + oa);
+      b.store(out + ob);
+    }
+    out += d_step;
+    h += ln.rpw;
   }
 }
 
-template <typename T, int VEC, bool INTER, int U>
+template <typename T, bool INTER, int STAGES>
 __global__ void __launch_bounds__(kRopeWarps * 32) qk_norm_rope_kernel(const RopeArgs p, const RopePlan pl) {
   extern __shared__ __align__(16) unsigned char smem_rope[];
+  wait_for_prior();
   if (blockIdx.x >= pl.row_ctas) {
-    store_v_tile<T, VEC>(p, blockIdx.x - pl.row_ctas, smem_rope);
+    store_v_tile<T>(p, blockIdx.x - pl.row_ctas, smem_rope);
     return;
   }
   const int lane = threadIdx.x & 31;
   const unsigned w = blockIdx.x * kRopeWarps + (threadIdx.x >> 5);
-  const unsigned per = (unsigned)(pl.q_chunks + pl.k_chunks + pl.v_chunks);
-  const unsigned tok = w / per;
+  const unsigned tok = w / pl.warps_per_token;
   if (tok >= p.num_tokens) return;
-  int chunk = (int)(w - tok * per);
-  const int kind = chunk < pl.q_chunks ? 0 : (chunk < pl.q_chunks + pl.k_chunks ? 1 : 2);
-  if (kind > 0) chunk -= pl.q_chunks;
-  if (kind > 1) chunk -= pl.k_chunks;
-  const bool to_cache = kind > 0 && p.k_cache != nullptr;
+  const int all = pl.q_groups + pl.k_groups + pl.v_groups;
+  const int g0 = (int)(w - tok * pl.warps_per_token) * pl.span, g1 = g0 + pl.span < all ? g0 + pl.span : all;
+
+  const int half = p.rot >> 1;
+  RopeLane ln;
+  ln.lpr = 1 << pl.lpr_shift;
+  ln.rpw = 32 >> pl.lpr_shift;
+  ln.sub = lane >> pl.lpr_shift;
+  const int li = lane & (ln.lpr - 1);
+  ln.on = li * 8 < p.head_size;
+  ln.rotated = li * 8 < p.rot;
+  ln.da = !INTER && ln.rotated ? 4 * li : 8 * li;
+  ln.db = !INTER && ln.rotated ? ln.da + half : ln.da + 4;
   const int64_t pos = load_index(p.positions, p.pos_i64, tok);
-  const int64_t slot = to_cache ? load_index(p.slots, p.slots_i64, tok) : 0;
-
-  const int lpr = 1 << pl.lpr_shift, rpw = 32 >> pl.lpr_shift;
-  const int sub = lane >> pl.lpr_shift, li = lane & (lpr - 1);
-  const int D = p.head_size, d0 = li * VEC, half = p.rot >> 1;
-  const int heads = kind ? p.num_kv_heads : p.num_heads;
-  const int h0 = chunk * rpw * U + sub;
-  const bool on = d0 < D;
-  const T* src = reinterpret_cast<const T*>(kind == 0 ? p.q : (kind == 1 ? p.k : p.v));
-  const int64_t s_tok = kind == 0 ? p.q_tok : (kind == 1 ? p.k_tok : p.v_tok);
-  const int64_t s_head = kind == 0 ? p.q_head : (kind == 1 ? p.k_head : p.v_head);
-  src += (int64_t)tok * s_tok + d0;
-
-  // every load of the warp's rows before any is used
-  Vec<T, VEC> x[U];
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int h = h0 + u * rpw;
-    if (on && h < heads) x[u].load(src + (int64_t)h * s_head);
-    else
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) x[u].e[e] = from_float<T>(0.f);
-  }
   int64_t blk = 0;
   int off = 0;
-  if (to_cache && !token_place(p, slot, chunk == 0 && kind == 1 && lane == 0, &blk, &off)) return;
+  bool place = false;  // the token has a cache place
+  if (p.k_cache != nullptr && g1 > pl.q_groups)
+    place = token_place(p, load_index(p.slots, p.slots_i64, tok), lane == 0, &blk, &off);
+  const bool pos_ok = pos >= 0 && pos < p.table_rows;
+  if (pos >= p.table_rows && lane == 0) set_status(&g_layer_ops_status, KVC_STATUS_INDEX_OOB);
+  float4 c = make_float4(1.f, 1.f, 1.f, 1.f), s = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (ln.rotated && pos_ok) {
+    const float* cs = p.table + pos * p.table_stride + 4 * li;
+    c = __ldg(reinterpret_cast<const float4*>(cs));
+    s = __ldg(reinterpret_cast<const float4*>(cs + half));
+  }
+  const bool w_f32 = p.weight_type == ElemType::F32;
+  Quad<T>* ring = reinterpret_cast<Quad<T>*>(smem_rope) + (threadIdx.x >> 5) * (STAGES * 64) + lane;
 
-  if (kind == 2) {
-    T* vc = reinterpret_cast<T*>(p.v_cache) + blk * p.vc_block;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int h = h0 + u * rpw;
-      if (!on || h >= heads) continue;
-      T* dst = vc + (int64_t)h * p.vc_head;
+  if (g0 < pl.q_groups && pos_ok)
+    rope_rows<T, INTER, STAGES>(ln, ring, reinterpret_cast<const T*>(p.q) + (int64_t)tok * p.q_tok, (int)p.q_head,
+                           reinterpret_cast<T*>(p.q_out) + (int64_t)tok * p.qo_tok, (int)p.qo_head, ln.da, ln.db,
+                           p.num_heads, g0, g1 < pl.q_groups ? g1 : pl.q_groups, p.q_weight, w_f32, p.eps, pl.inv_d, c,
+                           s);
+  const int k0 = g0 > pl.q_groups ? g0 - pl.q_groups : 0;
+  int k1 = g1 - pl.q_groups;
+  k1 = k1 < pl.k_groups ? k1 : pl.k_groups;
+  if (k0 < k1 && pos_ok && (place || p.k_cache == nullptr)) {
+    T* dst;
+    int d_head, oa = ln.da, ob = ln.db;
+    if (p.k_cache == nullptr) {
+      dst = reinterpret_cast<T*>(p.k_out) + (int64_t)tok * p.ko_tok;
+      d_head = (int)p.ko_head;
+    } else {
+      dst = reinterpret_cast<T*>(p.k_cache) + blk * p.kc_block;
+      d_head = (int)p.kc_head;
+      if (p.paged) {  // 16-byte places [d / X][offset] of the page
+        constexpr int X = 16 / (int)sizeof(T);
+        oa = (oa / X * p.block_size + off) * X + oa % X;
+        ob = (ob / X * p.block_size + off) * X + ob % X;
+      } else {
+        dst += (int64_t)off * p.kc_tok;
+      }
+    }
+    rope_rows<T, INTER, STAGES>(ln, ring, reinterpret_cast<const T*>(p.k) + (int64_t)tok * p.k_tok, (int)p.k_head, dst, d_head, oa,
+                           ob, p.num_kv_heads, k0, k1, p.k_weight, w_f32, p.eps, pl.inv_d, c, s);
+  }
+  const int vg = pl.q_groups + pl.k_groups;
+  if (g1 > vg && place) {  // values: as they are
+    const T* src = reinterpret_cast<const T*>(p.v) + (int64_t)tok * p.v_tok;
+    T* dst = reinterpret_cast<T*>(p.v_cache) + blk * p.vc_block + (p.paged ? (int64_t)off : (int64_t)off * p.vc_tok);
+    const int d = 8 * li;
+    for (int g = g0 > vg ? g0 - vg : 0; g < g1 - vg; ++g) {
+      const int h = g * ln.rpw + ln.sub;
+      if (!ln.on || h >= p.num_kv_heads) continue;
+      Quad<T> a, b;
+      a.load(src + h * p.v_head + d);
+      b.load(src + h * p.v_head + d + 4);
+      T* o = dst + h * p.vc_head;
       if (p.paged) {
+        const T* ea = reinterpret_cast<const T*>(&a.w);
+        const T* eb = reinterpret_cast<const T*>(&b.w);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) dst[(int64_t)(d0 + e) * p.block_size + off] = x[u].e[e];
+        for (int e = 0; e < 4; ++e) {
+          o[(d + e) * p.block_size] = ea[e];
+          o[(d + 4 + e) * p.block_size] = eb[e];
+        }
       } else {
-        x[u].store(dst + (int64_t)off * p.vc_tok + d0);
+        a.store(o + d);
+        b.store(o + d + 4);
       }
-    }
-    return;
-  }
-  if (pos < 0 || pos >= p.table_rows) {  // (the whole warp: one token)
-    if (pos >= 0 && lane == 0) set_status(&g_layer_ops_status, KVC_STATUS_INDEX_OOB);
-    return;
-  }
-
-  // this lane's cosines and sines (in the half layout an element's own, so that
-  // the pair is formed by one exchange with the lane that holds the other half)
-  constexpr int NC = INTER ? VEC / 2 : VEC;
-  float c[NC], s[NC];
-  const bool rotated = on && d0 < p.rot;
-  const bool upper = !INTER && d0 >= half;
-  const float* cs = p.table + pos * p.table_stride + (INTER ? d0 / 2 : (upper ? d0 - half : d0));
-#pragma unroll
-  for (int i = 0; i < NC; i += 2) {
-    const float2 a = rotated ? __ldg(reinterpret_cast<const float2*>(cs + i)) : make_float2(1.f, 1.f);
-    const float2 b = rotated ? __ldg(reinterpret_cast<const float2*>(cs + half + i)) : make_float2(0.f, 0.f);
-    c[i] = a.x;
-    c[i + 1] = a.y;
-    s[i] = upper ? b.x : (INTER ? b.x : -b.x);
-    s[i + 1] = upper ? b.y : (INTER ? b.y : -b.y);
-  }
-  const void* wp = kind ? p.k_weight : p.q_weight;
-  float wt[VEC];
-#pragma unroll
-  for (int e = 0; e < VEC; ++e) wt[e] = 1.f;
-  if (wp && on) {
-    if (p.weight_type == ElemType::F32) {
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) wt[e] = __ldg(reinterpret_cast<const float*>(wp) + d0 + e);
-    } else {
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) wt[e] = to_float(reinterpret_cast<const T*>(wp)[d0 + e]);
-    }
-  }
-  // the lane that holds the other element of each pair (half layout)
-  const int mate = rotated ? (upper ? lane - half / VEC : lane + half / VEC) : lane;
-  T* dst = reinterpret_cast<T*>(kind == 0 ? p.q_out : p.k_out);
-  const int64_t o_head = kind == 0 ? p.qo_head : p.ko_head;
-  if (to_cache) dst = reinterpret_cast<T*>(p.k_cache) + blk * p.kc_block;
-  else dst += (int64_t)tok * (kind == 0 ? p.qo_tok : p.ko_tok) + d0;
-  constexpr int X = 16 / (int)sizeof(T);
-
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int h = h0 + u * rpw;
-    float y[VEC];
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) y[e] = to_float(x[u].e[e]);
-    if (wp) {
-      float ss = 0.f;
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) ss = fmaf(y[e], y[e], ss);
-      for (int o = 1; o < lpr; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      const float inv = rsqrtf(ss / (float)D + p.eps);
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) y[e] *= inv * wt[e];
-    }
-    Vec<T, VEC> out;
-    if constexpr (INTER) {
-#pragma unroll
-      for (int i = 0; i < VEC / 2; ++i) {
-        const float a = y[2 * i], b = y[2 * i + 1];
-        out.e[2 * i] = from_float<T>(rotated ? a * c[i] - b * s[i] : a);
-        out.e[2 * i + 1] = from_float<T>(rotated ? fmaf(b, c[i], a * s[i]) : b);
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const float m = __shfl_sync(0xffffffffu, y[e], mate);
-        out.e[e] = from_float<T>(rotated ? fmaf(m, s[e], y[e] * c[e]) : y[e]);
-      }
-    }
-    if (!on || h >= heads) continue;
-    if (!to_cache) {
-      out.store(dst + (int64_t)h * o_head);
-    } else if (p.paged) {  // 16-byte places [d / X][offset] of the page
-      T* page = dst + (int64_t)h * p.kc_head;
-      if constexpr (VEC >= X) {
-#pragma unroll
-        for (int i = 0; i < VEC / X; ++i)
-          *reinterpret_cast<uint4*>(page + ((int64_t)(d0 / X + i) * p.block_size + off) * X) =
-              reinterpret_cast<const uint4*>(out.e)[i];
-      } else {
-        out.store(page + ((int64_t)(d0 / X) * p.block_size + off) * X + d0 % X);
-      }
-    } else {
-      out.store(dst + (int64_t)off * p.kc_tok + (int64_t)h * p.kc_head + d0);
     }
   }
 }
@@ -553,6 +736,7 @@ constexpr int kRopeMaxHead = 512;
 template <typename T, typename C>
 __global__ void __launch_bounds__(kRopeWarps * 32) qk_norm_rope_any_kernel(const RopeArgs p) {
   __shared__ float row_s[kRopeWarps][kRopeMaxHead];
+  wait_for_prior();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const unsigned per = (unsigned)(p.num_heads + p.num_kv_heads * (p.k_cache ? 2 : 1));
   const unsigned w = blockIdx.x * kRopeWarps + warp, tok = w / per;
@@ -627,58 +811,69 @@ template <typename T, typename C>
 static cudaError_t launch_rope_any(const RopeArgs& a, cudaStream_t stream) {
   const int64_t rows = a.num_tokens * (a.num_heads + (int64_t)a.num_kv_heads * (a.k_cache ? 2 : 1));
   if (a.head_size > kRopeMaxHead || rows > 0x7fffffffll) return cudaErrorInvalidValue;
-  qk_norm_rope_any_kernel<T, C><<<(unsigned)((rows + kRopeWarps - 1) / kRopeWarps), kRopeWarps * 32, 0, stream>>>(a);
-  count_launch();
-  return cudaGetLastError();
+  return launch_dependent(qk_norm_rope_any_kernel<T, C>, dim3((unsigned)((rows + kRopeWarps - 1) / kRopeWarps)),
+                          kRopeWarps * 32, 0, stream, a);
 }
 
-template <typename T, int VEC, bool INTER, int U>
-static cudaError_t launch_rope_u(const RopeArgs& a, RopePlan pl, bool v_tiles, cudaStream_t stream) {
+template <typename T, bool INTER, int STAGES>
+static cudaError_t launch_rope_u(const RopeArgs& a, RopePlan pl, bool v_tiles, int span, cudaStream_t stream) {
   const int rpw = 32 >> pl.lpr_shift;
-  pl.q_chunks = (a.num_heads + rpw * U - 1) / (rpw * U);
-  pl.k_chunks = (a.num_kv_heads + rpw * U - 1) / (rpw * U);
-  pl.v_chunks = a.k_cache && !v_tiles ? pl.k_chunks : 0;
-  const int64_t warps = a.num_tokens * (pl.q_chunks + pl.k_chunks + pl.v_chunks);
+  pl.q_groups = (a.num_heads + rpw - 1) / rpw;
+  pl.k_groups = (a.num_kv_heads + rpw - 1) / rpw;
+  pl.v_groups = a.k_cache && !v_tiles ? pl.k_groups : 0;
+  const int all = pl.q_groups + pl.k_groups + pl.v_groups;
+  pl.span = span;
+  pl.warps_per_token = (unsigned)((all + pl.span - 1) / pl.span);
+  const int64_t warps = a.num_tokens * pl.warps_per_token;
   const int64_t tiles = v_tiles ? (a.num_tokens + kVTile - 1) / kVTile * a.num_kv_heads : 0;
   const int64_t ctas = (warps + kRopeWarps - 1) / kRopeWarps;
   if (ctas + tiles > 0x7fffffffll / kRopeWarps) return cudaErrorInvalidValue;
   pl.row_ctas = (unsigned)ctas;
-  const size_t smem = v_tiles ? (size_t)kVTile * (a.head_size + (sizeof(T) == 2 ? 2 : 1)) * sizeof(T) : 0;
-  qk_norm_rope_kernel<T, VEC, INTER, U><<<(unsigned)(ctas + tiles), kRopeWarps * 32, smem, stream>>>(a, pl);
-  count_launch();
-  return cudaGetLastError();
+  size_t smem = STAGES > 1 ? (size_t)kRopeWarps * STAGES * 64 * sizeof(Quad<T>) : 0;
+  const size_t tile = v_tiles ? (size_t)kVTile * (a.head_size * sizeof(T) + 16) : 0;
+  if (tile > smem) smem = tile;
+  return launch_dependent(qk_norm_rope_kernel<T, INTER, STAGES>, dim3((unsigned)(ctas + tiles)), kRopeWarps * 32, smem,
+                          stream, a, pl);
 }
 
-template <typename T, int VEC>
-static cudaError_t launch_rope_vec(const RopeArgs& a, cudaStream_t stream) {
+template <typename T>
+static cudaError_t launch_rope_vec(RopeArgs a, cudaStream_t stream) {
   RopePlan pl = {};
-  while ((VEC << pl.lpr_shift) < a.head_size) ++pl.lpr_shift;
+  while ((8 << pl.lpr_shift) < a.head_size) ++pl.lpr_shift;
+  pl.inv_d = 1.f / (float)a.head_size;
+  // Many tokens: a token's rows to one warp, kRopeStages of its groups in flight
+  // through the lanes' rings; else one group to a warp.  bf16, 32 + 8 heads of
+  // 128 (20 groups to a token), one group / rings: 512 tokens 8.3 / 12.4 us, 1024
+  // 12.4 / 12.4, 2048 24.5 / 16.4, 6000 61.5 / 32.8.  Without enough tokens the
+  // rings leave SMs with too few warps, with few groups a ring hardly fills.
   const int rpw = 32 >> pl.lpr_shift;
-  const int64_t rows = a.num_tokens * (a.num_heads + (int64_t)a.num_kv_heads * (a.k_cache ? 2 : 1));
-  // four passes to a warp once that still fills the GPU (16 warps to an SM)
-  const bool four = rows >= (int64_t)sm_count() * 16 * 4 * rpw;
+  const int64_t groups = a.num_tokens * ((a.num_heads + rpw - 1) / rpw + (a.num_kv_heads + rpw - 1) / rpw);
+  const bool whole = a.num_tokens >= 7 * (int64_t)sm_count() && groups >= 128 * (int64_t)sm_count();
   const bool v_tiles = a.k_cache && a.paged && a.num_tokens >= 1024;
+  a.v_wide = a.block_size % 8 == 0 && reinterpret_cast<uintptr_t>(a.v_cache) % 16 == 0 && a.vc_block % 8 == 0 &&
+             a.vc_head % 8 == 0;
   if (a.interleaved)
-    return four ? launch_rope_u<T, VEC, true, 4>(a, pl, v_tiles, stream)
-                : launch_rope_u<T, VEC, true, 1>(a, pl, v_tiles, stream);
-  return four ? launch_rope_u<T, VEC, false, 4>(a, pl, v_tiles, stream)
-              : launch_rope_u<T, VEC, false, 1>(a, pl, v_tiles, stream);
+    return whole ? launch_rope_u<T, true, kRopeStages>(a, pl, v_tiles, 1 << 20, stream)
+                 : launch_rope_u<T, true, 1>(a, pl, v_tiles, 1, stream);
+  return whole ? launch_rope_u<T, false, kRopeStages>(a, pl, v_tiles, 1 << 20, stream)
+               : launch_rope_u<T, false, 1>(a, pl, v_tiles, 1, stream);
 }
 
-// Whether every row the launch touches can be moved VEC elements at a time.
-static bool rope_vec_ok(const RopeArgs& a, int vec, int es) {
-  const int D = a.head_size;
-  const int64_t align = vec * es < 16 ? vec * es : 16;
-  // the rotated part is whole vectors, and so is each half of it in the half layout
-  if (D % vec || D > 32 * vec || a.rot % (a.interleaved ? vec : 2 * vec) || a.type != a.cache_type) return false;
+// Whether every row the launch touches is whole quads of 8 (16-bit) or 16 bytes.
+static bool rope_vec_ok(const RopeArgs& a, int es) {
+  const int64_t align = 4 * es;
+  if (a.head_size % 8 || a.head_size > 256 || a.rot % 8 || a.type != a.cache_type) return false;
+  // (head strides are 32-bit in the kernel)
+  for (int64_t s : {a.q_head, a.k_head, a.v_head, a.qo_head, a.ko_head, a.kc_head, a.vc_head})
+    if (s > 0x7fffffffll || s < -0x7fffffffll) return false;
   auto rows = [&](const void* base, int64_t s1, int64_t s2, int64_t s3) {
     return reinterpret_cast<uintptr_t>(base) % align == 0 && (s1 * es) % align == 0 && (s2 * es) % align == 0 &&
            (s3 * es) % align == 0;
   };
   if (!rows(a.q, a.q_tok, a.q_head, 0) || !rows(a.k, a.k_tok, a.k_head, 0) || !rows(a.q_out, a.qo_tok, a.qo_head, 0))
     return false;
-  if ((reinterpret_cast<uintptr_t>(a.table) & 7u) || (a.table_stride & 1)) return false;  // (float2 loads)
-  if ((a.rot >> 1) & 1) return false;
+  // the table's rows as four floats at a time (half a multiple of 4)
+  if ((reinterpret_cast<uintptr_t>(a.table) & 15u) || (a.table_stride & 3)) return false;
   if (!a.k_cache) return rows(a.k_out, a.ko_tok, a.ko_head, 0);
   return rows(a.v, a.v_tok, a.v_head, 0) && rows(a.k_cache, a.kc_block, a.kc_head, a.kc_tok) &&
          (a.paged || rows(a.v_cache, a.vc_block, a.vc_head, a.vc_tok));
@@ -686,9 +881,7 @@ static bool rope_vec_ok(const RopeArgs& a, int vec, int es) {
 
 template <typename T>
 static cudaError_t launch_rope_t(const RopeArgs& a, cudaStream_t stream) {
-  if (rope_vec_ok(a, 8, sizeof(T))) return launch_rope_vec<T, 8>(a, stream);
-  if (rope_vec_ok(a, 4, sizeof(T))) return launch_rope_vec<T, 4>(a, stream);
-  return launch_rope_any<T, T>(a, stream);
+  return rope_vec_ok(a, sizeof(T)) ? launch_rope_vec<T>(a, stream) : launch_rope_any<T, T>(a, stream);
 }
 
 cudaError_t launch_qk_norm_rope(const RopeArgs& a, cudaStream_t stream) {
