@@ -204,18 +204,17 @@ __global__ void __launch_bounds__(kTablesThreads) step_tables_kernel(StepTablesA
   const uint64_t threads = (uint64_t)gridDim.x * kTablesThreads;
   const uint64_t me = (uint64_t)blockIdx.x * kTablesThreads + tid;
 
-  // new blocks: free list -> table rows
-  for (uint64_t k = me; k < nblk; k += threads) {
-    const int i = find_request(blk_off, n, (uint32_t)k);
+  // new blocks: free list -> table rows (the first one's id is on its way while
+  // the tokens are done)
+  auto free_id = [&](uint64_t k) {
     const uint64_t f = base_blk + k;
-    const int64_t col = ((int64_t)first_tok[i] + bs - 1) / bs + (int64_t)((uint32_t)k - blk_off[i]);
-    const bool have = f < (uint64_t)p.num_free;
-    bad |= !have || col >= p.table_len;
-    if (col < p.table_len) p.tables[(int64_t)(b0 + i) * p.table_stride + col] = have ? p.free_blocks[f] : -1;
-  }
+    return f < (uint64_t)p.num_free ? p.free_blocks[f] : -1;
+  };
+  int32_t next_id = me < nblk ? free_id(me) : -1;
 
-  // new tokens, four consecutive rows to a thread; the last chunk also fills the
-  // rows past the batch (capacity of a captured step) with -1
+  // new tokens, four consecutive rows to a thread, the block ids of all four read
+  // before one is used; the last chunk also fills the rows past the batch (capacity
+  // of a captured step) with -1
   const int64_t row0 = (int64_t)(base_tok < (uint64_t)p.num_tokens ? base_tok : (uint64_t)p.num_tokens);
   int64_t row1 = last_chunk ? p.num_tokens : row0 + (int64_t)ntok;
   if (row1 > p.num_tokens) row1 = p.num_tokens;
@@ -223,42 +222,40 @@ __global__ void __launch_bounds__(kTablesThreads) step_tables_kernel(StepTablesA
   for (int64_t g = row0 / 4 + (int64_t)me; g * 4 < row1; g += (int64_t)threads) {
     int32_t pos[4];
     int64_t slot[4];
+    uint32_t in_blk[4];
+    const int32_t* id_at[4];  // (nullptr: no block)
     int i = -1;
-    int64_t id = -1;      // block of the token before, to be carried on inside it
-    uint32_t in_blk = 0;  // its place in that block
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int64_t r = g * 4 + e;
       pos[e] = -1;
       slot[e] = -1;
+      in_blk[e] = 0u;
+      id_at[e] = nullptr;
       if (r < row0 || r - row0 >= (int64_t)ntok) continue;
       const uint32_t x = (uint32_t)(r - row0);
-      const bool same = i >= 0 && x < tok_off[i + 1];
-      if (!same) i = find_request(tok_off, n, x);
+      if (i < 0 || x >= tok_off[i + 1]) i = find_request(tok_off, n, x);
       const int32_t t = first_tok[i] + (int32_t)(x - tok_off[i]);
+      const uint32_t col = (uint32_t)t / bs, had = ((uint32_t)first_tok[i] + bs - 1) / bs;
       pos[e] = t;
-      if (same && in_blk + 1 < bs) {
-        ++in_blk;
-      } else {
-        const uint32_t col = (uint32_t)t / bs, had = ((uint32_t)first_tok[i] + bs - 1) / bs;
-        in_blk = (uint32_t)t - col * bs;
-        const uint64_t f = base_blk + blk_off[i] + (col - had);
-        id = -1;
-        if ((int64_t)col < p.table_len) {
-          if (col < had) id = p.tables[(int64_t)(b0 + i) * p.table_stride + col];
-          else if (f < (uint64_t)p.num_free) id = p.free_blocks[f];
-        }
+      in_blk[e] = (uint32_t)t - col * bs;
+      const uint64_t f = base_blk + blk_off[i] + (col - had);
+      if ((int64_t)col < p.table_len) {
+        if (col < had) id_at[e] = p.tables + (int64_t)(b0 + i) * p.table_stride + col;
+        else if (f < (uint64_t)p.num_free) id_at[e] = p.free_blocks + f;
       }
-      if (id >= 0) slot[e] = id * (int64_t)bs + in_blk;
-      bad |= id < 0;
     }
-    if (!p.slots_i64) {
+    int32_t id[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (slot[e] > 0x7fffffffll) {
-          slot[e] = -1;
-          bad = true;
-        }
+    for (int e = 0; e < 4; ++e) id[e] = id_at[e] ? *id_at[e] : -1;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (id[e] >= 0) slot[e] = (int64_t)id[e] * (int64_t)bs + in_blk[e];
+      bad |= pos[e] >= 0 && id[e] < 0;
+      if (!p.slots_i64 && slot[e] > 0x7fffffffll) {
+        slot[e] = -1;
+        bad = true;
+      }
     }
     if (vec && g * 4 >= row0 && g * 4 + 4 <= row1) {
       reinterpret_cast<int4*>(p.positions)[g] = make_int4(pos[0], pos[1], pos[2], pos[3]);
@@ -279,14 +276,23 @@ __global__ void __launch_bounds__(kTablesThreads) step_tables_kernel(StepTablesA
       }
     }
   }
+
+  for (uint64_t k = me; k < nblk; k += threads) {
+    const int i = find_request(blk_off, n, (uint32_t)k);
+    const int64_t col = ((int64_t)first_tok[i] + bs - 1) / bs + (int64_t)((uint32_t)k - blk_off[i]);
+    bad |= base_blk + k >= (uint64_t)p.num_free || col >= p.table_len;
+    if (col < p.table_len) p.tables[(int64_t)(b0 + i) * p.table_stride + col] = next_id;
+    if (k + threads < nblk) next_id = free_id(k + threads);
+  }
   if (bad) set_status(&g_layer_ops_status, KVC_STATUS_INDEX_OOB);
 }
 
 cudaError_t launch_step_tables(const StepTablesArgs& a, cudaStream_t stream) {
   const int64_t chunks = a.num_seqs > 0 ? ((int64_t)a.num_seqs + kTablesChunk - 1) / kTablesChunk : 1;
   if (chunks > 65535) return cudaErrorInvalidValue;
-  // a thread's four rows at a time, up to two CTAs to an SM
-  int64_t slices = (a.num_tokens + 4 * kTablesThreads - 1) / (4 * kTablesThreads);
+  // four rows to every fourth thread (the latency of a CTA's scan hides better
+  // behind more CTAs than behind fuller ones), up to two CTAs to an SM
+  int64_t slices = (a.num_tokens + kTablesThreads - 1) / kTablesThreads;
   const int64_t most = 2 * (int64_t)sm_count() / chunks;
   if (slices > most) slices = most;
   if (slices < 1) slices = 1;
