@@ -212,6 +212,27 @@ static cudaError_t launch_prefill_mma_any(const PrefillArgs& a, cudaStream_t str
   return cudaErrorNotSupported;
 }
 
+// K viewed as rows of one 8-dim chunk of one page of one head: [nb * H * D/8][BS * 8]
+// (needs the dense paged layout).
+static bool make_k_gather_map(const PrefillArgs& a, int D, int BS, CUtensorMap* map) {
+  auto enc = tensor_map_encoder();
+  if (!enc) return false;
+  const cuuint64_t dims[2] = {(cuuint64_t)BS * 8, (cuuint64_t)a.num_blocks * a.num_kv_heads * (D / 8)};
+  const cuuint64_t strides[1] = {(cuuint64_t)BS * 16};
+  const cuuint32_t box[2] = {(cuuint32_t)BS * 8, 1};
+  const cuuint32_t ones[2] = {1, 1};
+  return enc(map, a.q_type == ElemType::BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+             const_cast<void*>(a.k_cache), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) ==
+         CUDA_SUCCESS;
+}
+
+// KVC_PREFILL_ISSUE=single: the producer's lane 0 issues every copy (tuning runs).
+static int umma_single_issue() {
+  const char* v = getenv("KVC_PREFILL_ISSUE");
+  return v && v[0] == 's' ? 1 : 0;
+}
+
 template <typename T, int D, int BS, bool GK>
 static cudaError_t launch_prefill_umma(const PrefillArgs& a, cudaStream_t stream) {
   using UG = UmmaGeom<D, BS>;

@@ -104,7 +104,7 @@ __global__ void __launch_bounds__((kPrefillConsumers + 1) * 32) prefill_kernel(P
   const int prefix = bad ? 0 : (int)(kvl - ql);
   const int64_t R_last = (R0 + kPrefillRows < rows ? R0 + kPrefillRows : rows) - 1;
   const int t_first = (int)(R0 / G), t_last = (int)(R_last / G);
-  Seen seen;
+  Seen seen = {};
   if constexpr (WINDOW)
     seen = seen_range(prefix + t_first, prefix + t_last, p.window, p.sinks, FLASH ? p.block_size : BS);
   const int jump = WINDOW ? seen.jump : 0;

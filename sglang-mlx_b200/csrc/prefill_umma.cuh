@@ -64,6 +64,12 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
       "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
       "r"(a), "l"(b), "r"(idesc), "r"(accumulate));
 }
+// D[tmem] (+)= A[smem descriptor] * B[smem descriptor]
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
+}
 __device__ __forceinline__ void commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(mma_detail::smem_u32(bar))
                : "memory");
@@ -175,6 +181,7 @@ struct UmmaItem {
   bool bad, skip, first_tile;
 };
 
+// WINDOW: the sliding-window extend (window_umma.cuh).
 template <bool CASCADE, bool WINDOW = false>
 __device__ __forceinline__ UmmaItem umma_item(const PrefillArgs& p, int idx, int tiles_x, int ny) {
   constexpr int KT = kUmmaTile;
@@ -237,12 +244,7 @@ __device__ __forceinline__ UmmaItem umma_item(const PrefillArgs& p, int idx, int
 // tiles_x x ny x num_kv_heads items) until none is left, keeping TMEM, its
 // barriers and its ring across them (every barrier phase below counts this
 // CTA's tiles or items).
-// WINDOW: prefill / extend under a sliding window whose first p.sinks tokens stay
-// visible.  An item's keys are its sink blocks and its window's blocks, numbered
-// without the gap (struct Seen): the tiles are filled page by page, so the few
-// sink tokens share a tile with the window's first pages, and a tile starts at
-// the window's first block, not at a multiple of 128 tokens.
-template <typename T, int D, int BS, bool GK, bool CASCADE = false, bool WINDOW = false>
+template <typename T, int D, int BS, bool GK, bool CASCADE = false>
 __global__ void __launch_bounds__(kUmmaThreads, 1)
     prefill_umma_kernel(const PrefillArgs p, const __grid_constant__ TmaMaps maps, int tiles_x, int ny, int slot) {
   using namespace mma_detail;
@@ -296,10 +298,10 @@ __global__ void __launch_bounds__(kUmmaThreads, 1)
       asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&maps.v)) : "memory");
       if (GK) asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&maps.k)) : "memory");
     }
-    it0 = umma_item<CASCADE, WINDOW>(p, blockIdx.x, tiles_x, ny);
+    it0 = umma_item<CASCADE>(p, blockIdx.x, tiles_x, ny);
     const uint32_t* t0row = p.block_tables + (CASCADE ? (int64_t)0 : (int64_t)it0.y * p.table_stride);
     if (!it0.skip && lane < PAGES && it0.ntiles > 0 && it0.kv_beg + lane * BS < it0.kv_end)
-      first_id = __ldg(t0row + (WINDOW ? it0.seen.real_block(lane) : (it0.kv_beg + lane * BS) / BS));
+      first_id = __ldg(t0row + (it0.kv_beg + lane * BS) / BS);
   }
 
   if (threadIdx.x == 0) {
@@ -367,7 +369,7 @@ __global__ void __launch_bounds__(kUmmaThreads, 1)
     UmmaSched* sched = &g_umma_sched[slot];
     for (int idx = blockIdx.x; idx < n_items && !stop;) {
       const bool first = idx == (int)blockIdx.x;  // (claimed items are all past the grid)
-      const UmmaItem it = first ? it0 : umma_item<CASCADE, WINDOW>(p, idx, tiles_x, ny);
+      const UmmaItem it = first ? it0 : umma_item<CASCADE>(p, idx, tiles_x, ny);
       if (!CASCADE && it.bad && it.first_tile && it.kvh == 0 && lane == 0)
         set_status(&g_decode_status, KVC_STATUS_INDEX_OOB);
       // the next item is claimed once this one's loads are issued
@@ -406,8 +408,7 @@ __global__ void __launch_bounds__(kUmmaThreads, 1)
       auto load_id = [&](int j) -> uint32_t {
         uint32_t id = 0xffffffffu;
         const int tok = kv_beg + j * KT + lane * BS;
-        if (lane < PAGES && j < ntiles && tok < kv_end)
-          id = __ldg(table + (WINDOW ? it.seen.real_block(tok / BS) : tok / BS));
+        if (lane < PAGES && j < ntiles && tok < kv_end) id = __ldg(table + tok / BS);
         return id;
       };
       uint32_t id = first ? first_id : load_id(0);
@@ -555,7 +556,7 @@ __global__ void __launch_bounds__(kUmmaThreads, 1)
         mbar_arrive(&item_empty[sl]);
         ++nread;
         if (idx >= n_items) break;
-        const UmmaItem it = umma_item<CASCADE, WINDOW>(p, idx, tiles_x, ny);
+        const UmmaItem it = umma_item<CASCADE>(p, idx, tiles_x, ny);
         if (it.skip || it.ntiles == 0) continue;  // (no Q is handed over for an item without keys)
         if (abort_now() || !umma::wait(q_ready, (uint32_t)(nit & 1))) {
           ok = false;
@@ -674,7 +675,6 @@ __global__ void __launch_bounds__(kUmmaThreads, 1)
     struct RowItem {
       int64_t q0;
       int y, kvh, kv_beg, kv_end, ntiles;
-      int v_beg;               // window form: the item's first window position (virtual)
       int t, g, end_r, beg_r;  // t: the new token (prefill) or the sequence (cascade) of the row
       bool in_tile;            // a row (else padding of the last tile)
     };
@@ -696,7 +696,7 @@ __global__ void __launch_bounds__(kUmmaThreads, 1)
         if (lane == 0) mbar_arrive(&item_empty[sl]);
         ++nread;
         if (idx >= n_items) return false;
-        const UmmaItem it = umma_item<CASCADE, WINDOW>(p, idx, tiles_x, ny);
+        const UmmaItem it = umma_item<CASCADE>(p, idx, tiles_x, ny);
         if (it.skip) continue;
         ri.q0 = it.q0;
         ri.y = it.y;
@@ -704,7 +704,6 @@ __global__ void __launch_bounds__(kUmmaThreads, 1)
         ri.kv_beg = it.kv_beg;
         ri.kv_end = it.kv_end;
         ri.ntiles = it.ntiles;
-        if constexpr (WINDOW) ri.v_beg = it.seen.beg;
         bool on;  // a row that sees keys
         const int64_t R = it.R0 + r;
         ri.in_tile = R < it.rows;
@@ -816,8 +815,7 @@ __global__ void __launch_bounds__(kUmmaThreads, 1)
 #pragma unroll
           for (int c = 0; c < HK; ++c) {
             const int tok = t0 + c;
-            const bool vis = (tok >= beg_r || (WINDOW && tok < p.sinks)) && tok < end_r &&
-                             ((pm >> ((half * HK + c) / BS)) & 1u);
+            const bool vis = tok >= beg_r && tok < end_r && ((pm >> ((half * HK + c) / BS)) & 1u);
             x[c] = vis ? x[c] * qk_scale : -INFINITY;
             mx = fmaxf(mx, x[c]);
           }
@@ -903,24 +901,6 @@ __global__ void __launch_bounds__(kUmmaThreads, 1)
                 const int ch = tk / 8;
                 const int phys = BS == 32 ? (ch ^ ((d >> 1) & 3)) : (ch ^ ((d >> 2) & 1));
                 *reinterpret_cast<uint16_t*>(vpage + d * BS * 2 + phys * 16 + (tk % 8) * 2) = 0;
-              }
-            }
-            fence_proxy_async();
-          }
-        }
-        // window form: V of the tokens between the sinks and the first row's window
-        // start, which share their pages with seen ones, becomes 0 for the same reason
-        if constexpr (WINDOW) {
-          const int u0 = p.sinks > tile0 ? p.sinks : tile0;
-          const int u1 = cur.v_beg < tile0 + KT ? cur.v_beg : tile0 + KT;
-          if (half == 0 && u0 < u1) {
-            const int d = r;
-            if (d < D) {
-              uint8_t* vst = ring + (size_t)st * UG::STAGE + PAGES * PAGE;
-              for (int tk = u0 - tile0; tk < u1 - tile0; ++tk) {
-                const int ch = (tk % BS) / 8;
-                const int phys = BS == 32 ? (ch ^ ((d >> 1) & 3)) : (ch ^ ((d >> 2) & 1));
-                *reinterpret_cast<uint16_t*>(vst + (tk / BS) * PAGE + d * BS * 2 + phys * 16 + (tk % 8) * 2) = 0;
               }
             }
             fence_proxy_async();
@@ -1021,27 +1001,6 @@ __global__ void __launch_bounds__(kUmmaThreads, 1)
       atomicExch(&g_umma_sched[slot].done, 0u);
     }
   }
-}
-
-// K viewed as rows of one 8-dim chunk of one page of one head: [nb * H * D/8][BS * 8]
-// (needs the dense paged layout).
-static bool make_k_gather_map(const PrefillArgs& a, int D, int BS, CUtensorMap* map) {
-  auto enc = tensor_map_encoder();
-  if (!enc) return false;
-  const cuuint64_t dims[2] = {(cuuint64_t)BS * 8, (cuuint64_t)a.num_blocks * a.num_kv_heads * (D / 8)};
-  const cuuint64_t strides[1] = {(cuuint64_t)BS * 16};
-  const cuuint32_t box[2] = {(cuuint32_t)BS * 8, 1};
-  const cuuint32_t ones[2] = {1, 1};
-  return enc(map, a.q_type == ElemType::BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
-             const_cast<void*>(a.k_cache), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
-             CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) ==
-         CUDA_SUCCESS;
-}
-
-// KVC_PREFILL_ISSUE=single: the producer's lane 0 issues every copy (tuning runs).
-static int umma_single_issue() {
-  const char* v = getenv("KVC_PREFILL_ISSUE");
-  return v && v[0] == 's' ? 1 : 0;
 }
 
 // The persistent grid: one CTA per SM (the ring and TMEM allow one), fewer

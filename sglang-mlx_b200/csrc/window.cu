@@ -11,6 +11,7 @@
 #include "decode_mma.cuh"
 #include "prefill.cuh"
 #include "prefill_umma.cuh"
+#include "window_umma.cuh"
 
 namespace kvc {
 
@@ -706,34 +707,60 @@ cudaError_t launch_window_decode(const DecodeArgs& a, const WindowArgs& w, cudaS
 }
 
 // ---------------------------------------------------------------------------
-// Extend: the prefill kernels in their WINDOW form; which one serves a call goes
-// by the same rule as the causal prefill (attention_dispatch.cuh).
+// Extend.  The tcgen05 kernel (window_umma.cuh) serves 16- and 32-token pages and
+// every dense token-major cache; the mma.sync prefill kernel in its WINDOW form the
+// rest (8-token pages, strided token rows, output rows that 16-byte stores cannot
+// write).
 // ---------------------------------------------------------------------------
-template <typename T, int D, int BS, bool GK>
+// K as rows of one 8-dim chunk of one page, [rows][BS * 8], over whatever lies
+// between the pages of a strided cache.
+static bool make_k_chunk_map(const PrefillArgs& a, int D, int BS, CUtensorMap* map) {
+  auto enc = tensor_map_encoder();
+  const int64_t row = (int64_t)BS * 8;
+  if (!enc || a.k_block_stride % row || a.k_head_stride % row || a.k_block_stride < 0 || a.k_head_stride < 0) return false;
+  const int64_t rows = ((a.num_blocks - 1) * a.k_block_stride + (a.num_kv_heads - 1) * a.k_head_stride) / row + D / 8;
+  if (rows <= 0 || rows > 0x7fffffffll) return false;
+  const cuuint64_t dims[2] = {(cuuint64_t)row, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)row * 2};
+  const cuuint32_t box[2] = {(cuuint32_t)row, 1};
+  const cuuint32_t ones[2] = {1, 1};
+  return enc(map, a.q_type == ElemType::BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+             const_cast<void*>(a.k_cache), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) ==
+         CUDA_SUCCESS;
+}
+
+template <typename T, int D, int BS, int LOAD>
 static cudaError_t launch_window_umma(const PrefillArgs& a, cudaStream_t stream) {
-  using UG = UmmaGeom<D, BS>;
+  using WG = WinUmmaGeom<D, BS, LOAD>;
   DecodeParams dp;
   memset(&dp, 0, sizeof(dp));
   dp.k_cache = a.k_cache;
   dp.v_cache = a.v_cache;
   dp.num_blocks = a.num_blocks;
   dp.num_kv_heads = a.num_kv_heads;
+  dp.block_size = a.block_size;
   dp.k_head_stride = a.k_head_stride;
   dp.k_block_stride = a.k_block_stride;
   dp.v_head_stride = a.v_head_stride;
   dp.v_block_stride = a.v_block_stride;
+  dp.k_tok_stride = a.k_tok_stride;
+  dp.v_tok_stride = a.v_tok_stride;
   TmaMaps maps;
   memset(&maps, 0, sizeof(maps));
-  if (!make_tensor_maps(dp, std::is_same<T, __nv_bfloat16>::value ? ElemType::BF16 : ElemType::F16, D, BS, BS, BS * 2,
-                        kTiles, &maps))
+  const ElemType et = std::is_same<T, __nv_bfloat16>::value ? ElemType::BF16 : ElemType::F16;
+  if (LOAD == kPages) {
+    if (!make_tensor_maps(dp, et, D, BS, BS, BS * 2, kTiles, &maps) || !make_k_chunk_map(a, D, BS, &maps.k))
+      return cudaErrorNotSupported;
+  } else if (!make_tensor_maps(dp, et, D, 16, 16, 128, LOAD == kRows ? kFlashTma : kFlashGather, &maps)) {
     return cudaErrorNotSupported;
-  if (GK && !make_k_gather_map(a, D, BS, &maps.k)) return cudaErrorNotSupported;
-  auto kern = prefill_umma_kernel<T, D, BS, GK, false, true>;
+  }
+  auto kern = window_umma_kernel<T, D, BS, LOAD>;
   static std::atomic<bool> configured[64];  // per device; setting the attribute twice is harmless
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev >= 0 && dev < 64 && !configured[dev]) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, UG::SMEM);
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, WG::SMEM);
     if (e != cudaSuccess) return e;
     configured[dev] = true;
   }
@@ -741,28 +768,41 @@ static cudaError_t launch_window_umma(const PrefillArgs& a, cudaStream_t stream)
   const int64_t tiles = ((int64_t)a.max_q_len * G + kUmmaRows - 1) / kUmmaRows;
   const int64_t items = tiles * a.num_seqs * a.num_kv_heads;
   if (items > 0x7fffffffll - 1024) return cudaErrorInvalidValue;
-  const int ctas = umma_persistent_ctas(dev, items);
-  const int slot = umma_sched_slot(stream);
-  PrefillArgs aa = a;
-  aa.single_issue = umma_single_issue();
-  kern<<<ctas, kUmmaThreads, UG::SMEM, stream>>>(aa, maps, (int)tiles, (int)a.num_seqs, slot);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)umma_persistent_ctas(dev, items));
+  cfg.blockDim = dim3(kUmmaThreads);
+  cfg.dynamicSmemBytes = WG::SMEM;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e =
+      cudaLaunchKernelEx(&cfg, kern, a, maps, (int)tiles, (int)a.num_seqs, umma_sched_slot(stream));
   count_launch();
-  return cudaGetLastError();
+  return e != cudaSuccess ? e : cudaGetLastError();
 }
 
 template <typename T, int D>
 static cudaError_t launch_window_prefill_t(const PrefillArgs& a, cudaStream_t stream) {
-  const bool rows16 = (reinterpret_cast<uintptr_t>(a.out) & 15u) == 0 && ((a.out_tok_stride | a.out_head_stride) & 7) == 0;
-  if (!a.token_major && (a.block_size == 16 || a.block_size == 32) && rows16) {
-    const int64_t BS = a.block_size;
-    const bool dense = a.k_head_stride == D * BS && a.k_block_stride == (int64_t)a.num_kv_heads * D * BS &&
-                       a.num_blocks * a.num_kv_heads * (D / 8) < 0x7fffffffll;  // (row indices are 32-bit)
-    cudaError_t e;
-    if (BS == 32) e = dense ? launch_window_umma<T, D, 32, true>(a, stream) : launch_window_umma<T, D, 32, false>(a, stream);
-    else e = dense ? launch_window_umma<T, D, 16, true>(a, stream) : launch_window_umma<T, D, 16, false>(a, stream);
-    if (e != cudaErrorNotSupported) return e;
+  cudaError_t e = cudaErrorNotSupported;
+  if ((reinterpret_cast<uintptr_t>(a.out) & 15u) == 0 && ((a.out_tok_stride | a.out_head_stride) & 7) == 0) {
+    if (!a.token_major) {
+      if (a.block_size == 32) e = launch_window_umma<T, D, 32, kPages>(a, stream);
+      else if (a.block_size == 16) e = launch_window_umma<T, D, 16, kPages>(a, stream);
+    } else {
+      const int64_t H = a.num_kv_heads, bs = a.block_size;
+      // (block size 1, the pool's [slots, H, D]: a block is one row and carries no token stride)
+      const int64_t ktok = bs == 1 ? a.k_block_stride : a.k_tok_stride, vtok = bs == 1 ? a.v_block_stride : a.v_tok_stride;
+      const bool blocks = a.k_block_stride == bs * ktok && a.v_block_stride == bs * vtok &&
+                          a.num_blocks * bs * H < (int64_t)1 << 31;
+      const bool dense = blocks && a.k_head_stride == D && ktok == H * D && a.v_head_stride == D && vtok == H * D;
+      if (blocks && bs % 16 == 0) e = launch_window_umma<T, D, 16, kRows>(a, stream);
+      else if (dense) e = launch_window_umma<T, D, 16, kSlots>(a, stream);
+    }
   }
-  return launch_prefill_layout<T, D, true>(a, a.token_major, stream);
+  return e != cudaErrorNotSupported ? e : launch_prefill_layout<T, D, true>(a, a.token_major, stream);
 }
 
 cudaError_t launch_window_prefill(const PrefillArgs& a, cudaStream_t stream) {

@@ -1,0 +1,789 @@
+// window_umma.cuh — tcgen05 extend attention over a sliding window with sinks
+// (sm_100a), for the paged layout and for token-major caches.
+//
+// Included by window.cu after prefill_umma.cuh, whose work items (umma_item: 128
+// (new token, query head) rows of one sequence and KV head), persistent grid and
+// descriptors it shares.  An item's keys are its sink blocks and its window's
+// blocks without the gap between them (struct Seen), in tiles of 128 tokens that
+// are filled block by block, so the few sink tokens share a tile with the window's
+// first blocks and no tile is spent on alignment.
+//
+// What sets it apart from the causal kernel: that one's two halves of softmax warps
+// (each thread one row and 64 of a tile's 128 tokens) share one O and so must agree
+// on a row maximum before every exponential, an exchange of about 630 of a tile's
+// 3260 cycles.  Here each half accumulates into an O of its own with its own lazy
+// maximum and sum, and the two meet once per item:
+//   out = (w_0 O_0 + w_1 O_1) / (w_0 l_0 + w_1 l_1),  w_h = 2^(m_h - max(m_0, m_1)).
+// The second O takes the tensor memory that Q had, so Q goes to shared memory
+// (S = Q K^T from two descriptors, N = 128), and K and V have rings of their own: K
+// is free after S, V after P V.
+//   TMEM (512 columns): S 2 x 128 (P over it: per half 32 columns of hi pairs and
+//   32 of lo pairs), O 2 x D.
+//   Warps 0-7 softmax (warp w and w + 4: the two halves of rows 32 (w & 3) ..),
+//   warp 8 producer, warp 9 (one lane) products.
+//
+// LOAD: how a tile reaches shared memory.
+//   kPages  paged layout, 16- or 32-token pages: K by 4-row gathers of 8-dim
+//           chunk rows ([D/8][128][8], no swizzle), V a page at a time ([D][bs],
+//           rows swizzled over bs * 2 bytes: K-major for P V).
+//   kRows   token-major, blocks of 16k dense rows: 16 rows x 64 dims to a copy,
+//           128-byte swizzle; K is K-major as it lies, V is MN-major (its
+//           dims, the N of P V, run along the row).
+//   kSlots  token-major, any block size (the pool's slot lists): the same tile
+//           from 4-row gathers, each token's row where its own slot is.
+// Every wait is bounded; a timeout sets KVC_STATUS_WAIT_TIMEOUT and an abort flag
+// that ends every loop; TMEM is freed after a final commit.
+#pragma once
+
+namespace kvc {
+
+constexpr int kPages = 0, kRows = 1, kSlots = 2;
+constexpr uint32_t kLayoutSw128 = 2;
+
+template <int D, int BS, int LOAD>
+struct WinUmmaGeom {
+  static constexpr int TILE = kUmmaTile * D * 2;  // bytes of one K (or V) tile
+  static constexpr int KS = D == 128 ? 3 : 4, VS = D == 128 ? 2 : 4;  // ring stages
+  static constexpr int Q_OFF = (KS + VS) * TILE;
+  static constexpr int XBUF_OFF = Q_OFF + 2 * TILE;          // [2 halves][128 rows] (max, sum)
+  static constexpr int BAR_OFF = XBUF_OFF + 2 * 128 * 8;
+  static constexpr int NBARS = 2 * KS + 2 * VS + 2 + 4 + 1 + 1 + 1 + 1 + 1 + 4;
+  static constexpr int MASK_OFF = BAR_OFF + NBARS * 8;       // [8 tiles][4] loaded blocks (kSlots: tokens)
+  static constexpr int MISC_OFF = MASK_OFF + 8 * 16;         // abort, tmem address, two item slots
+  static constexpr int SMEM = MISC_OFF + 16;
+  static constexpr int UNIT = LOAD == kPages ? BS : (LOAD == kRows ? 16 : 1);  // tokens to a mask bit
+  static constexpr int UNITS = LOAD == kSlots ? 128 : kUmmaTile / UNIT;
+  static constexpr uint32_t SCOL = 0, OCOL = 256;
+  static_assert(OCOL + 2 * D <= 512, "TMEM columns");
+  static_assert(SMEM <= 227 * 1024, "shared memory");
+};
+
+template <typename T, int D, int BS, int LOAD>
+__global__ void __launch_bounds__(kUmmaThreads, 1)
+    window_umma_kernel(const PrefillArgs p, const __grid_constant__ TmaMaps maps, int tiles_x, int ny, int slot) {
+  using namespace mma_detail;
+  using WG = WinUmmaGeom<D, BS, LOAD>;
+  constexpr int KT = kUmmaTile, TILE = WG::TILE, KS = WG::KS, VS = WG::VS, UNIT = WG::UNIT;
+  constexpr int PAGES = KT / BS, PAGE = D * BS * 2;  // kPages
+  constexpr int HALF = KT * 128;                     // token-major: bytes of 64 dims of a tile
+  constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+  constexpr bool SPLIT = BF16;  // bf16 P as hi + lo (one rounding misses the tolerance on rows of few keys)
+  // (no static shared memory: the dynamic window then starts on a 1024-byte
+  // boundary, as the 128-byte swizzle needs; checked below)
+  extern __shared__ __align__(1024) uint8_t smem_wu[];
+  uint8_t* kring = smem_wu;
+  uint8_t* vring = smem_wu + KS * TILE;
+  uint8_t* qsm = smem_wu + WG::Q_OFF;
+  float2* xbuf = reinterpret_cast<float2*>(smem_wu + WG::XBUF_OFF);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem_wu + WG::BAR_OFF);
+  uint64_t* k_full = bars;
+  uint64_t* k_empty = k_full + KS;
+  uint64_t* v_full = k_empty + KS;
+  uint64_t* v_empty = v_full + VS;
+  uint64_t* s_full = v_empty + VS;  // [2 buffers]
+  uint64_t* p_full = s_full + 2;    // [2 buffers][2 halves]
+  uint64_t* pv_done = p_full + 4;
+  uint64_t* o_done = pv_done + 1;
+  uint64_t* q_ready = o_done + 1;
+  uint64_t* all_done = q_ready + 1;
+  uint64_t* xchg = all_done + 1;
+  uint64_t* item_full = xchg + 1;
+  uint64_t* item_empty = item_full + 2;
+  uint32_t* masks = reinterpret_cast<uint32_t*>(smem_wu + WG::MASK_OFF);
+  volatile int* s_abort = reinterpret_cast<volatile int*>(smem_wu + WG::MISC_OFF);
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(smem_wu + WG::MISC_OFF + 4);
+  volatile int* s_item = reinterpret_cast<volatile int*>(smem_wu + WG::MISC_OFF + 8);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int G = p.num_heads / p.num_kv_heads;
+  const int n_items = tiles_x * ny * p.num_kv_heads;
+  const bool dynamic = n_items > (int)gridDim.x;
+  grid_dependents_launch();
+  if ((smem_u32(smem_wu) & 1023u) != 0) {  // (the same for every thread)
+    grid_dependency_wait();
+    if (threadIdx.x == 0) set_status(&g_decode_status, KVC_STATUS_WAIT_TIMEOUT);
+    return;
+  }
+  if (threadIdx.x == 0) {
+    *s_abort = 0;
+    for (int s = 0; s < KS; ++s) {
+      mbar_init(&k_full[s], 1);
+      mbar_init(&k_empty[s], 1);
+    }
+    for (int s = 0; s < VS; ++s) {
+      mbar_init(&v_full[s], 1);
+      mbar_init(&v_empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&s_full[b], 2);
+      mbar_init(&item_full[b], 1);
+      mbar_init(&item_empty[b], 9);
+    }
+    for (int b = 0; b < 4; ++b) mbar_init(&p_full[b], 4);
+    mbar_init(pv_done, 1);
+    mbar_init(o_done, 1);
+    mbar_init(q_ready, 8);
+    mbar_init(all_done, 1);
+    mbar_init(xchg, 8);
+    mbar_fence_init();
+  }
+  // V of blocks that a tile does not load meets P = 0 (0 * NaN = NaN): the ring
+  // starts from zeros
+  for (int i = threadIdx.x; i < VS * TILE / 16; i += kUmmaThreads)
+    reinterpret_cast<uint4*>(vring)[i] = make_uint4(0u, 0u, 0u, 0u);
+  fence_proxy_async();
+  if (warp == kMmaWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(s_tmem)),
+                 "r"(512));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  } else if (warp == kProducerWarp && lane == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&maps.v)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&maps.k)) : "memory");
+  }
+  umma::fence_before();
+  __syncthreads();
+  umma::fence_after();
+  const uint32_t tmem = *s_tmem;
+  // (a programmatic dependent: the set-up above overlaps the kernel before this one)
+  grid_dependency_wait();
+  auto abort_now = [&]() -> bool { return *s_abort != 0; };
+  auto give_up = [&]() {
+    *s_abort = 1;
+    set_status(&g_decode_status, KVC_STATUS_WAIT_TIMEOUT);
+  };
+
+  if (warp == kProducerWarp) {
+    // ---- producer: claims items, hands each to the other warps, loads its tiles
+    int gt = 0, npub = 0;  // tiles issued, items handed over
+    int nk = 0, nv = 0;    // K and V tiles asked for
+    bool stop = false;
+    auto publish = [&](int idx) -> bool {  // (lane 0)
+      const int sl = npub & 1;
+      if (npub >= 2 && !umma::wait(&item_empty[sl], (uint32_t)(((npub >> 1) - 1) & 1))) return false;
+      s_item[sl] = idx;
+      mbar_arrive(&item_full[sl]);
+      ++npub;
+      return true;
+    };
+    UmmaSched* sched = &g_umma_sched[slot];
+    // every lane learns whether lane 0's wait came through and nobody gave up
+    auto warp_wait = [&](bool need, uint64_t* bar, uint32_t parity) -> bool {
+      bool ok = true;
+      if (need && lane == 0) ok = umma::wait(bar, parity);
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+      if (!ok && lane == 0) give_up();
+      return ok && !__shfl_sync(0xffffffffu, abort_now() ? 1 : 0, 0);
+    };
+    for (int idx = blockIdx.x; idx < n_items && !stop;) {
+      const UmmaItem it = umma_item<false, true>(p, idx, tiles_x, ny);
+      if (it.bad && it.first_tile && it.kvh == 0 && lane == 0) set_status(&g_decode_status, KVC_STATUS_INDEX_OOB);
+      auto claim = [&]() -> int {
+        unsigned nx = (unsigned)n_items;
+        if (dynamic && lane == 0) nx = gridDim.x + atomicAdd(&sched->next, 1u);
+        nx = __shfl_sync(0xffffffffu, nx, 0);
+        return nx < (unsigned)n_items ? (int)nx : n_items;
+      };
+      if (it.skip) {
+        idx = claim();
+        continue;
+      }
+      // the item's query rows toward L2, ahead of the softmax warps' loads
+      if (!it.bad && it.ntiles > 0) {
+        const int64_t nrows = it.rows - it.R0 < kUmmaRows ? it.rows - it.R0 : kUmmaRows;
+        for (int r = lane; r < nrows; r += 32) {
+          const int64_t R = it.R0 + r, t = R / G;
+          const char* a = reinterpret_cast<const char*>(reinterpret_cast<const T*>(p.q) + (it.q0 + t) * p.q_tok_stride +
+                                                        (int64_t)(it.kvh * G + (int)(R - t * G)) * p.q_head_stride);
+#pragma unroll
+          for (int b = 0; b < D * 2; b += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(a + b));
+        }
+      }
+      bool handed = true;
+      if (lane == 0) handed = publish(idx);
+      if (!__shfl_sync(0xffffffffu, handed, 0)) {
+        if (lane == 0) give_up();
+        break;
+      }
+      const int kvh = it.kvh, kv_end = it.kv_end, ntiles = it.ntiles;
+      const uint32_t* table = p.block_tables + (int64_t)it.y * p.table_stride;
+      const int tbs = p.block_size;
+      // ids of tile j: lane i holds unit i's (kSlots: tokens 4i .. 4i + 3)
+      auto load_ids = [&](int j, uint32_t (&id)[4]) {
+        if constexpr (LOAD == kSlots) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int tok = j * KT + 4 * lane + e;
+            id[e] = j < ntiles && tok < kv_end ? __ldg(table + it.seen.real_block(tbs == 1 ? tok : tok / tbs)) : 0xffffffffu;
+          }
+        } else {
+          const int tok = j * KT + lane * UNIT;
+          id[0] = lane < WG::UNITS && j < ntiles && tok < kv_end
+                      ? __ldg(table + it.seen.real_block(LOAD == kPages ? tok / BS : tok / tbs))
+                      : 0xffffffffu;
+        }
+      };
+      uint32_t id[4];
+      load_ids(0, id);
+      for (int j = 0; j < ntiles; ++j) {
+        const int g = gt + j, ks = g % KS, vs = g % VS, t0 = j * KT;
+        if (!warp_wait(g >= KS, &k_empty[ks], (uint32_t)(((g / KS) - 1) & 1))) {
+          stop = true;
+          break;
+        }
+        uint8_t* kst = kring + (size_t)ks * TILE;
+        uint8_t* vst = vring + (size_t)vs * TILE;
+        uint32_t* tm = masks + (g & 7) * 4;
+        uint32_t next[4];
+        if constexpr (LOAD == kSlots) {
+          // a token without a block gathers a loaded token's row (and is masked)
+          uint32_t ok = 0, oob = 0;
+          int row[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int tok = t0 + 4 * lane + e;
+            const bool in = tok < kv_end, good = in && (int64_t)id[e] < p.num_blocks;
+            ok |= good ? 1u << e : 0u;
+            oob |= in && !good ? 1u : 0u;
+            row[e] = good ? (int)((tbs == 1 ? (int64_t)id[e] : (int64_t)id[e] * tbs + tok % tbs) * p.num_kv_heads + kvh) : -1;
+          }
+          if (oob) set_status(&g_decode_status, KVC_STATUS_BLOCK_OOB);
+          const uint32_t any = __ballot_sync(0xffffffffu, ok != 0u);
+          int spare = ok ? row[__ffs(ok) - 1] : 0;
+          spare = __shfl_sync(0xffffffffu, spare, any ? __ffs(any) - 1 : 0);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) row[e] = row[e] >= 0 ? row[e] : spare;
+          // lanes 8w .. 8w + 7 hold the 32 tokens of word w
+          uint32_t word = ok << (4 * (lane & 7));
+#pragma unroll
+          for (int o = 1; o < 8; o <<= 1) word |= __shfl_xor_sync(0xffffffffu, word, o);
+          if ((lane & 7) == 0) tm[lane >> 3] = word;
+          load_ids(j + 1, next);
+          __syncwarp();
+          if (lane == 0) {
+            if (any) mbar_arrive_expect_tx(&k_full[ks], (uint32_t)TILE);
+            else mbar_arrive(&k_full[ks]);
+          }
+          nk = g + 1;
+          __syncwarp();
+          if (any) {
+#pragma unroll
+            for (int h = 0; h < D / 64; ++h)
+              tma_gather4(kst + h * HALF + lane * 512, &maps.k, 64 * h, row[0], row[1], row[2], row[3], &k_full[ks]);
+          }
+          if (!warp_wait(g >= VS, &v_empty[vs], (uint32_t)(((g / VS) - 1) & 1))) {
+            stop = true;
+            break;
+          }
+          if (lane == 0) {
+            if (any) mbar_arrive_expect_tx(&v_full[vs], (uint32_t)TILE);
+            else mbar_arrive(&v_full[vs]);
+          }
+          nv = g + 1;
+          __syncwarp();
+          if (any) {
+#pragma unroll
+            for (int h = 0; h < D / 64; ++h)
+              tma_gather4(vst + h * HALF + lane * 512, &maps.v, 64 * h, row[0], row[1], row[2], row[3], &v_full[vs]);
+          }
+        } else {
+          const int tok = t0 + lane * UNIT;
+          const bool in = lane < WG::UNITS && tok < kv_end, good = in && (int64_t)id[0] < p.num_blocks;
+          if (in && !good) set_status(&g_decode_status, KVC_STATUS_BLOCK_OOB);
+          const uint32_t mask = __ballot_sync(0xffffffffu, good);
+          const uint32_t mine = id[0];
+          load_ids(j + 1, next);
+          if (lane == 0) {
+            tm[0] = mask;
+            const uint32_t unit_bytes = (uint32_t)(UNIT * D * 2);
+            if (!mask) mbar_arrive(&k_full[ks]);
+            else mbar_arrive_expect_tx(&k_full[ks], LOAD == kPages ? (uint32_t)TILE : (uint32_t)__popc(mask) * unit_bytes);
+          }
+          nk = g + 1;
+          __syncwarp();
+          const int row = LOAD == kRows ? (int)mine * tbs + tok % tbs : 0;  // (rows are below 2^31: the host checked)
+          if (mask) {
+            if constexpr (LOAD == kPages) {
+              // chunk row c of a page: row base + c; pages without keys gather a loaded page's rows
+              const int base = (int)(((int64_t)mine * p.k_block_stride + (int64_t)kvh * p.k_head_stride) / (BS * 8));
+              const int any = __shfl_sync(0xffffffffu, base, __ffs(mask) - 1);
+              int rb[PAGES];
+#pragma unroll
+              for (int i = 0; i < PAGES; ++i) {
+                const int b = __shfl_sync(0xffffffffu, base, i);
+                rb[i] = (mask >> i) & 1u ? b : any;
+              }
+              if (lane < D / 8) {
+#pragma unroll
+                for (int q = 0; q < PAGES; q += 4)
+                  tma_gather4(kst + lane * KT * 16 + q * BS * 16, &maps.k, 0, rb[q] + lane, rb[q + 1] + lane,
+                              rb[q + 2] + lane, rb[q + 3] + lane, &k_full[ks]);
+              }
+            } else if (good) {
+#pragma unroll
+              for (int h = 0; h < D / 64; ++h)
+                tma_load_3d(kst + h * HALF + lane * 16 * 128, &maps.k, 64 * h, kvh, row, &k_full[ks]);
+            }
+          }
+          if (!warp_wait(g >= VS, &v_empty[vs], (uint32_t)(((g / VS) - 1) & 1))) {
+            stop = true;
+            break;
+          }
+          if (lane == 0) {
+            if (mask) mbar_arrive_expect_tx(&v_full[vs], (uint32_t)__popc(mask) * (uint32_t)(UNIT * D * 2));
+            else mbar_arrive(&v_full[vs]);
+          }
+          nv = g + 1;
+          __syncwarp();
+          if (good) {
+            if constexpr (LOAD == kPages) {
+              tma_load_4d(vst + lane * PAGE, &maps.v, 0, 0, kvh, (int)mine, &v_full[vs]);
+            } else {
+#pragma unroll
+              for (int h = 0; h < D / 64; ++h)
+                tma_load_3d(vst + h * HALF + lane * 16 * 128, &maps.v, 64 * h, kvh, row, &v_full[vs]);
+            }
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) id[e] = next[e];
+      }
+      gt += ntiles;
+      if (!stop) idx = claim();
+    }
+    if (lane == 0 && !publish(n_items)) give_up();
+    // shared memory outlives every copy, after an abort too: bounded waits on the
+    // last copy asked for in each stage
+    if (lane == 0) {
+      for (int g = nk > KS ? nk - KS : 0; g < nk; ++g) umma::wait(&k_full[g % KS], (uint32_t)((g / KS) & 1));
+      for (int g = nv > VS ? nv - VS : 0; g < nv; ++g) umma::wait(&v_full[g % VS], (uint32_t)((g / VS) & 1));
+    }
+    __syncwarp();
+  } else if (warp == kMmaWarp) {
+    // ---- products (one lane)
+    if (lane == 0) {
+      const uint32_t idS = umma::instr_desc(BF16, 128, KT);
+      const uint32_t idO = umma::instr_desc(BF16, 128, D) | (LOAD == kPages ? 0u : 1u << 16);  // (B is MN-major)
+      const uint64_t q_desc0 = umma::smem_desc(smem_u32(qsm), kUmmaRows * 16, 128, umma::kLayoutNone);
+      const uint64_t k_desc0 = LOAD == kPages ? umma::smem_desc(smem_u32(kring), KT * 16, 128, umma::kLayoutNone)
+                                              : umma::smem_desc(smem_u32(kring), 16, 1024, kLayoutSw128);
+      const uint64_t v_desc0 =
+          LOAD != kPages ? umma::smem_desc(smem_u32(vring), HALF, 1024, kLayoutSw128)
+                         : (BS == 32 ? umma::smem_desc(smem_u32(vring), 16, 512, umma::kLayoutSw64)
+                                     : umma::smem_desc(smem_u32(vring), 16, 256, umma::kLayoutSw32));
+      int gt = 0, nit = 0, nread = 0;
+      bool ok = true;
+      for (;;) {
+        const int sl = nread & 1;
+        if (abort_now() || !umma::wait(&item_full[sl], (uint32_t)((nread >> 1) & 1))) {
+          ok = false;
+          break;
+        }
+        const int idx = s_item[sl];
+        mbar_arrive(&item_empty[sl]);
+        ++nread;
+        if (idx >= n_items) break;
+        const UmmaItem it = umma_item<false, true>(p, idx, tiles_x, ny);
+        if (it.skip || it.ntiles == 0) continue;
+        if (abort_now() || !umma::wait(q_ready, (uint32_t)(nit & 1))) {
+          ok = false;
+          break;
+        }
+        umma::fence_after();
+        const uint64_t qd = q_desc0 + (uint64_t)(((nit & 1) * TILE) >> 4);
+        ++nit;
+        const int kv_end = it.kv_end, ntiles = it.ntiles;
+        // O_h += P_h V_h of tile j (this CTA's tile g), both halves
+        auto issue_pv = [&](int j, int g) -> bool {
+          const int b = g & 1, vs = g % VS;
+          if (!umma::wait(&v_full[vs], (uint32_t)((g / VS) & 1))) return false;
+          const uint64_t vd = v_desc0 + (uint64_t)((vs * TILE) >> 4);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (!umma::wait(&p_full[2 * b + h], (uint32_t)((g >> 1) & 1))) return false;
+            // (an item's first product overwrites both O, which every softmax warp
+            // has read by the time it hands over its part of the first tile)
+            if (j == 0 && h == 0 && !umma::wait(&p_full[2 * b + 1], (uint32_t)((g >> 1) & 1))) return false;
+            umma::fence_after();
+            const int left = kv_end - (j * KT + h * 64), steps = left > 0 ? (left + 15) / 16 : 0;
+            const uint32_t pcol = tmem + WG::SCOL + b * 128 + h * 64, ocol = tmem + WG::OCOL + h * D;
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) {
+              if (ks < steps) {
+                const int tk = h * 64 + 16 * ks;
+                const uint64_t d =
+                    vd + (uint64_t)((LOAD == kPages ? (tk / BS) * PAGE + (tk % BS) * 2 : tk * 128) >> 4);
+                umma::mma_ts(ocol, pcol + 8 * ks, d, idO, (j > 0 || ks > 0) ? 1u : 0u);
+                if (SPLIT) umma::mma_ts(ocol, pcol + 32 + 8 * ks, d, idO, 1u);
+              }
+            }
+          }
+          umma::commit(pv_done);
+          umma::commit(&v_empty[vs]);
+          return true;
+        };
+        for (int j = 0; j < ntiles && ok; ++j) {
+          const int g = gt + j, ks0 = g % KS, b = g & 1;
+          if (abort_now() || !umma::wait(&k_full[ks0], (uint32_t)((g / KS) & 1))) {
+            ok = false;
+            break;
+          }
+          umma::fence_after();
+          const uint64_t kd = k_desc0 + (uint64_t)((ks0 * TILE) >> 4);
+#pragma unroll
+          for (int ks = 0; ks < D / 16; ++ks)
+            umma::mma_ss(tmem + WG::SCOL + b * 128, qd + (uint64_t)((ks * 2 * kUmmaRows * 16) >> 4),
+                         kd + (uint64_t)((LOAD == kPages ? ks * 2 * KT * 16 : (ks / 4) * HALF + (ks % 4) * 32) >> 4), idS,
+                         ks > 0 ? 1u : 0u);
+          umma::commit(&s_full[b]);
+          mbar_arrive(&s_full[b]);  // (release: the tile's masks, seen through k_full, are seen by whoever waits)
+          umma::commit(&k_empty[ks0]);
+          if (j >= 1 && !issue_pv(j - 1, g - 1)) ok = false;
+        }
+        if (ok && !abort_now()) ok = issue_pv(ntiles - 1, gt + ntiles - 1);
+        umma::commit(o_done);
+        gt += ntiles;
+      }
+      if (!ok) give_up();
+      umma::commit(all_done);
+      umma::wait(all_done, 0);
+    }
+    __syncwarp();
+  } else {
+    // ---- softmax / epilogue.  Decisions ahead of warp-collective TMEM accesses
+    // are made for the whole warp.
+    auto uwait = [&](uint64_t* bar, uint32_t parity) -> bool {
+      return __all_sync(0xffffffffu, umma::wait(bar, parity));
+    };
+    auto uabort = [&]() -> bool { return __any_sync(0xffffffffu, abort_now()); };
+    const int half = warp >> 2, r = threadIdx.x & 127;
+    const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    constexpr int HK = 64;      // tokens of a tile per half
+    constexpr int HD = D / 2;   // output columns per half
+    const float qk_scale = p.scale * kLog2e;
+    bool ok = true;
+    int gt = 0, nread = 0, nq = 0, nx = 0;
+    struct RowItem {
+      int64_t q0;
+      int kvh, kv_end, ntiles, v_beg;
+      int t, g, end_r, beg_r;
+      bool in_tile;
+    };
+    // the next item with work, its Q rows staged into shared buffer nq & 1 ([D/8
+    // chunks][128 rows][8], half of the chunks per half) and handed over; every
+    // product that read this buffer, two items back, completed before that item's
+    // epilogue
+    auto next_item = [&](RowItem& ri) -> bool {
+      for (;;) {
+        const int sl = nread & 1;
+        if (uabort() || !uwait(&item_full[sl], (uint32_t)((nread >> 1) & 1))) {
+          ok = false;
+          return false;
+        }
+        const int idx = s_item[sl];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&item_empty[sl]);
+        ++nread;
+        if (idx >= n_items) return false;
+        const UmmaItem it = umma_item<false, true>(p, idx, tiles_x, ny);
+        if (it.skip) continue;
+        ri.q0 = it.q0;
+        ri.kvh = it.kvh;
+        ri.kv_end = it.kv_end;
+        ri.ntiles = it.ntiles;
+        ri.v_beg = it.seen.beg;
+        const int64_t R = it.R0 + r;
+        ri.in_tile = R < it.rows;
+        ri.t = ri.in_tile ? (int)(R / G) : 0;
+        ri.g = ri.in_tile ? (int)(R - (int64_t)ri.t * G) : 0;
+        const bool on = ri.in_tile && !it.bad;
+        ri.end_r = on ? it.prefix + ri.t + 1 : 0;
+        ri.beg_r = ri.end_r > p.window ? ri.end_r - p.window : 0;
+        if (it.ntiles > 0) {
+          const T* qrow = reinterpret_cast<const T*>(p.q) + (it.q0 + ri.t) * p.q_tok_stride +
+                          (int64_t)(it.kvh * G + ri.g) * p.q_head_stride + half * HD;
+          uint4 qv[HD / 8];
+          if (on && (reinterpret_cast<uintptr_t>(qrow) & 15u) == 0) {  // 16-byte loads where the row allows
+#pragma unroll
+            for (int i = 0; i < HD / 8; ++i) qv[i] = __ldg(reinterpret_cast<const uint4*>(qrow) + i);
+          } else {
+            const uint32_t* q32 = reinterpret_cast<const uint32_t*>(qrow);
+#pragma unroll
+            for (int i = 0; i < HD / 8; ++i)
+              qv[i] = on ? make_uint4(__ldg(q32 + 4 * i), __ldg(q32 + 4 * i + 1), __ldg(q32 + 4 * i + 2), __ldg(q32 + 4 * i + 3))
+                         : make_uint4(0u, 0u, 0u, 0u);
+          }
+          uint8_t* qb = qsm + (nq & 1) * TILE + (half * (HD / 8)) * (kUmmaRows * 16) + r * 16;
+#pragma unroll
+          for (int i = 0; i < HD / 8; ++i) *reinterpret_cast<uint4*>(qb + i * (kUmmaRows * 16)) = qv[i];
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(q_ready);
+          ++nq;
+        }
+        return true;
+      }
+    };
+    RowItem cur;
+    bool have_cur = next_item(cur);
+    while (ok && have_cur) {
+      const int kv_end = cur.kv_end, ntiles = cur.ntiles, end_r = cur.end_r, beg_r = cur.beg_r;
+      float m_ref = -INFINITY, l = 0.f;
+      for (int j = 0; j < ntiles; ++j) {
+        const int gg = gt + j, b = gg & 1, vs = gg % VS;
+        if (uabort() || !uwait(&s_full[b], (uint32_t)((gg >> 1) & 1))) {
+          ok = false;
+          break;
+        }
+        umma::fence_after();
+        const int tile0 = j * KT, t0 = tile0 + half * HK;  // first token of my half
+        const uint32_t* tm = masks + (gg & 7) * 4;
+        float x[HK];
+#pragma unroll
+        for (int c = 0; c < HK; c += 32) {
+          uint32_t v[32];
+          umma::ld32(lane_base + WG::SCOL + b * 128 + half * HK + c, v);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) x[c + i] = __uint_as_float(v[i]);
+        }
+        // bit c / UNIT of m0 (c < 32) and m1: the block of token t0 + c is loaded
+        uint32_t m0, m1;
+        bool all_in;
+        if constexpr (LOAD == kSlots) {
+          m0 = tm[2 * half];
+          m1 = tm[2 * half + 1];
+          all_in = (m0 & m1) == 0xffffffffu;
+        } else {
+          constexpr int UH = HK / UNIT;
+          const uint32_t mine = (tm[0] >> (half * UH)) & ((1u << UH) - 1u);
+          m0 = mine & ((1u << (UH / 2)) - 1u);
+          m1 = mine >> (UH / 2);
+          all_in = mine == (1u << UH) - 1u;
+        }
+        umma::wait_ld();
+        // a half tile every row of the warp sees whole needs no per-token mask
+        const bool whole = __all_sync(0xffffffffu, all_in && t0 >= beg_r && t0 + HK <= end_r);
+        float mx;  // row max of my scaled scores (log2 units)
+        if (whole) {
+          float h0 = -INFINITY, h1 = -INFINITY;
+          if (qk_scale >= 0.f) {
+#pragma unroll
+            for (int c = 0; c < HK; c += 2) {
+              h0 = fmaxf(h0, x[c]);
+              h1 = fmaxf(h1, x[c + 1]);
+            }
+            mx = fmaxf(h0, h1) * qk_scale;
+          } else {
+#pragma unroll
+            for (int c = 0; c < HK; c += 2) {
+              h0 = fmaxf(h0, -x[c]);
+              h1 = fmaxf(h1, -x[c + 1]);
+            }
+            mx = -fmaxf(h0, h1) * qk_scale;
+          }
+        } else {
+          // seen: tokens [max(beg, 0), end) and [0, sinks) of this half, as bits
+          auto below = [](int n) -> uint64_t { return n <= 0 ? 0ull : (n >= 64 ? ~0ull : (1ull << n) - 1ull); };
+          uint64_t vis = below(end_r - t0) & (~below(beg_r - t0) | below(p.sinks - t0));
+          if (!all_in) {
+            uint64_t in = 0;
+            if constexpr (LOAD == kSlots) {
+              in = (uint64_t)m1 << 32 | m0;
+            } else {
+              constexpr int UH = HK / UNIT;
+              const uint32_t mine = m0 | m1 << (UH / 2);
+#pragma unroll
+              for (int u = 0; u < UH; ++u) in |= (mine >> u) & 1u ? below(UNIT) << (u * UNIT % 64) : 0ull;
+            }
+            vis &= in;
+          }
+          const uint32_t v0 = (uint32_t)vis, v1 = (uint32_t)(vis >> 32);
+          mx = -INFINITY;
+#pragma unroll
+          for (int c = 0; c < HK; ++c) {
+            x[c] = ((c < 32 ? v0 : v1) >> (c & 31)) & 1u ? x[c] * qk_scale : -INFINITY;
+            mx = fmaxf(mx, x[c]);
+          }
+        }
+        // lazy max: rescale only when it rises by more than 2^8
+        float alpha = 1.f;
+        if (mx > m_ref + 8.f) {
+          alpha = m_ref == -INFINITY ? 0.f : fast_exp2(m_ref - mx);
+          m_ref = mx;
+        }
+        const float neg_ref = m_ref == -INFINITY ? 0.f : -m_ref;
+        float2 ps = make_float2(0.f, 0.f);
+        uint32_t hi[32], lo[32];
+        // hi = the upper 16 bits of each fp32 (a bf16, truncated), lo = the exact
+        // remainder rounded to bf16; f16 P is one rounding
+        auto pack_pair = [&](int i, float2 pp) {
+          ps = add_x2(ps, pp);
+          if constexpr (SPLIT) {
+            const uint32_t u0 = __float_as_uint(pp.x), u1 = __float_as_uint(pp.y);
+            hi[i] = __byte_perm(u0, u1, 0x7632);
+            const float2 rem =
+                sub_x2(pp, make_float2(__uint_as_float(u0 & 0xFFFF0000u), __uint_as_float(u1 & 0xFFFF0000u)));
+            lo[i] = MmaOp<T>::pack(rem.x, rem.y);
+          } else {
+            hi[i] = MmaOp<T>::pack(pp.x, pp.y);
+            lo[i] = 0u;
+          }
+        };
+        if (whole) {
+          const float2 sc = make_float2(qk_scale, qk_scale), nr = make_float2(neg_ref, neg_ref);
+#pragma unroll
+          for (int i = 0; i < HK / 2; ++i) {
+            const float2 e = fma_x2(make_float2(x[2 * i], x[2 * i + 1]), sc, nr);
+            pack_pair(i, make_float2(fast_exp2(e.x), fast_exp2(e.y)));
+          }
+        } else {
+          const float2 nr = make_float2(neg_ref, neg_ref);
+#pragma unroll
+          for (int i = 0; i < HK / 2; ++i) {
+            const float2 e = add_x2(make_float2(x[2 * i], x[2 * i + 1]), nr);
+            pack_pair(i, make_float2(fast_exp2(e.x), fast_exp2(e.y)));
+          }
+        }
+        l = l * alpha + (ps.x + ps.y);
+        // (P needs no wait: it goes over this tile's own S, whose last reader, P V
+        // two tiles back, completed before this S did)
+        if (j >= 1 && __any_sync(0xffffffffu, alpha != 1.f)) {
+          if (!uwait(pv_done, (uint32_t)((gg - 1) & 1))) {
+            ok = false;
+            break;
+          }
+          umma::fence_after();
+#pragma unroll
+          for (int c = 0; c < D; c += 16) {
+            uint32_t v[16];
+            umma::ld16(lane_base + WG::OCOL + half * D + c, v);
+            umma::wait_ld();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * alpha);
+            umma::st16(lane_base + WG::OCOL + half * D + c, v);
+          }
+        }
+        // V of tokens nobody sees, in blocks that are loaded for others, becomes 0
+        // (their slots may hold anything, and 0 * NaN = NaN): between the sinks and
+        // the first row's window, and past the last row's end.  Each half clears
+        // its own tokens.
+        const int a0 = p.sinks > t0 ? p.sinks : t0, a1 = cur.v_beg < t0 + HK ? cur.v_beg : t0 + HK;
+        const int e1 = (kv_end + 15) / 16 * 16 < t0 + HK ? (kv_end + 15) / 16 * 16 : t0 + HK;
+        const int e0 = kv_end > t0 ? kv_end : t0;
+        if (a0 < a1 || e0 < e1) {
+          if (!uwait(&v_full[vs], (uint32_t)((gg / VS) & 1))) {
+            ok = false;
+            break;
+          }
+          uint8_t* vst = vring + (size_t)vs * TILE;
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            const int c0 = (w ? e0 : a0) - tile0, c1 = (w ? e1 : a1) - tile0;
+            if constexpr (LOAD == kPages) {
+              if (r < D)
+                for (int tk = c0; tk < c1; ++tk) {
+                  const int ch = (tk % BS) / 8;
+                  const int phys = BS == 32 ? (ch ^ ((r >> 1) & 3)) : (ch ^ ((r >> 2) & 1));
+                  *reinterpret_cast<uint16_t*>(vst + (tk / BS) * PAGE + r * BS * 2 + phys * 16 + (tk % 8) * 2) = 0;
+                }
+            } else {
+              for (int i = r; i < (c1 - c0) * (D / 8); i += 128) {
+                const int tk = c0 + i / (D / 8), ch = i % (D / 8);
+                *reinterpret_cast<uint4*>(vst + (ch >> 3) * HALF + tk * 128 + (ch & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+              }
+            }
+          }
+          fence_proxy_async();
+        }
+        umma::st32(lane_base + WG::SCOL + b * 128 + half * 64, hi);
+        if constexpr (SPLIT) umma::st32(lane_base + WG::SCOL + b * 128 + half * 64 + 32, lo);
+        umma::wait_st();
+        umma::fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[2 * b + half]);
+      }
+      // the next item's Q goes in while this item's last P V runs
+      RowItem nxt;
+      const bool have_nxt = ok && next_item(nxt);
+      bool have = ok && ntiles > 0;
+      if (have) {
+        // (a barrier of its own, once per item: the other half may be a tile behind,
+        // and the parity of pv_done cannot tell the last P V from the one two back)
+        have = uwait(o_done, (uint32_t)(nx & 1));
+        if (!have) ok = false;
+        umma::fence_after();
+      }
+      // the halves' (max, sum) of this row: one exchange per item (the buffer is
+      // free again before any warp can be at its next item's: that item's products
+      // need every warp)
+      float m_o = -INFINITY, l_o = 0.f;
+      if (ntiles > 0) {
+        xbuf[half * 128 + r] = make_float2(m_ref, l);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(xchg);
+        if (!uwait(xchg, (uint32_t)(nx & 1))) ok = false;
+        ++nx;
+        const float2 o = xbuf[(half ^ 1) * 128 + r];
+        m_o = o.x;
+        l_o = o.y;
+      }
+      have = have && ok;
+      const float M = fmaxf(m_ref, m_o);
+      const float w_me = m_ref == -INFINITY ? 0.f : fast_exp2(m_ref - M);
+      const float w_o = m_o == -INFINITY ? 0.f : fast_exp2(m_o - M);
+      const float total = w_me * l + w_o * l_o;
+      // a row with no visible key (or after an abort) is 0; a half without any has
+      // an O that nothing has written, and takes no part
+      const bool nonzero = have && total > 0.f;
+      const float inv = nonzero ? 1.f / total : 0.f;
+      const float f0 = (half == 0 ? w_me : w_o) * inv, f1 = (half == 0 ? w_o : w_me) * inv;
+      const bool u0 = nonzero && f0 != 0.f, u1 = nonzero && f1 != 0.f;
+      T* orow = reinterpret_cast<T*>(p.out) + (cur.q0 + cur.t) * p.out_tok_stride +
+                (int64_t)(cur.kvh * G + cur.g) * p.out_head_stride + half * HD;
+#pragma unroll
+      for (int c = 0; c < HD; c += 16) {
+        uint32_t v[16], w[16];
+        umma::ld16(lane_base + WG::OCOL + half * HD + c, v);
+        umma::ld16(lane_base + WG::OCOL + D + half * HD + c, w);
+        umma::wait_ld();
+        if (cur.in_tile) {
+          uint32_t packed[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            float y[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float o0 = u0 ? __uint_as_float(v[2 * i + e]) * f0 : 0.f;
+              y[e] = u1 ? fmaf(__uint_as_float(w[2 * i + e]), f1, o0) : o0;
+            }
+            packed[i] = pack_out<T>(y[0], y[1]);
+          }
+#pragma unroll
+          for (int i = 0; i < 8; i += 4)
+            *reinterpret_cast<uint4*>(orow + c + 2 * i) =
+                make_uint4(packed[i], packed[i + 1], packed[i + 2], packed[i + 3]);
+        }
+      }
+      umma::fence_before();
+      gt += ntiles;
+      cur = nxt;
+      have_cur = have_nxt;
+    }
+    if (!ok && lane == 0) give_up();
+  }
+
+  umma::fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    umma::fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+  }
+  if (dynamic && threadIdx.x == 0) {
+    __threadfence();
+    if (atomicAdd(&g_umma_sched[slot].done, 1u) == gridDim.x - 1) {
+      atomicExch(&g_umma_sched[slot].next, 0u);
+      atomicExch(&g_umma_sched[slot].done, 0u);
+    }
+  }
+}
+
+}  // namespace kvc

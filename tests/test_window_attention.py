@@ -275,6 +275,16 @@ def test_extend_many_sequences_and_a_long_prefix(gpu):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("layout,bs,d", [("paged", 32, 128), ("paged", 16, 64), ("flash", 16, 64), ("pool", 1, 128)])
+def test_extend_more_items_than_sms(gpu, layout, bs, d):
+    """Each CTA takes several (128-row tile, sequence, KV head) items, of one tile and of more."""
+    rng = np.random.default_rng(35)
+    new = rng.integers(1, 60, 100)
+    lens = new + rng.integers(0, 400, 100)
+    check_extend(Case(35, "bfloat16", lens, 16, 4, d, bs, layout, new=new), 150, 4)
+
+
+@pytest.mark.gpu
 def test_extend_of_one_token(gpu):
     check_extend(Case(34, "float16", [5, 64, 700], 8, 2, 64, 16), 90, 4)
 
