@@ -770,7 +770,7 @@ static cudaError_t launch_window_umma(const PrefillArgs& a, cudaStream_t stream)
   if (items > 0x7fffffffll - 1024) return cudaErrorInvalidValue;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)umma_persistent_ctas(dev, items));
-  cfg.blockDim = dim3(kUmmaThreads);
+  cfg.blockDim = dim3(kWinThreads);
   cfg.dynamicSmemBytes = WG::SMEM;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];

@@ -20,7 +20,13 @@
 //   TMEM (512 columns): S 2 x 128 (P over it: per half 32 columns of hi pairs and
 //   32 of lo pairs), O 2 x D.
 //   Warps 0-7 softmax (warp w and w + 4: the two halves of rows 32 (w & 3) ..),
-//   warp 8 producer, warp 9 (one lane) products.
+//   warp 8 K, warp 9 (one lane) products, warp 10 V, warp 11 items and Q.
+// K and V have a warp each because V waits for a product that comes a softmax
+// later than K's: behind V's wait in one warp, K came 800 cycles late for S.  Warp
+// 11 claims and decodes an item while the one before it runs and copies its Q
+// rows: done by the softmax warps between two items, that cost 12000 cycles an
+// item, against 3300 a tile.  The products run over the tiles of all items in one
+// sequence, S of the next tile (or item) ahead of P V of this one.
 //
 // LOAD: how a tile reaches shared memory.
 //   kPages  paged layout, 16- or 32-token pages: K by 4-row gathers of 8-dim
@@ -40,6 +46,20 @@ namespace kvc {
 constexpr int kPages = 0, kRows = 1, kSlots = 2;
 constexpr uint32_t kLayoutSw128 = 2;
 
+constexpr int kWinThreads = 384;
+constexpr int kKWarp = 8, kVWarp = 10, kItemWarp = 11;
+constexpr int kWinItems = 4;  // item slots
+
+// A decoded work item, handed by warp 11 to the others.
+struct WinItem {
+  int64_t q0;         // row of q / out of the sequence's first new token
+  Seen seen;
+  int t0, g0, nrows;  // (new token, head of the group) of the item's first row; rows
+  int y, kvh, prefix; // prefix less the gap: row's end = prefix + token + 1, virtual
+  int kv_end, ntiles;
+  int state;          // 0 work, 1 rows to be zeroed (bad indices), 2 no further item
+};
+
 template <int D, int BS, int LOAD>
 struct WinUmmaGeom {
   static constexpr int TILE = kUmmaTile * D * 2;  // bytes of one K (or V) tile
@@ -47,10 +67,11 @@ struct WinUmmaGeom {
   static constexpr int Q_OFF = (KS + VS) * TILE;
   static constexpr int XBUF_OFF = Q_OFF + 2 * TILE;          // [2 halves][128 rows] (max, sum)
   static constexpr int BAR_OFF = XBUF_OFF + 2 * 128 * 8;
-  static constexpr int NBARS = 2 * KS + 2 * VS + 2 + 4 + 1 + 1 + 1 + 1 + 1 + 4;
+  static constexpr int NBARS = 2 * KS + 2 * VS + 2 + 4 + 1 + 1 + 4 + 1 + 1 + 2 * kWinItems;
   static constexpr int MASK_OFF = BAR_OFF + NBARS * 8;       // [8 tiles][4] loaded blocks (kSlots: tokens)
-  static constexpr int MISC_OFF = MASK_OFF + 8 * 16;         // abort, tmem address, two item slots
-  static constexpr int SMEM = MISC_OFF + 16;
+  static constexpr int ITEM_OFF = (MASK_OFF + 8 * 16 + 15) / 16 * 16;
+  static constexpr int MISC_OFF = ITEM_OFF + kWinItems * (int)sizeof(WinItem);  // abort, tmem address
+  static constexpr int SMEM = MISC_OFF + 8;
   static constexpr int UNIT = LOAD == kPages ? BS : (LOAD == kRows ? 16 : 1);  // tokens to a mask bit
   static constexpr int UNITS = LOAD == kSlots ? 128 : kUmmaTile / UNIT;
   static constexpr uint32_t SCOL = 0, OCOL = 256;
@@ -59,7 +80,7 @@ struct WinUmmaGeom {
 };
 
 template <typename T, int D, int BS, int LOAD>
-__global__ void __launch_bounds__(kUmmaThreads, 1)
+__global__ void __launch_bounds__(kWinThreads, 1)
     window_umma_kernel(const PrefillArgs p, const __grid_constant__ TmaMaps maps, int tiles_x, int ny, int slot) {
   using namespace mma_detail;
   using WG = WinUmmaGeom<D, BS, LOAD>;
@@ -84,15 +105,16 @@ __global__ void __launch_bounds__(kUmmaThreads, 1)
   uint64_t* p_full = s_full + 2;    // [2 buffers][2 halves]
   uint64_t* pv_done = p_full + 4;
   uint64_t* o_done = pv_done + 1;
-  uint64_t* q_ready = o_done + 1;
-  uint64_t* all_done = q_ready + 1;
+  uint64_t* q_full = o_done + 1;    // [2 buffers]
+  uint64_t* q_empty = q_full + 2;
+  uint64_t* all_done = q_empty + 2;
   uint64_t* xchg = all_done + 1;
-  uint64_t* item_full = xchg + 1;
-  uint64_t* item_empty = item_full + 2;
+  uint64_t* item_full = xchg + 1;   // [kWinItems]
+  uint64_t* item_empty = item_full + kWinItems;
   uint32_t* masks = reinterpret_cast<uint32_t*>(smem_wu + WG::MASK_OFF);
+  WinItem* items = reinterpret_cast<WinItem*>(smem_wu + WG::ITEM_OFF);
   volatile int* s_abort = reinterpret_cast<volatile int*>(smem_wu + WG::MISC_OFF);
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(smem_wu + WG::MISC_OFF + 4);
-  volatile int* s_item = reinterpret_cast<volatile int*>(smem_wu + WG::MISC_OFF + 8);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int G = p.num_heads / p.num_kv_heads;
@@ -116,27 +138,30 @@ __global__ void __launch_bounds__(kUmmaThreads, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&s_full[b], 2);
-      mbar_init(&item_full[b], 1);
-      mbar_init(&item_empty[b], 9);
+      mbar_init(&q_full[b], 1);
+      mbar_init(&q_empty[b], 1);
     }
     for (int b = 0; b < 4; ++b) mbar_init(&p_full[b], 4);
+    for (int b = 0; b < kWinItems; ++b) {
+      mbar_init(&item_full[b], 1);
+      mbar_init(&item_empty[b], 11);
+    }
     mbar_init(pv_done, 1);
     mbar_init(o_done, 1);
-    mbar_init(q_ready, 8);
     mbar_init(all_done, 1);
     mbar_init(xchg, 8);
     mbar_fence_init();
   }
   // V of blocks that a tile does not load meets P = 0 (0 * NaN = NaN): the ring
   // starts from zeros
-  for (int i = threadIdx.x; i < VS * TILE / 16; i += kUmmaThreads)
+  for (int i = threadIdx.x; i < VS * TILE / 16; i += kWinThreads)
     reinterpret_cast<uint4*>(vring)[i] = make_uint4(0u, 0u, 0u, 0u);
   fence_proxy_async();
   if (warp == kMmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(s_tmem)),
                  "r"(512));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
-  } else if (warp == kProducerWarp && lane == 0) {
+  } else if (warp == kKWarp && lane == 0) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&maps.v)) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&maps.k)) : "memory");
   }
@@ -152,58 +177,129 @@ __global__ void __launch_bounds__(kUmmaThreads, 1)
     set_status(&g_decode_status, KVC_STATUS_WAIT_TIMEOUT);
   };
 
-  if (warp == kProducerWarp) {
-    // ---- producer: claims items, hands each to the other warps, loads its tiles
-    int gt = 0, npub = 0;  // tiles issued, items handed over
-    int nk = 0, nv = 0;    // K and V tiles asked for
-    bool stop = false;
-    auto publish = [&](int idx) -> bool {  // (lane 0)
-      const int sl = npub & 1;
-      if (npub >= 2 && !umma::wait(&item_empty[sl], (uint32_t)(((npub >> 1) - 1) & 1))) return false;
-      s_item[sl] = idx;
-      mbar_arrive(&item_full[sl]);
-      ++npub;
-      return true;
-    };
+  // Item k of this CTA, for a whole warp: false on a failed wait.
+  auto take_item = [&](int k, WinItem& it) -> bool {
+    const int sl = k % kWinItems;
+    if (!__all_sync(0xffffffffu, umma::wait(&item_full[sl], (uint32_t)((k / kWinItems) & 1)))) return false;
+    it = items[sl];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&item_empty[sl]);
+    return true;
+  };
+
+  if (warp == kItemWarp) {
+    // ---- items and their Q
     UmmaSched* sched = &g_umma_sched[slot];
-    // every lane learns whether lane 0's wait came through and nobody gave up
-    auto warp_wait = [&](bool need, uint64_t* bar, uint32_t parity) -> bool {
-      bool ok = true;
-      if (need && lane == 0) ok = umma::wait(bar, parity);
-      ok = __shfl_sync(0xffffffffu, ok, 0);
-      if (!ok && lane == 0) give_up();
-      return ok && !__shfl_sync(0xffffffffu, abort_now() ? 1 : 0, 0);
-    };
-    for (int idx = blockIdx.x; idx < n_items && !stop;) {
-      const UmmaItem it = umma_item<false, true>(p, idx, tiles_x, ny);
-      if (it.bad && it.first_tile && it.kvh == 0 && lane == 0) set_status(&g_decode_status, KVC_STATUS_INDEX_OOB);
-      auto claim = [&]() -> int {
-        unsigned nx = (unsigned)n_items;
-        if (dynamic && lane == 0) nx = gridDim.x + atomicAdd(&sched->next, 1u);
-        nx = __shfl_sync(0xffffffffu, nx, 0);
-        return nx < (unsigned)n_items ? (int)nx : n_items;
-      };
-      if (it.skip) {
-        idx = claim();
-        continue;
-      }
-      // the item's query rows toward L2, ahead of the softmax warps' loads
-      if (!it.bad && it.ntiles > 0) {
-        const int64_t nrows = it.rows - it.R0 < kUmmaRows ? it.rows - it.R0 : kUmmaRows;
-        for (int r = lane; r < nrows; r += 32) {
-          const int64_t R = it.R0 + r, t = R / G;
-          const char* a = reinterpret_cast<const char*>(reinterpret_cast<const T*>(p.q) + (it.q0 + t) * p.q_tok_stride +
-                                                        (int64_t)(it.kvh * G + (int)(R - t * G)) * p.q_head_stride);
-#pragma unroll
-          for (int b = 0; b < D * 2; b += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(a + b));
+    int npub = 0, nq = 0;  // items handed over, of them with keys
+    bool ok = true;
+    auto publish = [&](const WinItem& it) -> bool {
+      const int sl = npub % kWinItems;
+      bool fine = true;
+      if (lane == 0) {
+        if (npub >= kWinItems) fine = umma::wait(&item_empty[sl], (uint32_t)((npub / kWinItems - 1) & 1));
+        if (fine) {
+          items[sl] = it;
+          mbar_arrive(&item_full[sl]);  // (release)
         }
       }
-      bool handed = true;
-      if (lane == 0) handed = publish(idx);
-      if (!__shfl_sync(0xffffffffu, handed, 0)) {
-        if (lane == 0) give_up();
+      ++npub;
+      return __shfl_sync(0xffffffffu, fine, 0) && !__shfl_sync(0xffffffffu, abort_now() ? 1 : 0, 0);
+    };
+    for (int idx = blockIdx.x; idx < n_items && ok;) {
+      const UmmaItem u = umma_item<false, true>(p, idx, tiles_x, ny);
+      if (u.bad && u.first_tile && u.kvh == 0 && lane == 0) set_status(&g_decode_status, KVC_STATUS_INDEX_OOB);
+      if (!u.skip) {
+        WinItem it;
+        it.q0 = u.q0;
+        it.seen = u.seen;
+        it.t0 = (int)(u.R0 / G);
+        it.g0 = (int)(u.R0 - (int64_t)it.t0 * G);
+        it.nrows = (int)(u.rows - u.R0 < kUmmaRows ? u.rows - u.R0 : kUmmaRows);
+        it.y = u.y;
+        it.kvh = u.kvh;
+        it.prefix = u.prefix;
+        it.kv_end = u.kv_end;
+        it.ntiles = u.ntiles;
+        it.state = u.bad ? 1 : 0;
+        ok = publish(it);
+        if (ok && it.ntiles > 0) {
+          // Q rows into buffer nq & 1 ([D/8 chunks][128 rows][8 dims]; rows past the
+          // last are zero), whose last reader is S of the item two back
+          const int buf = nq & 1;
+          bool free = true;
+          if (nq >= 2 && lane == 0) free = umma::wait(&q_empty[buf], (uint32_t)(((nq >> 1) - 1) & 1));
+          ok = __shfl_sync(0xffffffffu, free, 0);
+          if (ok) {
+            const T* qbase = reinterpret_cast<const T*>(p.q);
+            const T* row[4];
+            bool on[4], wide = true;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int r = i * 32 + lane, x = it.g0 + r, dt = x / G;
+              on[i] = r < it.nrows;
+              row[i] = on[i] ? qbase + (it.q0 + it.t0 + dt) * p.q_tok_stride +
+                                   (int64_t)(it.kvh * G + (x - dt * G)) * p.q_head_stride
+                             : qbase;
+              wide = wide && (!on[i] || (reinterpret_cast<uintptr_t>(row[i]) & 15u) == 0);
+            }
+            // (a row past the last reads nothing, but its address must be aligned too)
+            wide = __all_sync(0xffffffffu, wide) && (reinterpret_cast<uintptr_t>(qbase) & 15u) == 0;
+            uint8_t* qb = qsm + buf * TILE + lane * 16;
+            if (wide) {
+#pragma unroll 4
+              for (int c = 0; c < D / 8; ++c)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  cp_async16_zfill(qb + c * (kUmmaRows * 16) + i * 512, row[i] + c * 8, on[i] ? 16u : 0u);
+              asm volatile("cp.async.wait_all;" ::: "memory");
+            } else {
+              for (int c = 0; c < D / 8; ++c)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  const uint32_t* q32 = reinterpret_cast<const uint32_t*>(row[i] + c * 8);
+                  *reinterpret_cast<uint4*>(qb + c * (kUmmaRows * 16) + i * 512) =
+                      on[i] ? make_uint4(__ldg(q32), __ldg(q32 + 1), __ldg(q32 + 2), __ldg(q32 + 3))
+                            : make_uint4(0u, 0u, 0u, 0u);
+                }
+            }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&q_full[buf]);
+            ++nq;
+          }
+        }
+      }
+      // the next item, once Q of this one is in (so at most one item is claimed ahead)
+      unsigned nx = (unsigned)n_items;
+      if (dynamic && lane == 0) nx = gridDim.x + atomicAdd(&sched->next, 1u);
+      nx = __shfl_sync(0xffffffffu, nx, 0);
+      idx = nx < (unsigned)n_items ? (int)nx : n_items;
+    }
+    if (ok) {
+      WinItem it;
+      memset(&it, 0, sizeof(it));
+      it.state = 2;
+      ok = publish(it);
+    }
+    if (!ok && lane == 0) give_up();
+    __syncwarp();
+  } else if (warp == kKWarp || warp == kVWarp) {
+    // ---- one ring's tiles, K or V
+    const bool is_k = warp == kKWarp;
+    const int stages = is_k ? KS : VS;
+    uint64_t* full = is_k ? k_full : v_full;
+    uint64_t* empty = is_k ? k_empty : v_empty;
+    uint8_t* ring = is_k ? kring : vring;
+    const CUtensorMap* map = is_k ? &maps.k : &maps.v;
+    int g = 0, st = 0, round = 0;  // tiles asked for, the next one's stage and turn of the ring
+    bool ok = true;
+    for (int k = 0; ok; ++k) {
+      WinItem it;
+      if (!take_item(k, it)) {
+        ok = false;
         break;
       }
+      if (it.state == 2) break;
       const int kvh = it.kvh, kv_end = it.kv_end, ntiles = it.ntiles;
       const uint32_t* table = p.block_tables + (int64_t)it.y * p.table_stride;
       const int tbs = p.block_size;
@@ -225,65 +321,52 @@ __global__ void __launch_bounds__(kUmmaThreads, 1)
       uint32_t id[4];
       load_ids(0, id);
       for (int j = 0; j < ntiles; ++j) {
-        const int g = gt + j, ks = g % KS, vs = g % VS, t0 = j * KT;
-        if (!warp_wait(g >= KS, &k_empty[ks], (uint32_t)(((g / KS) - 1) & 1))) {
-          stop = true;
+        const int t0 = j * KT;
+        bool free = true;
+        if (round > 0 && lane == 0) free = umma::wait(&empty[st], (uint32_t)((round - 1) & 1));
+        free = __shfl_sync(0xffffffffu, free, 0);
+        if (!free || __shfl_sync(0xffffffffu, abort_now() ? 1 : 0, 0)) {
+          ok = false;
           break;
         }
-        uint8_t* kst = kring + (size_t)ks * TILE;
-        uint8_t* vst = vring + (size_t)vs * TILE;
+        uint8_t* dst = ring + (size_t)st * TILE;
         uint32_t* tm = masks + (g & 7) * 4;
         uint32_t next[4];
         if constexpr (LOAD == kSlots) {
           // a token without a block gathers a loaded token's row (and is masked)
-          uint32_t ok = 0, oob = 0;
+          uint32_t good4 = 0, oob = 0;
           int row[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int tok = t0 + 4 * lane + e;
             const bool in = tok < kv_end, good = in && (int64_t)id[e] < p.num_blocks;
-            ok |= good ? 1u << e : 0u;
+            good4 |= good ? 1u << e : 0u;
             oob |= in && !good ? 1u : 0u;
             row[e] = good ? (int)((tbs == 1 ? (int64_t)id[e] : (int64_t)id[e] * tbs + tok % tbs) * p.num_kv_heads + kvh) : -1;
           }
           if (oob) set_status(&g_decode_status, KVC_STATUS_BLOCK_OOB);
-          const uint32_t any = __ballot_sync(0xffffffffu, ok != 0u);
-          int spare = ok ? row[__ffs(ok) - 1] : 0;
+          const uint32_t any = __ballot_sync(0xffffffffu, good4 != 0u);
+          int spare = good4 ? row[__ffs(good4) - 1] : 0;
           spare = __shfl_sync(0xffffffffu, spare, any ? __ffs(any) - 1 : 0);
 #pragma unroll
           for (int e = 0; e < 4; ++e) row[e] = row[e] >= 0 ? row[e] : spare;
-          // lanes 8w .. 8w + 7 hold the 32 tokens of word w
-          uint32_t word = ok << (4 * (lane & 7));
+          if (is_k) {  // lanes 8w .. 8w + 7 hold the 32 tokens of word w
+            uint32_t word = good4 << (4 * (lane & 7));
 #pragma unroll
-          for (int o = 1; o < 8; o <<= 1) word |= __shfl_xor_sync(0xffffffffu, word, o);
-          if ((lane & 7) == 0) tm[lane >> 3] = word;
+            for (int o = 1; o < 8; o <<= 1) word |= __shfl_xor_sync(0xffffffffu, word, o);
+            if ((lane & 7) == 0) tm[lane >> 3] = word;
+          }
           load_ids(j + 1, next);
           __syncwarp();
           if (lane == 0) {
-            if (any) mbar_arrive_expect_tx(&k_full[ks], (uint32_t)TILE);
-            else mbar_arrive(&k_full[ks]);
+            if (any) mbar_arrive_expect_tx(&full[st], (uint32_t)TILE);
+            else mbar_arrive(&full[st]);
           }
-          nk = g + 1;
           __syncwarp();
           if (any) {
 #pragma unroll
             for (int h = 0; h < D / 64; ++h)
-              tma_gather4(kst + h * HALF + lane * 512, &maps.k, 64 * h, row[0], row[1], row[2], row[3], &k_full[ks]);
-          }
-          if (!warp_wait(g >= VS, &v_empty[vs], (uint32_t)(((g / VS) - 1) & 1))) {
-            stop = true;
-            break;
-          }
-          if (lane == 0) {
-            if (any) mbar_arrive_expect_tx(&v_full[vs], (uint32_t)TILE);
-            else mbar_arrive(&v_full[vs]);
-          }
-          nv = g + 1;
-          __syncwarp();
-          if (any) {
-#pragma unroll
-            for (int h = 0; h < D / 64; ++h)
-              tma_gather4(vst + h * HALF + lane * 512, &maps.v, 64 * h, row[0], row[1], row[2], row[3], &v_full[vs]);
+              tma_gather4(dst + h * HALF + lane * 512, map, 64 * h, row[0], row[1], row[2], row[3], &full[st]);
           }
         } else {
           const int tok = t0 + lane * UNIT;
@@ -293,70 +376,56 @@ __global__ void __launch_bounds__(kUmmaThreads, 1)
           const uint32_t mine = id[0];
           load_ids(j + 1, next);
           if (lane == 0) {
-            tm[0] = mask;
-            const uint32_t unit_bytes = (uint32_t)(UNIT * D * 2);
-            if (!mask) mbar_arrive(&k_full[ks]);
-            else mbar_arrive_expect_tx(&k_full[ks], LOAD == kPages ? (uint32_t)TILE : (uint32_t)__popc(mask) * unit_bytes);
+            if (is_k) tm[0] = mask;
+            if (!mask) mbar_arrive(&full[st]);
+            else
+              mbar_arrive_expect_tx(&full[st], LOAD == kPages && is_k ? (uint32_t)TILE
+                                                                      : (uint32_t)__popc(mask) * (uint32_t)(UNIT * D * 2));
           }
-          nk = g + 1;
           __syncwarp();
-          const int row = LOAD == kRows ? (int)mine * tbs + tok % tbs : 0;  // (rows are below 2^31: the host checked)
           if (mask) {
             if constexpr (LOAD == kPages) {
-              // chunk row c of a page: row base + c; pages without keys gather a loaded page's rows
-              const int base = (int)(((int64_t)mine * p.k_block_stride + (int64_t)kvh * p.k_head_stride) / (BS * 8));
-              const int any = __shfl_sync(0xffffffffu, base, __ffs(mask) - 1);
-              int rb[PAGES];
+              if (is_k) {
+                // chunk row c of a page: row base + c; pages without keys gather a loaded page's rows
+                const int base = (int)(((int64_t)mine * p.k_block_stride + (int64_t)kvh * p.k_head_stride) / (BS * 8));
+                const int any = __shfl_sync(0xffffffffu, base, __ffs(mask) - 1);
+                int rb[PAGES];
 #pragma unroll
-              for (int i = 0; i < PAGES; ++i) {
-                const int b = __shfl_sync(0xffffffffu, base, i);
-                rb[i] = (mask >> i) & 1u ? b : any;
-              }
-              if (lane < D / 8) {
+                for (int i = 0; i < PAGES; ++i) {
+                  const int b = __shfl_sync(0xffffffffu, base, i);
+                  rb[i] = (mask >> i) & 1u ? b : any;
+                }
+                if (lane < D / 8) {
 #pragma unroll
-                for (int q = 0; q < PAGES; q += 4)
-                  tma_gather4(kst + lane * KT * 16 + q * BS * 16, &maps.k, 0, rb[q] + lane, rb[q + 1] + lane,
-                              rb[q + 2] + lane, rb[q + 3] + lane, &k_full[ks]);
+                  for (int q = 0; q < PAGES; q += 4)
+                    tma_gather4(dst + lane * KT * 16 + q * BS * 16, map, 0, rb[q] + lane, rb[q + 1] + lane,
+                                rb[q + 2] + lane, rb[q + 3] + lane, &full[st]);
+                }
+              } else if (good) {
+                tma_load_4d(dst + lane * PAGE, map, 0, 0, kvh, (int)mine, &full[st]);
               }
             } else if (good) {
+              const int row = (int)mine * tbs + tok % tbs;  // (rows are below 2^31: the host checked)
 #pragma unroll
               for (int h = 0; h < D / 64; ++h)
-                tma_load_3d(kst + h * HALF + lane * 16 * 128, &maps.k, 64 * h, kvh, row, &k_full[ks]);
+                tma_load_3d(dst + h * HALF + lane * 16 * 128, map, 64 * h, kvh, row, &full[st]);
             }
           }
-          if (!warp_wait(g >= VS, &v_empty[vs], (uint32_t)(((g / VS) - 1) & 1))) {
-            stop = true;
-            break;
-          }
-          if (lane == 0) {
-            if (mask) mbar_arrive_expect_tx(&v_full[vs], (uint32_t)__popc(mask) * (uint32_t)(UNIT * D * 2));
-            else mbar_arrive(&v_full[vs]);
-          }
-          nv = g + 1;
-          __syncwarp();
-          if (good) {
-            if constexpr (LOAD == kPages) {
-              tma_load_4d(vst + lane * PAGE, &maps.v, 0, 0, kvh, (int)mine, &v_full[vs]);
-            } else {
-#pragma unroll
-              for (int h = 0; h < D / 64; ++h)
-                tma_load_3d(vst + h * HALF + lane * 16 * 128, &maps.v, 64 * h, kvh, row, &v_full[vs]);
-            }
-          }
+        }
+        ++g;
+        if (++st == stages) {
+          st = 0;
+          ++round;
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) id[e] = next[e];
       }
-      gt += ntiles;
-      if (!stop) idx = claim();
     }
-    if (lane == 0 && !publish(n_items)) give_up();
+    if (!ok && lane == 0) give_up();
     // shared memory outlives every copy, after an abort too: bounded waits on the
     // last copy asked for in each stage
-    if (lane == 0) {
-      for (int g = nk > KS ? nk - KS : 0; g < nk; ++g) umma::wait(&k_full[g % KS], (uint32_t)((g / KS) & 1));
-      for (int g = nv > VS ? nv - VS : 0; g < nv; ++g) umma::wait(&v_full[g % VS], (uint32_t)((g / VS) & 1));
-    }
+    if (lane == 0)
+      for (int i = g > stages ? g - stages : 0; i < g; ++i) umma::wait(&full[i % stages], (uint32_t)((i / stages) & 1));
     __syncwarp();
   } else if (warp == kMmaWarp) {
     // ---- products (one lane)
@@ -370,59 +439,58 @@ __global__ void __launch_bounds__(kUmmaThreads, 1)
           LOAD != kPages ? umma::smem_desc(smem_u32(vring), HALF, 1024, kLayoutSw128)
                          : (BS == 32 ? umma::smem_desc(smem_u32(vring), 16, 512, umma::kLayoutSw64)
                                      : umma::smem_desc(smem_u32(vring), 16, 256, umma::kLayoutSw32));
-      int gt = 0, nit = 0, nread = 0;
+      // S of tile g, then P V of tile g - 1, over the tiles of all items
+      int g = 0, nq = 0;                        // tiles, items with keys so far
+      int pv_left = 0, pv_j = -1;               // the tile whose P V is due: keys from its first token on, its place
+      bool pv_last = false;                     // .. and whether its item ends with it
       bool ok = true;
-      for (;;) {
-        const int sl = nread & 1;
-        if (abort_now() || !umma::wait(&item_full[sl], (uint32_t)((nread >> 1) & 1))) {
-          ok = false;
-          break;
-        }
-        const int idx = s_item[sl];
-        mbar_arrive(&item_empty[sl]);
-        ++nread;
-        if (idx >= n_items) break;
-        const UmmaItem it = umma_item<false, true>(p, idx, tiles_x, ny);
-        if (it.skip || it.ntiles == 0) continue;
-        if (abort_now() || !umma::wait(q_ready, (uint32_t)(nit & 1))) {
-          ok = false;
-          break;
-        }
-        umma::fence_after();
-        const uint64_t qd = q_desc0 + (uint64_t)(((nit & 1) * TILE) >> 4);
-        ++nit;
-        const int kv_end = it.kv_end, ntiles = it.ntiles;
-        // O_h += P_h V_h of tile j (this CTA's tile g), both halves
-        auto issue_pv = [&](int j, int g) -> bool {
-          const int b = g & 1, vs = g % VS;
-          if (!umma::wait(&v_full[vs], (uint32_t)((g / VS) & 1))) return false;
-          const uint64_t vd = v_desc0 + (uint64_t)((vs * TILE) >> 4);
+      auto issue_pv = [&]() -> bool {
+        const int t = g - 1, b = t & 1, vs = t % VS;
+        if (!umma::wait(&v_full[vs], (uint32_t)((t / VS) & 1))) return false;
+        const uint64_t vd = v_desc0 + (uint64_t)((vs * TILE) >> 4);
+        // an item's first product overwrites both O, which every softmax warp has
+        // read by the time it hands over its part of the first tile
+        if (pv_j == 0 && !umma::wait(&p_full[2 * b + 1], (uint32_t)((t >> 1) & 1))) return false;
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            if (!umma::wait(&p_full[2 * b + h], (uint32_t)((g >> 1) & 1))) return false;
-            // (an item's first product overwrites both O, which every softmax warp
-            // has read by the time it hands over its part of the first tile)
-            if (j == 0 && h == 0 && !umma::wait(&p_full[2 * b + 1], (uint32_t)((g >> 1) & 1))) return false;
-            umma::fence_after();
-            const int left = kv_end - (j * KT + h * 64), steps = left > 0 ? (left + 15) / 16 : 0;
-            const uint32_t pcol = tmem + WG::SCOL + b * 128 + h * 64, ocol = tmem + WG::OCOL + h * D;
+        for (int h = 0; h < 2; ++h) {
+          if (!umma::wait(&p_full[2 * b + h], (uint32_t)((t >> 1) & 1))) return false;
+          umma::fence_after();
+          const int left = pv_left - h * 64, steps = left > 0 ? (left + 15) / 16 : 0;
+          const uint32_t pcol = tmem + WG::SCOL + b * 128 + h * 64, ocol = tmem + WG::OCOL + h * D;
 #pragma unroll
-            for (int ks = 0; ks < 4; ++ks) {
-              if (ks < steps) {
-                const int tk = h * 64 + 16 * ks;
-                const uint64_t d =
-                    vd + (uint64_t)((LOAD == kPages ? (tk / BS) * PAGE + (tk % BS) * 2 : tk * 128) >> 4);
-                umma::mma_ts(ocol, pcol + 8 * ks, d, idO, (j > 0 || ks > 0) ? 1u : 0u);
-                if (SPLIT) umma::mma_ts(ocol, pcol + 32 + 8 * ks, d, idO, 1u);
-              }
+          for (int ks = 0; ks < 4; ++ks) {
+            if (ks < steps) {
+              const int tk = h * 64 + 16 * ks;
+              const uint64_t d = vd + (uint64_t)((LOAD == kPages ? (tk / BS) * PAGE + (tk % BS) * 2 : tk * 128) >> 4);
+              umma::mma_ts(ocol, pcol + 8 * ks, d, idO, (pv_j > 0 || ks > 0) ? 1u : 0u);
+              if (SPLIT) umma::mma_ts(ocol, pcol + 32 + 8 * ks, d, idO, 1u);
             }
           }
-          umma::commit(pv_done);
-          umma::commit(&v_empty[vs]);
-          return true;
-        };
-        for (int j = 0; j < ntiles && ok; ++j) {
-          const int g = gt + j, ks0 = g % KS, b = g & 1;
+        }
+        umma::commit(pv_done);
+        umma::commit(&v_empty[vs]);
+        if (pv_last) umma::commit(o_done);
+        return true;
+      };
+      for (int k = 0; ok; ++k) {
+        const int sl = k % kWinItems;
+        if (abort_now() || !umma::wait(&item_full[sl], (uint32_t)((k / kWinItems) & 1))) {
+          ok = false;
+          break;
+        }
+        const int kv_end = items[sl].kv_end, ntiles = items[sl].ntiles, state = items[sl].state;
+        mbar_arrive(&item_empty[sl]);
+        if (state == 2) break;
+        if (ntiles == 0) continue;
+        const int buf = nq & 1;
+        if (abort_now() || !umma::wait(&q_full[buf], (uint32_t)((nq >> 1) & 1))) {
+          ok = false;
+          break;
+        }
+        ++nq;
+        const uint64_t qd = q_desc0 + (uint64_t)((buf * TILE) >> 4);
+        for (int j = 0; j < ntiles; ++j) {
+          const int ks0 = g % KS, b = g & 1;
           if (abort_now() || !umma::wait(&k_full[ks0], (uint32_t)((g / KS) & 1))) {
             ok = false;
             break;
@@ -437,12 +505,18 @@ __global__ void __launch_bounds__(kUmmaThreads, 1)
           umma::commit(&s_full[b]);
           mbar_arrive(&s_full[b]);  // (release: the tile's masks, seen through k_full, are seen by whoever waits)
           umma::commit(&k_empty[ks0]);
-          if (j >= 1 && !issue_pv(j - 1, g - 1)) ok = false;
+          if (j == ntiles - 1) umma::commit(&q_empty[buf]);
+          if (pv_j >= 0 && !issue_pv()) {
+            ok = false;
+            break;
+          }
+          ++g;
+          pv_j = j;
+          pv_left = kv_end - j * KT;
+          pv_last = j == ntiles - 1;
         }
-        if (ok && !abort_now()) ok = issue_pv(ntiles - 1, gt + ntiles - 1);
-        umma::commit(o_done);
-        gt += ntiles;
       }
+      if (ok && pv_j >= 0) ok = issue_pv();
       if (!ok) give_up();
       umma::commit(all_done);
       umma::wait(all_done, 0);
@@ -461,72 +535,19 @@ __global__ void __launch_bounds__(kUmmaThreads, 1)
     constexpr int HD = D / 2;   // output columns per half
     const float qk_scale = p.scale * kLog2e;
     bool ok = true;
-    int gt = 0, nread = 0, nq = 0, nx = 0;
-    struct RowItem {
-      int64_t q0;
-      int kvh, kv_end, ntiles, v_beg;
-      int t, g, end_r, beg_r;
-      bool in_tile;
-    };
-    // the next item with work, its Q rows staged into shared buffer nq & 1 ([D/8
-    // chunks][128 rows][8], half of the chunks per half) and handed over; every
-    // product that read this buffer, two items back, completed before that item's
-    // epilogue
-    auto next_item = [&](RowItem& ri) -> bool {
-      for (;;) {
-        const int sl = nread & 1;
-        if (uabort() || !uwait(&item_full[sl], (uint32_t)((nread >> 1) & 1))) {
-          ok = false;
-          return false;
-        }
-        const int idx = s_item[sl];
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&item_empty[sl]);
-        ++nread;
-        if (idx >= n_items) return false;
-        const UmmaItem it = umma_item<false, true>(p, idx, tiles_x, ny);
-        if (it.skip) continue;
-        ri.q0 = it.q0;
-        ri.kvh = it.kvh;
-        ri.kv_end = it.kv_end;
-        ri.ntiles = it.ntiles;
-        ri.v_beg = it.seen.beg;
-        const int64_t R = it.R0 + r;
-        ri.in_tile = R < it.rows;
-        ri.t = ri.in_tile ? (int)(R / G) : 0;
-        ri.g = ri.in_tile ? (int)(R - (int64_t)ri.t * G) : 0;
-        const bool on = ri.in_tile && !it.bad;
-        ri.end_r = on ? it.prefix + ri.t + 1 : 0;
-        ri.beg_r = ri.end_r > p.window ? ri.end_r - p.window : 0;
-        if (it.ntiles > 0) {
-          const T* qrow = reinterpret_cast<const T*>(p.q) + (it.q0 + ri.t) * p.q_tok_stride +
-                          (int64_t)(it.kvh * G + ri.g) * p.q_head_stride + half * HD;
-          uint4 qv[HD / 8];
-          if (on && (reinterpret_cast<uintptr_t>(qrow) & 15u) == 0) {  // 16-byte loads where the row allows
-#pragma unroll
-            for (int i = 0; i < HD / 8; ++i) qv[i] = __ldg(reinterpret_cast<const uint4*>(qrow) + i);
-          } else {
-            const uint32_t* q32 = reinterpret_cast<const uint32_t*>(qrow);
-#pragma unroll
-            for (int i = 0; i < HD / 8; ++i)
-              qv[i] = on ? make_uint4(__ldg(q32 + 4 * i), __ldg(q32 + 4 * i + 1), __ldg(q32 + 4 * i + 2), __ldg(q32 + 4 * i + 3))
-                         : make_uint4(0u, 0u, 0u, 0u);
-          }
-          uint8_t* qb = qsm + (nq & 1) * TILE + (half * (HD / 8)) * (kUmmaRows * 16) + r * 16;
-#pragma unroll
-          for (int i = 0; i < HD / 8; ++i) *reinterpret_cast<uint4*>(qb + i * (kUmmaRows * 16)) = qv[i];
-          fence_proxy_async();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(q_ready);
-          ++nq;
-        }
-        return true;
+    int gt = 0, nx = 0;  // tiles and items with keys so far
+    for (int k = 0; ok; ++k) {
+      WinItem it;
+      if (uabort() || !take_item(k, it)) {
+        ok = false;
+        break;
       }
-    };
-    RowItem cur;
-    bool have_cur = next_item(cur);
-    while (ok && have_cur) {
-      const int kv_end = cur.kv_end, ntiles = cur.ntiles, end_r = cur.end_r, beg_r = cur.beg_r;
+      if (it.state == 2) break;
+      const int kv_end = it.kv_end, ntiles = it.ntiles;
+      const bool in_tile = r < it.nrows;
+      const int x0 = it.g0 + r, dt = x0 / G, row_t = it.t0 + dt, row_g = x0 - dt * G;
+      const int end_r = in_tile && it.state == 0 ? it.prefix + row_t + 1 : 0;
+      const int beg_r = end_r > p.window ? end_r - p.window : 0;
       float m_ref = -INFINITY, l = 0.f;
       for (int j = 0; j < ntiles; ++j) {
         const int gg = gt + j, b = gg & 1, vs = gg % VS;
@@ -564,21 +585,20 @@ __global__ void __launch_bounds__(kUmmaThreads, 1)
         const bool whole = __all_sync(0xffffffffu, all_in && t0 >= beg_r && t0 + HK <= end_r);
         float mx;  // row max of my scaled scores (log2 units)
         if (whole) {
-          float h0 = -INFINITY, h1 = -INFINITY;
+          // (the largest raw score, or the smallest for a negative scale; four chains)
+          float h[4] = {x[0], x[1], x[2], x[3]};
           if (qk_scale >= 0.f) {
 #pragma unroll
-            for (int c = 0; c < HK; c += 2) {
-              h0 = fmaxf(h0, x[c]);
-              h1 = fmaxf(h1, x[c + 1]);
-            }
-            mx = fmaxf(h0, h1) * qk_scale;
+            for (int c = 4; c < HK; c += 4)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) h[e] = fmaxf(h[e], x[c + e]);
+            mx = fmaxf(fmaxf(h[0], h[1]), fmaxf(h[2], h[3])) * qk_scale;
           } else {
 #pragma unroll
-            for (int c = 0; c < HK; c += 2) {
-              h0 = fmaxf(h0, -x[c]);
-              h1 = fmaxf(h1, -x[c + 1]);
-            }
-            mx = -fmaxf(h0, h1) * qk_scale;
+            for (int c = 4; c < HK; c += 4)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) h[e] = fminf(h[e], x[c + e]);
+            mx = fminf(fminf(h[0], h[1]), fminf(h[2], h[3])) * qk_scale;
           }
         } else {
           // seen: tokens [max(beg, 0), end) and [0, sinks) of this half, as bits
@@ -612,40 +632,35 @@ __global__ void __launch_bounds__(kUmmaThreads, 1)
         }
         const float neg_ref = m_ref == -INFINITY ? 0.f : -m_ref;
         float2 ps = make_float2(0.f, 0.f);
-        uint32_t hi[32], lo[32];
-        // hi = the upper 16 bits of each fp32 (a bf16, truncated), lo = the exact
-        // remainder rounded to bf16; f16 P is one rounding
-        auto pack_pair = [&](int i, float2 pp) {
-          ps = add_x2(ps, pp);
-          if constexpr (SPLIT) {
-            const uint32_t u0 = __float_as_uint(pp.x), u1 = __float_as_uint(pp.y);
-            hi[i] = __byte_perm(u0, u1, 0x7632);
-            const float2 rem =
-                sub_x2(pp, make_float2(__uint_as_float(u0 & 0xFFFF0000u), __uint_as_float(u1 & 0xFFFF0000u)));
-            lo[i] = MmaOp<T>::pack(rem.x, rem.y);
-          } else {
-            hi[i] = MmaOp<T>::pack(pp.x, pp.y);
-            lo[i] = 0u;
-          }
-        };
-        if (whole) {
-          const float2 sc = make_float2(qk_scale, qk_scale), nr = make_float2(neg_ref, neg_ref);
+        // P over this tile's own S, 16 pairs of tokens at a time, so that the stores
+        // overlap the next pairs' exponentials: hi = the upper 16 bits of each fp32
+        // (a bf16, truncated), lo = the exact remainder rounded to bf16; f16 P is
+        // one rounding.  (No wait: S's last reader, P V two tiles back, completed
+        // before this S did.)
+        const float2 sc = make_float2(qk_scale, qk_scale), nr = make_float2(neg_ref, neg_ref);
 #pragma unroll
-          for (int i = 0; i < HK / 2; ++i) {
-            const float2 e = fma_x2(make_float2(x[2 * i], x[2 * i + 1]), sc, nr);
-            pack_pair(i, make_float2(fast_exp2(e.x), fast_exp2(e.y)));
-          }
-        } else {
-          const float2 nr = make_float2(neg_ref, neg_ref);
+        for (int q = 0; q < 2; ++q) {
+          uint32_t hi[16], lo[16];
 #pragma unroll
-          for (int i = 0; i < HK / 2; ++i) {
-            const float2 e = add_x2(make_float2(x[2 * i], x[2 * i + 1]), nr);
-            pack_pair(i, make_float2(fast_exp2(e.x), fast_exp2(e.y)));
+          for (int i = 0; i < 16; ++i) {
+            const float2 xx = make_float2(x[32 * q + 2 * i], x[32 * q + 2 * i + 1]);
+            const float2 e = whole ? fma_x2(xx, sc, nr) : add_x2(xx, nr);  // (masked: exp2(-inf) = 0)
+            const float2 pp = make_float2(fast_exp2(e.x), fast_exp2(e.y));
+            ps = add_x2(ps, pp);
+            if constexpr (SPLIT) {
+              const uint32_t u0 = __float_as_uint(pp.x), u1 = __float_as_uint(pp.y);
+              hi[i] = __byte_perm(u0, u1, 0x7632);
+              const float2 rem =
+                  sub_x2(pp, make_float2(__uint_as_float(u0 & 0xFFFF0000u), __uint_as_float(u1 & 0xFFFF0000u)));
+              lo[i] = MmaOp<T>::pack(rem.x, rem.y);
+            } else {
+              hi[i] = MmaOp<T>::pack(pp.x, pp.y);
+            }
           }
+          umma::st16(lane_base + WG::SCOL + b * 128 + half * 64 + 16 * q, hi);
+          if constexpr (SPLIT) umma::st16(lane_base + WG::SCOL + b * 128 + half * 64 + 32 + 16 * q, lo);
         }
         l = l * alpha + (ps.x + ps.y);
-        // (P needs no wait: it goes over this tile's own S, whose last reader, P V
-        // two tiles back, completed before this S did)
         if (j >= 1 && __any_sync(0xffffffffu, alpha != 1.f)) {
           if (!uwait(pv_done, (uint32_t)((gg - 1) & 1))) {
             ok = false;
@@ -666,7 +681,7 @@ __global__ void __launch_bounds__(kUmmaThreads, 1)
         // (their slots may hold anything, and 0 * NaN = NaN): between the sinks and
         // the first row's window, and past the last row's end.  Each half clears
         // its own tokens.
-        const int a0 = p.sinks > t0 ? p.sinks : t0, a1 = cur.v_beg < t0 + HK ? cur.v_beg : t0 + HK;
+        const int a0 = p.sinks > t0 ? p.sinks : t0, a1 = it.seen.beg < t0 + HK ? it.seen.beg : t0 + HK;
         const int e1 = (kv_end + 15) / 16 * 16 < t0 + HK ? (kv_end + 15) / 16 * 16 : t0 + HK;
         const int e0 = kv_end > t0 ? kv_end : t0;
         if (a0 < a1 || e0 < e1) {
@@ -694,16 +709,11 @@ __global__ void __launch_bounds__(kUmmaThreads, 1)
           }
           fence_proxy_async();
         }
-        umma::st32(lane_base + WG::SCOL + b * 128 + half * 64, hi);
-        if constexpr (SPLIT) umma::st32(lane_base + WG::SCOL + b * 128 + half * 64 + 32, lo);
         umma::wait_st();
         umma::fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[2 * b + half]);
       }
-      // the next item's Q goes in while this item's last P V runs
-      RowItem nxt;
-      const bool have_nxt = ok && next_item(nxt);
       bool have = ok && ntiles > 0;
       if (have) {
         // (a barrier of its own, once per item: the other half may be a tile behind,
@@ -737,15 +747,15 @@ __global__ void __launch_bounds__(kUmmaThreads, 1)
       const float inv = nonzero ? 1.f / total : 0.f;
       const float f0 = (half == 0 ? w_me : w_o) * inv, f1 = (half == 0 ? w_o : w_me) * inv;
       const bool u0 = nonzero && f0 != 0.f, u1 = nonzero && f1 != 0.f;
-      T* orow = reinterpret_cast<T*>(p.out) + (cur.q0 + cur.t) * p.out_tok_stride +
-                (int64_t)(cur.kvh * G + cur.g) * p.out_head_stride + half * HD;
+      T* orow = reinterpret_cast<T*>(p.out) + (it.q0 + row_t) * p.out_tok_stride +
+                (int64_t)(it.kvh * G + row_g) * p.out_head_stride + half * HD;
 #pragma unroll
       for (int c = 0; c < HD; c += 16) {
         uint32_t v[16], w[16];
         umma::ld16(lane_base + WG::OCOL + half * HD + c, v);
         umma::ld16(lane_base + WG::OCOL + D + half * HD + c, w);
         umma::wait_ld();
-        if (cur.in_tile) {
+        if (in_tile) {
           uint32_t packed[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
@@ -765,8 +775,6 @@ __global__ void __launch_bounds__(kUmmaThreads, 1)
       }
       umma::fence_before();
       gt += ntiles;
-      cur = nxt;
-      have_cur = have_nxt;
     }
     if (!ok && lane == 0) give_up();
   }
