@@ -49,6 +49,35 @@ constexpr uint32_t kLayoutSw128 = 2;
 constexpr int kWinThreads = 384;
 constexpr int kKWarp = 8, kVWarp = 10, kItemWarp = 11;
 constexpr int kWinItems = 4;  // item slots
+// bf16 P is rounded once (8 bits: 1.1e-3 rms of the output, under the 1.7e-3 of the
+// output's own rounding) where every row of an item sees at least this many keys,
+// and carried as hi + lo (16 bits, a second product per 16 tokens) where some row
+// sees fewer: single weights are large there, and nearly cancelling V rows would
+// show the rounding (2e-3 absolute is missed with 3 keys).  16 x 512 tokens, window
+// 1024: 1 / 2 products TIMES_HERE us.
+constexpr int kSplitKeys = 64;
+
+// Products whose accumulation is known as the code is written, with the second
+// operand's descriptor as its low word (the address, which is all that changes:
+// shared addresses stay below 256 KB, no carry) and its constant high word.  The
+// one lane that issues them competes with eight softmax warps for issue slots: at
+// 160 cycles a product (64-bit descriptor arithmetic, a predicate and a branch
+// each) they, not the tensor cores, set the pace.
+template <bool ADD>
+__device__ __forceinline__ void mma_ts_lo(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t b_hi, uint32_t idesc) {
+  asm volatile(
+      "{\n.reg .pred p;\n.reg .b64 b;\nmov.b64 b, {%2, %3};\nsetp.ne.b32 p, %5, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n}\n" ::"r"(d),
+      "r"(a), "r"(b_lo), "r"(b_hi), "r"(idesc), "n"(ADD ? 1 : 0));
+}
+template <bool ADD>
+__device__ __forceinline__ void mma_ss_lo(uint32_t d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi,
+                                          uint32_t idesc) {
+  asm volatile(
+      "{\n.reg .pred p;\n.reg .b64 a, b;\nmov.b64 a, {%1, %2};\nmov.b64 b, {%3, %4};\nsetp.ne.b32 p, %6, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %5, p;\n}\n" ::"r"(d),
+      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "n"(ADD ? 1 : 0));
+}
 
 // A decoded work item, handed by warp 11 to the others.
 struct WinItem {
@@ -57,6 +86,7 @@ struct WinItem {
   int t0, g0, nrows;  // (new token, head of the group) of the item's first row; rows
   int y, kvh, prefix; // prefix less the gap: row's end = prefix + token + 1, virtual
   int kv_end, ntiles;
+  int split;          // bf16: some row sees fewer than kSplitKeys keys
   int state;          // 0 work, 1 rows to be zeroed (bad indices), 2 no further item
 };
 
@@ -67,7 +97,7 @@ struct WinUmmaGeom {
   static constexpr int Q_OFF = (KS + VS) * TILE;
   static constexpr int XBUF_OFF = Q_OFF + 2 * TILE;          // [2 halves][128 rows] (max, sum)
   static constexpr int BAR_OFF = XBUF_OFF + 2 * 128 * 8;
-  static constexpr int NBARS = 2 * KS + 2 * VS + 2 + 4 + 1 + 1 + 4 + 1 + 1 + 2 * kWinItems;
+  static constexpr int NBARS = 2 * KS + 3 * VS + 2 + 4 + 1 + 1 + 4 + 1 + 1 + 2 * kWinItems;
   static constexpr int MASK_OFF = BAR_OFF + NBARS * 8;       // [8 tiles][4] loaded blocks (kSlots: tokens)
   static constexpr int ITEM_OFF = (MASK_OFF + 8 * 16 + 15) / 16 * 16;
   static constexpr int MISC_OFF = ITEM_OFF + kWinItems * (int)sizeof(WinItem);  // abort, tmem address
@@ -88,7 +118,6 @@ __global__ void __launch_bounds__(kWinThreads, 1)
   constexpr int PAGES = KT / BS, PAGE = D * BS * 2;  // kPages
   constexpr int HALF = KT * 128;                     // token-major: bytes of 64 dims of a tile
   constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
-  constexpr bool SPLIT = BF16;  // bf16 P as hi + lo (one rounding misses the tolerance on rows of few keys)
   // (no static shared memory: the dynamic window then starts on a 1024-byte
   // boundary, as the 128-byte swizzle needs; checked below)
   extern __shared__ __align__(1024) uint8_t smem_wu[];
@@ -101,7 +130,8 @@ __global__ void __launch_bounds__(kWinThreads, 1)
   uint64_t* k_empty = k_full + KS;
   uint64_t* v_full = k_empty + KS;
   uint64_t* v_empty = v_full + VS;
-  uint64_t* s_full = v_empty + VS;  // [2 buffers]
+  uint64_t* v_ready = v_empty + VS;  // what nobody sees is cleared
+  uint64_t* s_full = v_ready + VS;   // [2 buffers]
   uint64_t* p_full = s_full + 2;    // [2 buffers][2 halves]
   uint64_t* pv_done = p_full + 4;
   uint64_t* o_done = pv_done + 1;
@@ -135,11 +165,12 @@ __global__ void __launch_bounds__(kWinThreads, 1)
     for (int s = 0; s < VS; ++s) {
       mbar_init(&v_full[s], 1);
       mbar_init(&v_empty[s], 1);
+      mbar_init(&v_ready[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&s_full[b], 2);
       mbar_init(&q_full[b], 1);
-      mbar_init(&q_empty[b], 1);
+      mbar_init(&q_empty[b], 8);
     }
     for (int b = 0; b < 4; ++b) mbar_init(&p_full[b], 4);
     for (int b = 0; b < kWinItems; ++b) {
@@ -220,11 +251,16 @@ __global__ void __launch_bounds__(kWinThreads, 1)
         it.prefix = u.prefix;
         it.kv_end = u.kv_end;
         it.ntiles = u.ntiles;
+        {  // keys of the item's first row, which sees the fewest
+          const int i1 = u.prefix + u.seen.jump + it.t0 + 1;  // its position + 1
+          const int64_t cap = (int64_t)p.window + p.sinks;
+          it.split = BF16 && (i1 < kSplitKeys || cap < kSplitKeys);
+        }
         it.state = u.bad ? 1 : 0;
         ok = publish(it);
         if (ok && it.ntiles > 0) {
           // Q rows into buffer nq & 1 ([D/8 chunks][128 rows][8 dims]; rows past the
-          // last are zero), whose last reader is S of the item two back
+          // last are zero), free once the item two back has left its output rows in it
           const int buf = nq & 1;
           bool free = true;
           if (nq >= 2 && lane == 0) free = umma::wait(&q_empty[buf], (uint32_t)(((nq >> 1) - 1) & 1));
@@ -412,6 +448,57 @@ __global__ void __launch_bounds__(kWinThreads, 1)
             }
           }
         }
+        if (!is_k) {
+          // V of tokens nobody sees, in blocks that are loaded for others, becomes 0
+          // (their slots may hold anything, and 0 * NaN = NaN): between the sinks and
+          // the first row's window, and past the last row's end up to the 16 tokens
+          // of a product.  This warp runs ahead of the products.
+          const int a0 = p.sinks > t0 ? p.sinks : t0, a1 = it.seen.beg < t0 + KT ? it.seen.beg : t0 + KT;
+          const int e0 = kv_end > t0 ? kv_end : t0, e1r = (kv_end + 15) / 16 * 16, e1 = e1r < t0 + KT ? e1r : t0 + KT;
+          if (a0 < a1 || e0 < e1) {
+            if (!__all_sync(0xffffffffu, umma::wait(&full[st], (uint32_t)(round & 1)))) {
+              ok = false;
+              break;
+            }
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+              const int c0 = (w ? e0 : a0) - t0, c1 = (w ? e1 : a1) - t0;
+              if constexpr (LOAD == kPages) {
+                // 8 tokens (16 bytes) of one dim's row of a page at a time
+                for (int tk = c0 & ~7; tk < c1; tk += 8) {
+                  const int ch = (tk % BS) / 8, lo = c0 - tk, hi = c1 - tk;
+                  uint32_t keep[4];
+#pragma unroll
+                  for (int i = 0; i < 4; ++i)
+                    keep[i] = (2 * i < lo || 2 * i >= hi ? 0x0000ffffu : 0u) |
+                              (2 * i + 1 < lo || 2 * i + 1 >= hi ? 0xffff0000u : 0u);
+                  const bool whole = lo <= 0 && hi >= 8;
+                  for (int d = lane; d < D; d += 32) {
+                    const int phys = BS == 32 ? (ch ^ ((d >> 1) & 3)) : (ch ^ ((d >> 2) & 1));
+                    uint4* w16 = reinterpret_cast<uint4*>(dst + (tk / BS) * PAGE + d * BS * 2 + phys * 16);
+                    uint4 v = make_uint4(0u, 0u, 0u, 0u);
+                    if (!whole) {
+                      v = *w16;
+                      v.x &= keep[0];
+                      v.y &= keep[1];
+                      v.z &= keep[2];
+                      v.w &= keep[3];
+                    }
+                    *w16 = v;
+                  }
+                }
+              } else {
+                for (int i = lane; i < (c1 - c0) * (D / 8); i += 32) {
+                  const int tk = c0 + i / (D / 8), ch = i % (D / 8);
+                  *reinterpret_cast<uint4*>(dst + (ch >> 3) * HALF + tk * 128 + (ch & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                }
+              }
+            }
+            fence_proxy_async();
+            __syncwarp();
+          }
+          if (lane == 0) mbar_arrive(&v_ready[st]);
+        }
         ++g;
         if (++st == stages) {
           st = 0;
@@ -442,28 +529,44 @@ __global__ void __launch_bounds__(kWinThreads, 1)
       // S of tile g, then P V of tile g - 1, over the tiles of all items
       int g = 0, nq = 0;                        // tiles, items with keys so far
       int pv_left = 0, pv_j = -1;               // the tile whose P V is due: keys from its first token on, its place
-      bool pv_last = false;                     // .. and whether its item ends with it
+      bool pv_last = false, pv_split = false;   // .. whether its item ends with it, and has lo parts
       bool ok = true;
       auto issue_pv = [&]() -> bool {
         const int t = g - 1, b = t & 1, vs = t % VS;
-        if (!umma::wait(&v_full[vs], (uint32_t)((t / VS) & 1))) return false;
+        if (!umma::wait(&v_ready[vs], (uint32_t)((t / VS) & 1)) || !umma::wait(&v_full[vs], (uint32_t)((t / VS) & 1)))
+          return false;
         const uint64_t vd = v_desc0 + (uint64_t)((vs * TILE) >> 4);
         // an item's first product overwrites both O, which every softmax warp has
         // read by the time it hands over its part of the first tile
         if (pv_j == 0 && !umma::wait(&p_full[2 * b + 1], (uint32_t)((t >> 1) & 1))) return false;
+        const uint32_t vd_lo = (uint32_t)vd, vd_hi = (uint32_t)(vd >> 32);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           if (!umma::wait(&p_full[2 * b + h], (uint32_t)((t >> 1) & 1))) return false;
           umma::fence_after();
-          const int left = pv_left - h * 64, steps = left > 0 ? (left + 15) / 16 : 0;
+          const int left = pv_left - h * 64;
           const uint32_t pcol = tmem + WG::SCOL + b * 128 + h * 64, ocol = tmem + WG::OCOL + h * D;
+          // 16 tokens of V: k-step ks of this half
+          auto vlo = [&](int ks) -> uint32_t {
+            const int tk = h * 64 + 16 * ks;
+            return vd_lo + (uint32_t)((LOAD == kPages ? (tk / BS) * PAGE + (tk % BS) * 2 : tk * 128) >> 4);
+          };
+          if (left > 0) {
+            if (pv_j > 0) mma_ts_lo<true>(ocol, pcol, vlo(0), vd_hi, idO);
+            else mma_ts_lo<false>(ocol, pcol, vlo(0), vd_hi, idO);
+          }
+          if (left > 48 && !(BF16 && pv_split)) {
 #pragma unroll
-          for (int ks = 0; ks < 4; ++ks) {
-            if (ks < steps) {
-              const int tk = h * 64 + 16 * ks;
-              const uint64_t d = vd + (uint64_t)((LOAD == kPages ? (tk / BS) * PAGE + (tk % BS) * 2 : tk * 128) >> 4);
-              umma::mma_ts(ocol, pcol + 8 * ks, d, idO, (pv_j > 0 || ks > 0) ? 1u : 0u);
-              if (SPLIT) umma::mma_ts(ocol, pcol + 32 + 8 * ks, d, idO, 1u);
+            for (int ks = 1; ks < 4; ++ks) mma_ts_lo<true>(ocol, pcol + 8 * ks, vlo(ks), vd_hi, idO);
+          } else if (left > 0) {
+            const int steps = left > 48 ? 4 : (left + 15) / 16;
+            if (BF16 && pv_split) mma_ts_lo<true>(ocol, pcol + 32, vlo(0), vd_hi, idO);
+#pragma unroll
+            for (int ks = 1; ks < 4; ++ks) {
+              if (ks < steps) {
+                mma_ts_lo<true>(ocol, pcol + 8 * ks, vlo(ks), vd_hi, idO);
+                if (BF16 && pv_split) mma_ts_lo<true>(ocol, pcol + 32 + 8 * ks, vlo(ks), vd_hi, idO);
+              }
             }
           }
         }
@@ -478,7 +581,7 @@ __global__ void __launch_bounds__(kWinThreads, 1)
           ok = false;
           break;
         }
-        const int kv_end = items[sl].kv_end, ntiles = items[sl].ntiles, state = items[sl].state;
+        const int kv_end = items[sl].kv_end, ntiles = items[sl].ntiles, state = items[sl].state, split = items[sl].split;
         mbar_arrive(&item_empty[sl]);
         if (state == 2) break;
         if (ntiles == 0) continue;
@@ -491,21 +594,22 @@ __global__ void __launch_bounds__(kWinThreads, 1)
         const uint64_t qd = q_desc0 + (uint64_t)((buf * TILE) >> 4);
         for (int j = 0; j < ntiles; ++j) {
           const int ks0 = g % KS, b = g & 1;
-          if (abort_now() || !umma::wait(&k_full[ks0], (uint32_t)((g / KS) & 1))) {
+          if (!umma::wait(&k_full[ks0], (uint32_t)((g / KS) & 1))) {
             ok = false;
             break;
           }
           umma::fence_after();
           const uint64_t kd = k_desc0 + (uint64_t)((ks0 * TILE) >> 4);
+          const uint32_t qlo = (uint32_t)qd, qhi = (uint32_t)(qd >> 32), klo = (uint32_t)kd, khi = (uint32_t)(kd >> 32);
+          mma_ss_lo<false>(tmem + WG::SCOL + b * 128, qlo, qhi, klo, khi, idS);
 #pragma unroll
-          for (int ks = 0; ks < D / 16; ++ks)
-            umma::mma_ss(tmem + WG::SCOL + b * 128, qd + (uint64_t)((ks * 2 * kUmmaRows * 16) >> 4),
-                         kd + (uint64_t)((LOAD == kPages ? ks * 2 * KT * 16 : (ks / 4) * HALF + (ks % 4) * 32) >> 4), idS,
-                         ks > 0 ? 1u : 0u);
+          for (int ks = 1; ks < D / 16; ++ks)
+            mma_ss_lo<true>(tmem + WG::SCOL + b * 128, qlo + (uint32_t)((ks * 2 * kUmmaRows * 16) >> 4), qhi,
+                            klo + (uint32_t)((LOAD == kPages ? ks * 2 * KT * 16 : (ks / 4) * HALF + (ks % 4) * 32) >> 4),
+                            khi, idS);
           umma::commit(&s_full[b]);
           mbar_arrive(&s_full[b]);  // (release: the tile's masks, seen through k_full, are seen by whoever waits)
           umma::commit(&k_empty[ks0]);
-          if (j == ntiles - 1) umma::commit(&q_empty[buf]);
           if (pv_j >= 0 && !issue_pv()) {
             ok = false;
             break;
@@ -514,6 +618,7 @@ __global__ void __launch_bounds__(kWinThreads, 1)
           pv_j = j;
           pv_left = kv_end - j * KT;
           pv_last = j == ntiles - 1;
+          pv_split = split != 0;
         }
       }
       if (ok && pv_j >= 0) ok = issue_pv();
@@ -533,7 +638,9 @@ __global__ void __launch_bounds__(kWinThreads, 1)
     const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     constexpr int HK = 64;      // tokens of a tile per half
     constexpr int HD = D / 2;   // output columns per half
-    const float qk_scale = p.scale * kLog2e;
+    // (a zero scale would make 0 * inf of a hidden score: the least normal number
+    // instead, whose scores round to the same exponentials)
+    const float qk_scale = p.scale == 0.f ? 1.1754944e-38f : p.scale * kLog2e;
     bool ok = true;
     int gt = 0, nx = 0;  // tiles and items with keys so far
     for (int k = 0; ok; ++k) {
@@ -543,14 +650,15 @@ __global__ void __launch_bounds__(kWinThreads, 1)
         break;
       }
       if (it.state == 2) break;
-      const int kv_end = it.kv_end, ntiles = it.ntiles;
+      const int ntiles = it.ntiles;
       const bool in_tile = r < it.nrows;
       const int x0 = it.g0 + r, dt = x0 / G, row_t = it.t0 + dt, row_g = x0 - dt * G;
+      const int64_t o_off = (it.q0 + row_t) * p.out_tok_stride + (int64_t)(it.kvh * G + row_g) * p.out_head_stride;
       const int end_r = in_tile && it.state == 0 ? it.prefix + row_t + 1 : 0;
       const int beg_r = end_r > p.window ? end_r - p.window : 0;
       float m_ref = -INFINITY, l = 0.f;
       for (int j = 0; j < ntiles; ++j) {
-        const int gg = gt + j, b = gg & 1, vs = gg % VS;
+        const int gg = gt + j, b = gg & 1;
         if (uabort() || !uwait(&s_full[b], (uint32_t)((gg >> 1) & 1))) {
           ok = false;
           break;
@@ -583,25 +691,8 @@ __global__ void __launch_bounds__(kWinThreads, 1)
         umma::wait_ld();
         // a half tile every row of the warp sees whole needs no per-token mask
         const bool whole = __all_sync(0xffffffffu, all_in && t0 >= beg_r && t0 + HK <= end_r);
-        float mx;  // row max of my scaled scores (log2 units)
-        if (whole) {
-          // (the largest raw score, or the smallest for a negative scale; four chains)
-          float h[4] = {x[0], x[1], x[2], x[3]};
-          if (qk_scale >= 0.f) {
-#pragma unroll
-            for (int c = 4; c < HK; c += 4)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) h[e] = fmaxf(h[e], x[c + e]);
-            mx = fmaxf(fmaxf(h[0], h[1]), fmaxf(h[2], h[3])) * qk_scale;
-          } else {
-#pragma unroll
-            for (int c = 4; c < HK; c += 4)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) h[e] = fminf(h[e], x[c + e]);
-            mx = fminf(fminf(h[0], h[1]), fminf(h[2], h[3])) * qk_scale;
-          }
-        } else {
-          // seen: tokens [max(beg, 0), end) and [0, sinks) of this half, as bits
+        if (!whole) {
+          // seen: tokens [beg, end) and [0, sinks) of this half, as bits
           auto below = [](int n) -> uint64_t { return n <= 0 ? 0ull : (n >= 64 ? ~0ull : (1ull << n) - 1ull); };
           uint64_t vis = below(end_r - t0) & (~below(beg_r - t0) | below(p.sinks - t0));
           if (!all_in) {
@@ -617,11 +708,28 @@ __global__ void __launch_bounds__(kWinThreads, 1)
             vis &= in;
           }
           const uint32_t v0 = (uint32_t)vis, v1 = (uint32_t)(vis >> 32);
-          mx = -INFINITY;
+          // (a hidden score is whatever the scale takes to -inf)
+          const float hidden = qk_scale >= 0.f ? -INFINITY : INFINITY;
 #pragma unroll
-          for (int c = 0; c < HK; ++c) {
-            x[c] = ((c < 32 ? v0 : v1) >> (c & 31)) & 1u ? x[c] * qk_scale : -INFINITY;
-            mx = fmaxf(mx, x[c]);
+          for (int c = 0; c < HK; ++c) x[c] = ((c < 32 ? v0 : v1) >> (c & 31)) & 1u ? x[c] : hidden;
+        }
+        // row max of my scaled scores (log2 units): the largest raw score, or the
+        // smallest for a negative scale; four chains
+        float mx;
+        {
+          float h[4] = {x[0], x[1], x[2], x[3]};
+          if (qk_scale >= 0.f) {
+#pragma unroll
+            for (int c = 4; c < HK; c += 4)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) h[e] = fmaxf(h[e], x[c + e]);
+            mx = fmaxf(fmaxf(h[0], h[1]), fmaxf(h[2], h[3])) * qk_scale;
+          } else {
+#pragma unroll
+            for (int c = 4; c < HK; c += 4)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) h[e] = fminf(h[e], x[c + e]);
+            mx = fminf(fminf(h[0], h[1]), fminf(h[2], h[3])) * qk_scale;
           }
         }
         // lazy max: rescale only when it rises by more than 2^8
@@ -633,33 +741,38 @@ __global__ void __launch_bounds__(kWinThreads, 1)
         const float neg_ref = m_ref == -INFINITY ? 0.f : -m_ref;
         float2 ps = make_float2(0.f, 0.f);
         // P over this tile's own S, 16 pairs of tokens at a time, so that the stores
-        // overlap the next pairs' exponentials: hi = the upper 16 bits of each fp32
-        // (a bf16, truncated), lo = the exact remainder rounded to bf16; f16 P is
-        // one rounding.  (No wait: S's last reader, P V two tiles back, completed
-        // before this S did.)
+        // overlap the next pairs' exponentials: one rounding, or hi = the upper 16
+        // bits of each fp32 (a bf16, truncated) and lo = the exact remainder rounded
+        // to bf16.  (No wait: S's last reader, P V two tiles back, completed before
+        // this S did.)
         const float2 sc = make_float2(qk_scale, qk_scale), nr = make_float2(neg_ref, neg_ref);
+        auto exponentials = [&](auto two) {
+          constexpr bool TWO = decltype(two)::value;
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          uint32_t hi[16], lo[16];
+          for (int q = 0; q < 2; ++q) {
+            uint32_t hi[16], lo[16];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float2 xx = make_float2(x[32 * q + 2 * i], x[32 * q + 2 * i + 1]);
-            const float2 e = whole ? fma_x2(xx, sc, nr) : add_x2(xx, nr);  // (masked: exp2(-inf) = 0)
-            const float2 pp = make_float2(fast_exp2(e.x), fast_exp2(e.y));
-            ps = add_x2(ps, pp);
-            if constexpr (SPLIT) {
-              const uint32_t u0 = __float_as_uint(pp.x), u1 = __float_as_uint(pp.y);
-              hi[i] = __byte_perm(u0, u1, 0x7632);
-              const float2 rem =
-                  sub_x2(pp, make_float2(__uint_as_float(u0 & 0xFFFF0000u), __uint_as_float(u1 & 0xFFFF0000u)));
-              lo[i] = MmaOp<T>::pack(rem.x, rem.y);
-            } else {
-              hi[i] = MmaOp<T>::pack(pp.x, pp.y);
+            for (int i = 0; i < 16; ++i) {
+              const float2 xx = make_float2(x[32 * q + 2 * i], x[32 * q + 2 * i + 1]);
+              const float2 e = fma_x2(xx, sc, nr);  // (hidden: exp2(-inf) = 0)
+              const float2 pp = make_float2(fast_exp2(e.x), fast_exp2(e.y));
+              ps = add_x2(ps, pp);
+              if constexpr (TWO) {
+                const uint32_t u0 = __float_as_uint(pp.x), u1 = __float_as_uint(pp.y);
+                hi[i] = __byte_perm(u0, u1, 0x7632);
+                const float2 rem =
+                    sub_x2(pp, make_float2(__uint_as_float(u0 & 0xFFFF0000u), __uint_as_float(u1 & 0xFFFF0000u)));
+                lo[i] = MmaOp<T>::pack(rem.x, rem.y);
+              } else {
+                hi[i] = MmaOp<T>::pack(pp.x, pp.y);
+              }
             }
+            umma::st16(lane_base + WG::SCOL + b * 128 + half * 64 + 16 * q, hi);
+            if constexpr (TWO) umma::st16(lane_base + WG::SCOL + b * 128 + half * 64 + 32 + 16 * q, lo);
           }
-          umma::st16(lane_base + WG::SCOL + b * 128 + half * 64 + 16 * q, hi);
-          if constexpr (SPLIT) umma::st16(lane_base + WG::SCOL + b * 128 + half * 64 + 32 + 16 * q, lo);
-        }
+        };
+        if (BF16 && it.split) exponentials(std::true_type{});
+        else exponentials(std::false_type{});
         l = l * alpha + (ps.x + ps.y);
         if (j >= 1 && __any_sync(0xffffffffu, alpha != 1.f)) {
           if (!uwait(pv_done, (uint32_t)((gg - 1) & 1))) {
@@ -676,38 +789,6 @@ __global__ void __launch_bounds__(kWinThreads, 1)
             for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * alpha);
             umma::st16(lane_base + WG::OCOL + half * D + c, v);
           }
-        }
-        // V of tokens nobody sees, in blocks that are loaded for others, becomes 0
-        // (their slots may hold anything, and 0 * NaN = NaN): between the sinks and
-        // the first row's window, and past the last row's end.  Each half clears
-        // its own tokens.
-        const int a0 = p.sinks > t0 ? p.sinks : t0, a1 = it.seen.beg < t0 + HK ? it.seen.beg : t0 + HK;
-        const int e1 = (kv_end + 15) / 16 * 16 < t0 + HK ? (kv_end + 15) / 16 * 16 : t0 + HK;
-        const int e0 = kv_end > t0 ? kv_end : t0;
-        if (a0 < a1 || e0 < e1) {
-          if (!uwait(&v_full[vs], (uint32_t)((gg / VS) & 1))) {
-            ok = false;
-            break;
-          }
-          uint8_t* vst = vring + (size_t)vs * TILE;
-#pragma unroll
-          for (int w = 0; w < 2; ++w) {
-            const int c0 = (w ? e0 : a0) - tile0, c1 = (w ? e1 : a1) - tile0;
-            if constexpr (LOAD == kPages) {
-              if (r < D)
-                for (int tk = c0; tk < c1; ++tk) {
-                  const int ch = (tk % BS) / 8;
-                  const int phys = BS == 32 ? (ch ^ ((r >> 1) & 3)) : (ch ^ ((r >> 2) & 1));
-                  *reinterpret_cast<uint16_t*>(vst + (tk / BS) * PAGE + r * BS * 2 + phys * 16 + (tk % 8) * 2) = 0;
-                }
-            } else {
-              for (int i = r; i < (c1 - c0) * (D / 8); i += 128) {
-                const int tk = c0 + i / (D / 8), ch = i % (D / 8);
-                *reinterpret_cast<uint4*>(vst + (ch >> 3) * HALF + tk * 128 + (ch & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
-              }
-            }
-          }
-          fence_proxy_async();
         }
         umma::wait_st();
         umma::fence_before();
@@ -747,33 +828,55 @@ __global__ void __launch_bounds__(kWinThreads, 1)
       const float inv = nonzero ? 1.f / total : 0.f;
       const float f0 = (half == 0 ? w_me : w_o) * inv, f1 = (half == 0 ? w_o : w_me) * inv;
       const bool u0 = nonzero && f0 != 0.f, u1 = nonzero && f1 != 0.f;
-      T* orow = reinterpret_cast<T*>(p.out) + (it.q0 + row_t) * p.out_tok_stride +
-                (int64_t)(it.kvh * G + row_g) * p.out_head_stride + half * HD;
+      if (ntiles > 0) {
+        // through the item's Q buffer (S is done with it) to whole 128- or 64-byte
+        // pieces of rows: 16-byte chunk c of row r at c ^ (r & 7), this warp's rows
+        // and half of the columns only
+        constexpr int RB = D * 2, CPR = HD / 8;  // bytes of a row, chunks of my half of it
+        uint8_t* ob = qsm + ((nx - 1) & 1) * TILE;
 #pragma unroll
-      for (int c = 0; c < HD; c += 16) {
-        uint32_t v[16], w[16];
-        umma::ld16(lane_base + WG::OCOL + half * HD + c, v);
-        umma::ld16(lane_base + WG::OCOL + D + half * HD + c, w);
-        umma::wait_ld();
-        if (in_tile) {
-          uint32_t packed[8];
+        for (int c = 0; c < HD; c += 32) {
+          uint32_t v[32], w[32];
+          umma::ld32(lane_base + WG::OCOL + half * HD + c, v);
+          umma::ld32(lane_base + WG::OCOL + D + half * HD + c, w);
+          umma::wait_ld();
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            float y[2];
+          for (int i = 0; i < 32; i += 8) {
+            uint32_t packed[4];
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const float o0 = u0 ? __uint_as_float(v[2 * i + e]) * f0 : 0.f;
-              y[e] = u1 ? fmaf(__uint_as_float(w[2 * i + e]), f1, o0) : o0;
+            for (int k2 = 0; k2 < 4; ++k2) {
+              float y[2];
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const float o0 = u0 ? __uint_as_float(v[i + 2 * k2 + e]) * f0 : 0.f;
+                y[e] = u1 ? fmaf(__uint_as_float(w[i + 2 * k2 + e]), f1, o0) : o0;
+              }
+              packed[k2] = pack_out<T>(y[0], y[1]);
             }
-            packed[i] = pack_out<T>(y[0], y[1]);
+            const int ch = half * CPR + (c + i) / 8;
+            *reinterpret_cast<uint4*>(ob + r * RB + ((ch & ~7) | ((ch ^ r) & 7)) * 16) =
+                make_uint4(packed[0], packed[1], packed[2], packed[3]);
           }
-#pragma unroll
-          for (int i = 0; i < 8; i += 4)
-            *reinterpret_cast<uint4*>(orow + c + 2 * i) =
-                make_uint4(packed[i], packed[i + 1], packed[i + 2], packed[i + 3]);
         }
+        umma::fence_before();
+        __syncwarp();
+        // lane -> chunk lane % CPR of row (lane / CPR) + 32 / CPR * i of my warp's 32
+        const int ch = half * CPR + lane % CPR;
+#pragma unroll
+        for (int i = 0; i < CPR; ++i) {
+          const int from = lane / CPR + (32 / CPR) * i, rr = (warp & 3) * 32 + from;
+          const int64_t off = __shfl_sync(0xffffffffu, o_off, from);  // (that row's own thread knows where it goes)
+          if (rr < it.nrows)
+            *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) + off + ch * 8) =
+                *reinterpret_cast<const uint4*>(ob + rr * RB + ((ch & ~7) | ((ch ^ rr) & 7)) * 16);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&q_empty[(nx - 1) & 1]);
+      } else if (in_tile) {  // (bad indices: zeros)
+        T* orow = reinterpret_cast<T*>(p.out) + o_off + half * HD;
+#pragma unroll
+        for (int c = 0; c < HD; c += 8) *reinterpret_cast<uint4*>(orow + c) = make_uint4(0u, 0u, 0u, 0u);
       }
-      umma::fence_before();
       gt += ntiles;
     }
     if (!ok && lane == 0) give_up();
