@@ -1147,7 +1147,7 @@ int kvc_paged_attention_window(kvc_dltensor* out, const kvc_dltensor* query, con
   if (a.num_seqs == 0) return KVC_OK;
   DeviceGuard g(device);
   if (!g.ok()) return fail(KVC_ECUDA, "cudaSetDevice failed");
-  WindowArgs w = {window_size, sink_size};
+  WindowArgs w = {window_size, sink_size, nullptr, 0, 0, 0};
   cudaError_t e = launch_window_decode(a, w, static_cast<cudaStream_t>(stream));
   if (e == cudaErrorMisalignedAddress)
     return fail(KVC_EINVAL, "key_cache/value_cache rows, blocks and heads must start on 16-byte boundaries");

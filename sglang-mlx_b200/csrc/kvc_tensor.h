@@ -291,6 +291,11 @@ cudaError_t launch_qk_norm_rope(const RopeArgs& a, cudaStream_t stream);
 // Sliding window with sinks over the paged cache (window.cu): decode and extend.
 struct WindowArgs {
   int window, sinks;
+  // extend only: [num_seqs + 1] first rows, the bound on a sequence's new tokens,
+  // rows of q, entries of a table row
+  const uint32_t* indptr;
+  int max_q_len;
+  int64_t num_tokens, table_len;
 };
 cudaError_t launch_window_decode(const DecodeArgs& a, const WindowArgs& w, cudaStream_t stream);
 cudaError_t launch_window_prefill(const PrefillArgs& a, cudaStream_t stream);

@@ -40,75 +40,108 @@ __device__ __forceinline__ uint32_t cluster_rank() {
 }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
-// Stores into the shared memory of CTA `rank` of the cluster, at this CTA's address `dst`.
-__device__ __forceinline__ void store_remote(const float* dst, uint32_t rank, float v) {
+// This CTA's shared address `p` in CTA `rank` of the cluster, and stores to it.
+__device__ __forceinline__ uint32_t remote_address(const void* p, uint32_t rank) {
   uint32_t a;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
                : "=r"(a)
-               : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(dst))), "r"(rank));
-  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(a), "f"(v) : "memory");
+               : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(p))), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ void store_remote(const float2* dst, uint32_t rank, float2 v) {
+  asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(remote_address(dst, rank)), "f"(v.x), "f"(v.y)
+               : "memory");
+}
+__device__ __forceinline__ void store_remote(const float4* dst, uint32_t rank, float4 v) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(remote_address(dst, rank)), "f"(v.x), "f"(v.y),
+               "f"(v.z), "f"(v.w)
+               : "memory");
+}
+
+__device__ __forceinline__ void add_scaled(float4& a, float w, float4 b) {
+  a.x += w * b.x;
+  a.y += w * b.y;
+  a.z += w * b.z;
+  a.w += w * b.w;
+}
+
+// a / L as four elements of an output row, of any alignment; 0 where L is 0.
+template <typename T>
+__device__ __forceinline__ void store_quotient(T* dst, float4 a, float L, float eps) {
+  const float n = L + eps;
+  const bool any = L > 0.f;
+  struct alignas(4 * sizeof(T)) Four {
+    T e[4];
+  } v = {{from_float<T>(any ? a.x / n : 0.f), from_float<T>(any ? a.y / n : 0.f), from_float<T>(any ? a.z / n : 0.f),
+          from_float<T>(any ? a.w / n : 0.f)}};
+  if ((reinterpret_cast<uintptr_t>(dst) & (sizeof(Four) - 1)) == 0) {
+    *reinterpret_cast<Four*>(dst) = v;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) dst[i] = v.e[i];
+  }
 }
 
 // The exchange area of one CTA: [C][nh] (max, sum) pairs, then [C][S] values of
-// its slice of the nh * D elements, S = ceil(nh * D / C).
+// its slice of the nh * D elements, four to a value, S = ceil(nh * D / 4 / C).
 __host__ __device__ constexpr int exchange_floats(int nh, int D) {
-  return kMaxCluster * nh * 2 + nh * D + kMaxCluster;
+  return kMaxCluster * nh * 2 + nh * D + 4 * kMaxCluster;
 }
 
-// Joins the CTA states of a cluster.  state(g, &M, &L): the CTA's max (natural
-// log units) and sum of row g; value(i): its unnormalised element i = g * D + d.
-// Every thread of every CTA of the cluster calls it; each CTA has arrived once
-// on the cluster barrier before (its shared memory is live).
-template <typename T, typename FState, typename FValue>
-__device__ __forceinline__ void cluster_join(const DecodeParams& p, int seq, int h0, int nh, int D, int C, int rank,
-                                             float* xch, FState state, FValue value) {
-  T* out = reinterpret_cast<T*>(p.out) + (int64_t)seq * p.out_seq_stride + (int64_t)h0 * p.out_head_stride;
+// Joins the CTA states of a cluster.  part(g, d, &M, &L): the CTA's unnormalised
+// elements d .. d + 3 of row g, and the row's max (natural log units) and sum;
+// dest(g): the output row.  `eps` is added to a row's sum (a row that sees nothing
+// has sum 0 and gives 0).  Every thread of every CTA of the cluster calls it; each
+// CTA has arrived once on the cluster barrier before (its shared memory is live).
+template <typename T, typename FPart, typename FDest>
+__device__ __forceinline__ void cluster_join(int nh, int D, int C, int rank, float* xch, float eps, FPart part, FDest dest) {
+  const int n4 = nh * D / 4;
   if (C == 1) {
-    for (int i = threadIdx.x; i < nh * D; i += blockDim.x) {
-      const int g = i / D, d = i - g * D;
+    for (int i = threadIdx.x; i < n4; i += blockDim.x) {
+      const int g = 4 * i / D, d = 4 * i - g * D;
       float M, L;
-      state(g, &M, &L);
-      out[(int64_t)g * p.out_head_stride + d] = from_float<T>(value(i) / (L + 1e-6f));
+      const float4 a = part(g, d, &M, &L);
+      store_quotient(dest(g) + d, a, L, eps);
     }
     return;
   }
-  const int S = (nh * D + C - 1) / C;
-  float* ml = xch;                          // [C][nh][2]
-  float* val = xch + kMaxCluster * nh * 2;  // [C][S]
+  const int S = (n4 + C - 1) / C;
+  float2* ml = reinterpret_cast<float2*>(xch);                          // [C][nh]
+  float4* val = reinterpret_cast<float4*>(xch + kMaxCluster * nh * 2);  // [C][S]
   cluster_wait();  // every CTA of the cluster runs: its exchange area may be written
-  for (int i = threadIdx.x; i < nh * C; i += blockDim.x) {
-    const int r = i / nh, g = i - r * nh;
+  for (int i = threadIdx.x; i < n4; i += blockDim.x) {
+    const int g = 4 * i / D, d = 4 * i - g * D, r = i / S;
     float M, L;
-    state(g, &M, &L);
-    store_remote(ml + (rank * nh + g) * 2, (uint32_t)r, M);
-    store_remote(ml + (rank * nh + g) * 2 + 1, (uint32_t)r, L);
-  }
-  for (int i = threadIdx.x; i < nh * D; i += blockDim.x) {
-    const int r = i / S;
-    store_remote(val + rank * S + (i - r * S), (uint32_t)r, value(i));
+    const float4 a = part(g, d, &M, &L);
+    store_remote(val + rank * S + (i - r * S), (uint32_t)r, a);
+    // the row's state goes to every CTA, one by each of the row's threads
+    for (int c = d / 4; c < C; c += D / 4) store_remote(ml + rank * nh + g, (uint32_t)c, make_float2(M, L));
   }
   cluster_arrive();
   cluster_wait();
-  for (int j = threadIdx.x; j < S && rank * S + j < nh * D; j += blockDim.x) {
-    const int i = rank * S + j, g = i / D, d = i - g * D;
+  for (int j = threadIdx.x; j < S && rank * S + j < n4; j += blockDim.x) {
+    const int i = rank * S + j, g = 4 * i / D, d = 4 * i - g * D;
     float M = -INFINITY;
-    for (int c = 0; c < C; ++c) M = fmaxf(M, ml[(c * nh + g) * 2]);
-    float L = 0.f, A = 0.f;
+    for (int c = 0; c < C; ++c) M = fmaxf(M, ml[c * nh + g].x);
+    float L = 0.f;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int c = 0; c < C; ++c) {
-      const float m = ml[(c * nh + g) * 2];
-      const float w = m == -INFINITY ? 0.f : expf(m - M);
-      L += w * ml[(c * nh + g) * 2 + 1];
-      A += w * val[c * S + j];
+      const float2 s = ml[c * nh + g];
+      const float w = s.x == -INFINITY ? 0.f : expf(s.x - M);
+      L += w * s.y;
+      add_scaled(a, w, val[c * S + j]);
     }
-    out[(int64_t)g * p.out_head_stride + d] = from_float<T>(A / (L + 1e-6f));
+    store_quotient(dest(g) + d, a, L, eps);
   }
 }
 
-// Tensor-core form: the G <= 16 query heads of a KV head are the rows of the
-// decode's m16n8k16 tile (mma_group, decode_mma.cuh); each warp streams every
-// NW-th group of GT tokens of the CTA's run through its own ring of STAGES
-// stages, as paged_decode_mma_kernel does.  MODE: kBulk (whole pages), kSwizzledV
-// (32-token pages), kFlashTma (token rows in blocks of 16k), kFlash (token rows).
+// Tensor-core form: 16 (new token, query head of the group) rows of one KV head
+// are the rows of the decode's m16n8k16 tile (mma_group, decode_mma.cuh); each warp
+// streams every NW-th group of GT tokens of the CTA's run through its own ring of
+// STAGES stages, as paged_decode_mma_kernel does.  MODE: kBulk (whole pages),
+// kSwizzledV (32-token pages), kFlashTma (token rows in blocks of 16k), kFlash
+// (token rows).  EXT: several such tiles to a sequence and KV head (grid.z): the
+// extend's few new tokens (indptr), or, without indptr, more than 16 heads of one.
 template <int D, int BS, int NW, int STAGES, int GT, int MODE>
 struct WindowGeom {
   using Geo = MmaGeom<D, BS, NW, STAGES, GT, MODE>;
@@ -116,7 +149,7 @@ struct WindowGeom {
   static constexpr int SMEM = XCH_OFF + exchange_floats(16, D) * 4;
 };
 
-template <typename T, int D, int BS, int NW, int STAGES, int GTOK, int MODE>
+template <typename T, int D, int BS, int NW, int STAGES, int GTOK, int MODE, bool EXT>
 __global__ void __launch_bounds__(NW * 32)
     window_decode_kernel(const DecodeParams p, const WindowArgs wa, const __grid_constant__ TmaMaps tm) {
   using namespace mma_detail;
@@ -132,15 +165,50 @@ __global__ void __launch_bounds__(NW * 32)
   const int r = lane >> 2, q4 = lane & 3;
   const int G = p.num_heads / p.num_kv_heads, h0 = kvh * G;
   grid_dependents_launch();
+  const int rbs = Geo::TROWS || Geo::FLASH ? p.block_size : BS;
+  // rows R0 .. R0 + nh - 1 of the sequence's new tokens, whose first is row q0 of
+  // q / out and position `prefix`
+  const int R0 = EXT ? blockIdx.z * 16 : 0;
   const uint32_t ctx = p.context_lens[seq];
-  if (ctx == 0 || ctx > (uint32_t)p.max_seq_len) {  // (the same for the whole cluster)
+  int64_t q0 = seq;
+  int rows = G, prefix = (int)ctx - 1;
+  bool zero = ctx == 0 || ctx > (uint32_t)p.max_seq_len;
+  if (EXT && wa.indptr) {
+    const int64_t a = wa.indptr[seq], b = wa.indptr[seq + 1];
+    const int64_t ql = b - a;
+    q0 = a;
+    if (ql <= 0 || R0 >= ql * G) {  // (the same for the whole cluster, as every early end here)
+      grid_dependency_wait();
+      return;
+    }
+    // rows past q may not be written; other index errors give zeros
+    zero = ql > wa.max_q_len || (int64_t)ctx < ql || (int64_t)ctx > wa.table_len * (int64_t)rbs || ctx > 0x7fffff00u;
+    const bool past = b > wa.num_tokens;
+    if ((zero || past) && threadIdx.x == 0 && R0 == 0 && blockIdx.x == 0) set_status(&g_decode_status, KVC_STATUS_INDEX_OOB);
+    if (past) {
+      grid_dependency_wait();
+      return;
+    }
+    rows = (int)(ql * G < 0x7fffffff ? ql * G : 0x7fffffff);
+    prefix = (int)((int64_t)ctx - ql);
+  }
+  const int nh = EXT ? (rows - R0 < 16 ? rows - R0 : 16) : G;
+  // row R0 + g: new token t, head of the group
+  auto token_of = [&](int g) { return EXT ? (R0 + g) / G : 0; };
+  auto dest = [&](int g) -> T* {
+    if constexpr (!EXT)  // (fewer registers live across the loop: 256 sequences, window 1024: 170 -> 165 us)
+      return reinterpret_cast<T*>(p.out) + (int64_t)seq * p.out_seq_stride + (int64_t)(h0 + g) * p.out_head_stride;
+    const int t = token_of(g);
+    return reinterpret_cast<T*>(p.out) + (q0 + t) * p.out_seq_stride + (int64_t)(h0 + R0 + g - t * G) * p.out_head_stride;
+  };
+  if (zero) {
     grid_dependency_wait();
-    if (rank == 0) write_zero_heads<T>(p, seq, h0, G, D);
+    if (rank == 0)
+      for (int i = threadIdx.x; i < nh * D; i += NW * 32) dest(i / D)[i % D] = from_float<T>(0.f);
     return;
   }
   if (C > 1) cluster_arrive();
-  const int rbs = Geo::TROWS || Geo::FLASH ? p.block_size : BS;
-  const Seen seen = seen_range((int)ctx - 1, (int)ctx - 1, wa.window, wa.sinks, rbs);
+  const Seen seen = seen_range(prefix + token_of(0), prefix + token_of(nh - 1), wa.window, wa.sinks, rbs);
   // this CTA's run of groups
   const int all = (seen.end + GT - 1) / GT, per = (all + C - 1) / C;
   const int begin = rank * per * GT;
@@ -284,18 +352,30 @@ __global__ void __launch_bounds__(NW * 32)
     store_ids(0, first);
   }
   uint32_t qa[KS][4];
-  const T* qp = reinterpret_cast<const T*>(p.q) + (int64_t)seq * p.q_seq_stride;
+  const int t_lo = token_of(r), t_hi = token_of(r + 8);
+  const T* q_lo = reinterpret_cast<const T*>(p.q) + (q0 + t_lo) * p.q_seq_stride +
+                  (int64_t)(h0 + R0 + r - t_lo * G) * p.q_head_stride;
+  const T* q_hi = reinterpret_cast<const T*>(p.q) + (q0 + t_hi) * p.q_seq_stride +
+                  (int64_t)(h0 + R0 + r + 8 - t_hi * G) * p.q_head_stride;
+  // what this lane's two rows see (rows past the last: nothing)
+  int end_lo = 2147483647, end_hi = 2147483647, beg_lo = seen.beg, beg_hi = seen.beg;
+  if constexpr (EXT) {
+    end_lo = r < nh ? prefix + t_lo + 1 - seen.jump : 0;
+    end_hi = r + 8 < nh ? prefix + t_hi + 1 - seen.jump : 0;
+    beg_lo = end_lo > wa.window ? end_lo - wa.window : 0;
+    beg_hi = end_hi > wa.window ? end_hi - wa.window : 0;
+  }
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) {
     const int d0 = ks * 16 + 2 * q4;
     qa[ks][0] = qa[ks][1] = qa[ks][2] = qa[ks][3] = 0u;
-    if (r < G) {
-      const T* row = qp + (int64_t)(h0 + r) * p.q_head_stride;
+    if (r < nh) {
+      const T* row = q_lo;
       qa[ks][0] = *reinterpret_cast<const uint32_t*>(row + d0);
       qa[ks][2] = *reinterpret_cast<const uint32_t*>(row + d0 + 8);
     }
-    if (r + 8 < G) {
-      const T* row = qp + (int64_t)(h0 + r + 8) * p.q_head_stride;
+    if (r + 8 < nh) {
+      const T* row = q_hi;
       qa[ks][1] = *reinterpret_cast<const uint32_t*>(row + d0);
       qa[ks][3] = *reinterpret_cast<const uint32_t*>(row + d0 + 8);
     }
@@ -324,8 +404,8 @@ __global__ void __launch_bounds__(NW * 32)
     }
     const uint8_t* st = ring + (size_t)s * Geo::STAGE;
     mma_group<T, Geo, D, true, true>(gs, qa, smem_u32(st), smem_u32(st + NBOX * BOX), begin + (warp + k * NW) * GT, end,
-                                     masks[s], 0, qk_scale, false, 0.f, 0.f, lane, 2147483647, 2147483647, seen.beg,
-                                     seen.beg, wa.sinks, seen.beg);
+                                     masks[s], 0, qk_scale, false, 0.f, 0.f, lane, end_lo, end_hi, beg_lo, beg_hi,
+                                     wa.sinks, seen.beg);
     __syncwarp();
     if (k + STAGES < n_mine) {
       fence_proxy_async();
@@ -344,12 +424,14 @@ __global__ void __launch_bounds__(NW * 32)
   float* red_o = reinterpret_cast<float*>(smem);  // [NW][16][D]
   float* red_ml = red_o + NW * 16 * D;            // [NW][16][2]
   {
+    // (16-byte pieces of a row in an order of its own, so that the rows' stores meet
+    // in no bank; rows past the last stay unwritten)
     float* ow = red_o + (size_t)warp * 16 * D;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int d = 8 * nt + 2 * q4;
-      *reinterpret_cast<float2*>(ow + r * D + d) = make_float2(gs.o[nt][0], gs.o[nt][1]);
-      *reinterpret_cast<float2*>(ow + (r + 8) * D + d) = make_float2(gs.o[nt][2], gs.o[nt][3]);
+      const int d = ((2 * nt + (q4 >> 1)) ^ r) * 4 + 2 * (q4 & 1);
+      if (r < nh) *reinterpret_cast<float2*>(ow + r * D + d) = make_float2(gs.o[nt][0], gs.o[nt][1]);
+      if (r + 8 < nh) *reinterpret_cast<float2*>(ow + (r + 8) * D + d) = make_float2(gs.o[nt][2], gs.o[nt][3]);
     }
     if (q4 == 0) {
       red_ml[(warp * 16 + r) * 2] = gs.m_lo;
@@ -359,33 +441,23 @@ __global__ void __launch_bounds__(NW * 32)
     }
   }
   __syncthreads();
-  auto top = [&](int g) -> float {  // log2 units
-    float M = -INFINITY;
+  auto part = [&](int g, int d, float* M, float* L) -> float4 {
+    float m = -INFINITY, l = 0.f;  // log2 units
 #pragma unroll
-    for (int w = 0; w < NW; ++w) M = fmaxf(M, red_ml[(w * 16 + g) * 2]);
-    return M;
-  };
-  auto weight = [&](int w, int g, float M) -> float {
-    const float m = red_ml[(w * 16 + g) * 2];
-    return m == -INFINITY ? 0.f : fast_exp2(m - M);
-  };
-  auto state = [&](int g, float* M, float* L) {
-    const float m = top(g);
-    float l = 0.f;
+    for (int w = 0; w < NW; ++w) m = fmaxf(m, red_ml[(w * 16 + g) * 2]);
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int w = 0; w < NW; ++w) l += weight(w, g, m) * red_ml[(w * 16 + g) * 2 + 1];
+    for (int w = 0; w < NW; ++w) {
+      const float2 s = *reinterpret_cast<const float2*>(red_ml + (w * 16 + g) * 2);
+      const float e = s.x == -INFINITY ? 0.f : fast_exp2(s.x - m);
+      l += e * s.y;
+      add_scaled(a, e, *reinterpret_cast<const float4*>(red_o + (size_t)w * 16 * D + g * D + (d ^ ((g & 7) * 4))));
+    }
     *M = m * kLn2;
     *L = l;
-  };
-  auto value = [&](int i) -> float {
-    const int g = i / D;
-    const float m = top(g);
-    float a = 0.f;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) a += weight(w, g, m) * red_o[(size_t)w * 16 * D + i];
     return a;
   };
-  cluster_join<T>(p, seq, h0, G, D, C, rank, reinterpret_cast<float*>(smem + WG::XCH_OFF), state, value);
+  cluster_join<T>(nh, D, C, rank, reinterpret_cast<float*>(smem + WG::XCH_OFF), EXT && wa.indptr ? 0.f : 1e-6f, part, dest);
 }
 
 // CUDA-core form, for every other pair of types, head size and group: the
@@ -399,7 +471,7 @@ __global__ void __launch_bounds__(kWinWarps * 32) window_decode_any_kernel(const
   __shared__ float qs[GC][D];
   __shared__ float ps[kWinWarps][GC][32];
   __shared__ float red_ml[kWinWarps][GC][2];
-  __shared__ float red_o[kWinWarps][GC * D];
+  __shared__ __align__(16) float red_o[kWinWarps][GC * D];
   extern __shared__ __align__(16) float xch[];
   const int C = (int)cluster_size(), rank = (int)cluster_rank();
   const int G = p.num_heads / p.num_kv_heads, per_kv = (G + GC - 1) / GC;
@@ -516,48 +588,59 @@ __global__ void __launch_bounds__(kWinWarps * 32) window_decode_any_kernel(const
     for (int i = 0; i < DPL; ++i)
       if (lane + 32 * i < D) red_o[warp][g * D + lane + 32 * i] = o[g][i];
   __syncthreads();
-  auto top = [&](int g) -> float {
-    float M = -INFINITY;
+  auto part = [&](int g, int d, float* M, float* L) -> float4 {
+    float top = -INFINITY, l = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWinWarps; ++w) M = fmaxf(M, red_ml[w][g][0]);
-    return M;
-  };
-  auto weight = [&](int w, int g, float M) -> float {
-    return red_ml[w][g][0] == -INFINITY ? 0.f : expf(red_ml[w][g][0] - M);
-  };
-  auto state = [&](int g, float* M, float* L) {
-    *M = top(g);
-    float s = 0.f;
+    for (int w = 0; w < kWinWarps; ++w) top = fmaxf(top, red_ml[w][g][0]);
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int w = 0; w < kWinWarps; ++w) s += weight(w, g, *M) * red_ml[w][g][1];
-    *L = s;
-  };
-  auto value = [&](int i) -> float {
-    const int g = i / D;
-    const float M = top(g);
-    float a = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWinWarps; ++w) a += weight(w, g, M) * red_o[w][i];
+    for (int w = 0; w < kWinWarps; ++w) {
+      const float e = red_ml[w][g][0] == -INFINITY ? 0.f : expf(red_ml[w][g][0] - top);
+      l += e * red_ml[w][g][1];
+      add_scaled(a, e, *reinterpret_cast<const float4*>(&red_o[w][g * D + d]));
+    }
+    *M = top;
+    *L = l;
     return a;
   };
-  cluster_join<Q_T>(p, seq, h0, nh, D, C, rank, xch, state, value);
+  auto dest = [&](int g) -> Q_T* {
+    return reinterpret_cast<Q_T*>(p.out) + (int64_t)seq * p.out_seq_stride + (int64_t)(h0 + g) * p.out_head_stride;
+  };
+  cluster_join<Q_T>(nh, D, C, rank, xch, 1e-6f, part, dest);
 }
 
 // ---- launches -------------------------------------------------------------------
-// CTAs to a cluster: the smallest power of two (at most 16) that brings the
-// launch to one CTA per SM, while a CTA keeps at least `least` tokens of the
-// longest run a sequence can see.
-static int window_cluster(const DecodeParams& p, const WindowArgs& w, int units, int least) {
+// How a CTA of the tensor-core form is cut: kNarrow (two or three to an SM), kWide
+// (one, with the SM's shared memory: more warps, each with fewer groups one after
+// another), kSmall (four).
+enum Form { kNarrow, kWide, kSmall };
+
+// The longest run that a query can see, in whole blocks.
+static int64_t longest_seen(const DecodeParams& p, const WindowArgs& w) {
   const int64_t sinks = (w.sinks + (int64_t)p.block_size - 1) / p.block_size * p.block_size;
-  int64_t seen = sinks + w.window + p.block_size;
-  if (seen > p.max_seq_len) seen = p.max_seq_len;
+  const int64_t seen = sinks + w.window + p.block_size;
+  return seen < p.max_seq_len ? seen : p.max_seq_len;
+}
+
+// CTAs to a cluster, a power of two, while a CTA keeps at least `least` tokens of
+// the longest run.  Where two CTAs fit an SM: the smallest (at most 16) that brings
+// the launch to one CTA per SM.  kWide: the largest that keeps it within one per SM,
+// at most 8, and 8 only to three quarters of the SMs: GPCs of 16 to 20 SMs hold two
+// such clusters each at best (one sequence of 8 KV heads 6.9 us, two 13.2 with
+// clusters of 8).
+static int window_cluster(const DecodeParams& p, const WindowArgs& w, int64_t units, int least, Form form) {
+  const int64_t seen = longest_seen(p, w), n = units * p.num_seqs, sms = decode_sm_count();
+  auto grow = [&](int c) {
+    if (form != kWide) return c < kMaxCluster && n * c < sms;
+    return c < 4 ? 2 * n * c <= sms : c == 4 && 4 * n * 8 <= 3 * sms;
+  };
   int c = 1;
-  while (c < kMaxCluster && (int64_t)units * p.num_seqs * c < decode_sm_count() && seen >= (int64_t)least * 2 * c) c *= 2;
+  while (grow(c) && seen >= (int64_t)least * 2 * c) c *= 2;
   return c;
 }
 
 template <typename K, typename... Args>
-static cudaError_t launch_clustered(K kern, int smem, int cluster, unsigned units, unsigned seqs, int threads,
+static cudaError_t launch_clustered(K kern, int smem, int cluster, unsigned units, unsigned seqs, unsigned tiles, int threads,
                                     std::atomic<bool>* configured, cudaStream_t stream, Args... args) {
   int dev = 0;
   cudaGetDevice(&dev);
@@ -568,7 +651,7 @@ static cudaError_t launch_clustered(K kern, int smem, int cluster, unsigned unit
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(units * (unsigned)cluster, seqs);
+  cfg.gridDim = dim3(units * (unsigned)cluster, seqs, tiles);
   cfg.blockDim = dim3((unsigned)threads);
   cfg.dynamicSmemBytes = (size_t)smem;
   cfg.stream = stream;
@@ -586,7 +669,7 @@ static cudaError_t launch_clustered(K kern, int smem, int cluster, unsigned unit
   return e != cudaSuccess ? e : cudaGetLastError();
 }
 
-template <typename T, int D, int BS, int NW, int STAGES, int GT, int MODE>
+template <typename T, int D, int BS, int NW, int STAGES, int GT, int MODE, bool EXT, Form FORM>
 static cudaError_t launch_window_nw(const DecodeParams& p, const WindowArgs& w, cudaStream_t stream) {
   using WG = WindowGeom<D, BS, NW, STAGES, GT, MODE>;
   TmaMaps maps;
@@ -596,30 +679,69 @@ static cudaError_t launch_window_nw(const DecodeParams& p, const WindowArgs& w, 
     if (!make_tensor_maps(p, et, D, BS, WG::Geo::VBS, WG::Geo::VSWZ, MODE, &maps)) return cudaErrorNotSupported;
   }
   static std::atomic<bool> configured[64];
-  return launch_clustered(window_decode_kernel<T, D, BS, NW, STAGES, GT, MODE>, WG::SMEM,
-                          window_cluster(p, w, p.num_kv_heads, NW * GT), (unsigned)p.num_kv_heads,
-                          (unsigned)p.num_seqs, NW * 32, configured, stream, p, w, maps);
+  // 16-row tiles of a sequence
+  const int64_t rows = (EXT ? (int64_t)w.max_q_len : 1) * (p.num_heads / p.num_kv_heads), tiles = (rows + 15) / 16;
+  if (tiles > 65535) return cudaErrorInvalidValue;
+  return launch_clustered(window_decode_kernel<T, D, BS, NW, STAGES, GT, MODE, EXT>, WG::SMEM,
+                          window_cluster(p, w, p.num_kv_heads * tiles, FORM == kWide ? NW * GT / 2 : NW * GT, FORM),
+                          (unsigned)p.num_kv_heads, (unsigned)p.num_seqs, (unsigned)tiles, NW * 32, configured, stream,
+                          p, w, maps);
 }
 
-template <typename T, int D>
-static cudaError_t launch_window_mma(const DecodeParams& p, const DecodeArgs& a, const WindowArgs& w,
-                                     cudaStream_t stream) {
-  constexpr int NW = D == 128 ? 6 : 4, ST = D == 128 ? 2 : 3;  // as the decode (decode_mma.cuh)
-  if (a.flash) {
-    const bool rows_ok = a.block_size % 16 == 0 && a.k_block_stride == (int64_t)a.block_size * a.k_tok_stride &&
-                         a.v_block_stride == (int64_t)a.block_size * a.v_tok_stride &&
-                         a.num_blocks * (int64_t)a.block_size < (int64_t)1 << 31;
-    if (rows_ok) {
-      const cudaError_t e = launch_window_nw<T, D, 16, NW, ST, 16, kFlashTma>(p, w, stream);
+// Token-major blocks whose rows a tensor map can address: 16k rows one after another.
+static bool token_row_map(const DecodeParams& p) {
+  return p.block_size % 16 == 0 && p.k_block_stride == (int64_t)p.block_size * p.k_tok_stride &&
+         p.v_block_stride == (int64_t)p.block_size * p.v_tok_stride &&
+         p.num_blocks * (int64_t)p.block_size < (int64_t)1 << 31;
+}
+
+template <typename T, int D, bool EXT, Form FORM>
+static cudaError_t launch_window_layout(const DecodeParams& p, bool flash, const WindowArgs& w, cudaStream_t stream) {
+  // 16-token groups: as the decode (decode_mma.cuh), or 12 warps, or half the
+  // decode's; 32-token pages: 2 warps (three CTAs to an SM), or 6 (12 at D = 64)
+  constexpr int NW = FORM == kWide ? 12 : (D == 128 ? 6 : 4) / (FORM == kSmall ? 2 : 1), ST = D == 128 ? 2 : 3;
+  constexpr int NP = FORM == kWide ? (D == 128 ? 6 : 12) : 2;
+  if (flash) {
+    if (token_row_map(p)) {
+      const cudaError_t e = launch_window_nw<T, D, 16, NW, ST, 16, kFlashTma, EXT, FORM>(p, w, stream);
       if (e != cudaErrorNotSupported) return e;
     }
-    return launch_window_nw<T, D, 16, NW, ST, 16, kFlash>(p, w, stream);
+    return launch_window_nw<T, D, 16, NW, ST, 16, kFlash, EXT, FORM>(p, w, stream);
   }
-  if (a.block_size == 8) return launch_window_nw<T, D, 8, NW, ST, 16, kBulk>(p, w, stream);
-  if (a.block_size == 16) return launch_window_nw<T, D, 16, NW, ST, 16, kBulk>(p, w, stream);
-  const cudaError_t e = launch_window_nw<T, D, 32, 2, 2, 32, kSwizzledV>(p, w, stream);
+  if (p.block_size == 8) return launch_window_nw<T, D, 8, NW, ST, 16, kBulk, EXT, FORM>(p, w, stream);
+  if (p.block_size == 16) return launch_window_nw<T, D, 16, NW, ST, 16, kBulk, EXT, FORM>(p, w, stream);
+  constexpr Form FP = FORM == kSmall ? kNarrow : FORM;  // (kNarrow is as small)
+  const cudaError_t e = launch_window_nw<T, D, 32, NP, 2, 32, kSwizzledV, EXT, FP>(p, w, stream);
   if (e != cudaErrorNotSupported) return e;
-  return launch_window_nw<T, D, 32, 2, 2, 32, kBulk>(p, w, stream);
+  return launch_window_nw<T, D, 32, NP, 2, 32, kBulk, EXT, FP>(p, w, stream);
+}
+
+// 16-row tiles of a call: (tiles of a sequence) x sequences x KV heads.
+static int64_t window_units(const DecodeParams& p, int64_t new_tokens) {
+  return (new_tokens * (p.num_heads / p.num_kv_heads) + 15) / 16 * p.num_seqs * p.num_kv_heads;
+}
+
+// kWide where a CTA of it for every tile fits the GPU at once, and 32-token pages,
+// single token rows or the extend's masks make a group's work long: decode of one
+// sequence, 8 KV heads, 32-token pages, window 128 / 4096: 9.4 / 11.8 us narrow, 6.1
+// / 10.5 wide; slot lists, 4 / 16 sequences, window 1024: 22.5 / 29 and 17 / 18.7;
+// 16-token pages 6.3 / 10.9 and 6.4 / 10.5 (narrow); extend of 4 x 2 tokens, 4 KV
+// heads, window 1024: 15.7 narrow, 9.7 wide.
+// kSmall where every SM gets four tiles or more and a tile is short, so that what
+// counts is how many CTAs an SM has in their start and end: decode, 8 KV heads, 128
+// sequences, window 128 / 256 / 1024: D = 128, 16-token pages 29.2 / 39.6 / 91 us
+// narrow, 28.5 / 38.7 / 103 small (256 sequences, window 64 / 128: 44 / 51 and 37 /
+// 48); D = 64 15.2 / 21.3 / 50.2 and 12.1 / 17.3 / 48.0; slot lists 47 / 63 / 159 and
+// 29 / 45 / 140.
+template <typename T, int D, bool EXT>
+static cudaError_t launch_window_mma(const DecodeParams& p, bool flash, const WindowArgs& w, cudaStream_t stream) {
+  const int64_t units = window_units(p, EXT ? w.max_q_len : 1), sms = decode_sm_count();
+  const bool slots = flash && !token_row_map(p), pages32 = !flash && p.block_size == 32;
+  if (units <= sms && (EXT || slots || pages32)) return launch_window_layout<T, D, EXT, kWide>(p, flash, w, stream);
+  if constexpr (!EXT)
+    if (units >= 4 * sms && !pages32 && longest_seen(p, w) <= (D == 64 || slots ? 1280 : 320))
+      return launch_window_layout<T, D, EXT, kSmall>(p, flash, w, stream);
+  return launch_window_layout<T, D, EXT, kNarrow>(p, flash, w, stream);
 }
 
 template <typename Q_T, typename CACHE_T, int D>
@@ -628,8 +750,8 @@ static cudaError_t launch_window_any(const DecodeParams& p, const WindowArgs& w,
   const int units = p.num_kv_heads * ((G + kWinGC - 1) / kWinGC);
   static std::atomic<bool> configured[64];
   return launch_clustered(window_decode_any_kernel<Q_T, CACHE_T, D>, exchange_floats(kWinGC, D) * 4,
-                          window_cluster(p, w, units, kWinWarps * p.block_size), (unsigned)units, (unsigned)p.num_seqs,
-                          kWinWarps * 32, configured, stream, p, w);
+                          window_cluster(p, w, units, kWinWarps * p.block_size, kNarrow), (unsigned)units, (unsigned)p.num_seqs,
+                          1, kWinWarps * 32, configured, stream, p, w);
 }
 
 template <typename Q_T, typename CACHE_T>
@@ -683,17 +805,25 @@ cudaError_t launch_window_decode(const DecodeArgs& a, const WindowArgs& w, cudaS
   p.v_tok_stride = a.v_tok_stride;
   p.table_stride = a.table_stride;
   p.scale = a.scale;
-  // tensor cores: 16-bit query and cache of one type, head size 64 / 128, up to
-  // 16 query heads to a KV head, query rows read as pairs of elements
+  // tensor cores: 16-bit query and cache of one type, head size 64 / 128, query
+  // rows read as pairs of elements
   const bool mma = a.q_type == a.cache_type && a.q_type != ElemType::F32 && (a.head_size == 64 || a.head_size == 128) &&
-                   a.num_heads / a.num_kv_heads <= 16 && (reinterpret_cast<uintptr_t>(a.q) & 3u) == 0 &&
+                   (reinterpret_cast<uintptr_t>(a.q) & 3u) == 0 &&
                    ((a.q_seq_stride | a.q_head_stride) & 1) == 0;
+  if (mma && a.num_heads / a.num_kv_heads > 16) {
+    const WindowArgs one = {w.window, w.sinks, nullptr, 1, a.num_seqs, 0};
+    if (a.q_type == ElemType::BF16)
+      return a.head_size == 128 ? launch_window_mma<__nv_bfloat16, 128, true>(p, a.flash, one, stream)
+                                : launch_window_mma<__nv_bfloat16, 64, true>(p, a.flash, one, stream);
+    return a.head_size == 128 ? launch_window_mma<__half, 128, true>(p, a.flash, one, stream)
+                              : launch_window_mma<__half, 64, true>(p, a.flash, one, stream);
+  }
   if (mma) {
     if (a.q_type == ElemType::BF16)
-      return a.head_size == 128 ? launch_window_mma<__nv_bfloat16, 128>(p, a, w, stream)
-                                : launch_window_mma<__nv_bfloat16, 64>(p, a, w, stream);
-    return a.head_size == 128 ? launch_window_mma<__half, 128>(p, a, w, stream)
-                              : launch_window_mma<__half, 64>(p, a, w, stream);
+      return a.head_size == 128 ? launch_window_mma<__nv_bfloat16, 128, false>(p, a.flash, w, stream)
+                                : launch_window_mma<__nv_bfloat16, 64, false>(p, a.flash, w, stream);
+    return a.head_size == 128 ? launch_window_mma<__half, 128, false>(p, a.flash, w, stream)
+                              : launch_window_mma<__half, 64, false>(p, a.flash, w, stream);
   }
   if (a.flash) return cudaErrorNotSupported;  // no CUDA-core kernel for token-major caches
   const int D = a.head_size;
@@ -707,10 +837,9 @@ cudaError_t launch_window_decode(const DecodeArgs& a, const WindowArgs& w, cudaS
 }
 
 // ---------------------------------------------------------------------------
-// Extend.  The tcgen05 kernel (window_umma.cuh) serves 16- and 32-token pages and
-// every dense token-major cache; the mma.sync prefill kernel in its WINDOW form the
-// rest (8-token pages, strided token rows, output rows that 16-byte stores cannot
-// write).
+// Extend.  The tcgen05 kernel (window_umma.cuh) serves every paged cache and every
+// dense token-major one; the mma.sync prefill kernel in its WINDOW form the rest
+// (strided token rows, output rows that 16-byte stores cannot write).
 // ---------------------------------------------------------------------------
 // K as rows of one 8-dim chunk of one page, [rows][BS * 8], over whatever lies
 // between the pages of a strided cache.
@@ -750,7 +879,7 @@ static cudaError_t launch_window_umma(const PrefillArgs& a, cudaStream_t stream)
   memset(&maps, 0, sizeof(maps));
   const ElemType et = std::is_same<T, __nv_bfloat16>::value ? ElemType::BF16 : ElemType::F16;
   if (LOAD == kPages) {
-    if (!make_tensor_maps(dp, et, D, BS, BS, BS * 2, kTiles, &maps) || !make_k_chunk_map(a, D, BS, &maps.k))
+    if ((BS > 8 && !make_tensor_maps(dp, et, D, BS, BS, BS * 2, kTiles, &maps)) || !make_k_chunk_map(a, D, BS, &maps.k))
       return cudaErrorNotSupported;
   } else if (!make_tensor_maps(dp, et, D, 16, 16, 128, LOAD == kRows ? kFlashTma : kFlashGather, &maps)) {
     return cudaErrorNotSupported;
@@ -784,13 +913,57 @@ static cudaError_t launch_window_umma(const PrefillArgs& a, cudaStream_t stream)
   return e != cudaSuccess ? e : cudaGetLastError();
 }
 
+// Few new tokens: the decode's kernel over 16-row tiles, split over clusters.
+template <typename T, int D>
+static cudaError_t launch_window_few(const PrefillArgs& a, cudaStream_t stream) {
+  DecodeParams p;
+  memset(&p, 0, sizeof(p));
+  p.out = a.out;
+  p.q = a.q;
+  p.k_cache = a.k_cache;
+  p.v_cache = a.v_cache;
+  p.block_tables = a.block_tables;
+  p.context_lens = a.kv_lens;
+  p.num_seqs = a.num_seqs;
+  p.num_heads = a.num_heads;
+  p.num_kv_heads = a.num_kv_heads;
+  p.block_size = a.block_size;
+  p.max_seq_len = (int)(a.table_len * a.block_size < 0x7fffffffll ? a.table_len * a.block_size : 0x7fffffffll);
+  p.num_partitions = 1;
+  p.num_blocks = a.num_blocks;
+  p.q_seq_stride = a.q_tok_stride;
+  p.q_head_stride = a.q_head_stride;
+  p.out_seq_stride = a.out_tok_stride;
+  p.out_head_stride = a.out_head_stride;
+  p.k_block_stride = a.k_block_stride;
+  p.k_head_stride = a.k_head_stride;
+  p.v_block_stride = a.v_block_stride;
+  p.v_head_stride = a.v_head_stride;
+  p.k_tok_stride = a.k_tok_stride;
+  p.v_tok_stride = a.v_tok_stride;
+  p.table_stride = a.table_stride;
+  p.scale = a.scale;
+  WindowArgs w = {a.window, a.sinks, a.qo_indptr, a.max_q_len, a.num_tokens, a.table_len};
+  return launch_window_mma<T, D, true>(p, a.token_major, w, stream);
+}
+
 template <typename T, int D>
 static cudaError_t launch_window_prefill_t(const PrefillArgs& a, cudaStream_t stream) {
+  // A 16-row tile for every SM or fewer: the decode's kernel, which splits the keys
+  // too (4 sequences, 4 KV heads, 7 heads each, window 1024; 16 / 64 / 112 / 224
+  // tiles: 9.7 / 13.4 / 17.8 / 31.7 us against 18.6 of 128-row items one after
+  // another).  Against the mma.sync kernel it holds out to three times as many (4
+  // sequences, 16-token pages, output rows off 16 bytes: 224 tiles 25 against 49 us,
+  // 448 tiles 48 against 51).
+  const int64_t units = ((int64_t)a.max_q_len * (a.num_heads / a.num_kv_heads) + 15) / 16 * a.num_seqs * a.num_kv_heads;
+  const int64_t sms = decode_sm_count();
+  if (units <= sms) return launch_window_few<T, D>(a, stream);
   cudaError_t e = cudaErrorNotSupported;
   if ((reinterpret_cast<uintptr_t>(a.out) & 15u) == 0 && ((a.out_tok_stride | a.out_head_stride) & 7) == 0) {
     if (!a.token_major) {
       if (a.block_size == 32) e = launch_window_umma<T, D, 32, kPages>(a, stream);
       else if (a.block_size == 16) e = launch_window_umma<T, D, 16, kPages>(a, stream);
+      else if (a.block_size == 8) e = launch_window_umma<T, D, 8, kPages>(a, stream);
     } else {
       const int64_t H = a.num_kv_heads, bs = a.block_size;
       // (block size 1, the pool's [slots, H, D]: a block is one row and carries no token stride)
@@ -802,7 +975,9 @@ static cudaError_t launch_window_prefill_t(const PrefillArgs& a, cudaStream_t st
       else if (dense) e = launch_window_umma<T, D, 16, kSlots>(a, stream);
     }
   }
-  return e != cudaErrorNotSupported ? e : launch_prefill_layout<T, D, true>(a, a.token_major, stream);
+  if (e != cudaErrorNotSupported) return e;
+  if (units <= 3 * sms) return launch_window_few<T, D>(a, stream);
+  return launch_prefill_layout<T, D, true>(a, a.token_major, stream);
 }
 
 cudaError_t launch_window_prefill(const PrefillArgs& a, cudaStream_t stream) {

@@ -29,9 +29,9 @@
 // sequence, S of the next tile (or item) ahead of P V of this one.
 //
 // LOAD: how a tile reaches shared memory.
-//   kPages  paged layout, 16- or 32-token pages: K by 4-row gathers of 8-dim
-//           chunk rows ([D/8][128][8], no swizzle), V a page at a time ([D][bs],
-//           rows swizzled over bs * 2 bytes: K-major for P V).
+//   kPages  paged layout: K by 4-row gathers of 8-dim chunk rows ([D/8][128][8],
+//           no swizzle), V a page at a time ([D][bs], K-major for P V: rows swizzled
+//           over their bs * 2 bytes, or as they are for 8 tokens).
 //   kRows   token-major, blocks of 16k dense rows: 16 rows x 64 dims to a copy,
 //           128-byte swizzle; K is K-major as it lies, V is MN-major (its
 //           dims, the N of P V, run along the row).
@@ -54,7 +54,7 @@ constexpr int kWinItems = 4;  // item slots
 // and carried as hi + lo (16 bits, a second product per 16 tokens) where some row
 // sees fewer: single weights are large there, and nearly cancelling V rows would
 // show the rounding (2e-3 absolute is missed with 3 keys).  16 x 512 tokens, window
-// 1024: 1 / 2 products TIMES_HERE us.
+// 1024: 1 / 2 products 131 / 164 us.
 constexpr int kSplitKeys = 64;
 
 // Products whose accumulation is known as the code is written, with the second
@@ -438,7 +438,11 @@ __global__ void __launch_bounds__(kWinThreads, 1)
                                 rb[q + 2] + lane, rb[q + 3] + lane, &full[st]);
                 }
               } else if (good) {
-                tma_load_4d(dst + lane * PAGE, map, 0, 0, kvh, (int)mine, &full[st]);
+                if constexpr (BS == 8)
+                  bulk_g2s(dst + lane * PAGE, reinterpret_cast<const T*>(p.v_cache) + (int64_t)mine * p.v_block_stride +
+                                                  (int64_t)kvh * p.v_head_stride, PAGE, &full[st]);
+                else
+                  tma_load_4d(dst + lane * PAGE, map, 0, 0, kvh, (int)mine, &full[st]);
               }
             } else if (good) {
               const int row = (int)mine * tbs + tok % tbs;  // (rows are below 2^31: the host checked)
@@ -474,7 +478,7 @@ __global__ void __launch_bounds__(kWinThreads, 1)
                               (2 * i + 1 < lo || 2 * i + 1 >= hi ? 0xffff0000u : 0u);
                   const bool whole = lo <= 0 && hi >= 8;
                   for (int d = lane; d < D; d += 32) {
-                    const int phys = BS == 32 ? (ch ^ ((d >> 1) & 3)) : (ch ^ ((d >> 2) & 1));
+                    const int phys = BS == 32 ? (ch ^ ((d >> 1) & 3)) : (BS == 16 ? (ch ^ ((d >> 2) & 1)) : 0);
                     uint4* w16 = reinterpret_cast<uint4*>(dst + (tk / BS) * PAGE + d * BS * 2 + phys * 16);
                     uint4 v = make_uint4(0u, 0u, 0u, 0u);
                     if (!whole) {
@@ -524,8 +528,9 @@ __global__ void __launch_bounds__(kWinThreads, 1)
                                               : umma::smem_desc(smem_u32(kring), 16, 1024, kLayoutSw128);
       const uint64_t v_desc0 =
           LOAD != kPages ? umma::smem_desc(smem_u32(vring), HALF, 1024, kLayoutSw128)
-                         : (BS == 32 ? umma::smem_desc(smem_u32(vring), 16, 512, umma::kLayoutSw64)
-                                     : umma::smem_desc(smem_u32(vring), 16, 256, umma::kLayoutSw32));
+                         : (BS == 32   ? umma::smem_desc(smem_u32(vring), 16, 512, umma::kLayoutSw64)
+                            : BS == 16 ? umma::smem_desc(smem_u32(vring), 16, 256, umma::kLayoutSw32)
+                                       : umma::smem_desc(smem_u32(vring), PAGE, 128, umma::kLayoutNone));
       // S of tile g, then P V of tile g - 1, over the tiles of all items
       int g = 0, nq = 0;                        // tiles, items with keys so far
       int pv_left = 0, pv_j = -1;               // the tile whose P V is due: keys from its first token on, its place

@@ -289,6 +289,103 @@ def test_extend_of_one_token(gpu):
     check_extend(Case(34, "float16", [5, 64, 700], 8, 2, 64, 16), 90, 4)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("window,sinks", WINDOWS)
+@pytest.mark.parametrize("layout,bs,d", [("paged", 8, 128), ("paged", 16, 128), ("paged", 32, 128), ("paged", 16, 64),
+                                         ("paged", 32, 64), ("flash", 16, 128), ("flash", 32, 64), ("flash", 5, 64),
+                                         ("pool", 1, 128), ("pool", 1, 64)])
+def test_extend_few_tokens(gpu, layout, bs, d, window, sinks):
+    """At most one 16-row tile to an SM: tiles of several tokens, whole and ragged, split over a cluster."""
+    c = Case(36, "bfloat16", [1, 40, 133, 300, 555, 2000], 6, 2, d, bs, layout, new=[1, 7, 33, 0, 20, 2])
+    check_extend(c, window, sinks, f"{layout} {bs} {d}")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seqs", [2, 8, 40])
+def test_extend_unaligned_output_rows(gpu, seqs):
+    """Output rows that start at 4 bytes past a 16-byte boundary, from few 16-row tiles to many."""
+    rng = np.random.default_rng(37)
+    new = rng.integers(20, 61, seqs)
+    c = Case(37, "bfloat16", new + rng.integers(0, 300, seqs), 16, 4, 128, 16, new=new)
+    ref = c.reference(70, 3, 0.0)
+    q, kc, vc, tables, lens = c.upload()
+    wide = DeviceArray.zeros((q.shape[0], 16, 136), "bfloat16")
+    mk.paged_prefill_window(q, kc, vc, tables, c.indptr, lens, 4, c.scale, 16, 70, 3, out=wide[:, :, 2:130])
+    got = wide.to_numpy()
+    assert_close(got[:, :, 2:130], ref, *tolerance("bfloat16"))
+    assert not got[:, :, :2].any() and not got[:, :, 130:].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seqs", [2, 40])
+@pytest.mark.parametrize("bs", [5, 16])
+def test_extend_strided_token_rows(gpu, seqs, bs):
+    """A token-major cache that is a slice of wider rows."""
+    rng = np.random.default_rng(38)
+    new = rng.integers(20, 61, seqs)
+    c = Case(38, "float16", new + rng.integers(0, 300, seqs), 16, 4, 64, bs, "flash", new=new)
+    ref = c.reference(70, 3, 0.0)
+    q, _, _, tables, lens = c.upload()
+    caches = []
+    for rows in (c.k_rows, c.v_rows):
+        wide = np.full((c.blocks, bs, 6, 64), NAN, np.float32)
+        wide[:, :, 1:5] = rows.reshape(c.blocks, bs, 4, 64)
+        caches.append(DeviceArray.from_numpy(wide, dtype="float16")[:, :, 1:5])
+    got = mk.paged_prefill_window(q, caches[0], caches[1], tables, c.indptr, lens, 4, c.scale, bs, 70, 3).to_numpy()
+    assert_close(got, ref, *tolerance("float16"))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seqs", [3, 40])
+def test_extend_index_errors(gpu, seqs):
+    """Lengths that the host cannot see: the status word names the error, the sequence's
+    rows are 0, rows past the query are not written, and the other sequences are right."""
+    rng = np.random.default_rng(39)
+    new = rng.integers(20, 61, seqs)
+    c = Case(39, "bfloat16", new + rng.integers(0, 300, seqs), 16, 4, 64, 16, new=new)
+    ref = c.reference(70, 3, 0.0)
+    q, kc, vc, tables, _ = c.upload()
+    for bad in (int(new[1]) - 1, c.max_seq_len + 1):
+        kl = c.lens.astype(np.int32)
+        kl[1] = bad
+        _lib.get_status(0, clear=True)
+        got = mk.paged_prefill_window(q, kc, vc, tables, c.indptr, kl, 4, c.scale, 16, 70, 3).to_numpy()
+        assert _lib.get_status(0, clear=True) == _lib.STATUS_INDEX_OOB
+        want = ref.copy()
+        want[c.indptr[1]:c.indptr[2]] = 0
+        assert_close(got, want, *tolerance("bfloat16"))
+    last = int(c.indptr[-2])  # the last sequence reaches past a query one row shorter than its tokens
+    out = DeviceArray.zeros(q.shape, "bfloat16")
+    mk.paged_prefill_window(q[:-1], kc, vc, tables, DeviceArray.from_numpy(c.indptr), c.lens.astype(np.int32), 4, c.scale,
+                            16, 70, 3, max_q_len=int(new.max()), out=out[:-1])
+    assert _lib.get_status(0, clear=True) == _lib.STATUS_INDEX_OOB
+    got = out.to_numpy()
+    assert_close(got[:last], ref[:last], *tolerance("bfloat16"))
+    assert not got[last:].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seqs", [2, 40])
+def test_extend_bits_repeat(gpu, seqs):
+    """The same call gives the same bits, on any stream; max_q_len may be larger than needed."""
+    rng = np.random.default_rng(41)
+    new = rng.integers(20, 61, seqs)
+    c = Case(41, "bfloat16", new + rng.integers(0, 900, seqs), 16, 4, 128, 32, new=new)
+    ref = c.reference(200, 3, 0.0)
+    q, kc, vc, tables, lens = c.upload()
+    args = (q, kc, vc, tables, DeviceArray.from_numpy(c.indptr), lens, 4, c.scale, 32, 200, 3)
+    for longest in (int(new.max()), q.shape[0]):
+        first = mk.paged_prefill_window(*args, max_q_len=longest)
+        assert_close(first.to_numpy(), ref, *tolerance("bfloat16"))
+        for _ in range(3):
+            s = Stream()
+            out = DeviceArray.zeros(q.shape, "bfloat16")
+            mk.synchronize()
+            mk.paged_prefill_window(*args, max_q_len=longest, out=out, stream=s)
+            s.synchronize()
+            np.testing.assert_array_equal(out.to_numpy(raw=True), first.to_numpy(raw=True))
+
+
 # ---- refusals -------------------------------------------------------------------
 
 
