@@ -65,9 +65,7 @@ __device__ __forceinline__ uint32_t pack_out<__nv_bfloat16>(float a, float b) {
 
 // MODE: kBulk (paged layout, BS-token pages) or kFlashBulk (token-major rows;
 // BS is then only a template placeholder and p.block_size is read at run time).
-// WINDOW: a sliding window whose first p.sinks tokens stay visible; key positions
-// below are then the tile's virtual ones (struct Seen).
-template <typename T, int D, int BS, int STAGES, int MODE, bool WINDOW = false>
+template <typename T, int D, int BS, int STAGES, int MODE>
 __global__ void __launch_bounds__((kPrefillConsumers + 1) * 32) prefill_kernel(PrefillParams p) {
   using namespace mma_detail;
   using PG = PrefillGeom<D, BS, STAGES, MODE>;
@@ -104,12 +102,8 @@ __global__ void __launch_bounds__((kPrefillConsumers + 1) * 32) prefill_kernel(P
   const int prefix = bad ? 0 : (int)(kvl - ql);
   const int64_t R_last = (R0 + kPrefillRows < rows ? R0 + kPrefillRows : rows) - 1;
   const int t_first = (int)(R0 / G), t_last = (int)(R_last / G);
-  Seen seen = {};
-  if constexpr (WINDOW)
-    seen = seen_range(prefix + t_first, prefix + t_last, p.window, p.sinks, FLASH ? p.block_size : BS);
-  const int jump = WINDOW ? seen.jump : 0;
-  const int kv_end = bad ? 0 : prefix + t_last + 1 - jump;
-  int kv_beg = !WINDOW && p.window > 0 ? prefix + t_first + 1 - p.window : 0;
+  const int kv_end = bad ? 0 : prefix + t_last + 1;
+  int kv_beg = p.window > 0 ? prefix + t_first + 1 - p.window : 0;
   kv_beg = kv_beg > 0 ? kv_beg / GT * GT : 0;  // groups start GT-aligned (whole pages)
   const int ngroups = kv_end > kv_beg ? (kv_end - kv_beg + GT - 1) / GT : 0;
   if (q1 > p.num_tokens) return;  // rows outside q / out: nothing may be written
@@ -134,8 +128,7 @@ __global__ void __launch_bounds__((kPrefillConsumers + 1) * 32) prefill_kernel(P
       uint32_t id = 0xffffffffu;
       if (lane < NID && k < ngroups) {
         const int tok = kv_beg + k * GT + lane * VBS;
-        const int vb = FLASH ? tok / p.block_size : tok / BS;
-        if (tok < kv_end) id = __ldg(table + (WINDOW ? seen.real_block(vb) : vb));
+        if (tok < kv_end) id = __ldg(table + (FLASH ? tok / p.block_size : tok / BS));
       }
       return id;
     };
@@ -239,18 +232,13 @@ __global__ void __launch_bounds__((kPrefillConsumers + 1) * 32) prefill_kernel(P
   const int t_lo = (int)(R_lo / G), g_lo = (int)(R_lo - (int64_t)t_lo * G);
   const int t_hi = (int)(R_hi / G), g_hi = (int)(R_hi - (int64_t)t_hi * G);
   const bool on_lo = R_lo < rows, on_hi = R_hi < rows;
-  const int end_lo = on_lo && !bad ? prefix + t_lo + 1 - jump : 0;
-  const int end_hi = on_hi && !bad ? prefix + t_hi + 1 - jump : 0;
+  const int end_lo = on_lo && !bad ? prefix + t_lo + 1 : 0;
+  const int end_hi = on_hi && !bad ? prefix + t_hi + 1 : 0;
   const int beg_lo = p.window > 0 ? end_lo - p.window : 0;
   const int beg_hi = p.window > 0 ? end_hi - p.window : 0;
-  // key range any row of this warp sees: groups outside it are skipped (rows
-  // past the tile's last see nothing and must not widen the window form's start)
+  // key range any row of this warp sees: groups outside it are skipped
   int w_end = end_lo > end_hi ? end_lo : end_hi;
   int w_beg = beg_lo < beg_hi ? beg_lo : beg_hi;
-  if constexpr (WINDOW) {
-    w_beg = end_lo > 0 ? beg_lo : 0x7fffffff;
-    if (end_hi > 0 && beg_hi < w_beg) w_beg = beg_hi;
-  }
 #pragma unroll
   for (int o = 4; o < 32; o <<= 1) {
     w_end = max(w_end, __shfl_xor_sync(0xffffffffu, w_end, o));
@@ -291,12 +279,11 @@ __global__ void __launch_bounds__((kPrefillConsumers + 1) * 32) prefill_kernel(P
       break;
     }
     const int tok0 = kv_beg + k * GT;
-    if (tok0 < w_end && (tok0 + GT > w_beg || (WINDOW && tok0 < p.sinks))) {
+    if (tok0 < w_end && tok0 + GT > w_beg) {
       const uint8_t* st = smem + (size_t)s * Geo::STAGE;
       // bf16 P keeps the hi + lo split: one bf16 P misses 2e-3 abs / 1e-2 rel on short rows
-      mma_group<T, Geo, D, true, WINDOW>(gs, qa, smem_u32(st), smem_u32(st + NBOX * BOX), tok0, kv_end, masks[s], 0,
-                                         qk_scale, false, 0.f, 0.f, lane, end_lo, end_hi, beg_lo, beg_hi,
-                                         WINDOW ? p.sinks : 0, WINDOW ? w_beg : 0);
+      mma_group<T, Geo, D>(gs, qa, smem_u32(st), smem_u32(st + NBOX * BOX), tok0, kv_end, masks[s], 0, qk_scale,
+                           false, 0.f, 0.f, lane, end_lo, end_hi, beg_lo, beg_hi);
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(&empty[s]);
@@ -317,11 +304,11 @@ __global__ void __launch_bounds__((kPrefillConsumers + 1) * 32) prefill_kernel(P
   if (on_hi) store_row(t_hi, g_hi, inv_hi, 1);
 }
 
-template <typename T, int D, int BS, int MODE, bool WINDOW = false>
+template <typename T, int D, int BS, int MODE>
 static cudaError_t launch_prefill(const PrefillParams& p, cudaStream_t stream) {
   constexpr int STAGES = 4;
   using PG = PrefillGeom<D, BS, STAGES, MODE>;
-  auto kern = prefill_kernel<T, D, BS, STAGES, MODE, WINDOW>;
+  auto kern = prefill_kernel<T, D, BS, STAGES, MODE>;
   static std::atomic<bool> configured[64];  // per device; setting the attribute twice is harmless
   int dev = 0;
   cudaGetDevice(&dev);
@@ -340,12 +327,12 @@ static cudaError_t launch_prefill(const PrefillParams& p, cudaStream_t stream) {
   return cudaGetLastError();
 }
 
-template <typename T, int D, bool WINDOW = false>
+template <typename T, int D>
 static cudaError_t launch_prefill_layout(const PrefillParams& p, bool token_major, cudaStream_t stream) {
-  if (token_major) return launch_prefill<T, D, 16, kFlashBulk, WINDOW>(p, stream);
-  if (p.block_size == 8) return launch_prefill<T, D, 8, kBulk, WINDOW>(p, stream);
-  if (p.block_size == 16) return launch_prefill<T, D, 16, kBulk, WINDOW>(p, stream);
-  if (p.block_size == 32) return launch_prefill<T, D, 32, kBulk, WINDOW>(p, stream);
+  if (token_major) return launch_prefill<T, D, 16, kFlashBulk>(p, stream);
+  if (p.block_size == 8) return launch_prefill<T, D, 8, kBulk>(p, stream);
+  if (p.block_size == 16) return launch_prefill<T, D, 16, kBulk>(p, stream);
+  if (p.block_size == 32) return launch_prefill<T, D, 32, kBulk>(p, stream);
   return cudaErrorNotSupported;
 }
 

@@ -1,7 +1,7 @@
 // window.cu — attention over a sliding window with a few first tokens that stay
 // visible (sinks), on the paged and token-major caches, for sm_100a: one new
 // token per sequence (decode, below) and the new tokens of a ragged batch
-// (extend: the prefill kernels in their WINDOW form).
+// (extend).
 //
 // The query at position i of a sequence sees position j <= i when j < sinks or
 // j > i - window:
@@ -140,7 +140,7 @@ __device__ __forceinline__ void cluster_join(int nh, int D, int C, int rank, flo
 // streams every NW-th group of GT tokens of the CTA's run through its own ring of
 // STAGES stages, as paged_decode_mma_kernel does.  MODE: kBulk (whole pages),
 // kSwizzledV (32-token pages), kFlashTma (token rows in blocks of 16k), kFlash
-// (token rows).  EXT: several such tiles to a sequence and KV head (grid.z): the
+// (token rows).  EXT: several such tiles to a sequence and KV head: the
 // extend's few new tokens (indptr), or, without indptr, more than 16 heads of one.
 template <int D, int BS, int NW, int STAGES, int GT, int MODE>
 struct WindowGeom {
@@ -160,7 +160,8 @@ __global__ void __launch_bounds__(NW * 32)
   extern __shared__ __align__(128) uint8_t smem[];
 
   const int C = (int)cluster_size(), rank = (int)cluster_rank();
-  const int kvh = blockIdx.x / C, seq = blockIdx.y;
+  const int unit = blockIdx.x / C, seq = blockIdx.y;
+  const int tile = EXT ? unit / p.num_kv_heads : 0, kvh = unit - tile * p.num_kv_heads;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r = lane >> 2, q4 = lane & 3;
   const int G = p.num_heads / p.num_kv_heads, h0 = kvh * G;
@@ -168,7 +169,7 @@ __global__ void __launch_bounds__(NW * 32)
   const int rbs = Geo::TROWS || Geo::FLASH ? p.block_size : BS;
   // rows R0 .. R0 + nh - 1 of the sequence's new tokens, whose first is row q0 of
   // q / out and position `prefix`
-  const int R0 = EXT ? blockIdx.z * 16 : 0;
+  const int R0 = tile * 16;
   const uint32_t ctx = p.context_lens[seq];
   int64_t q0 = seq;
   int rows = G, prefix = (int)ctx - 1;
@@ -184,7 +185,7 @@ __global__ void __launch_bounds__(NW * 32)
     // rows past q may not be written; other index errors give zeros
     zero = ql > wa.max_q_len || (int64_t)ctx < ql || (int64_t)ctx > wa.table_len * (int64_t)rbs || ctx > 0x7fffff00u;
     const bool past = b > wa.num_tokens;
-    if ((zero || past) && threadIdx.x == 0 && R0 == 0 && blockIdx.x == 0) set_status(&g_decode_status, KVC_STATUS_INDEX_OOB);
+    if ((zero || past) && threadIdx.x == 0 && blockIdx.x == 0) set_status(&g_decode_status, KVC_STATUS_INDEX_OOB);
     if (past) {
       grid_dependency_wait();
       return;
@@ -623,11 +624,11 @@ static int64_t longest_seen(const DecodeParams& p, const WindowArgs& w) {
 }
 
 // CTAs to a cluster, a power of two, while a CTA keeps at least `least` tokens of
-// the longest run.  Where two CTAs fit an SM: the smallest (at most 16) that brings
-// the launch to one CTA per SM.  kWide: the largest that keeps it within one per SM,
+// the longest run.  kWide: the largest that keeps the launch within one CTA per SM,
 // at most 8, and 8 only to three quarters of the SMs: GPCs of 16 to 20 SMs hold two
-// such clusters each at best (one sequence of 8 KV heads 6.9 us, two 13.2 with
-// clusters of 8).
+// such clusters each at best (two sequences of 8 KV heads, 32-token pages, window
+// 1024: 13.2 us in clusters of 8, 7.3 of 4).  Else the smallest (at most 16) that
+// brings the launch to one CTA per SM.
 static int window_cluster(const DecodeParams& p, const WindowArgs& w, int64_t units, int least, Form form) {
   const int64_t seen = longest_seen(p, w), n = units * p.num_seqs, sms = decode_sm_count();
   auto grow = [&](int c) {
@@ -640,8 +641,9 @@ static int window_cluster(const DecodeParams& p, const WindowArgs& w, int64_t un
 }
 
 template <typename K, typename... Args>
-static cudaError_t launch_clustered(K kern, int smem, int cluster, unsigned units, unsigned seqs, unsigned tiles, int threads,
+static cudaError_t launch_clustered(K kern, int smem, int cluster, int64_t units, unsigned seqs, int threads,
                                     std::atomic<bool>* configured, cudaStream_t stream, Args... args) {
+  if (units * cluster > 0x7fffffffll) return cudaErrorInvalidValue;
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64 || !configured[dev]) {  // setting the attributes twice is harmless
@@ -651,7 +653,7 @@ static cudaError_t launch_clustered(K kern, int smem, int cluster, unsigned unit
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(units * (unsigned)cluster, seqs, tiles);
+  cfg.gridDim = dim3((unsigned)units * (unsigned)cluster, seqs);
   cfg.blockDim = dim3((unsigned)threads);
   cfg.dynamicSmemBytes = (size_t)smem;
   cfg.stream = stream;
@@ -681,11 +683,10 @@ static cudaError_t launch_window_nw(const DecodeParams& p, const WindowArgs& w, 
   static std::atomic<bool> configured[64];
   // 16-row tiles of a sequence
   const int64_t rows = (EXT ? (int64_t)w.max_q_len : 1) * (p.num_heads / p.num_kv_heads), tiles = (rows + 15) / 16;
-  if (tiles > 65535) return cudaErrorInvalidValue;
+  const int64_t units = p.num_kv_heads * tiles;
   return launch_clustered(window_decode_kernel<T, D, BS, NW, STAGES, GT, MODE, EXT>, WG::SMEM,
-                          window_cluster(p, w, p.num_kv_heads * tiles, FORM == kWide ? NW * GT / 2 : NW * GT, FORM),
-                          (unsigned)p.num_kv_heads, (unsigned)p.num_seqs, (unsigned)tiles, NW * 32, configured, stream,
-                          p, w, maps);
+                          window_cluster(p, w, units, FORM == kWide ? NW * GT / 2 : NW * GT, FORM), units,
+                          (unsigned)p.num_seqs, NW * 32, configured, stream, p, w, maps);
 }
 
 // Token-major blocks whose rows a tensor map can address: 16k rows one after another.
@@ -721,26 +722,28 @@ static int64_t window_units(const DecodeParams& p, int64_t new_tokens) {
   return (new_tokens * (p.num_heads / p.num_kv_heads) + 15) / 16 * p.num_seqs * p.num_kv_heads;
 }
 
-// kWide where a CTA of it for every tile fits the GPU at once, and 32-token pages,
-// single token rows or the extend's masks make a group's work long: decode of one
-// sequence, 8 KV heads, 32-token pages, window 128 / 4096: 9.4 / 11.8 us narrow, 6.1
-// / 10.5 wide; slot lists, 4 / 16 sequences, window 1024: 22.5 / 29 and 17 / 18.7;
-// 16-token pages 6.3 / 10.9 and 6.4 / 10.5 (narrow); extend of 4 x 2 tokens, 4 KV
-// heads, window 1024: 15.7 narrow, 9.7 wide.
-// kSmall where every SM gets four tiles or more and a tile is short, so that what
-// counts is how many CTAs an SM has in their start and end: decode, 8 KV heads, 128
-// sequences, window 128 / 256 / 1024: D = 128, 16-token pages 29.2 / 39.6 / 91 us
-// narrow, 28.5 / 38.7 / 103 small (256 sequences, window 64 / 128: 44 / 51 and 37 /
-// 48); D = 64 15.2 / 21.3 / 50.2 and 12.1 / 17.3 / 48.0; slot lists 47 / 63 / 159 and
-// 29 / 45 / 140.
+// kWide where every tile gets an SM or more (decode, 8 KV heads, window 1024, 1 / 2 /
+// 4 / 8 / 16 sequences: 32-token pages 7.8 / 15.0 / 10.8 / 13.1 / 20.0 us narrow, 6.1
+// / 7.3 / 8.0 / 11.5 / 16.7 wide; 16-token pages 6.3 / 7.1 / 9.3 / 10.5 / 16.8 and 6.3
+// / 6.6 / 8.1 / 10.6 / 16.0; slot lists 7.4 / 14.1 / 21.7 / 19.7 / 29.5 and 7.2 / 8.2
+// / 9.9 / 12.4 / 18.7).
+// kSmall where every SM gets four tiles or more, so that it pays to have more CTAs in
+// their start and end, and the groups are short (D = 64, single token rows) or few
+// (decode, 8 KV heads, 128 sequences, window 64 / 128 / 256 / 1024: D = 128, 16-token
+// pages 19.3 / 24.2 / 33.6 / 87.9 us narrow, 17.6 / 24.5 / 35.1 / 99.6 small, and with
+// 256 sequences 34.7 / 43.1 / 58.7 / 162.8 and 29.8 / 41.2 / 58.8 / 168.9; D = 64 9.4 /
+// 13.6 / 19.7 / 48.5 and 7.2 / 11.3 / 16.6 / 47.8; slot lists 31 / 41 / 57 / 153 and 19
+// / 26 / 42 / 136; 64 sequences of D = 64, under four tiles to an SM: 4.9 / 6.3 / 10.3
+// / 26.1 and 5.5 / 7.9 / 12.9 / 39.8).
 template <typename T, int D, bool EXT>
 static cudaError_t launch_window_mma(const DecodeParams& p, bool flash, const WindowArgs& w, cudaStream_t stream) {
   const int64_t units = window_units(p, EXT ? w.max_q_len : 1), sms = decode_sm_count();
-  const bool slots = flash && !token_row_map(p), pages32 = !flash && p.block_size == 32;
-  if (units <= sms && (EXT || slots || pages32)) return launch_window_layout<T, D, EXT, kWide>(p, flash, w, stream);
-  if constexpr (!EXT)
-    if (units >= 4 * sms && !pages32 && longest_seen(p, w) <= (D == 64 || slots ? 1280 : 320))
+  if (units <= sms) return launch_window_layout<T, D, EXT, kWide>(p, flash, w, stream);
+  if constexpr (!EXT) {
+    const bool slots = flash && !token_row_map(p), pages32 = !flash && p.block_size == 32;
+    if (units >= 4 * sms && !pages32 && (D == 64 || slots || longest_seen(p, w) <= 160))
       return launch_window_layout<T, D, EXT, kSmall>(p, flash, w, stream);
+  }
   return launch_window_layout<T, D, EXT, kNarrow>(p, flash, w, stream);
 }
 
@@ -750,8 +753,8 @@ static cudaError_t launch_window_any(const DecodeParams& p, const WindowArgs& w,
   const int units = p.num_kv_heads * ((G + kWinGC - 1) / kWinGC);
   static std::atomic<bool> configured[64];
   return launch_clustered(window_decode_any_kernel<Q_T, CACHE_T, D>, exchange_floats(kWinGC, D) * 4,
-                          window_cluster(p, w, units, kWinWarps * p.block_size, kNarrow), (unsigned)units, (unsigned)p.num_seqs,
-                          1, kWinWarps * 32, configured, stream, p, w);
+                          window_cluster(p, w, units, kWinWarps * p.block_size, kNarrow), units, (unsigned)p.num_seqs,
+                          kWinWarps * 32, configured, stream, p, w);
 }
 
 template <typename Q_T, typename CACHE_T>
@@ -837,9 +840,10 @@ cudaError_t launch_window_decode(const DecodeArgs& a, const WindowArgs& w, cudaS
 }
 
 // ---------------------------------------------------------------------------
-// Extend.  The tcgen05 kernel (window_umma.cuh) serves every paged cache and every
-// dense token-major one; the mma.sync prefill kernel in its WINDOW form the rest
-// (strided token rows, output rows that 16-byte stores cannot write).
+// Extend.  The tcgen05 kernel (window_umma.cuh) serves every paged and token-major
+// cache that tensor maps describe (pages a whole number of K chunk rows apart, token
+// rows that hold all heads a fixed distance apart, fewer than 2^31 of either); the
+// decode's kernel serves few new tokens, and any number from the other caches.
 // ---------------------------------------------------------------------------
 // K as rows of one 8-dim chunk of one page, [rows][BS * 8], over whatever lies
 // between the pages of a strided cache.
@@ -859,8 +863,26 @@ static bool make_k_chunk_map(const PrefillArgs& a, int D, int BS, CUtensorMap* m
          CUDA_SUCCESS;
 }
 
-template <typename T, int D, int BS, int LOAD>
-static cudaError_t launch_window_umma(const PrefillArgs& a, cudaStream_t stream) {
+// Token rows of a token-major cache, [rows][all heads of a row]: row `token` of block
+// b is row b * (block stride / token stride) + token.
+static bool make_token_row_map(const PrefillArgs& a, const void* base, int D, int64_t block, int64_t tok, int64_t head,
+                               CUtensorMap* map) {
+  auto enc = tensor_map_encoder();
+  if (!enc || tok <= 0 || block <= 0 || head < 0 || block % tok) return false;
+  const int64_t width = (a.num_kv_heads - 1) * head + D;
+  const int64_t rows = (a.num_blocks - 1) * (block / tok) + a.block_size;
+  if (width > tok || rows <= 0 || rows > 0x7fffffffll || width > 0x7fffffffll) return false;
+  const cuuint64_t dims[2] = {(cuuint64_t)width, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)tok * 2};
+  const cuuint32_t box[2] = {64, 1};
+  const cuuint32_t ones[2] = {1, 1};
+  return enc(map, a.q_type == ElemType::BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+             const_cast<void*>(base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int D, int BS, int LOAD, bool OUT16>
+static cudaError_t launch_window_umma_out(const PrefillArgs& a, cudaStream_t stream) {
   using WG = WinUmmaGeom<D, BS, LOAD>;
   DecodeParams dp;
   memset(&dp, 0, sizeof(dp));
@@ -881,10 +903,18 @@ static cudaError_t launch_window_umma(const PrefillArgs& a, cudaStream_t stream)
   if (LOAD == kPages) {
     if ((BS > 8 && !make_tensor_maps(dp, et, D, BS, BS, BS * 2, kTiles, &maps)) || !make_k_chunk_map(a, D, BS, &maps.k))
       return cudaErrorNotSupported;
-  } else if (!make_tensor_maps(dp, et, D, 16, 16, 128, LOAD == kRows ? kFlashTma : kFlashGather, &maps)) {
-    return cudaErrorNotSupported;
+  } else if (LOAD == kRows) {
+    if (!make_tensor_maps(dp, et, D, 16, 16, 128, kFlashTma, &maps)) return cudaErrorNotSupported;
+  } else {
+    // (block size 1, the pool's [slots, H, D]: a block is one row and carries no token stride)
+    const bool one = a.block_size == 1;
+    if (!make_token_row_map(a, a.k_cache, D, a.k_block_stride, one ? a.k_block_stride : a.k_tok_stride, a.k_head_stride,
+                            &maps.k) ||
+        !make_token_row_map(a, a.v_cache, D, a.v_block_stride, one ? a.v_block_stride : a.v_tok_stride, a.v_head_stride,
+                            &maps.v))
+      return cudaErrorNotSupported;
   }
-  auto kern = window_umma_kernel<T, D, BS, LOAD>;
+  auto kern = window_umma_kernel<T, D, BS, LOAD, OUT16>;
   static std::atomic<bool> configured[64];  // per device; setting the attribute twice is harmless
   int dev = 0;
   cudaGetDevice(&dev);
@@ -913,7 +943,14 @@ static cudaError_t launch_window_umma(const PrefillArgs& a, cudaStream_t stream)
   return e != cudaSuccess ? e : cudaGetLastError();
 }
 
-// Few new tokens: the decode's kernel over 16-row tiles, split over clusters.
+template <typename T, int D, int BS, int LOAD>
+static cudaError_t launch_window_umma(const PrefillArgs& a, cudaStream_t stream) {
+  return (reinterpret_cast<uintptr_t>(a.out) & 15u) == 0 && ((a.out_tok_stride | a.out_head_stride) & 7) == 0
+             ? launch_window_umma_out<T, D, BS, LOAD, true>(a, stream)
+             : launch_window_umma_out<T, D, BS, LOAD, false>(a, stream);
+}
+
+// The decode's kernel over 16-row tiles, split over clusters.
 template <typename T, int D>
 static cudaError_t launch_window_few(const PrefillArgs& a, cudaStream_t stream) {
   DecodeParams p;
@@ -952,32 +989,24 @@ static cudaError_t launch_window_prefill_t(const PrefillArgs& a, cudaStream_t st
   // A 16-row tile for every SM or fewer: the decode's kernel, which splits the keys
   // too (4 sequences, 4 KV heads, 7 heads each, window 1024; 16 / 64 / 112 / 224
   // tiles: 9.7 / 13.4 / 17.8 / 31.7 us against 18.6 of 128-row items one after
-  // another).  Against the mma.sync kernel it holds out to three times as many (4
-  // sequences, 16-token pages, output rows off 16 bytes: 224 tiles 25 against 49 us,
-  // 448 tiles 48 against 51).
+  // another).
   const int64_t units = ((int64_t)a.max_q_len * (a.num_heads / a.num_kv_heads) + 15) / 16 * a.num_seqs * a.num_kv_heads;
   const int64_t sms = decode_sm_count();
   if (units <= sms) return launch_window_few<T, D>(a, stream);
   cudaError_t e = cudaErrorNotSupported;
-  if ((reinterpret_cast<uintptr_t>(a.out) & 15u) == 0 && ((a.out_tok_stride | a.out_head_stride) & 7) == 0) {
-    if (!a.token_major) {
-      if (a.block_size == 32) e = launch_window_umma<T, D, 32, kPages>(a, stream);
-      else if (a.block_size == 16) e = launch_window_umma<T, D, 16, kPages>(a, stream);
-      else if (a.block_size == 8) e = launch_window_umma<T, D, 8, kPages>(a, stream);
-    } else {
-      const int64_t H = a.num_kv_heads, bs = a.block_size;
-      // (block size 1, the pool's [slots, H, D]: a block is one row and carries no token stride)
-      const int64_t ktok = bs == 1 ? a.k_block_stride : a.k_tok_stride, vtok = bs == 1 ? a.v_block_stride : a.v_tok_stride;
-      const bool blocks = a.k_block_stride == bs * ktok && a.v_block_stride == bs * vtok &&
-                          a.num_blocks * bs * H < (int64_t)1 << 31;
-      const bool dense = blocks && a.k_head_stride == D && ktok == H * D && a.v_head_stride == D && vtok == H * D;
-      if (blocks && bs % 16 == 0) e = launch_window_umma<T, D, 16, kRows>(a, stream);
-      else if (dense) e = launch_window_umma<T, D, 16, kSlots>(a, stream);
-    }
+  if (!a.token_major) {
+    if (a.block_size == 32) e = launch_window_umma<T, D, 32, kPages>(a, stream);
+    else if (a.block_size == 16) e = launch_window_umma<T, D, 16, kPages>(a, stream);
+    else if (a.block_size == 8) e = launch_window_umma<T, D, 8, kPages>(a, stream);
+  } else {
+    const int64_t bs = a.block_size;
+    if (bs % 16 == 0 && a.k_block_stride == bs * a.k_tok_stride && a.v_block_stride == bs * a.v_tok_stride &&
+        a.num_blocks * bs < (int64_t)1 << 31)
+      e = launch_window_umma<T, D, 16, kRows>(a, stream);
+    if (e == cudaErrorNotSupported) e = launch_window_umma<T, D, 16, kSlots>(a, stream);
   }
-  if (e != cudaErrorNotSupported) return e;
-  if (units <= 3 * sms) return launch_window_few<T, D>(a, stream);
-  return launch_prefill_layout<T, D, true>(a, a.token_major, stream);
+  // (a cache that no tensor map describes: per-lane or bulk copies)
+  return e != cudaErrorNotSupported ? e : launch_window_few<T, D>(a, stream);
 }
 
 cudaError_t launch_window_prefill(const PrefillArgs& a, cudaStream_t stream) {

@@ -35,8 +35,8 @@
 //   kRows   token-major, blocks of 16k dense rows: 16 rows x 64 dims to a copy,
 //           128-byte swizzle; K is K-major as it lies, V is MN-major (its
 //           dims, the N of P V, run along the row).
-//   kSlots  token-major, any block size (the pool's slot lists): the same tile
-//           from 4-row gathers, each token's row where its own slot is.
+//   kSlots  token-major, any block size (the pool's slot lists) and row distance: the
+//           same tile from 4-row gathers, each token's row where its own slot is.
 // Every wait is bounded; a timeout sets KVC_STATUS_WAIT_TIMEOUT and an abort flag
 // that ends every loop; TMEM is freed after a final commit.
 #pragma once
@@ -56,6 +56,21 @@ constexpr int kWinItems = 4;  // item slots
 // show the rounding (2e-3 absolute is missed with 3 keys).  16 x 512 tokens, window
 // 1024: 1 / 2 products 131 / 164 us.
 constexpr int kSplitKeys = 64;
+
+// 16 bytes of an output row: one store, or, where the rows do not start on 16-byte
+// boundaries, four (a row's pairs are 4-byte aligned: the host checked).
+template <bool OUT16>
+__device__ __forceinline__ void store_row16(void* dst, uint4 v) {
+  if constexpr (OUT16) {
+    *reinterpret_cast<uint4*>(dst) = v;
+  } else {
+    uint32_t* d = reinterpret_cast<uint32_t*>(dst);
+    d[0] = v.x;
+    d[1] = v.y;
+    d[2] = v.z;
+    d[3] = v.w;
+  }
+}
 
 // Products whose accumulation is known as the code is written, with the second
 // operand's descriptor as its low word (the address, which is all that changes:
@@ -109,7 +124,9 @@ struct WinUmmaGeom {
   static_assert(SMEM <= 227 * 1024, "shared memory");
 };
 
-template <typename T, int D, int BS, int LOAD>
+// OUT16: output rows start on 16-byte boundaries (a run-time choice costs the softmax
+// warps registers: 16 x 512 tokens 131 -> 136 us).
+template <typename T, int D, int BS, int LOAD, bool OUT16>
 __global__ void __launch_bounds__(kWinThreads, 1)
     window_umma_kernel(const PrefillArgs p, const __grid_constant__ TmaMaps maps, int tiles_x, int ny, int slot) {
   using namespace mma_detail;
@@ -327,6 +344,10 @@ __global__ void __launch_bounds__(kWinThreads, 1)
     uint64_t* empty = is_k ? k_empty : v_empty;
     uint8_t* ring = is_k ? kring : vring;
     const CUtensorMap* map = is_k ? &maps.k : &maps.v;
+    // kSlots: rows of the map from one block to the next (all rows are below 2^31: the host checked)
+    const int64_t rows_per_block = LOAD != kSlots || p.block_size == 1 ? 1
+                                   : is_k                              ? p.k_block_stride / p.k_tok_stride
+                                                                       : p.v_block_stride / p.v_tok_stride;
     int g = 0, st = 0, round = 0;  // tiles asked for, the next one's stage and turn of the ring
     bool ok = true;
     for (int k = 0; ok; ++k) {
@@ -339,6 +360,7 @@ __global__ void __launch_bounds__(kWinThreads, 1)
       const int kvh = it.kvh, kv_end = it.kv_end, ntiles = it.ntiles;
       const uint32_t* table = p.block_tables + (int64_t)it.y * p.table_stride;
       const int tbs = p.block_size;
+      const int col = (int)(kvh * (is_k ? p.k_head_stride : p.v_head_stride));  // kSlots: the head's first column
       // ids of tile j: lane i holds unit i's (kSlots: tokens 4i .. 4i + 3)
       auto load_ids = [&](int j, uint32_t (&id)[4]) {
         if constexpr (LOAD == kSlots) {
@@ -378,7 +400,7 @@ __global__ void __launch_bounds__(kWinThreads, 1)
             const bool in = tok < kv_end, good = in && (int64_t)id[e] < p.num_blocks;
             good4 |= good ? 1u << e : 0u;
             oob |= in && !good ? 1u : 0u;
-            row[e] = good ? (int)((tbs == 1 ? (int64_t)id[e] : (int64_t)id[e] * tbs + tok % tbs) * p.num_kv_heads + kvh) : -1;
+            row[e] = good ? (int)(id[e] * rows_per_block) + (tbs == 1 ? 0 : tok % tbs) : -1;
           }
           if (oob) set_status(&g_decode_status, KVC_STATUS_BLOCK_OOB);
           const uint32_t any = __ballot_sync(0xffffffffu, good4 != 0u);
@@ -402,7 +424,7 @@ __global__ void __launch_bounds__(kWinThreads, 1)
           if (any) {
 #pragma unroll
             for (int h = 0; h < D / 64; ++h)
-              tma_gather4(dst + h * HALF + lane * 512, map, 64 * h, row[0], row[1], row[2], row[3], &full[st]);
+              tma_gather4(dst + h * HALF + lane * 512, map, col + 64 * h, row[0], row[1], row[2], row[3], &full[st]);
           }
         } else {
           const int tok = t0 + lane * UNIT;
@@ -872,15 +894,15 @@ __global__ void __launch_bounds__(kWinThreads, 1)
           const int from = lane / CPR + (32 / CPR) * i, rr = (warp & 3) * 32 + from;
           const int64_t off = __shfl_sync(0xffffffffu, o_off, from);  // (that row's own thread knows where it goes)
           if (rr < it.nrows)
-            *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) + off + ch * 8) =
-                *reinterpret_cast<const uint4*>(ob + rr * RB + ((ch & ~7) | ((ch ^ rr) & 7)) * 16);
+            store_row16<OUT16>(reinterpret_cast<T*>(p.out) + off + ch * 8,
+                               *reinterpret_cast<const uint4*>(ob + rr * RB + ((ch & ~7) | ((ch ^ rr) & 7)) * 16));
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&q_empty[(nx - 1) & 1]);
       } else if (in_tile) {  // (bad indices: zeros)
         T* orow = reinterpret_cast<T*>(p.out) + o_off + half * HD;
 #pragma unroll
-        for (int c = 0; c < HD; c += 8) *reinterpret_cast<uint4*>(orow + c) = make_uint4(0u, 0u, 0u, 0u);
+        for (int c = 0; c < HD; c += 8) store_row16<OUT16>(orow + c, make_uint4(0u, 0u, 0u, 0u));
       }
       gt += ntiles;
     }

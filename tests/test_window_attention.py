@@ -336,6 +336,31 @@ def test_extend_strided_token_rows(gpu, seqs, bs):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("seqs", [2, 40])
+@pytest.mark.parametrize("layout,bs,pad", [("paged", 16, 8), ("paged", 32, 8), ("paged", 8, 64), ("flash", 16, 8),
+                                           ("flash", 5, 8), ("flash", 5, 256), ("flash", 16, 512)])
+def test_extend_blocks_any_distance_apart(gpu, layout, bs, pad, seqs):
+    """Elements between one block and the next: whole K chunks or token rows (which tensor maps can step over) or not."""
+    import torch
+
+    rng = np.random.default_rng(42)
+    new = rng.integers(20, 61, seqs)
+    c = Case(42, "float16", new + rng.integers(0, 300, seqs), 16, 4, 64, bs, layout, new=new)
+    ref = c.reference(70, 3, 0.0)
+    q, kc, vc, tables, lens = c.upload()
+    spread = []
+    for a in (kc, vc):
+        a = torch.from_numpy(a.to_numpy())
+        flat = torch.full((c.blocks, a[0].numel() + pad), NAN, dtype=torch.float16)
+        flat[:, :a[0].numel()] = a.reshape(c.blocks, -1)
+        spread.append(torch.as_strided(flat.cuda(), a.shape, (flat.shape[1],) + a.stride()[1:]))
+    torch.cuda.synchronize()
+    got = mk.paged_prefill_window(q, spread[0], spread[1], tables, c.indptr, lens, 4, c.scale, bs, 70, 3).to_numpy()
+    assert_close(got, ref, *tolerance("float16"))
+    assert _lib.get_status(0, clear=True) == 0
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("seqs", [3, 40])
 def test_extend_index_errors(gpu, seqs):
     """Lengths that the host cannot see: the status word names the error, the sequence's
@@ -384,6 +409,23 @@ def test_extend_bits_repeat(gpu, seqs):
             mk.paged_prefill_window(*args, max_q_len=longest, out=out, stream=s)
             s.synchronize()
             np.testing.assert_array_equal(out.to_numpy(raw=True), first.to_numpy(raw=True))
+
+
+@pytest.mark.gpu
+def test_window_serving_example(gpu):
+    """The example's chunked prompts and decode steps, blocks behind the window reused.  Tolerance: values of at
+    most about 4.5, one fp16 rounding of the output (2^-11 relative) and of P (2^-11 each), of the rotated q and
+    the cached k where the fp32 result rounds differently (one step, rare): under 4 x 4.5 x 2^-11 = 8.8e-3."""
+    import importlib.util
+    import os
+
+    path = os.path.join(os.path.dirname(__file__), "..", "examples", "window_serving.py")
+    spec = importlib.util.spec_from_file_location("window_serving", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    lines = []
+    assert example.main(steps=24, requests=5, log=lines.append) < 8.8e-3
+    assert len(lines) == 24 and _lib.get_status(0, clear=True) == 0
 
 
 # ---- refusals -------------------------------------------------------------------
