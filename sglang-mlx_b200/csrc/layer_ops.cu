@@ -67,7 +67,11 @@ static int sm_count() {
 // KB out of L2, cheaper than a second launch or a wait between CTAs) and then
 // does slice s of the chunk's new blocks and new tokens, found by binary search
 // in the scanned offsets.  A token in a new block reads the free list, not the
-// table, so no CTA needs what another one writes.
+// table, so no CTA needs what another one writes.  A few KB move: what counts is the
+// chain of launch, loads, scan, search and stores (64 requests with one token each
+// 4.9 us back to back, 528 of a mixed step 6.8; 256 prompts of up to 4096 tokens, 7.2
+// MB of positions and slots, 6.6; an empty kernel launched the same way takes about
+// 2.1).
 // ---------------------------------------------------------------------------
 constexpr int kTablesThreads = 512;
 constexpr int kTablesChunk = 2 * kTablesThreads;
@@ -334,7 +338,11 @@ cudaError_t launch_rotary_table(const RotaryTableArgs& a, cudaStream_t stream) {
 //   y_d = x_d w_d / sqrt(sum_e x_e^2 / D + eps)          (or y = x)
 //   half layout         (y_i, y_{i + half}),   interleaved   (y_2i, y_2i+1):
 //   (a, b) -> (a c_i - b s_i, b c_i + a s_i)
-// in 32 bits, rounded once to the output's type.
+// in 32 bits, rounded once to the output's type.  Memory sets the pace for many tokens
+// (8192 tokens of 28 + 4 heads of 128, fp16, 136 MB: 25.6 us, 5.3 TB/s; with norm and
+// append to 32-token pages 34.4 us, 4.5 TB/s), latency for few (256 tokens of 32 + 8
+// heads: 4.0 us; with the append 7.5, half of it V's elements, each a sector of its
+// own).
 // ---------------------------------------------------------------------------
 // Two fp32 lanes per instruction (the f32x2 arithmetic of sm_100), rounded as two
 // scalar operations are.
@@ -855,6 +863,12 @@ static cudaError_t launch_rope_vec(RopeArgs a, cudaStream_t stream) {
   const int rpw = 32 >> pl.lpr_shift;
   const int64_t groups = a.num_tokens * ((a.num_heads + rpw - 1) / rpw + (a.num_kv_heads + rpw - 1) / rpw);
   const bool whole = a.num_tokens >= 7 * (int64_t)sm_count() && groups >= 128 * (int64_t)sm_count();
+  // V by tiles of 32 tokens: 16-byte stores where slots run on, but a poor scatter
+  // where they do not.  bf16, heads of 128, 64 / 256 / 1024 tokens, one by one and by
+  // tiles: a prompt's slots (28 + 4 heads) 3.3 / 4.9 / 13.1 us and 2.7 / 3.4 / 9.4
+  // (8192: 65 and 35), one slot of each request (32 + 8 heads) 4.9 / 7.6 / 25.7 and
+  // 7.0 / 12.8 / 39.5.  The host does not see the slots: fewer than 1024 new tokens
+  // are taken for a decode step's.
   const bool v_tiles = a.k_cache && a.paged && a.num_tokens >= 1024;
   a.v_wide = a.block_size % 8 == 0 && reinterpret_cast<uintptr_t>(a.v_cache) % 16 == 0 && a.vc_block % 8 == 0 &&
              a.vc_head % 8 == 0;
