@@ -420,3 +420,65 @@ def test_rotary_table_refusals():
     assert _lib.lib.kvc_rotary_table(_fake((4, 64), "float32"), f, 1.0, None) == 1 and "finite" in _lib.last_error()
     with pytest.raises(ValueError):
         mk.rotary_table(0, 64)
+
+
+# ---- the two ways into the library ----------------------------------------------
+
+
+def _step_calls():
+    """The five calls with preallocated outputs, on small inputs: (name, call) pairs; a call returns its outputs."""
+    rng = np.random.default_rng(7)
+    T, H, KH, D, bs, nb = 3, 4, 2, 64, 16, 8
+    half = lambda *s: DeviceArray.from_numpy(rng.standard_normal(s).astype(np.float16))  # noqa: E731
+    i32 = lambda a: DeviceArray.from_numpy(np.asarray(a, np.int32))  # noqa: E731
+    q, k, v, w = half(T, H, D), half(T, KH, D), half(T, KH, D), half(D)
+    kc, vc = half(nb, KH, D // 8, bs, 8), half(nb, KH, D, bs)
+    rope = mk.rotary_table(40, D)
+    pos, slots = i32([4, 17, 30]), DeviceArray.from_numpy(np.asarray([4, 33, 62], np.int64))
+    tables, lens, ind = i32([[0, -1], [1, 2], [4, 3]]), i32([5, 18, 31]), i32([0, 1, 2, 3])
+    like = lambda a: DeviceArray.zeros(a.shape, a.dtype)  # noqa: E731
+
+    def tabs():
+        t = i32(np.full((2, 4), -1))
+        outs = [i32(np.zeros(n)) for n in (2, 3, 5)] + [DeviceArray.from_numpy(np.zeros(5, np.int64)), i32([0])]
+        r = mk.build_step_tables(t, i32([0, 0]), i32([2, 3]), i32([5, 6, 7]), 4, kv_lens=outs[0], qo_indptr=outs[1],
+                                 positions=outs[2], slot_mapping=outs[3], blocks_used=outs[4])
+        return list(r)
+
+    def append():
+        kk, vv = like(kc), like(vc)
+        return list(mk.qk_norm_rope_append(q, k, v, pos, rope, kk, vv, slots, q_weight=w, k_weight=w, q_out=like(q)))
+
+    return [
+        ("tables", tabs),
+        ("rope", lambda: list(mk.qk_norm_rope(q, k, pos, rope, q_weight=w, k_weight=w, q_out=like(q), k_out=like(k)))),
+        ("append", append),
+        ("decode", lambda: [mk.paged_attention_window(q, kc, vc, tables, lens, KH, 0.125, bs, 32, 9, 2, out=like(q))]),
+        ("extend", lambda: [mk.paged_prefill_window(q, kc, vc, tables, ind, lens, KH, 0.125, bs, 9, 2, max_q_len=1,
+                                                    out=like(q))]),
+    ]
+
+
+@pytest.mark.gpu
+def test_direct_calls_are_the_general_ones(gpu, monkeypatch):
+    """With preallocated outputs a call goes to the library in one C call, where that module is built: the same bits."""
+    direct = [[o.to_numpy(raw=True) for o in call()] for _, call in _step_calls()]
+    monkeypatch.setattr(mk, "_calls", None)
+    for (name, call), first in zip(_step_calls(), direct):
+        for a, b in zip(call(), first):
+            np.testing.assert_array_equal(a.to_numpy(raw=True), b, err_msg=name)
+    assert _lib.get_status(0, clear=True) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("direct", [True, False])
+def test_refusals_are_the_same_either_way(gpu, monkeypatch, direct):
+    if not direct:
+        monkeypatch.setattr(mk, "_calls", None)
+    q = DeviceArray.zeros((2, 4, 64), "float16")
+    kc, vc = DeviceArray.zeros((3, 2, 8, 16, 8), "float16"), DeviceArray.zeros((3, 2, 64, 16), "float16")
+    t, n = DeviceArray.zeros((2, 1), "int32"), DeviceArray.zeros((2,), "int32")
+    with pytest.raises(ValueError, match="window_size must be positive"):
+        mk.paged_attention_window(q, kc, vc, t, n, 2, 0.125, 16, 16, 0, out=DeviceArray.zeros(q.shape, "float16"))
+    with pytest.raises(ValueError, match="out"):
+        mk.paged_attention_window(q, kc, vc, t, n, 2, 0.125, 16, 16, 4, out=DeviceArray.zeros((2, 4, 32), "float16"))
