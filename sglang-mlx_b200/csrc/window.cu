@@ -623,35 +623,58 @@ static int64_t longest_seen(const DecodeParams& p, const WindowArgs& w) {
   return seen < p.max_seq_len ? seen : p.max_seq_len;
 }
 
-// CTAs to a cluster, a power of two, while a CTA keeps at least `least` tokens of
-// the longest run.  kWide: the largest that keeps the launch within one CTA per SM,
-// at most 8, and 8 only to three quarters of the SMs: GPCs of 16 to 20 SMs hold two
-// such clusters each at best (two sequences of 8 KV heads, 32-token pages, window
-// 1024: 13.2 us in clusters of 8, 7.3 of 4).  Else the smallest (at most 16) that
-// brings the launch to one CTA per SM.
-static int window_cluster(const DecodeParams& p, const WindowArgs& w, int64_t units, int least, Form form) {
+// CTAs to a cluster of the CUDA-core form, whose CTAs share SMs: the smallest power
+// of two (at most 16) that brings the launch to one CTA per SM, while a CTA keeps at
+// least `least` tokens of the longest run.
+static int window_cluster(const DecodeParams& p, const WindowArgs& w, int64_t units, int least) {
   const int64_t seen = longest_seen(p, w), n = units * p.num_seqs, sms = decode_sm_count();
-  auto grow = [&](int c) {
-    if (form != kWide) return c < kMaxCluster && n * c < sms;
-    return c < 4 ? 2 * n * c <= sms : c == 4 && 4 * n * 8 <= 3 * sms;
-  };
   int c = 1;
-  while (grow(c) && seen >= (int64_t)least * 2 * c) c *= 2;
+  while (c < kMaxCluster && n * c < sms && seen >= (int64_t)least * 2 * c) c *= 2;
   return c;
+}
+
+// Shared memory and cluster sizes of a kernel, once per device (twice is harmless).
+template <typename K>
+static cudaError_t configure_clustered(K kern, int smem, std::atomic<bool>* configured) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 0 && dev < 64 && configured[dev]) return cudaSuccess;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e == cudaSuccess && dev >= 0 && dev < 64) configured[dev] = true;
+  return e;
+}
+
+// Clusters of c CTAs that run at once on the current device, asked once per size.
+template <typename K>
+static int active_clusters(K kern, int smem, int threads, int c, int dev, std::atomic<int> (*known)[kMaxCluster + 1]) {
+  const bool keep = dev >= 0 && dev < 64;
+  int n = keep ? known[dev][c].load() : 0;
+  if (n > 0) return n - 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)c);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)c;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) {
+    cudaGetLastError();
+    n = 0;
+  }
+  if (keep) known[dev][c] = n + 1;
+  return n;
 }
 
 template <typename K, typename... Args>
 static cudaError_t launch_clustered(K kern, int smem, int cluster, int64_t units, unsigned seqs, int threads,
                                     std::atomic<bool>* configured, cudaStream_t stream, Args... args) {
   if (units * cluster > 0x7fffffffll) return cudaErrorInvalidValue;
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev < 0 || dev >= 64 || !configured[dev]) {  // setting the attributes twice is harmless
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e != cudaSuccess) return e;
-    if (dev >= 0 && dev < 64) configured[dev] = true;
-  }
+  if (const cudaError_t e = configure_clustered(kern, smem, configured); e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)units * (unsigned)cluster, seqs);
   cfg.blockDim = dim3((unsigned)threads);
@@ -684,9 +707,23 @@ static cudaError_t launch_window_nw(const DecodeParams& p, const WindowArgs& w, 
   // 16-row tiles of a sequence
   const int64_t rows = (EXT ? (int64_t)w.max_q_len : 1) * (p.num_heads / p.num_kv_heads), tiles = (rows + 15) / 16;
   const int64_t units = p.num_kv_heads * tiles;
-  return launch_clustered(window_decode_kernel<T, D, BS, NW, STAGES, GT, MODE, EXT>, WG::SMEM,
-                          window_cluster(p, w, units, FORM == kWide ? NW * GT / 2 : NW * GT, FORM), units,
-                          (unsigned)p.num_seqs, NW * 32, configured, stream, p, w, maps);
+  auto kern = window_decode_kernel<T, D, BS, NW, STAGES, GT, MODE, EXT>;
+  int cluster = 1;
+  if constexpr (FORM == kWide) {
+    // the largest cluster (at most 16 CTAs) of which all run at once, one CTA to an
+    // SM, while a CTA keeps half of its warps' groups.  What fits a GPC is the
+    // device's own affair, hence the question (two sequences of 8 KV heads, window
+    // 4096 / 16384: powers of two up to 8 and three quarters of the SMs 15.0 / 44.8
+    // us, up to all SMs, where the last clusters wait, 20.4 / 50.7, so 12.5 / 33.3).
+    static std::atomic<int> known[64][kMaxCluster + 1];
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (const cudaError_t e = configure_clustered(kern, WG::SMEM, configured); e != cudaSuccess) return e;
+    const int64_t n = units * p.num_seqs, sms = decode_sm_count(), most = longest_seen(p, w) / (NW * GT / 2);
+    for (int c = (int)(most < kMaxCluster ? most : kMaxCluster); c > 1 && cluster == 1; --c)
+      if (n * c <= sms && active_clusters(kern, WG::SMEM, NW * 32, c, dev, known) >= n) cluster = c;
+  }
+  return launch_clustered(kern, WG::SMEM, cluster, units, (unsigned)p.num_seqs, NW * 32, configured, stream, p, w, maps);
 }
 
 // Token-major blocks whose rows a tensor map can address: 16k rows one after another.
@@ -723,10 +760,10 @@ static int64_t window_units(const DecodeParams& p, int64_t new_tokens) {
 }
 
 // kWide where every tile gets an SM or more (decode, 8 KV heads, window 1024, 1 / 2 /
-// 4 / 8 / 16 sequences: 32-token pages 7.8 / 15.0 / 10.8 / 13.1 / 20.0 us narrow, 6.1
-// / 7.3 / 8.0 / 11.5 / 16.7 wide; 16-token pages 6.3 / 7.1 / 9.3 / 10.5 / 16.8 and 6.3
-// / 6.6 / 8.1 / 10.6 / 16.0; slot lists 7.4 / 14.1 / 21.7 / 19.7 / 29.5 and 7.2 / 8.2
-// / 9.9 / 12.4 / 18.7).
+// 4 / 8 / 16 sequences: 32-token pages 7.8 / 15.0 / 10.8 / 13.1 / 20.0 us narrow (in
+// clusters of up to 16), 6.1 / 6.5 / 8.1 / 11.5 / 16.7 wide; slot lists 7.4 / 14.1 / 21.7
+// / 19.7 / 29.5 and 7.4 / 7.7 / 9.9 / 12.5 / 18.8; 16-token pages, window 4096, 9.6 /
+// 18.9 / 17.5 / 26.6 / 48.9 and 9.5 / 11.4 / 17.6 / 26.9 / 47.1).
 // kSmall where every SM gets four tiles or more, so that it pays to have more CTAs in
 // their start and end, and the groups are short (D = 64, single token rows) or few
 // (decode, 8 KV heads, 128 sequences, window 64 / 128 / 256 / 1024: D = 128, 16-token
@@ -753,7 +790,7 @@ static cudaError_t launch_window_any(const DecodeParams& p, const WindowArgs& w,
   const int units = p.num_kv_heads * ((G + kWinGC - 1) / kWinGC);
   static std::atomic<bool> configured[64];
   return launch_clustered(window_decode_any_kernel<Q_T, CACHE_T, D>, exchange_floats(kWinGC, D) * 4,
-                          window_cluster(p, w, units, kWinWarps * p.block_size, kNarrow), units, (unsigned)p.num_seqs,
+                          window_cluster(p, w, units, kWinWarps * p.block_size), units, (unsigned)p.num_seqs,
                           kWinWarps * 32, configured, stream, p, w);
 }
 
@@ -988,7 +1025,7 @@ template <typename T, int D>
 static cudaError_t launch_window_prefill_t(const PrefillArgs& a, cudaStream_t stream) {
   // A 16-row tile for every SM or fewer: the decode's kernel, which splits the keys
   // too (4 sequences, 4 KV heads, 7 heads each, window 1024; 16 / 64 / 112 / 224
-  // tiles: 9.7 / 13.4 / 17.8 / 31.7 us against 18.6 of 128-row items one after
+  // tiles: 7.2 / 11.0 / 15.4 / 27.6 us against 18.6 of 128-row items one after
   // another).
   const int64_t units = ((int64_t)a.max_q_len * (a.num_heads / a.num_kv_heads) + 15) / 16 * a.num_seqs * a.num_kv_heads;
   const int64_t sms = decode_sm_count();
