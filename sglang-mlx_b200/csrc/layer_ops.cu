@@ -340,7 +340,8 @@ cudaError_t launch_rotary_table(const RotaryTableArgs& a, cudaStream_t stream) {
 //   (a, b) -> (a c_i - b s_i, b c_i + a s_i)
 // in 32 bits, rounded once to the output's type.  Memory sets the pace for many tokens
 // (8192 tokens of 28 + 4 heads of 128, fp16, 136 MB: 25.6 us, 5.3 TB/s; with norm and
-// append to 32-token pages 34.4 us, 4.5 TB/s), latency for few (256 tokens of 32 + 8
+// append to 32-token pages 34.4 us, 4.5 TB/s; 28 + 4 heads in fp32 with norm 46.0 us, 5.9
+// TB/s, and with the append 51.1, 6.0 TB/s), latency for few (256 tokens of 32 + 8
 // heads: 4.0 us; with the append 7.5, half of it V's elements, each a sector of its
 // own).
 // ---------------------------------------------------------------------------
@@ -524,7 +525,11 @@ struct RopeLane {
 // registers (with 16 bytes to a lane and group, 32 warps to an SM and 5 groups
 // ahead, 80 KB to an SM; loads into registers reached 4.1 TB/s at 8192 tokens,
 // the ring 4.9).  Quad e of place i of lane l lies at (i * 2 + e) * 32 + l.
-constexpr int kRopeStages = 6;
+// 32-bit elements take twice the place: 4 stages are 32 KB to a CTA, while 6 would
+// be the whole 48 KB that a kernel has without asking for more, with none left for
+// the V tiles' static words.
+template <typename T>
+constexpr int kRopeStages = sizeof(T) == 4 ? 4 : 6;
 
 template <typename T>
 __device__ __forceinline__ void quad_async(Quad<T>* dst, const T* src) {
@@ -844,6 +849,8 @@ static cudaError_t launch_rope_u(const RopeArgs& a, RopePlan pl, bool v_tiles, i
   if (ctas + tiles > 0x7fffffffll / kRopeWarps) return cudaErrorInvalidValue;
   pl.row_ctas = (unsigned)ctas;
   size_t smem = STAGES > 1 ? (size_t)kRopeWarps * STAGES * 64 * sizeof(Quad<T>) : 0;
+  static_assert(STAGES == 1 || kRopeWarps * STAGES * 64 * sizeof(Quad<T>) <= 40 * 1024,
+                "dynamic shared memory beside the static words, within 48 KB");
   const size_t tile = v_tiles ? (size_t)kVTile * (a.head_size * sizeof(T) + 16) : 0;
   if (tile > smem) smem = tile;
   return launch_dependent(qk_norm_rope_kernel<T, INTER, STAGES>, dim3((unsigned)(ctas + tiles)), kRopeWarps * 32, smem,
@@ -855,7 +862,7 @@ static cudaError_t launch_rope_vec(RopeArgs a, cudaStream_t stream) {
   RopePlan pl = {};
   while ((8 << pl.lpr_shift) < a.head_size) ++pl.lpr_shift;
   pl.inv_d = 1.f / (float)a.head_size;
-  // Many tokens: a token's rows to one warp, kRopeStages of its groups in flight
+  // Many tokens: a token's rows to one warp, kRopeStages<T> of its groups in flight
   // through the lanes' rings; else one group to a warp.  bf16, 32 + 8 heads of
   // 128 (20 groups to a token), one group / rings: 512 tokens 8.3 / 12.4 us, 1024
   // 12.4 / 12.4, 2048 24.5 / 16.4, 6000 61.5 / 32.8.  Without enough tokens the
@@ -873,9 +880,9 @@ static cudaError_t launch_rope_vec(RopeArgs a, cudaStream_t stream) {
   a.v_wide = a.block_size % 8 == 0 && reinterpret_cast<uintptr_t>(a.v_cache) % 16 == 0 && a.vc_block % 8 == 0 &&
              a.vc_head % 8 == 0;
   if (a.interleaved)
-    return whole ? launch_rope_u<T, true, kRopeStages>(a, pl, v_tiles, 1 << 20, stream)
+    return whole ? launch_rope_u<T, true, kRopeStages<T>>(a, pl, v_tiles, 1 << 20, stream)
                  : launch_rope_u<T, true, 1>(a, pl, v_tiles, 1, stream);
-  return whole ? launch_rope_u<T, false, kRopeStages>(a, pl, v_tiles, 1 << 20, stream)
+  return whole ? launch_rope_u<T, false, kRopeStages<T>>(a, pl, v_tiles, 1 << 20, stream)
                : launch_rope_u<T, false, 1>(a, pl, v_tiles, 1, stream);
 }
 

@@ -332,6 +332,60 @@ def test_append(gpu, layout, bs, dtype, cache, d, rot, T):
         assert _lib.get_status(0, clear=True) == flagged
 
 
+# Many tokens: from 7 * 148 = 1036 of them with 128 * 148 = 18944 groups (a group: the rows of one tensor that a warp
+# holds at a time, 4 heads of 64, 2 of 80 to 128, 1 of 256) a warp takes all of a token's rows, through its lanes' copy rings.
+MANY = [(1100, 128, 128), (1100, 128, 64), (1900, 64, 64), (1100, 80, 40), (1040, 256, 256)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("T,d,rot", MANY)
+def test_qk_norm_rope_many_tokens(gpu, T, d, rot, dtype, interleaved):
+    """Slices of a fused projection with norms, and in place without a norm of k, with skipped tokens."""
+    c = Rope(T + rot, dtype, T, 32, 8, d, rot, True, "float32" if rot == 64 else None)
+    q, k = mk.qk_norm_rope(c.dq, c.dk, c.pos.astype(np.int32), c.table, interleaved=interleaved, **c.w)
+    want_q, want_k = c.want(interleaved)
+    close(q.to_numpy(), want_q, dtype)
+    close(k.to_numpy(), want_k, dtype)
+    pos = c.pos.copy()
+    skipped = [0, 500, T - 1]
+    pos[skipped] = -1, 5000, -7
+    want_k = plain_rope(c.k, None, c.cs, rot, interleaved, 0.0)
+    want_q[skipped], want_k[skipped] = c.q[skipped], c.k[skipped]
+    mk.qk_norm_rope(c.dq, c.dk, pos.astype(np.int64), c.table, q_weight=c.w["q_weight"], interleaved=interleaved,
+                    q_out=c.dq, k_out=c.dk)
+    close(c.dq.to_numpy(), want_q, dtype)
+    close(c.dk.to_numpy(), want_k, dtype)
+    assert _lib.get_status(0, clear=True) == _lib.STATUS_INDEX_OOB
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("layout,bs", [("paged", 16), ("paged", 32), ("flash", 16), ("pool", 1)])
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("T,d,rot", MANY)
+def test_append_many_tokens(gpu, T, d, rot, dtype, layout, bs):
+    c = Rope(T + d, dtype, T, 32, 8, d, rot, rot != 64, fused=bs != 1)
+    rng = np.random.default_rng(T + bs)
+    blocks = -(-T // bs) * 2 + 2
+    slots = np.concatenate([np.arange(T // 2) + 3, rng.permutation(np.arange(T // 2 + 3, blocks * bs))[:T - T // 2]])
+    slots[4], slots[7] = -1, blocks * bs + 5
+    ks, vs = cache_shapes(layout, blocks, bs, 8, d, dtype)
+    kc0 = kv_oracle.round_to(rng.standard_normal(ks).astype(np.float32), dtype)
+    vc0 = kv_oracle.round_to(rng.standard_normal(vs).astype(np.float32), dtype)
+    kc, vc = DeviceArray.from_numpy(kc0, dtype=dtype), DeviceArray.from_numpy(vc0, dtype=dtype)
+    interleaved = bs == 32 or d == 80
+    q, _, _ = mk.qk_norm_rope_append(c.dq, c.dk, c.dv, c.pos.astype(np.int32), c.table, kc, vc, slots.astype(np.int64),
+                                     interleaved=interleaved, **c.w)
+    want_q, want_k = c.want(interleaved)
+    close(q.to_numpy(), want_q, dtype)
+    kw, vw = kc0.astype(np.float64), vc0.astype(np.float64)
+    place(layout, kw, vw, slots, want_k, c.v, bs)
+    close(kc.to_numpy(), kw, dtype)
+    np.testing.assert_array_equal(vc.to_numpy(), vw.astype(np.float32))
+    assert _lib.get_status(0, clear=True) == _lib.STATUS_SLOT_OOB
+
+
 @pytest.mark.gpu
 def test_append_skipped_position_keeps_the_value(gpu):
     c = Rope(9, "bfloat16", 4, 4, 2, 128, 128, False)
