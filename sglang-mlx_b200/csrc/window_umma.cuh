@@ -200,11 +200,6 @@ __global__ void __launch_bounds__(kWinThreads, 1)
     mbar_init(xchg, 8);
     mbar_fence_init();
   }
-  // V of blocks that a tile does not load meets P = 0 (0 * NaN = NaN): the ring
-  // starts from zeros
-  for (int i = threadIdx.x; i < VS * TILE / 16; i += kWinThreads)
-    reinterpret_cast<uint4*>(vring)[i] = make_uint4(0u, 0u, 0u, 0u);
-  fence_proxy_async();
   if (warp == kMmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(s_tmem)),
                  "r"(512));
@@ -390,6 +385,7 @@ __global__ void __launch_bounds__(kWinThreads, 1)
         uint8_t* dst = ring + (size_t)st * TILE;
         uint32_t* tm = masks + (g & 7) * 4;
         uint32_t next[4];
+        uint32_t loaded = 0, bad4 = 0;  // units that are loaded; kSlots: which of my four tokens have no block
         if constexpr (LOAD == kSlots) {
           // a token without a block gathers a loaded token's row (and is masked)
           uint32_t good4 = 0, oob = 0;
@@ -399,10 +395,11 @@ __global__ void __launch_bounds__(kWinThreads, 1)
             const int tok = t0 + 4 * lane + e;
             const bool in = tok < kv_end, good = in && (int64_t)id[e] < p.num_blocks;
             good4 |= good ? 1u << e : 0u;
-            oob |= in && !good ? 1u : 0u;
+            oob |= in && !good ? 1u << e : 0u;
             row[e] = good ? (int)(id[e] * rows_per_block) + (tbs == 1 ? 0 : tok % tbs) : -1;
           }
           if (oob) set_status(&g_decode_status, KVC_STATUS_BLOCK_OOB);
+          bad4 = oob;
           const uint32_t any = __ballot_sync(0xffffffffu, good4 != 0u);
           int spare = good4 ? row[__ffs(good4) - 1] : 0;
           spare = __shfl_sync(0xffffffffu, spare, any ? __ffs(any) - 1 : 0);
@@ -432,6 +429,7 @@ __global__ void __launch_bounds__(kWinThreads, 1)
           if (in && !good) set_status(&g_decode_status, KVC_STATUS_BLOCK_OOB);
           const uint32_t mask = __ballot_sync(0xffffffffu, good);
           const uint32_t mine = id[0];
+          loaded = mask;
           load_ids(j + 1, next);
           if (lane == 0) {
             if (is_k) tm[0] = mask;
@@ -478,10 +476,22 @@ __global__ void __launch_bounds__(kWinThreads, 1)
           // V of tokens nobody sees, in blocks that are loaded for others, becomes 0
           // (their slots may hold anything, and 0 * NaN = NaN): between the sinks and
           // the first row's window, and past the last row's end up to the 16 tokens
-          // of a product.  This warp runs ahead of the products.
+          // of a product.  So does V of blocks past the cache, in whose place the
+          // stage holds another tile's tokens or another token's row.  This warp runs
+          // ahead of the products.
           const int a0 = p.sinks > t0 ? p.sinks : t0, a1 = it.seen.beg < t0 + KT ? it.seen.beg : t0 + KT;
           const int e0 = kv_end > t0 ? kv_end : t0, e1r = (kv_end + 15) / 16 * 16, e1 = e1r < t0 + KT ? e1r : t0 + KT;
-          if (a0 < a1 || e0 < e1) {
+          uint32_t holes;  // units (kSlots: of my four tokens) below kv_end without a block
+          bool any_hole;
+          if constexpr (LOAD == kSlots) {
+            holes = bad4;
+            any_hole = __any_sync(0xffffffffu, bad4 != 0u);
+          } else {
+            const int n = (kv_end - t0 + UNIT - 1) / UNIT;
+            holes = (n >= WG::UNITS ? (1u << WG::UNITS) - 1u : (1u << n) - 1u) & ~loaded;
+            any_hole = holes != 0u;
+          }
+          if (a0 < a1 || e0 < e1 || any_hole) {
             if (!__all_sync(0xffffffffu, umma::wait(&full[st], (uint32_t)(round & 1)))) {
               ok = false;
               break;
@@ -517,6 +527,25 @@ __global__ void __launch_bounds__(kWinThreads, 1)
                 for (int i = lane; i < (c1 - c0) * (D / 8); i += 32) {
                   const int tk = c0 + i / (D / 8), ch = i % (D / 8);
                   *reinterpret_cast<uint4*>(dst + (ch >> 3) * HALF + tk * 128 + (ch & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                }
+              }
+            }
+            if constexpr (LOAD == kSlots) {
+              for (; holes; holes &= holes - 1u) {
+                uint8_t* row = dst + (4 * lane + __ffs(holes) - 1) * 128;
+                for (int ch = 0; ch < D / 8; ++ch)
+                  *reinterpret_cast<uint4*>(row + (ch >> 3) * HALF + (ch & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+              }
+            } else {
+              for (; holes; holes &= holes - 1u) {
+                const int u = __ffs(holes) - 1;
+                if constexpr (LOAD == kPages) {
+                  for (int i = lane; i < PAGE / 16; i += 32)
+                    reinterpret_cast<uint4*>(dst + u * PAGE)[i] = make_uint4(0u, 0u, 0u, 0u);
+                } else {
+                  for (int i = lane; i < UNIT * (D / 8); i += 32)
+                    reinterpret_cast<uint4*>(dst + (i / (UNIT * 8)) * HALF + u * UNIT * 128)[i % (UNIT * 8)] =
+                        make_uint4(0u, 0u, 0u, 0u);
                 }
               }
             }

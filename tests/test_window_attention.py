@@ -390,6 +390,46 @@ def test_extend_index_errors(gpu, seqs):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("seqs", [3, 60])
+@pytest.mark.parametrize("sinks", [4, 0])
+@pytest.mark.parametrize("layout,bs,d", [("paged", 32, 128), ("paged", 32, 64), ("paged", 16, 128), ("paged", 8, 64),
+                                         ("flash", 32, 64), ("flash", 16, 128), ("flash", 5, 128), ("pool", 1, 64)])
+def test_extend_bad_blocks_are_skipped(gpu, layout, bs, d, seqs, sinks):
+    """Blocks past the cache are flagged and their tokens left out, whatever a row's other blocks, the unseen
+    places of those, or the sequences that ran before on the same SM hold."""
+    rng = np.random.default_rng(40 + bs)
+    new = rng.integers(20, 61, seqs)
+    c = Case(40, "bfloat16", new + rng.integers(0, 400, seqs), 16, 4, d, bs, layout, new=new)
+    window, flagged = 150, 0
+    # every third sequence misses a fifth of its blocks, among them neither the first nor the last two tokens'
+    lost = [np.zeros(int(n), bool) for n in c.lens]
+    bad = c.tables.copy()
+    for b in range(0, seqs, 3):
+        n = int(c.lens[b])
+        for blk in rng.permutation(np.arange(1, max(1, (n - 2) // bs)))[:max(1, n // bs // 5)]:
+            bad[b, blk] = c.blocks + int(rng.integers(0, 1000))
+            lost[b][blk * bs:(blk + 1) * bs] = True
+    ref = np.zeros(c.q.shape, np.float64)
+    for b, n in enumerate(c.lens):
+        for t in range(int(new[b])):
+            i, r = int(n - new[b]) + t, int(c.indptr[b]) + t
+            j = visible(i, window, sinks)
+            flagged |= _lib.STATUS_BLOCK_OOB if lost[b][j].any() else 0
+            j = j[~lost[b][j]]
+            for h in range(16 if len(j) else 0):
+                s = c.K[b][j, h // 4].astype(np.float64) @ c.q[r, h].astype(np.float64) * c.scale
+                e = np.exp(s - s.max())
+                ref[r, h] = e @ c.V[b][j, h // 4].astype(np.float64) / e.sum()
+    c.poison(window, sinks)
+    c.tables = np.where(bad >= c.blocks, bad, c.tables)
+    _lib.get_status(0, clear=True)
+    for _ in range(3):  # (the order of the items over the SMs is not fixed)
+        got = c.extend(window, sinks)
+        assert_close(got, ref, *tolerance("bfloat16"))
+        assert _lib.get_status(0, clear=True) == flagged
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("seqs", [2, 40])
 def test_extend_bits_repeat(gpu, seqs):
     """The same call gives the same bits, on any stream; max_q_len may be larger than needed."""
