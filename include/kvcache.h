@@ -401,7 +401,8 @@ int kvc_convert_fp8(kvc_dltensor* dst, const kvc_dltensor* src, float scale, int
  * (memory_pool.py:240-270).  window_size is positive; window_size >= the
  * context gives the unwindowed attention.  Block-table entries of blocks that no
  * query sees are not read (a server may have freed those blocks), and the values
- * in positions that no query of a sequence sees never matter.
+ * in positions that no query of a sequence sees never matter.  A query that sees a
+ * score of NaN or +inf gives NaN, one whose scores are all -inf gives 0.
  *
  * kvc_paged_attention_window: one new token per sequence, arguments and edge
  * rules of kvc_paged_attention_v1 (paged layout, every dtype pair, head size and

@@ -65,11 +65,12 @@ __device__ __forceinline__ void add_scaled(float4& a, float w, float4 b) {
   a.w += w * b.w;
 }
 
-// a / L as four elements of an output row, of any alignment; 0 where L is 0.
+// a / L as four elements of an output row, of any alignment; 0 where L is 0 (a NaN
+// sum, from a score that is NaN or +inf, gives NaN).
 template <typename T>
 __device__ __forceinline__ void store_quotient(T* dst, float4 a, float L, float eps) {
   const float n = L + eps;
-  const bool any = L > 0.f;
+  const bool any = L != 0.f;
   struct alignas(4 * sizeof(T)) Four {
     T e[4];
   } v = {{from_float<T>(any ? a.x / n : 0.f), from_float<T>(any ? a.y / n : 0.f), from_float<T>(any ? a.z / n : 0.f),

@@ -879,8 +879,9 @@ __global__ void __launch_bounds__(kWinThreads, 1)
       const float w_o = m_o == -INFINITY ? 0.f : fast_exp2(m_o - M);
       const float total = w_me * l + w_o * l_o;
       // a row with no visible key (or after an abort) is 0; a half without any has
-      // an O that nothing has written, and takes no part
-      const bool nonzero = have && total > 0.f;
+      // an O that nothing has written, and takes no part (unless the total is NaN,
+      // from a score that is NaN or +inf, which makes the row NaN)
+      const bool nonzero = have && total != 0.f;
       const float inv = nonzero ? 1.f / total : 0.f;
       const float f0 = (half == 0 ? w_me : w_o) * inv, f1 = (half == 0 ? w_o : w_me) * inv;
       const bool u0 = nonzero && f0 != 0.f, u1 = nonzero && f1 != 0.f;

@@ -430,6 +430,46 @@ def test_extend_bad_blocks_are_skipped(gpu, layout, bs, d, seqs, sinks):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("value", [NAN, np.inf])
+@pytest.mark.parametrize("dtype,d", [("float16", 128), ("bfloat16", 64), ("float32", 96)])
+def test_decode_nan_that_is_seen_shows(gpu, dtype, d, value):
+    """A key that is not finite makes the result of whoever sees it NaN, as the formula does, and of nobody else."""
+    c = Case(44, dtype, [300, 300, 300, 40], 4, 2, d, 16)
+    for b, j in ((0, 290), (1, 200), (3, 1)):  # in the window, in the gap, a sink
+        c.k_rows[c.tables[b, j // 16] * 16 + j % 16] = value
+        c.K[b][j] = value
+    c.q = kv_oracle.round_to(np.abs(c.q) + 0.5, c.dtype)
+    with np.errstate(invalid="ignore"):
+        ref = c.reference(50, 2, 1e-6)
+    assert np.isnan(ref[[0, 3]]).all() and np.isfinite(ref[[1, 2]]).all()
+    got = c.decode(50, 2)
+    assert np.isnan(got[[0, 3]]).all()
+    assert_close(got[[1, 2]], ref[[1, 2]], *tolerance(dtype))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seqs", [2, 40])
+@pytest.mark.parametrize("layout,bs", [("paged", 16), ("flash", 16), ("pool", 1)])
+@pytest.mark.parametrize("value", [NAN, np.inf])
+def test_extend_nan_that_is_seen_shows(gpu, layout, bs, seqs, value):
+    rng = np.random.default_rng(45)
+    new = rng.integers(20, 61, seqs)
+    c = Case(45, "bfloat16", new + rng.integers(60, 300, seqs), 16, 4, 64, bs, layout, new=new)
+    c.q = kv_oracle.round_to(np.abs(c.q) + 0.5, c.dtype)
+    for b in range(0, seqs, 2):
+        j = int(c.lens[b] - c.new[b] // 2)  # seen by the later half of the new tokens
+        c.k_rows[c.tables[b, j // bs] * bs + j % bs] = value
+        c.K[b][j] = value
+    with np.errstate(invalid="ignore"):
+        ref = c.reference(70, 3, 0.0)
+    nan = np.isnan(ref)
+    assert nan.any() and not nan.all()
+    got = c.extend(70, 3)
+    np.testing.assert_array_equal(np.isnan(got), nan)
+    assert_close(got[~nan], ref[~nan], *tolerance("bfloat16"))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("seqs", [2, 40])
 def test_extend_bits_repeat(gpu, seqs):
     """The same call gives the same bits, on any stream; max_q_len may be larger than needed."""
