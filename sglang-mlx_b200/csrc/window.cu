@@ -167,57 +167,6 @@ __global__ void __launch_bounds__(NW * 32)
   const int r = lane >> 2, q4 = lane & 3;
   const int G = p.num_heads / p.num_kv_heads, h0 = kvh * G;
   grid_dependents_launch();
-  const int rbs = Geo::TROWS || Geo::FLASH ? p.block_size : BS;
-  // rows R0 .. R0 + nh - 1 of the sequence's new tokens, whose first is row q0 of
-  // q / out and position `prefix`
-  const int R0 = tile * 16;
-  const uint32_t ctx = p.context_lens[seq];
-  int64_t q0 = seq;
-  int rows = G, prefix = (int)ctx - 1;
-  bool zero = ctx == 0 || ctx > (uint32_t)p.max_seq_len;
-  if (EXT && wa.indptr) {
-    const int64_t a = wa.indptr[seq], b = wa.indptr[seq + 1];
-    const int64_t ql = b - a;
-    q0 = a;
-    if (ql <= 0 || R0 >= ql * G) {  // (the same for the whole cluster, as every early end here)
-      grid_dependency_wait();
-      return;
-    }
-    // rows past q may not be written; other index errors give zeros
-    zero = ql > wa.max_q_len || (int64_t)ctx < ql || (int64_t)ctx > wa.table_len * (int64_t)rbs || ctx > 0x7fffff00u;
-    const bool past = b > wa.num_tokens;
-    if ((zero || past) && threadIdx.x == 0 && blockIdx.x == 0) set_status(&g_decode_status, KVC_STATUS_INDEX_OOB);
-    if (past) {
-      grid_dependency_wait();
-      return;
-    }
-    rows = (int)(ql * G < 0x7fffffff ? ql * G : 0x7fffffff);
-    prefix = (int)((int64_t)ctx - ql);
-  }
-  const int nh = EXT ? (rows - R0 < 16 ? rows - R0 : 16) : G;
-  // row R0 + g: new token t, head of the group
-  auto token_of = [&](int g) { return EXT ? (R0 + g) / G : 0; };
-  auto dest = [&](int g) -> T* {
-    if constexpr (!EXT)  // (fewer registers live across the loop: 256 sequences, window 1024: 170 -> 165 us)
-      return reinterpret_cast<T*>(p.out) + (int64_t)seq * p.out_seq_stride + (int64_t)(h0 + g) * p.out_head_stride;
-    const int t = token_of(g);
-    return reinterpret_cast<T*>(p.out) + (q0 + t) * p.out_seq_stride + (int64_t)(h0 + R0 + g - t * G) * p.out_head_stride;
-  };
-  if (zero) {
-    grid_dependency_wait();
-    if (rank == 0)
-      for (int i = threadIdx.x; i < nh * D; i += NW * 32) dest(i / D)[i % D] = from_float<T>(0.f);
-    return;
-  }
-  if (C > 1) cluster_arrive();
-  const Seen seen = seen_range(prefix + token_of(0), prefix + token_of(nh - 1), wa.window, wa.sinks, rbs);
-  // this CTA's run of groups
-  const int all = (seen.end + GT - 1) / GT, per = (all + C - 1) / C;
-  const int begin = rank * per * GT;
-  const int end = begin + per * GT < seen.end ? begin + per * GT : seen.end;
-  const int ngroups = end > begin ? (end - begin + GT - 1) / GT : 0;
-  const int n_mine = warp < ngroups ? (ngroups - warp + NW - 1) / NW : 0;
-
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Geo::BAR_OFF) + warp * STAGES;
   uint32_t* masks = reinterpret_cast<uint32_t*>(smem + Geo::MASK_OFF) + warp * STAGES;
   constexpr int IDC = Geo::IDC, IDV = IDC * GT / 32;
@@ -234,6 +183,53 @@ __global__ void __launch_bounds__(NW * 32)
   }
   __syncwarp();
 
+  // The kernel before this one may have written anything that is read from here on,
+  // lengths, tables and queries (an attention output as the next query) included.
+  grid_dependency_wait();
+  const int rbs = Geo::TROWS || Geo::FLASH ? p.block_size : BS;
+  // rows R0 .. R0 + nh - 1 of the sequence's new tokens, whose first is row q0 of
+  // q / out and position `prefix`
+  const int R0 = tile * 16;
+  const uint32_t ctx = p.context_lens[seq];
+  int64_t q0 = seq;
+  int rows = G, prefix = (int)ctx - 1;
+  bool zero = ctx == 0 || ctx > (uint32_t)p.max_seq_len;
+  if (EXT && wa.indptr) {
+    const int64_t a = wa.indptr[seq], b = wa.indptr[seq + 1];
+    const int64_t ql = b - a;
+    q0 = a;
+    if (ql <= 0 || R0 >= ql * G) return;  // (the same for the whole cluster, as every early end here)
+    // rows past q may not be written; other index errors give zeros
+    zero = ql > wa.max_q_len || (int64_t)ctx < ql || (int64_t)ctx > wa.table_len * (int64_t)rbs || ctx > 0x7fffff00u;
+    const bool past = b > wa.num_tokens;
+    if ((zero || past) && threadIdx.x == 0 && blockIdx.x == 0) set_status(&g_decode_status, KVC_STATUS_INDEX_OOB);
+    if (past) return;
+    rows = (int)(ql * G < 0x7fffffff ? ql * G : 0x7fffffff);
+    prefix = (int)((int64_t)ctx - ql);
+  }
+  const int nh = EXT ? (rows - R0 < 16 ? rows - R0 : 16) : G;
+  // row R0 + g: new token t, head of the group
+  auto token_of = [&](int g) { return EXT ? (R0 + g) / G : 0; };
+  auto dest = [&](int g) -> T* {
+    if constexpr (!EXT)  // (fewer registers live across the loop: 256 sequences, window 1024: 170 -> 165 us)
+      return reinterpret_cast<T*>(p.out) + (int64_t)seq * p.out_seq_stride + (int64_t)(h0 + g) * p.out_head_stride;
+    const int t = token_of(g);
+    return reinterpret_cast<T*>(p.out) + (q0 + t) * p.out_seq_stride + (int64_t)(h0 + R0 + g - t * G) * p.out_head_stride;
+  };
+  if (zero) {
+    if (rank == 0)
+      for (int i = threadIdx.x; i < nh * D; i += NW * 32) dest(i / D)[i % D] = from_float<T>(0.f);
+    return;
+  }
+  if (C > 1) cluster_arrive();
+  const Seen seen = seen_range(prefix + token_of(0), prefix + token_of(nh - 1), wa.window, wa.sinks, rbs);
+  // this CTA's run of groups
+  const int all = (seen.end + GT - 1) / GT, per = (all + C - 1) / C;
+  const int begin = rank * per * GT;
+  const int end = begin + per * GT < seen.end ? begin + per * GT : seen.end;
+  const int ngroups = end > begin ? (end - begin + GT - 1) / GT : 0;
+  const int n_mine = warp < ngroups ? (ngroups - warp + NW - 1) / NW : 0;
+
   const T* kbase = reinterpret_cast<const T*>(p.k_cache) + (int64_t)kvh * p.k_head_stride;
   const T* vbase = reinterpret_cast<const T*>(p.v_cache) + (int64_t)kvh * p.v_head_stride;
   const uint32_t* table = p.block_tables + (int64_t)seq * p.table_stride;
@@ -246,7 +242,7 @@ __global__ void __launch_bounds__(NW * 32)
     uint32_t b = 0xffffffffu;
     if constexpr (!Geo::TOKIDS) {
       const int tok = begin + (warp + k * NW) * GT + lane * VBS;
-      if (lane < NBOX && k < n_mine && tok < end) b = __ldg(table + seen.real_block(tok / rbs));
+      if (lane < NBOX && k < n_mine && tok < end) b = table[seen.real_block(tok / rbs)];
     }
     return b;
   };
@@ -255,7 +251,7 @@ __global__ void __launch_bounds__(NW * 32)
     for (int i = 0; i < IDV; ++i) {
       const int j = lane + 32 * i, kg = c * IDC + j / GT;
       const int tt = begin + (warp + kg * NW) * GT + j % GT;
-      v[i] = kg < n_mine && tt < end ? __ldg(table + seen.real_block(tok_blocks ? tt : tt / tbs)) : 0xffffffffu;
+      v[i] = kg < n_mine && tt < end ? table[seen.real_block(tok_blocks ? tt : tt / tbs)] : 0xffffffffu;
     }
   };
   auto store_ids = [&](int c, const uint32_t (&v)[IDV]) {
@@ -341,9 +337,7 @@ __global__ void __launch_bounds__(NW * 32)
     }
   };
 
-  // the first groups' ids and the query rows are on their way before the wait
-  // for the kernel before this one (tables, lengths and queries are written by
-  // none of this library's kernels that let their dependents start early)
+  // the first groups' ids and the query rows are on their way together
   uint32_t first_blk[STAGES], ids_next[IDV];
 #pragma unroll
   for (int s = 0; s < STAGES; ++s) first_blk[s] = load_block(s);
@@ -383,7 +377,6 @@ __global__ void __launch_bounds__(NW * 32)
     }
   }
   const float qk_scale = p.scale * kLog2e;
-  grid_dependency_wait();
 #pragma unroll
   for (int s = 0; s < STAGES; ++s)
     if (s < n_mine) issue(s, s, first_blk[s]);

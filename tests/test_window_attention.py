@@ -470,6 +470,40 @@ def test_extend_nan_that_is_seen_shows(gpu, layout, bs, seqs, value):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["decode", "decode fp32", "decode pool", "few", "many"])
+def test_output_is_the_next_query(gpu, kind):
+    """A kernel may start before the one ahead of it on the stream has ended, but reads nothing that this one writes
+    before it has: an attention output as the next call's query."""
+    dtype = "float32" if "fp32" in kind else "bfloat16"
+    new = None if kind.startswith("decode") else [9, 4] if kind == "few" else [700, 500]
+    layout, bs = ("pool", 1) if "pool" in kind else ("paged", 16)
+    a = Case(46, dtype, [9000, 7000], 8, 2, 128, bs, layout, new=new)
+    q, kc, vc, tables, lens = a.upload()
+    ind = DeviceArray.from_numpy(a.indptr)
+    window = 6000 if kind.startswith("decode") else 900
+
+    def call(query, lens, out):
+        if kind.startswith("decode"):
+            return mk.paged_attention_window(query, kc, vc, tables, lens, 2, a.scale, bs, a.max_seq_len, window, 3, out=out)
+        return mk.paged_prefill_window(query, kc, vc, tables, ind, lens, 2, a.scale, bs, window, 3,
+                                       max_q_len=max(new), out=out)
+
+    outs = [DeviceArray.zeros(q.shape, dtype) for _ in range(6)]
+    apart = [DeviceArray.zeros(q.shape, dtype) for _ in range(6)]
+    for _ in range(3):
+        for i in range(6):  # (one after another)
+            call(apart[i - 1] if i else q, lens, apart[i])
+            mk.synchronize()
+        for o in outs:
+            o.fill_zero()
+        mk.synchronize()
+        for i in range(6):
+            call(outs[i - 1] if i else q, lens, outs[i])
+        for i in range(6):
+            np.testing.assert_array_equal(outs[i].to_numpy(raw=True), apart[i].to_numpy(raw=True), err_msg=f"{kind} {i}")
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("seqs", [2, 40])
 def test_extend_bits_repeat(gpu, seqs):
     """The same call gives the same bits, on any stream; max_q_len may be larger than needed."""
