@@ -438,7 +438,10 @@ int kvc_paged_prefill_window(kvc_dltensor* out, const kvc_dltensor* query, const
  *   blocks_used   int32 [1]  entries of free_blocks taken
  *   prefix_lens, new_lens  int32 [num_seqs];  free_blocks  int32 [any]
  * N may exceed the total (the capacity of a captured step): the rows past it get
- * position -1 and slot -1, which the appends and kvc_qk_norm_rope skip.
+ * position -1 and slot -1, which the appends and kvc_qk_norm_rope skip.  kv_lens may
+ * be prefix_lens or new_lens (lengths kept on the device: a second launch updates
+ * them); apart from that, what is written shares no memory with the inputs or with
+ * one another (KVC_EINVAL).
  * KVC_STATUS_INDEX_OOB is set, and the affected slots are -1, when the total
  * exceeds N, the free list or a table row is too short (entries past the free
  * list are written as -1), a table entry that a new token falls into is

@@ -1179,6 +1179,15 @@ int kvc_paged_prefill_window(kvc_dltensor* out, const kvc_dltensor* query, const
 
 // ---- step tables, rotary positions (layer_ops.cu) ----------------------------------
 
+// Whether rows of `len` bytes, `stride` apart, meet the bytes [lo, hi).
+static bool rows_meet(const char* base, int64_t rows, int64_t len, int64_t stride, const char* lo, const char* hi) {
+  if (rows <= 0 || len <= 0 || lo >= hi) return false;
+  // the first row that ends past lo, if any, starts before hi
+  const int64_t gap = lo - (base + len);  // < 0: row 0 does
+  const int64_t i = gap < 0 ? 0 : gap / stride + 1;
+  return i < rows && base + i * stride < hi;
+}
+
 int kvc_step_tables(kvc_dltensor* block_tables, kvc_dltensor* kv_lens, kvc_dltensor* qo_indptr,
                     kvc_dltensor* positions, kvc_dltensor* slot_mapping, kvc_dltensor* blocks_used,
                     const kvc_dltensor* prefix_lens, const kvc_dltensor* new_lens, const kvc_dltensor* free_blocks,
@@ -1214,8 +1223,35 @@ int kvc_step_tables(kvc_dltensor* block_tables, kvc_dltensor* kv_lens, kvc_dlten
   if (B > 0x7fffffffll - 2048) return fail(KVC_EINVAL, "too many sequences");
   int device = -1;
   if (int rc = check_all_cuda({&bt, &kl, &qi, &po, &sm, &us, &pl, &nl, &fb}, &device)) return rc;
+  // what is written may not lie in what is read or written beside it, except that
+  // kv_lens may be prefix_lens or new_lens
+  const bool in_place = B > 0 && (kl.data == pl.data || kl.data == nl.data);
+  struct Span {
+    const char *lo, *hi;
+  };
+  auto span = [](const View& v) -> Span {
+    const char* at = static_cast<const char*>(v.data);
+    return {at, at + v.shape[0] * elem_size(v.dtype)};
+  };
+  auto meet = [](Span x, Span y) { return x.lo < x.hi && y.lo < y.hi && x.lo < y.hi && y.lo < x.hi; };
+  const View* written[] = {&kl, &qi, &po, &sm, &us};
+  const View* read[] = {&pl, &nl, &fb};
+  bool shared = false;
+  for (int i = 0; i < 5; ++i) {
+    const Span w = span(*written[i]);
+    for (int j = i + 1; j < 5; ++j) shared |= meet(w, span(*written[j]));
+    for (const View* r : read) shared |= meet(w, span(*r)) && !(written[i] == &kl && r != &fb && r->data == kl.data);
+    shared |= rows_meet(static_cast<const char*>(bt.data), B, bt.shape[1] * 4, B > 1 ? bt.stride(0) * 4 : 1, w.lo, w.hi);
+  }
+  for (const View* r : read)
+    shared |= rows_meet(static_cast<const char*>(bt.data), B, bt.shape[1] * 4, B > 1 ? bt.stride(0) * 4 : 1, span(*r).lo,
+                        span(*r).hi);
+  if (shared)
+    return fail(KVC_EINVAL, "block_tables, kv_lens, qo_indptr, positions, slot_mapping and blocks_used must not share "
+                            "memory with one another or with the inputs (kv_lens may be prefix_lens or new_lens)");
   StepTablesArgs a;
   memset(&a, 0, sizeof(a));
+  a.lens_in_place = in_place;
   a.tables = reinterpret_cast<int32_t*>(bt.data);
   a.table_stride = bt.stride(0);
   a.table_len = bt.shape[1];

@@ -177,6 +177,7 @@ struct StepTablesArgs {
   int32_t* blocks_used;
   int num_seqs, block_size;
   int64_t num_tokens;  // rows of positions / slots
+  bool lens_in_place;  // kv_lens is prefix_lens or new_lens
 };
 
 constexpr int kMaxRotaryHalf = 128;

@@ -67,7 +67,9 @@ static int sm_count() {
 // KB out of L2, cheaper than a second launch or a wait between CTAs) and then
 // does slice s of the chunk's new blocks and new tokens, found by binary search
 // in the scanned offsets.  A token in a new block reads the free list, not the
-// table, so no CTA needs what another one writes.  A few KB move: what counts is the
+// table, so no CTA needs what another one writes, and none may write what another
+// one still reads: lengths that are updated in place (kv_lens is prefix_lens or
+// new_lens) are left to a second kernel (0.85 us more).  A few KB move: what counts is the
 // chain of launch, loads, scan, search and stores (64 requests with one token each
 // 4.9 us back to back, 528 of a mixed step 6.8; 256 prompts of up to 4096 tokens, 7.2
 // MB of positions and slots, 6.6; an empty kernel launched the same way takes about
@@ -96,6 +98,26 @@ __device__ __forceinline__ int find_request(const uint32_t* off, int n, uint32_t
   return lo;
 }
 
+// A request's lengths: below zero, or past 2^31 - 1 together, is an input error, read
+// as zero (false).
+__device__ __forceinline__ bool request_lens(const StepTablesArgs& p, int b, uint32_t* pre, uint32_t* fresh) {
+  const int32_t x = p.prefix_lens[b], y = p.new_lens[b];
+  const bool ok = x >= 0 && y >= 0 && (int64_t)x + y <= 0x7fffffffll;
+  *pre = ok ? (uint32_t)x : 0u;
+  *fresh = ok ? (uint32_t)y : 0u;
+  return ok;
+}
+
+// The lengths in place: each thread reads a request's own before it writes them.
+__global__ void __launch_bounds__(256) step_lens_kernel(StepTablesArgs p) {
+  wait_for_prior();
+  const int b = blockIdx.x * 256 + threadIdx.x;
+  if (b >= p.num_seqs) return;
+  uint32_t pre, fresh;
+  request_lens(p, b, &pre, &fresh);
+  p.kv_lens[b] = (int32_t)(pre + fresh);
+}
+
 __global__ void __launch_bounds__(kTablesThreads) step_tables_kernel(StepTablesArgs p) {
   __shared__ uint32_t tok_off[kTablesChunk + 1], blk_off[kTablesChunk + 1];
   __shared__ int32_t first_tok[kTablesChunk];
@@ -108,14 +130,9 @@ __global__ void __launch_bounds__(kTablesThreads) step_tables_kernel(StepTablesA
   const uint32_t bs = (uint32_t)p.block_size;
   bool bad = false;
   wait_for_prior();
-  // request b's cached tokens, new tokens and new blocks (lengths below zero, or
-  // past 2^31 - 1 together, are input errors: flagged, read as zero)
+  // request b's cached tokens, new tokens and new blocks (input errors are flagged)
   auto request = [&](int b, uint32_t* pre, uint32_t* fresh, uint32_t* blocks) {
-    const int32_t x = p.prefix_lens[b], y = p.new_lens[b];
-    const bool ok = x >= 0 && y >= 0 && (int64_t)x + y <= 0x7fffffffll;
-    bad |= !ok;
-    *pre = ok ? (uint32_t)x : 0u;
-    *fresh = ok ? (uint32_t)y : 0u;
+    bad |= !request_lens(p, b, pre, fresh);
     *blocks = (*pre + *fresh + bs - 1) / bs - (*pre + bs - 1) / bs;
   };
 
@@ -180,7 +197,7 @@ __global__ void __launch_bounds__(kTablesThreads) step_tables_kernel(StepTablesA
       blk_off[i] = (uint32_t)(k < limit ? k : limit);
       first_tok[i] = (int32_t)pre[e];
       if (blockIdx.x == 0) {
-        p.kv_lens[b0 + i] = (int32_t)(pre[e] + fresh[e]);
+        if (!p.lens_in_place) p.kv_lens[b0 + i] = (int32_t)(pre[e] + fresh[e]);
         const uint64_t row = base_tok + t;
         p.qo_indptr[b0 + i] = (int32_t)(row < limit ? row : limit);
       }
@@ -300,7 +317,10 @@ cudaError_t launch_step_tables(const StepTablesArgs& a, cudaStream_t stream) {
   const int64_t most = 2 * (int64_t)sm_count() / chunks;
   if (slices > most) slices = most;
   if (slices < 1) slices = 1;
-  return launch_dependent(step_tables_kernel, dim3((unsigned)slices, (unsigned)chunks), kTablesThreads, 0, stream, a);
+  const cudaError_t e =
+      launch_dependent(step_tables_kernel, dim3((unsigned)slices, (unsigned)chunks), kTablesThreads, 0, stream, a);
+  if (e != cudaSuccess || !a.lens_in_place || a.num_seqs == 0) return e;
+  return launch_dependent(step_lens_kernel, dim3((unsigned)((a.num_seqs + 255) / 256)), 256, 0, stream, a);
 }
 
 // ---------------------------------------------------------------------------

@@ -70,6 +70,39 @@ def test_step_tables(gpu, B, bs, longest, most_new, extra, slot_dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("B,bs,longest,most_new", [(1, 16, 100, 1), (64, 16, 4096, 1), (300, 16, 500, 40),
+                                                   (1500, 16, 100, 3), (4000, 16, 60, 5), (5, 16, 10, 40000), (2, 16, 0, 0)])
+@pytest.mark.parametrize("into", ["prefix_lens", "new_lens"])
+def test_step_tables_update_lengths_in_place(gpu, B, bs, longest, most_new, into):
+    """A server that keeps its lengths on the device passes them as the output too: everything else as without."""
+    tables, prefix, new, free = tables_case(B * 37 + bs, B, bs, longest, most_new)
+    if B > 2:
+        new[1] = 0
+    capacity = int(new.sum()) + 3
+    want = plain_tables(tables, prefix, new, free, bs, capacity)
+    dev = {n: DeviceArray.from_numpy(np.asarray(a), dtype="int32") for n, a in
+           (("tables", tables), ("prefix_lens", prefix), ("new_lens", new), ("free", free))}
+    got = mk.build_step_tables(dev["tables"], dev["prefix_lens"], dev["new_lens"], dev["free"], bs, capacity,
+                               kv_lens=dev[into])
+    assert got.kv_lens is dev[into]
+    for g, w in zip(got, want):
+        np.testing.assert_array_equal(g.to_numpy().reshape(-1), np.asarray(w).reshape(-1))
+    other = "new_lens" if into == "prefix_lens" else "prefix_lens"
+    np.testing.assert_array_equal(dev[other].to_numpy(), new if other == "new_lens" else prefix)
+    assert _lib.get_status(0, clear=True) == 0
+
+
+@pytest.mark.gpu
+def test_step_tables_in_place_reads_bad_lengths_as_zero(gpu):
+    lens = DeviceArray.from_numpy(np.array([5, -3, 7, 2**31 - 5], np.int32))
+    new = DeviceArray.from_numpy(np.array([1, 4, -2, 9], np.int32))
+    tables = DeviceArray.from_numpy(np.full((4, 2), 1, np.int32))
+    mk.build_step_tables(tables, lens, new, DeviceArray.from_numpy(np.array([3], np.int32)), 16, 1, kv_lens=lens)
+    assert lens.to_numpy().tolist() == [6, 0, 0, 0]
+    assert _lib.get_status(0, clear=True) == _lib.STATUS_INDEX_OOB
+
+
+@pytest.mark.gpu
 def test_step_tables_no_requests(gpu):
     got = run_tables(np.zeros((0, 4), np.int32), [], [], [1, 2], 16, 3)
     assert got[2].tolist() == [0] and got[3].tolist() == [-1] * 3 and got[4].tolist() == [-1] * 3
@@ -463,6 +496,51 @@ def test_step_tables_refusals():
         assert text in _lib.last_error()
     with pytest.raises(ValueError, match="num_tokens is needed"):
         mk.build_step_tables(None, None, object(), None, 16)
+
+
+# what is laid out where: each array 64 KB from the next, as far as `at` does not say otherwise
+_TABLE_ARGS = dict(bt=((3, 4), "int32"), kl=((3,), "int32"), qi=((4,), "int32"), po=((9,), "int32"), sm=((9,), "int64"),
+                   us=((1,), "int32"), pl=((3,), "int32"), nl=((3,), "int32"), fb=((7,), "int32"))
+
+
+@pytest.mark.parametrize("at", [
+    dict(kl=("pl", 4)), dict(kl=("pl", -8)), dict(kl=("nl", 8)), dict(kl=("fb", 24)), dict(kl=("fb", 0)), dict(qi=("pl", 0)),
+    dict(qi=("nl", 0)), dict(po=("pl", 8)), dict(sm=("nl", -68)), dict(us=("pl", 8)), dict(us=("fb", 0)), dict(po=("sm", 68)),
+    dict(kl=("qi", 0)), dict(us=("kl", 4)), dict(bt=("fb", 24)), dict(fb=("bt", -24)), dict(kl=("bt", 44)), dict(pl=("bt", 0)),
+    dict(kl=("pl", 0), nl=("pl", 4)), dict(kl=("nl", 0), po=("nl", 8))])
+def test_step_tables_refuse_shared_memory(at):
+    """Every CTA reads all lengths while others write: what is written must lie apart (kv_lens exactly on the lengths
+    is allowed, and has a test of its own on a device)."""
+    ptr = {n: 0x100000 + 0x10000 * i for i, n in enumerate(_TABLE_ARGS)}
+    for n, (to, off) in at.items():
+        ptr[n] = ptr[to] + off
+    tensors = {}
+    for n, (shape, dtype) in _TABLE_ARGS.items():
+        strides = (4, 1) if len(shape) == 2 else (1,)
+        t, keep = dlpack.make_dltensor(ptr[n], shape, strides, dtype, 0)
+        tensors[n] = (ctypes.pointer(t), keep)
+    rc = _lib.lib.kvc_step_tables(*(tensors[n][0] for n in ("bt", "kl", "qi", "po", "sm", "us", "pl", "nl", "fb")), 16, None)
+    assert rc == 1 and "must not share memory" in _lib.last_error()
+
+
+@pytest.mark.gpu
+def test_step_tables_between_the_rows_of_a_wide_table(gpu):
+    """Block tables that are a slice of wider rows, whose other columns hold the other arrays of the call."""
+    import torch
+
+    wide = torch.full((4, 64), -1, dtype=torch.int32, device="cuda")
+    wide[0, 0], wide[1, 0] = 3, 9
+    prefix, new = wide[1, 16:20], wide[2, 16:20]
+    prefix.copy_(torch.tensor([5, 16, 0, 0]))
+    new.copy_(torch.tensor([20, 1, 0, 17]))
+    torch.cuda.synchronize()
+    out = mk.build_step_tables(wide[:, :8], prefix, new, torch.tensor([10, 11, 12, 13], dtype=torch.int32, device="cuda"), 16,
+                               38, kv_lens=wide[0, 24:28], qo_indptr=wide[3, 32:37])
+    mk.synchronize()
+    assert out.kv_lens.tolist() == [25, 17, 0, 17] and out.qo_indptr.tolist() == [0, 20, 21, 21, 38]
+    assert wide[:, :3].tolist() == [[3, 10, -1], [9, 11, -1], [-1, -1, -1], [12, 13, -1]]
+    assert prefix.tolist() == [5, 16, 0, 0] and new.tolist() == [20, 1, 0, 17]
+    assert _lib.get_status(0, clear=True) == 0
 
 
 def test_rotary_table_refusals():
