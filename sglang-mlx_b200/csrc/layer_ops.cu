@@ -17,9 +17,10 @@ __device__ unsigned int g_layer_ops_status = 0;
 
 // Every kernel here is a programmatic dependent of the kernel before it on the
 // stream: its launch overlaps that kernel's end, and it waits for it before it
-// reads or writes anything.  None lets its own dependents start early: the decode
-// kernels read queries, tables and lengths, which are written here, before they
-// wait.
+// reads or writes anything (with coherent loads: the non-coherent ones want data
+// that nothing writes while the kernel runs).  None lets its own dependents start
+// early: the whole-context decode kernels read queries, tables and lengths, which
+// are written here, before they wait.
 __device__ __forceinline__ void wait_for_prior() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 template <typename... P, typename... A>
@@ -582,8 +583,8 @@ __device__ __forceinline__ void rope_rows(const RopeLane& ln, Quad<T>* ring, con
       const float* w = reinterpret_cast<const float*>(weight);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        wt[i] = make_float2(__ldg(w + ln.da + 2 * i), __ldg(w + ln.da + 2 * i + 1));
-        wt[2 + i] = make_float2(__ldg(w + ln.db + 2 * i), __ldg(w + ln.db + 2 * i + 1));
+        wt[i] = make_float2(w[ln.da + 2 * i], w[ln.da + 2 * i + 1]);
+        wt[2 + i] = make_float2(w[ln.db + 2 * i], w[ln.db + 2 * i + 1]);
       }
     } else {
       const T* w = reinterpret_cast<const T*>(weight);
@@ -705,8 +706,8 @@ __global__ void __launch_bounds__(kRopeWarps * 32) qk_norm_rope_kernel(const Rop
   float4 c = make_float4(1.f, 1.f, 1.f, 1.f), s = make_float4(0.f, 0.f, 0.f, 0.f);
   if (ln.rotated && pos_ok) {
     const float* cs = p.table + pos * p.table_stride + 4 * li;
-    c = __ldg(reinterpret_cast<const float4*>(cs));
-    s = __ldg(reinterpret_cast<const float4*>(cs + half));
+    c = *reinterpret_cast<const float4*>(cs);
+    s = *reinterpret_cast<const float4*>(cs + half);
   }
   const bool w_f32 = p.weight_type == ElemType::F32;
   Quad<T>* ring = reinterpret_cast<Quad<T>*>(smem_rope) + (threadIdx.x >> 5) * (STAGES * 64) + lane;

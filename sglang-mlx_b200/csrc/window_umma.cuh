@@ -306,7 +306,7 @@ __global__ void __launch_bounds__(kWinThreads, 1)
                 for (int i = 0; i < 4; ++i) {
                   const uint32_t* q32 = reinterpret_cast<const uint32_t*>(row[i] + c * 8);
                   *reinterpret_cast<uint4*>(qb + c * (kUmmaRows * 16) + i * 512) =
-                      on[i] ? make_uint4(__ldg(q32), __ldg(q32 + 1), __ldg(q32 + 2), __ldg(q32 + 3))
+                      on[i] ? make_uint4(q32[0], q32[1], q32[2], q32[3])
                             : make_uint4(0u, 0u, 0u, 0u);
                 }
             }
@@ -362,12 +362,12 @@ __global__ void __launch_bounds__(kWinThreads, 1)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int tok = j * KT + 4 * lane + e;
-            id[e] = j < ntiles && tok < kv_end ? __ldg(table + it.seen.real_block(tbs == 1 ? tok : tok / tbs)) : 0xffffffffu;
+            id[e] = j < ntiles && tok < kv_end ? table[it.seen.real_block(tbs == 1 ? tok : tok / tbs)] : 0xffffffffu;
           }
         } else {
           const int tok = j * KT + lane * UNIT;
           id[0] = lane < WG::UNITS && j < ntiles && tok < kv_end
-                      ? __ldg(table + it.seen.real_block(LOAD == kPages ? tok / BS : tok / tbs))
+                      ? table[it.seen.real_block(LOAD == kPages ? tok / BS : tok / tbs)]
                       : 0xffffffffu;
         }
       };
