@@ -71,6 +71,10 @@ bool parse(const kvc_dltensor* t, const char* name, View* v) {
     v->strides[i] = t->strides && v->shape[i] != 1 ? t->strides[i] : expect;
     expect *= v->shape[i];
   }
+  if (t->data == nullptr && expect != 0) {
+    set_error(std::string(name) + ": null data pointer");
+    return false;
+  }
   v->data = static_cast<char*>(t->data) + t->byte_offset;
   v->on_cuda = (t->device.device_type == 2 || t->device.device_type == 13);
   v->on_host = (t->device.device_type == 1 || t->device.device_type == 3);

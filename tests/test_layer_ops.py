@@ -614,3 +614,54 @@ def test_refusals_are_the_same_either_way(gpu, monkeypatch, direct):
         mk.paged_attention_window(q, kc, vc, t, n, 2, 0.125, 16, 16, 0, out=DeviceArray.zeros(q.shape, "float16"))
     with pytest.raises(ValueError, match="out"):
         mk.paged_attention_window(q, kc, vc, t, n, 2, 0.125, 16, 16, 4, out=DeviceArray.zeros((2, 4, 32), "float16"))
+
+
+# ---- what a producer's tensors may be -------------------------------------------
+
+
+def _cpu_calls():
+    """The five calls on CPU torch tensors of fitting shapes, as (name, arguments, keywords, tensors' names)."""
+    import torch
+
+    f = lambda *s: torch.zeros(s, dtype=torch.float16)  # noqa: E731
+    i = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731
+    q, k = f(3, 4, 64), f(3, 2, 64)
+    kc, vc = f(8, 2, 8, 16, 8), f(8, 2, 64, 16)
+    cs = torch.zeros(40, 64)
+    slots = torch.zeros(3, dtype=torch.int64)
+    return [
+        ("paged_attention_window", [q, kc, vc, i(3, 2), i(3), 2, 0.125, 16, 32, 9, 2], dict(out=f(3, 4, 64))),
+        ("paged_prefill_window", [q, kc, vc, i(3, 2), i(4), i(3), 2, 0.125, 16, 9, 2], dict(max_q_len=1, out=f(3, 4, 64))),
+        ("build_step_tables", [i(3, 2), i(3), i(3), i(7), 16], dict(kv_lens=i(3), qo_indptr=i(4), positions=i(3),
+                                                                  slot_mapping=slots, blocks_used=i(1))),
+        ("qk_norm_rope", [q, k, i(3), cs], dict(q_weight=f(64), k_weight=f(64), q_out=f(3, 4, 64), k_out=f(3, 2, 64))),
+        ("qk_norm_rope_append", [q, k, f(3, 2, 64), i(3), cs, kc, vc, slots], dict(q_weight=f(64), q_out=f(3, 4, 64))),
+    ]
+
+
+@pytest.mark.filterwarnings("ignore")
+@pytest.mark.parametrize("direct", [True, False])
+@pytest.mark.parametrize("which", range(5))
+def test_tensors_without_memory_are_refused(monkeypatch, which, direct):
+    """A tensor that has elements but no address (as tracing makes them) does not reach a kernel."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    if not direct:
+        monkeypatch.setattr(mk, "_calls", None)
+    with FakeTensorMode():
+        name, args, kw = _cpu_calls()[which]
+    with pytest.raises(ValueError, match="null data pointer"):
+        getattr(mk, name)(*args, **kw, stream=0)
+
+
+def test_descriptors_without_memory_are_refused():
+    def null(shape, dtype="float16"):
+        ptr = _fake(shape, dtype)
+        ptr.contents.data = None
+        return ptr
+
+    assert _lib.lib.kvc_reshape_and_cache(_fake((3, 2, 64)), null((3, 2, 64)), _fake((5, 2, 8, 16, 8)),
+                                          _fake((5, 2, 64, 16)), _fake((3,), "int64"), None) == 1
+    assert "value: null data pointer" in _lib.last_error()
+    assert _lib.lib.kvc_rotary_table(null((4, 64), "float32"), (ctypes.c_double * 32)(), 1.0, None) == 1
+    assert "cos_sin: null data pointer" in _lib.last_error()
