@@ -6,8 +6,9 @@
 //
 // Every function takes its arguments by position and returns the library's
 // status code, or -1 when some argument needs the general path (host data, a
-// producer without the exchange API, or, for a call without a stream, a producer
-// whose current stream is not the legacy default stream): nothing has run then.
+// producer without the exchange API, a tensor that requires a gradient, which
+// __dlpack__ refuses, or, for a call without a stream, a producer whose current
+// stream is not the legacy default stream): nothing has run then.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 #include <stdint.h>
@@ -40,6 +41,7 @@ int g_num_producers = 0;
 PyTypeObject* g_device_array = nullptr;
 PyObject* g_name_dltensor = nullptr;
 PyObject* g_name_handle = nullptr;
+PyObject* g_name_requires_grad = nullptr;
 
 enum Fn { kWindowDecode, kWindowPrefill, kStepTables, kRope, kRopeAppend, kNumFns };
 const char* const kNames[kNumFns] = {"kvc_paged_attention_window", "kvc_paged_prefill_window", "kvc_step_tables",
@@ -115,6 +117,11 @@ struct Call {
     } else {
       const ExchangeAPI* api = exchange_api(type);
       if (!api) return false;
+      PyObject* grad = PyObject_GetAttr(o, g_name_requires_grad);
+      if (!grad) PyErr_Clear();
+      const bool plain = !grad || grad == Py_False;
+      Py_XDECREF(grad);
+      if (!plain) return false;
       if (api->dltensor_from_object(o, d) != 0) {
         PyErr_Clear();
         return false;
@@ -280,6 +287,7 @@ PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, g_methods,
 PyMODINIT_FUNC PyInit__calls(void) {
   g_name_dltensor = PyUnicode_InternFromString("_dltensor");
   g_name_handle = PyUnicode_InternFromString("handle");
-  if (!g_name_dltensor || !g_name_handle) return nullptr;
+  g_name_requires_grad = PyUnicode_InternFromString("requires_grad");
+  if (!g_name_dltensor || !g_name_handle || !g_name_requires_grad) return nullptr;
   return PyModule_Create(&g_module);
 }

@@ -135,6 +135,26 @@ def _exchange_api(cls):
     return found
 
 
+def _exchanged(obj, checked):
+    """(DLTensor of `obj` through the exchange API, checked), or (None, checked)
+    where it has none, fails, or has to be asked through `__dlpack__` (see
+    call_tensors).  `checked`: the stream needs no look any more."""
+    api = _exchange_api(type(obj))
+    if api is None or getattr(obj, "requires_grad", False):
+        return None, checked
+    t = DLTensor()
+    try:
+        if api[0](obj, ctypes.addressof(t)) != 0:
+            return None, checked
+        if not checked:
+            cur = ctypes.c_void_p()
+            checked = (t.device.device_type == KDL_CUDA
+                       and api[1](KDL_CUDA, t.device.device_id, ctypes.byref(cur)) == 0 and not cur.value)
+    except Exception:  # what is wrong with the tensor, __dlpack__ says
+        return None, checked
+    return (t if checked else None), checked
+
+
 def call_tensors(objs, names, stream):
     """DLTensor pointers for one call: a list of ctypes references (None for
     None) and what to keep alive until the call returns.
@@ -143,7 +163,8 @@ def call_tensors(objs, names, stream):
     stream synchronisation, so without an explicit `stream` (the call then runs
     on the legacy default stream) it is used only while the producer's current
     stream is that one; otherwise `__dlpack__` makes the default stream wait for
-    the producer's, as it does for every other call here.
+    the producer's, as it does for every other call here.  Nor does it refuse what
+    `__dlpack__` does (a tensor that requires a gradient): those go that way too.
     """
     refs, keep = [], []
     checked = stream is not None
@@ -151,19 +172,11 @@ def call_tensors(objs, names, stream):
         if obj is None:
             refs.append(None)
             continue
-        api = _exchange_api(type(obj))
-        if api is not None:
-            t = DLTensor()
-            ref = ctypes.byref(t)
-            if api[0](obj, ctypes.addressof(t)) == 0:
-                if not checked:
-                    cur = ctypes.c_void_p()
-                    checked = (t.device.device_type == KDL_CUDA
-                               and api[1](KDL_CUDA, t.device.device_id, ctypes.byref(cur)) == 0 and not cur.value)
-                if checked:
-                    refs.append(ref)
-                    keep.append(t)
-                    continue
+        t, checked = _exchanged(obj, checked)
+        if t is not None:
+            refs.append(ctypes.byref(t))
+            keep.append(t)
+            continue
         ptr, k = as_dltensor(obj, name)
         refs.append(ptr)
         keep.append(k)

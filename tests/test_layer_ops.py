@@ -639,6 +639,39 @@ def _cpu_calls():
     ]
 
 
+@pytest.mark.parametrize("direct", [True, False])
+@pytest.mark.parametrize("stream", [None, 0])
+@pytest.mark.parametrize("which", range(5))
+def test_tensors_under_autograd_are_refused(monkeypatch, which, stream, direct):
+    """As every other call does, through __dlpack__: a result would be cut off from the graph without a word."""
+    if not direct:
+        monkeypatch.setattr(mk, "_calls", None)
+    name, args, kw = _cpu_calls()[which]
+    for where in list(range(len(args))) + list(kw):
+        name, args, kw = _cpu_calls()[which]
+        t = args[where] if isinstance(where, int) else kw[where]
+        if not (hasattr(t, "is_floating_point") and t.is_floating_point()):
+            continue
+        t.requires_grad_()
+        with pytest.raises(BufferError, match="require gradient"):
+            getattr(mk, name)(*args, **kw, stream=stream)
+    name, args, kw = _cpu_calls()[which]  # (without one: what is wrong with these is that they are on the host)
+    with pytest.raises(ValueError, match="CUDA device"):
+        getattr(mk, name)(*args, **kw, stream=stream)
+
+
+@pytest.mark.parametrize("direct", [True, False])
+def test_tensors_that_are_not_strided_are_refused(monkeypatch, direct):
+    import torch
+
+    if not direct:
+        monkeypatch.setattr(mk, "_calls", None)
+    name, args, kw = _cpu_calls()[3]
+    args[3] = torch.eye(40, 64).to_sparse()
+    with pytest.raises(BufferError, match="strided"):
+        getattr(mk, name)(*args, **kw)
+
+
 @pytest.mark.filterwarnings("ignore")
 @pytest.mark.parametrize("direct", [True, False])
 @pytest.mark.parametrize("which", range(5))
@@ -665,3 +698,30 @@ def test_descriptors_without_memory_are_refused():
     assert "value: null data pointer" in _lib.last_error()
     assert _lib.lib.kvc_rotary_table(null((4, 64), "float32"), (ctypes.c_double * 32)(), 1.0, None) == 1
     assert "cos_sin: null data pointer" in _lib.last_error()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("side", [False, True])
+@pytest.mark.parametrize("direct", [True, False])
+def test_torch_tensors_give_the_same_bits(gpu, monkeypatch, direct, side):
+    """Through the exchange API, and from a stream other than the default one, which then is waited for."""
+    import torch
+
+    want = [[o.to_numpy(raw=True) for o in call()] for _, call in _step_calls()]
+    if not direct:
+        monkeypatch.setattr(mk, "_calls", None)
+
+    def with_torch(fn):
+        conv = lambda a: torch.from_dlpack(a) if isinstance(a, DeviceArray) else a  # noqa: E731
+        return lambda *a, **k: fn(*map(conv, a), **{n: conv(v) for n, v in k.items()})
+
+    for name in ("paged_attention_window", "paged_prefill_window", "build_step_tables", "qk_norm_rope", "qk_norm_rope_append"):
+        monkeypatch.setattr(mk, name, with_torch(getattr(mk, name)))
+    stream = torch.cuda.Stream() if side else torch.cuda.current_stream()
+    with torch.cuda.stream(stream):
+        got = [call() for _, call in _step_calls()]
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        for a, b in zip(g, w):
+            np.testing.assert_array_equal(a.cpu().numpy().view(b.dtype), b)
+    assert _lib.get_status(0, clear=True) == 0
