@@ -23,6 +23,9 @@ void set_error(const std::string& msg) { g_last_error = msg; }
 void count_launch() { g_launches.fetch_add(1, std::memory_order_relaxed); }
 
 static int fail(int code, const std::string& msg) {
+  // (an error of the CUDA runtime that a call has returned is not for the next
+  // launch's check to find)
+  if (code == KVC_ECUDA) cudaGetLastError();
   set_error(msg);
   return code;
 }

@@ -701,6 +701,16 @@ def test_descriptors_without_memory_are_refused():
 
 
 @pytest.mark.gpu
+def test_an_error_is_returned_once(gpu):
+    """A call that the CUDA runtime refused (here: a device that is not there) does not fail the calls after it."""
+    for _, call in _step_calls():
+        with pytest.raises(_lib.KVCacheError):
+            _lib.get_status(99)
+        call()
+    assert _lib.get_status(0, clear=True) == 0
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("side", [False, True])
 @pytest.mark.parametrize("direct", [True, False])
 def test_torch_tensors_give_the_same_bits(gpu, monkeypatch, direct, side):
