@@ -45,6 +45,11 @@ def _done(rc: int) -> bool:
     return rc == 0
 
 
+def _c_int(x) -> int:
+    """A whole number as the library's int, past its ends the nearest end (ctypes would wrap it round)."""
+    return min(max(int(x), -(1 << 31)), (1 << 31) - 1)
+
+
 DEFAULT_PARTITION_SIZE = 512
 
 
@@ -544,8 +549,8 @@ def paged_attention_window(query, key_cache, value_cache, block_tables, context_
         out = _out_like_query(query)
     t, keep = call_tensors((out, query, key_cache, value_cache, block_tables, context_lens),
                            ("out", "query", "key_cache", "value_cache", "block_tables", "context_lens"), stream)
-    rc = _L.kvc_paged_attention_window(t[0], t[1], t[2], t[3], t[4], t[5], int(num_kv_heads), float(scale),
-                                       int(block_size), int(max_seq_len), int(window_size), int(sink_size),
+    rc = _L.kvc_paged_attention_window(t[0], t[1], t[2], t[3], t[4], t[5], _c_int(num_kv_heads), float(scale),
+                                       _c_int(block_size), _c_int(max_seq_len), _c_int(window_size), _c_int(sink_size),
                                        _stream(stream))
     _lib.check(rc)
     return out
@@ -574,8 +579,8 @@ def paged_prefill_window(query, key_cache, value_cache, block_tables, qo_indptr,
         out = _out_like_query(query)
     t, keep = call_tensors((out, query, key_cache, value_cache, block_tables, qo_indptr, kv_lens),
                            ("out", "query", "key_cache", "value_cache", "block_tables", "qo_indptr", "kv_lens"), stream)
-    rc = _L.kvc_paged_prefill_window(t[0], t[1], t[2], t[3], t[4], t[5], t[6], int(num_kv_heads), float(scale),
-                                     int(block_size), int(max(0, max_q_len)), int(window_size), int(sink_size),
+    rc = _L.kvc_paged_prefill_window(t[0], t[1], t[2], t[3], t[4], t[5], t[6], _c_int(num_kv_heads), float(scale),
+                                     _c_int(block_size), _c_int(max(0, max_q_len)), _c_int(window_size), _c_int(sink_size),
                                      _stream(stream))
     _lib.check(rc)
     return out
@@ -634,7 +639,7 @@ def build_step_tables(block_tables, prefix_lens, new_lens, free_blocks, block_si
                             new_lens, free_blocks),
                            ("block_tables", "kv_lens", "qo_indptr", "positions", "slot_mapping", "blocks_used",
                             "prefix_lens", "new_lens", "free_blocks"), stream)
-    _lib.check(_L.kvc_step_tables(*t, int(block_size), _stream(stream)))
+    _lib.check(_L.kvc_step_tables(*t, _c_int(block_size), _stream(stream)))
     return StepTables(block_tables, kv_lens, qo_indptr, positions, slot_mapping, blocks_used)
 
 

@@ -672,6 +672,33 @@ def test_tensors_that_are_not_strided_are_refused(monkeypatch, direct):
         getattr(mk, name)(*args, **kw)
 
 
+@pytest.mark.parametrize("direct", [True, False])
+def test_whole_numbers_past_32_bits(monkeypatch, direct):
+    """A window or sinks past 2^31 (no limit) mean what they say, and other numbers do not wrap to small ones."""
+    if not direct:
+        monkeypatch.setattr(mk, "_calls", None)
+
+    def call(which, at, value, name=None):
+        fn, args, kw = _cpu_calls()[which]
+        if name is None:
+            args[at] = value
+        else:
+            kw[name] = value
+        with pytest.raises(ValueError) as e:
+            getattr(mk, fn)(*args, **kw)
+        return str(e.value)
+
+    for big in (2**31, 2**32, 2**32 + 5, 2**63, 2**80):
+        for which, at in ((0, 9), (0, 10), (1, 9), (1, 10)):  # windows and sinks: as far as the tensors, which are on the host
+            assert "CUDA device" in call(which, at, big)
+        assert "max_seq_len exceeds" in call(0, 8, big)
+        assert "num_heads must be divisible" in call(0, 5, big) and "num_heads must be divisible" in call(1, 6, big)
+        assert "match block_size" in call(0, 7, big) and "match block_size" in call(1, 8, big)
+        assert "CUDA device" in call(1, None, big, "max_q_len")
+        assert "window_size must be positive" in call(0, 9, -big) and "sink_size must be" in call(1, 10, -big)
+        assert "block_size must be positive" in call(2, 4, -big)
+
+
 @pytest.mark.filterwarnings("ignore")
 @pytest.mark.parametrize("direct", [True, False])
 @pytest.mark.parametrize("which", range(5))
