@@ -562,7 +562,7 @@ def paged_prefill_window(query, key_cache, value_cache, block_tables, qo_indptr,
     """Prefill / extend attention over a sliding window with sinks: as
     paged_prefill_attention, where the new token at position i sees position j <= i
     when j < sink_size or j > i - window_size.  Table entries of blocks that no
-    new token of their sequence sees are not read."""
+    new token of their sequence sees are not read.  A negative max_q_len is refused."""
     if _calls is not None and out is not None and max_q_len is not None and _done(_calls.paged_prefill_window(
             out, query, key_cache, value_cache, block_tables, qo_indptr, kv_lens, num_kv_heads, scale, block_size,
             max_q_len, window_size, sink_size, stream)):
@@ -580,7 +580,7 @@ def paged_prefill_window(query, key_cache, value_cache, block_tables, qo_indptr,
     t, keep = call_tensors((out, query, key_cache, value_cache, block_tables, qo_indptr, kv_lens),
                            ("out", "query", "key_cache", "value_cache", "block_tables", "qo_indptr", "kv_lens"), stream)
     rc = _L.kvc_paged_prefill_window(t[0], t[1], t[2], t[3], t[4], t[5], t[6], _c_int(num_kv_heads), float(scale),
-                                     _c_int(block_size), _c_int(max(0, max_q_len)), _c_int(window_size), _c_int(sink_size),
+                                     _c_int(block_size), _c_int(max_q_len), _c_int(window_size), _c_int(sink_size),
                                      _stream(stream))
     _lib.check(rc)
     return out

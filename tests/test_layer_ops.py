@@ -699,6 +699,20 @@ def test_whole_numbers_past_32_bits(monkeypatch, direct):
         assert "block_size must be positive" in call(2, 4, -big)
 
 
+@pytest.mark.parametrize("direct", [True, False])
+def test_a_negative_bound_on_new_tokens_is_refused(monkeypatch, direct):
+    """On both ways into the library: nothing would be written."""
+    if not direct:
+        monkeypatch.setattr(mk, "_calls", None)
+    for out in (True, False):
+        name, args, kw = _cpu_calls()[1]
+        kw["max_q_len"] = -1
+        if not out:
+            kw["out"] = args[0]
+        with pytest.raises(ValueError, match="max_q_len and window_size must be non-negative"):
+            getattr(mk, name)(*args, **kw)
+
+
 @pytest.mark.filterwarnings("ignore")
 @pytest.mark.parametrize("direct", [True, False])
 @pytest.mark.parametrize("which", range(5))
