@@ -923,6 +923,8 @@ static bool rope_vec_ok(const RopeArgs& a, int es) {
   // the table's rows as four floats at a time (half a multiple of 4)
   if ((reinterpret_cast<uintptr_t>(a.table) & 15u) || (a.table_stride & 3)) return false;
   if (!a.k_cache) return rows(a.k_out, a.ko_tok, a.ko_head, 0);
+  // (places within a head's page are 32-bit in the kernel)
+  if (a.paged && (int64_t)a.head_size * a.block_size > 0x7fffffffll) return false;
   return rows(a.v, a.v_tok, a.v_head, 0) && rows(a.k_cache, a.kc_block, a.kc_head, a.kc_tok) &&
          (a.paged || rows(a.v_cache, a.vc_block, a.vc_head, a.vc_tok));
 }

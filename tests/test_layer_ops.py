@@ -420,6 +420,31 @@ def test_append_many_tokens(gpu, T, d, rot, dtype, layout, bs):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T", [5, 1100])
+def test_append_to_a_page_past_32_bits(gpu, T):
+    """One block of 2^25 + 16 tokens: a head's page of 64 dims has more than 2^31 elements."""
+    import torch
+
+    bs, d = (1 << 25) + 16, 64
+    c = Rope(T, "float16", T, 2, 1, d, d, False, fused=False)
+    kc = torch.zeros((1, 1, d // 8, bs, 8), dtype=torch.float16, device="cuda")
+    vc = torch.zeros((1, 1, d, bs), dtype=torch.float16, device="cuda")
+    slots = np.arange(bs - T, bs)
+    slots[:2] = 0, 1 << 24
+    torch.cuda.synchronize()
+    mk.qk_norm_rope_append(c.dq, c.dk, c.dv, c.pos.astype(np.int32), c.table, kc, vc, slots)
+    mk.synchronize()
+    at = torch.from_numpy(slots).cuda()
+    got_k = kc[0, 0][:, at].permute(1, 0, 2).reshape(T, 1, d).float().cpu().numpy()
+    close(got_k, c.want(False)[1], "float16")
+    np.testing.assert_array_equal(vc[0, 0][:, at].t().reshape(T, 1, d).float().cpu().numpy(), c.v)
+    kc[0, 0][:, at] = 0
+    vc[0, 0][:, at] = 0
+    assert not kc.view(torch.int32).any() and not vc.view(torch.int32).any()  # nothing anywhere else
+    assert _lib.get_status(0, clear=True) == 0
+
+
+@pytest.mark.gpu
 def test_append_skipped_position_keeps_the_value(gpu):
     c = Rope(9, "bfloat16", 4, 4, 2, 128, 128, False)
     pos = np.array([5, -1, 7, 9], np.int32)
