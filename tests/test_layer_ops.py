@@ -3,6 +3,7 @@
 
 import ctypes
 import math
+import os
 
 import numpy as np
 import pytest
@@ -639,6 +640,17 @@ def test_refusals_are_the_same_either_way(gpu, monkeypatch, direct):
         mk.paged_attention_window(q, kc, vc, t, n, 2, 0.125, 16, 16, 0, out=DeviceArray.zeros(q.shape, "float16"))
     with pytest.raises(ValueError, match="out"):
         mk.paged_attention_window(q, kc, vc, t, n, 2, 0.125, 16, 16, 4, out=DeviceArray.zeros((2, 4, 32), "float16"))
+
+
+def test_direct_calls_are_built_for_this_interpreter():
+    """Under the interpreter's own tag: another one does not load them (and calls through ctypes instead)."""
+    import sysconfig
+
+    if not os.path.exists(os.path.join(sysconfig.get_paths()["include"], "Python.h")):
+        pytest.skip("built without the interpreter's headers")
+    assert mk._calls is not None
+    assert mk._calls.__file__.endswith("_calls" + sysconfig.get_config_var("EXT_SUFFIX"))
+    assert not os.path.exists(os.path.join(os.path.dirname(mk.__file__), "_calls.so"))
 
 
 # ---- what a producer's tensors may be -------------------------------------------
