@@ -18,7 +18,7 @@
 // (S = Q K^T from two descriptors, N = 128), and K and V have rings of their own: K
 // is free after S, V after P V.
 //   TMEM (512 columns): S 2 x 128 (P over it: per half 32 columns of hi pairs and
-//   32 of lo pairs), O 2 x D.
+//   32 of lo pairs, zeros where the rows have none), O 2 x D.
 //   Warps 0-7 softmax (warp w and w + 4: the two halves of rows 32 (w & 3) ..),
 //   warp 8 K, warp 9 (one lane) products, warp 10 V, warp 11 items and Q.
 // K and V have a warp each because V waits for a product that comes a softmax
@@ -49,13 +49,18 @@ constexpr uint32_t kLayoutSw128 = 2;
 constexpr int kWinThreads = 384;
 constexpr int kKWarp = 8, kVWarp = 10, kItemWarp = 11;
 constexpr int kWinItems = 4;  // item slots
-// bf16 P is rounded once (8 bits: 1.1e-3 rms of the output, under the 1.7e-3 of the
-// output's own rounding) where every row of an item sees at least this many keys,
-// and carried as hi + lo (16 bits, a second product per 16 tokens) where some row
-// sees fewer: single weights are large there, and nearly cancelling V rows would
-// show the rounding (2e-3 absolute is missed with 3 keys).  16 x 512 tokens, window
-// 1024: 1 / 2 products 131 / 164 us.
-constexpr int kSplitKeys = 64;
+// bf16 P is rounded once (8 bits) where no weight of a warp's 32 rows in a half tile is
+// more than 1 / kSharp of its row's sum so far (and so of its whole sum), and carried as
+// hi + lo (16 bits, a second product per 16 tokens) elsewhere: a few large weights on
+// nearly cancelling V rows show the rounding, many small ones average it out.  16 x 512
+// tokens, window 1024, N(0, 1) keys and values, queries N(0, f^2); elements of 2.2e7 past
+// 2e-3 + 1e-2 |value| at f = 2 / 6 (the worst by), and the time at f = 1:
+//   once wherever a row sees 64 keys   16 / 1746 (5e-3)      134.6 us
+//   kSharp 2                            1 / 4    (6e-4)      141.6
+//   kSharp 4                            0 / 0    (7e-4 to go) 144.7
+//   kSharp 8                            0 / 0    (1.4e-3)    150.3
+//   always hi + lo                      0 / 0                165.5
+constexpr float kSharp = 4.f;
 
 // 16 bytes of an output row: one store, or, where the rows do not start on 16-byte
 // boundaries, four (a row's pairs are 4-byte aligned: the host checked).
@@ -101,7 +106,6 @@ struct WinItem {
   int t0, g0, nrows;  // (new token, head of the group) of the item's first row; rows
   int y, kvh, prefix; // prefix less the gap: row's end = prefix + token + 1, virtual
   int kv_end, ntiles;
-  int split;          // bf16: some row sees fewer than kSplitKeys keys
   int state;          // 0 work, 1 rows to be zeroed (bad indices), 2 no further item
 };
 
@@ -115,8 +119,8 @@ struct WinUmmaGeom {
   static constexpr int NBARS = 2 * KS + 3 * VS + 2 + 4 + 1 + 1 + 4 + 1 + 1 + 2 * kWinItems;
   static constexpr int MASK_OFF = BAR_OFF + NBARS * 8;       // [8 tiles][4] loaded blocks (kSlots: tokens)
   static constexpr int ITEM_OFF = (MASK_OFF + 8 * 16 + 15) / 16 * 16;
-  static constexpr int MISC_OFF = ITEM_OFF + kWinItems * (int)sizeof(WinItem);  // abort, tmem address
-  static constexpr int SMEM = MISC_OFF + 8;
+  static constexpr int MISC_OFF = ITEM_OFF + kWinItems * (int)sizeof(WinItem);  // abort, tmem address, lo parts
+  static constexpr int SMEM = MISC_OFF + 8 + 16;
   static constexpr int UNIT = LOAD == kPages ? BS : (LOAD == kRows ? 16 : 1);  // tokens to a mask bit
   static constexpr int UNITS = LOAD == kSlots ? 128 : kUmmaTile / UNIT;
   static constexpr uint32_t SCOL = 0, OCOL = 256;
@@ -162,6 +166,8 @@ __global__ void __launch_bounds__(kWinThreads, 1)
   WinItem* items = reinterpret_cast<WinItem*>(smem_wu + WG::ITEM_OFF);
   volatile int* s_abort = reinterpret_cast<volatile int*>(smem_wu + WG::MISC_OFF);
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(smem_wu + WG::MISC_OFF + 4);
+  // [2 buffers][2 halves][4 warps]: the warp's rows of P have lo parts (else those are 0)
+  volatile uint8_t* s_lo = reinterpret_cast<volatile uint8_t*>(smem_wu + WG::MISC_OFF + 8);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int G = p.num_heads / p.num_kv_heads;
@@ -263,11 +269,6 @@ __global__ void __launch_bounds__(kWinThreads, 1)
         it.prefix = u.prefix;
         it.kv_end = u.kv_end;
         it.ntiles = u.ntiles;
-        {  // keys of the item's first row, which sees the fewest
-          const int i1 = u.prefix + u.seen.jump + it.t0 + 1;  // its position + 1
-          const int64_t cap = (int64_t)p.window + p.sinks;
-          it.split = BF16 && (i1 < kSplitKeys || cap < kSplitKeys);
-        }
         it.state = u.bad ? 1 : 0;
         ok = publish(it);
         if (ok && it.ntiles > 0) {
@@ -585,7 +586,7 @@ __global__ void __launch_bounds__(kWinThreads, 1)
       // S of tile g, then P V of tile g - 1, over the tiles of all items
       int g = 0, nq = 0;                        // tiles, items with keys so far
       int pv_left = 0, pv_j = -1;               // the tile whose P V is due: keys from its first token on, its place
-      bool pv_last = false, pv_split = false;   // .. whether its item ends with it, and has lo parts
+      bool pv_last = false;                     // .. whether its item ends with it
       bool ok = true;
       auto issue_pv = [&]() -> bool {
         const int t = g - 1, b = t & 1, vs = t % VS;
@@ -601,6 +602,7 @@ __global__ void __launch_bounds__(kWinThreads, 1)
           if (!umma::wait(&p_full[2 * b + h], (uint32_t)((t >> 1) & 1))) return false;
           umma::fence_after();
           const int left = pv_left - h * 64;
+          const bool two = BF16 && *reinterpret_cast<volatile uint32_t*>(smem_wu + WG::MISC_OFF + 8 + (2 * b + h) * 4) != 0u;
           const uint32_t pcol = tmem + WG::SCOL + b * 128 + h * 64, ocol = tmem + WG::OCOL + h * D;
           // 16 tokens of V: k-step ks of this half
           auto vlo = [&](int ks) -> uint32_t {
@@ -611,17 +613,17 @@ __global__ void __launch_bounds__(kWinThreads, 1)
             if (pv_j > 0) mma_ts_lo<true>(ocol, pcol, vlo(0), vd_hi, idO);
             else mma_ts_lo<false>(ocol, pcol, vlo(0), vd_hi, idO);
           }
-          if (left > 48 && !(BF16 && pv_split)) {
+          if (left > 48 && !two) {
 #pragma unroll
             for (int ks = 1; ks < 4; ++ks) mma_ts_lo<true>(ocol, pcol + 8 * ks, vlo(ks), vd_hi, idO);
           } else if (left > 0) {
             const int steps = left > 48 ? 4 : (left + 15) / 16;
-            if (BF16 && pv_split) mma_ts_lo<true>(ocol, pcol + 32, vlo(0), vd_hi, idO);
+            if (two) mma_ts_lo<true>(ocol, pcol + 32, vlo(0), vd_hi, idO);
 #pragma unroll
             for (int ks = 1; ks < 4; ++ks) {
               if (ks < steps) {
                 mma_ts_lo<true>(ocol, pcol + 8 * ks, vlo(ks), vd_hi, idO);
-                if (BF16 && pv_split) mma_ts_lo<true>(ocol, pcol + 32 + 8 * ks, vlo(ks), vd_hi, idO);
+                if (two) mma_ts_lo<true>(ocol, pcol + 32 + 8 * ks, vlo(ks), vd_hi, idO);
               }
             }
           }
@@ -637,7 +639,7 @@ __global__ void __launch_bounds__(kWinThreads, 1)
           ok = false;
           break;
         }
-        const int kv_end = items[sl].kv_end, ntiles = items[sl].ntiles, state = items[sl].state, split = items[sl].split;
+        const int kv_end = items[sl].kv_end, ntiles = items[sl].ntiles, state = items[sl].state;
         mbar_arrive(&item_empty[sl]);
         if (state == 2) break;
         if (ntiles == 0) continue;
@@ -674,7 +676,6 @@ __global__ void __launch_bounds__(kWinThreads, 1)
           pv_j = j;
           pv_left = kv_end - j * KT;
           pv_last = j == ntiles - 1;
-          pv_split = split != 0;
         }
       }
       if (ok && pv_j >= 0) ok = issue_pv();
@@ -796,40 +797,46 @@ __global__ void __launch_bounds__(kWinThreads, 1)
         }
         const float neg_ref = m_ref == -INFINITY ? 0.f : -m_ref;
         float2 ps = make_float2(0.f, 0.f);
-        // P over this tile's own S, 16 pairs of tokens at a time, so that the stores
-        // overlap the next pairs' exponentials: one rounding, or hi = the upper 16
-        // bits of each fp32 (a bf16, truncated) and lo = the exact remainder rounded
-        // to bf16.  (No wait: S's last reader, P V two tiles back, completed before
-        // this S did.)
+        // P over this tile's own S, the sum before the first store (what is carried
+        // depends on it: a sum of the tiles before alone, with the stores among the
+        // exponentials, carries lo parts oftener, 147.6 us against 144.7 at 16 x 512
+        // tokens): one rounding, or hi = the upper 16 bits of each fp32 (a bf16,
+        // truncated) and lo = the exact remainder rounded to bf16.  (No wait: S's last
+        // reader, P V two tiles back, completed before this S did.)
         const float2 sc = make_float2(qk_scale, qk_scale), nr = make_float2(neg_ref, neg_ref);
-        auto exponentials = [&](auto two) {
-          constexpr bool TWO = decltype(two)::value;
 #pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            uint32_t hi[16], lo[16];
+        for (int i = 0; i < HK / 2; ++i) {
+          const float2 e = fma_x2(make_float2(x[2 * i], x[2 * i + 1]), sc, nr);  // (hidden: exp2(-inf) = 0)
+          x[2 * i] = fast_exp2(e.x);
+          x[2 * i + 1] = fast_exp2(e.y);
+          ps = add_x2(ps, make_float2(x[2 * i], x[2 * i + 1]));
+        }
+        l = l * alpha + (ps.x + ps.y);
+        const bool two = BF16 && __any_sync(0xffffffffu, fast_exp2(mx + neg_ref) * kSharp > l);
+        const uint32_t pcol = lane_base + WG::SCOL + b * 128 + half * 64;
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          uint32_t hi[16], lo[16];
+          if (two) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-              const float2 xx = make_float2(x[32 * q + 2 * i], x[32 * q + 2 * i + 1]);
-              const float2 e = fma_x2(xx, sc, nr);  // (hidden: exp2(-inf) = 0)
-              const float2 pp = make_float2(fast_exp2(e.x), fast_exp2(e.y));
-              ps = add_x2(ps, pp);
-              if constexpr (TWO) {
-                const uint32_t u0 = __float_as_uint(pp.x), u1 = __float_as_uint(pp.y);
-                hi[i] = __byte_perm(u0, u1, 0x7632);
-                const float2 rem =
-                    sub_x2(pp, make_float2(__uint_as_float(u0 & 0xFFFF0000u), __uint_as_float(u1 & 0xFFFF0000u)));
-                lo[i] = MmaOp<T>::pack(rem.x, rem.y);
-              } else {
-                hi[i] = MmaOp<T>::pack(pp.x, pp.y);
-              }
+              const float p0 = x[32 * q + 2 * i], p1 = x[32 * q + 2 * i + 1];
+              const uint32_t u0 = __float_as_uint(p0), u1 = __float_as_uint(p1);
+              hi[i] = __byte_perm(u0, u1, 0x7632);
+              const float2 rem = sub_x2(make_float2(p0, p1),
+                                        make_float2(__uint_as_float(u0 & 0xFFFF0000u), __uint_as_float(u1 & 0xFFFF0000u)));
+              lo[i] = MmaOp<T>::pack(rem.x, rem.y);
             }
-            umma::st16(lane_base + WG::SCOL + b * 128 + half * 64 + 16 * q, hi);
-            if constexpr (TWO) umma::st16(lane_base + WG::SCOL + b * 128 + half * 64 + 32 + 16 * q, lo);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              hi[i] = MmaOp<T>::pack(x[32 * q + 2 * i], x[32 * q + 2 * i + 1]);
+              lo[i] = 0u;
+            }
           }
-        };
-        if (BF16 && it.split) exponentials(std::true_type{});
-        else exponentials(std::false_type{});
-        l = l * alpha + (ps.x + ps.y);
+          umma::st16(pcol + 16 * q, hi);
+          if constexpr (BF16) umma::st16(pcol + 32 + 16 * q, lo);
+        }
         if (j >= 1 && __any_sync(0xffffffffu, alpha != 1.f)) {
           if (!uwait(pv_done, (uint32_t)((gg - 1) & 1))) {
             ok = false;
@@ -849,7 +856,10 @@ __global__ void __launch_bounds__(kWinThreads, 1)
         umma::wait_st();
         umma::fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[2 * b + half]);
+        if (lane == 0) {
+          if constexpr (BF16) s_lo[(2 * b + half) * 4 + (warp & 3)] = two;
+          mbar_arrive(&p_full[2 * b + half]);
+        }
       }
       bool have = ok && ntiles > 0;
       if (have) {

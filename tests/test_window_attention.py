@@ -504,6 +504,20 @@ def test_output_is_the_next_query(gpu, kind):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("factor", [2, 3, 8])
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("layout,bs,d", [("paged", 16, 64), ("paged", 32, 128), ("flash", 16, 64), ("pool", 1, 128)])
+def test_extend_with_few_large_weights(gpu, layout, bs, d, dtype, factor):
+    """Scores of standard deviation `factor`: a few keys have most of a row's weight, and where their values nearly
+    cancel the weights' own rounding shows.  The tolerance is that of every other case."""
+    rng = np.random.default_rng(47)
+    new = rng.integers(30, 91, 40)
+    c = Case(47, dtype, new + rng.integers(0, 300, 40), 16, 4, d, bs, layout, new=new)
+    c.q = kv_oracle.round_to(c.q * factor, dtype)
+    check_extend(c, 130, 3, f"{layout} {dtype} x{factor}")
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("seqs", [2, 40])
 def test_extend_bits_repeat(gpu, seqs):
     """The same call gives the same bits, on any stream; max_q_len may be larger than needed."""
