@@ -707,8 +707,8 @@ static cudaError_t launch_window_nw(const DecodeParams& p, const WindowArgs& w, 
     // the largest cluster (at most 16 CTAs) of which all run at once, one CTA to an
     // SM, while a CTA keeps half of its warps' groups.  What fits a GPC is the
     // device's own affair, hence the question (two sequences of 8 KV heads, window
-    // 4096 / 16384: powers of two up to 8 and three quarters of the SMs 15.0 / 44.8
-    // us, up to all SMs, where the last clusters wait, 20.4 / 50.7, so 12.5 / 33.3).
+    // 4096 / 16384: powers of two up to 8 18.3 / 44.0 us, any size up to all SMs, where
+    // the last clusters wait, 18.3 / 42.5, so 12.1 / 28.7).
     static std::atomic<int> known[64][kMaxCluster + 1];
     int dev = 0;
     cudaGetDevice(&dev);
@@ -753,19 +753,19 @@ static int64_t window_units(const DecodeParams& p, int64_t new_tokens) {
   return (new_tokens * (p.num_heads / p.num_kv_heads) + 15) / 16 * p.num_seqs * p.num_kv_heads;
 }
 
-// kWide where every tile gets an SM or more (decode, 8 KV heads, window 1024, 1 / 2 /
-// 4 / 8 / 16 sequences: 32-token pages 7.8 / 15.0 / 10.8 / 13.1 / 20.0 us narrow (in
-// clusters of up to 16), 6.1 / 6.5 / 8.1 / 11.5 / 16.7 wide; slot lists 7.4 / 14.1 / 21.7
-// / 19.7 / 29.5 and 7.4 / 7.7 / 9.9 / 12.5 / 18.8; 16-token pages, window 4096, 9.6 /
-// 18.9 / 17.5 / 26.6 / 48.9 and 9.5 / 11.4 / 17.6 / 26.9 / 47.1).
+// kWide where every tile gets an SM or more (decode, 8 KV heads, 1 / 2 / 4 / 8 / 16
+// sequences: window 1024, 32-token pages 27.6 / 27.5 / 27.6 / 28.9 / 29.8 us narrow, 6.5 /
+// 7.0 / 8.4 / 12.4 / 17.4 wide; slot lists 22.3 / 22.3 / 22.3 / 22.9 / 23.5 and 7.6 / 8.1 /
+// 10.1 / 13.0 / 19.0; window 4096, 16-token pages 52.9 / 53.8 / 57.5 / 60.8 / 62.7 and 9.5 /
+// 12.0 / 18.0 / 28.5 / 48.0).
 // kSmall where every SM gets four tiles or more, so that it pays to have more CTAs in
 // their start and end, and the groups are short (D = 64, single token rows) or few
 // (decode, 8 KV heads, 128 sequences, window 64 / 128 / 256 / 1024: D = 128, 16-token
-// pages 19.3 / 24.2 / 33.6 / 87.9 us narrow, 17.6 / 24.5 / 35.1 / 99.6 small, and with
-// 256 sequences 34.7 / 43.1 / 58.7 / 162.8 and 29.8 / 41.2 / 58.8 / 168.9; D = 64 9.4 /
-// 13.6 / 19.7 / 48.5 and 7.2 / 11.3 / 16.6 / 47.8; slot lists 31 / 41 / 57 / 153 and 19
-// / 26 / 42 / 136; 64 sequences of D = 64, under four tiles to an SM: 4.9 / 6.3 / 10.3
-// / 26.1 and 5.5 / 7.9 / 12.9 / 39.8).
+// pages 19.4 / 24.5 / 33.9 / 89.8 us narrow, 17.3 / 23.0 / 34.7 / 101.4 small, and with
+// 256 sequences 34.1 / 42.9 / 58.2 / 166.2 and 29.2 / 38.1 / 57.8 / 171.9; D = 64 9.5 /
+// 13.4 / 20.2 / 49.9 and 7.3 / 11.6 / 17.3 / 51.7; slot lists 32.6 / 41.9 / 57.7 / 154.0 and
+// 20.0 / 27.3 / 43.1 / 138.2; 64 sequences of D = 64, under four tiles to an SM: 5.3 / 6.7 /
+// 11.0 / 28.1 and 6.1 / 8.7 / 13.3 / 39.9).
 template <typename T, int D, bool EXT>
 static cudaError_t launch_window_mma(const DecodeParams& p, bool flash, const WindowArgs& w, cudaStream_t stream) {
   const int64_t units = window_units(p, EXT ? w.max_q_len : 1), sms = decode_sm_count();
@@ -1019,7 +1019,7 @@ template <typename T, int D>
 static cudaError_t launch_window_prefill_t(const PrefillArgs& a, cudaStream_t stream) {
   // A 16-row tile for every SM or fewer: the decode's kernel, which splits the keys
   // too (4 sequences, 4 KV heads, 7 heads each, window 1024; 16 / 64 / 112 / 224
-  // tiles: 7.2 / 11.0 / 15.4 / 27.6 us against 18.6 of 128-row items one after
+  // tiles: 8.6 / 13.3 / 17.4 / 30.5 us against 20 of 128-row items one after
   // another).
   const int64_t units = ((int64_t)a.max_q_len * (a.num_heads / a.num_kv_heads) + 15) / 16 * a.num_seqs * a.num_kv_heads;
   const int64_t sms = decode_sm_count();
