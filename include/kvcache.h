@@ -92,7 +92,15 @@ int kvc_get_status(int device, uint32_t* flags, int clear);
  *   alibi_slopes [num_heads] f32, or NULL
  * Sequences with context_len == 0 or context_len > max_seq_len produce zeros
  * (paged_attention_kernels.metal:45-50).  Softmax denominator is
- * sum + 1e-6 (paged_attention_kernels.metal:144). */
+ * sum + 1e-6 (paged_attention_kernels.metal:144).
+ * Stream order, for this and the other whole-context decodes: their kernels start
+ * as programmatic dependents of the kernel ahead on the stream and wait for it
+ * before they touch the cache, the workspaces and out, but read the query, the
+ * tables, the lengths and the plan before that.  A kernel that lets its dependents
+ * start early must therefore not be the one just ahead that writes these; of this
+ * library's, the attention calls do so (an attention output that is the next
+ * decode's query needs another kernel or an event in between).  The window calls,
+ * kvc_step_tables and kvc_qk_norm_rope(_append) wait before they read anything. */
 int kvc_paged_attention_v1(kvc_dltensor* out, const kvc_dltensor* query,
                            const kvc_dltensor* key_cache, const kvc_dltensor* value_cache,
                            const kvc_dltensor* block_tables, const kvc_dltensor* context_lens,
@@ -402,7 +410,10 @@ int kvc_convert_fp8(kvc_dltensor* dst, const kvc_dltensor* src, float scale, int
  * context gives the unwindowed attention.  Block-table entries of blocks that no
  * query sees are not read (a server may have freed those blocks), and the values
  * in positions that no query of a sequence sees never matter.  A query that sees a
- * score of NaN or +inf gives NaN, one whose scores are all -inf gives 0.
+ * score of NaN or +inf gives NaN, one whose scores are all -inf gives 0.  Sums and
+ * maxima are float32; the weights of a float16 call are rounded to float16, those of
+ * a bfloat16 call carried in two parts (16 bits), but to one bfloat16 in prefills of
+ * many rows where each is at most a quarter of its row's sum.
  *
  * kvc_paged_attention_window: one new token per sequence, arguments and edge
  * rules of kvc_paged_attention_v1 (paged layout, every dtype pair, head size and
