@@ -813,3 +813,67 @@ def test_torch_tensors_give_the_same_bits(gpu, monkeypatch, direct, side):
         for a, b in zip(g, w):
             np.testing.assert_array_equal(a.cpu().numpy().view(b.dtype), b)
     assert _lib.get_status(0, clear=True) == 0
+
+
+CAPTURED_STEPS = """
+import sys
+sys.path.insert(0, sys.argv[1])
+import numpy as np
+from sglang_mlx_b200 import _lib, metal_kernels as mk
+from sglang_mlx_b200.device_array import DeviceArray, Graph, Stream
+
+B, H, KH, D, bs, steps = 3, 8, 2, 128, 16, 9
+rng = np.random.default_rng(1)
+i32 = lambda a: DeviceArray.from_numpy(np.asarray(a, np.int32))
+half = lambda *s: DeviceArray.from_numpy(rng.standard_normal(s).astype(np.float16))
+q, k, v, w, rope = half(B, H, D), half(B, KH, D), half(B, KH, D), half(D), mk.rotary_table(4096, D)
+k0, v0 = half(300, KH, D // 8, bs, 8).to_numpy(), half(300, KH, D, bs).to_numpy()
+one, free, st = i32([1] * B), i32([299]), Stream()
+
+
+class State:
+    def __init__(self):
+        self.kc, self.vc = DeviceArray.from_numpy(k0), DeviceArray.from_numpy(v0)
+        self.lens, self.tables = i32([3, 2000, 1601]), i32(np.arange(3 * 126).reshape(3, 126) % 299)
+        self.indptr, self.pos, self.used = i32([0] * (B + 1)), i32([0] * B), i32([0])
+        self.slots = DeviceArray.from_numpy(np.zeros(B, np.int64))
+        self.qr, self.out, self.out2 = (DeviceArray.zeros((B, H, D), "float16") for _ in range(3))
+
+    def step(self):
+        mk.build_step_tables(self.tables, self.lens, one, free, bs, kv_lens=self.lens, qo_indptr=self.indptr,
+                             positions=self.pos, slot_mapping=self.slots, blocks_used=self.used, stream=st)
+        mk.qk_norm_rope_append(q, k, v, self.pos, rope, self.kc, self.vc, self.slots, q_weight=w, k_weight=w,
+                               q_out=self.qr, stream=st)
+        mk.paged_attention_window(self.qr, self.kc, self.vc, self.tables, self.lens, KH, 0.09, bs, 2016, 900, 4, out=self.out,
+                                  stream=st)
+        mk.paged_prefill_window(self.qr, self.kc, self.vc, self.tables, self.indptr, self.lens, KH, 0.09, bs, 900, 4,
+                                max_q_len=1, out=self.out2, stream=st)
+
+    def seen(self):
+        st.synchronize()
+        return [a.to_numpy(raw=True) for a in (self.kc, self.vc, self.lens, self.pos, self.slots, self.out, self.out2)]
+
+
+a, b = State(), State()
+mk.synchronize()
+graph = Graph.capture(st, a.step)  # (the first calls of the process)
+for i in range(steps):
+    graph.replay(st)
+    b.step()
+    for x, y in zip(a.seen(), b.seen()):
+        np.testing.assert_array_equal(x, y)
+assert a.lens.to_numpy().tolist() == [3 + steps, 2000 + steps, 1601 + steps] and a.pos.to_numpy()[1] == 2000 + steps - 1
+assert _lib.get_status(0, clear=True) == 0
+print("captured")
+"""
+
+
+@pytest.mark.gpu
+def test_steps_captured_in_a_graph(gpu):
+    """A decode step with its lengths on the device, captured before any of its calls has run, then replayed."""
+    import subprocess
+    import sys
+
+    root = os.path.dirname(os.path.dirname(mk.__file__))
+    r = subprocess.run([sys.executable, "-c", CAPTURED_STEPS, root], capture_output=True, text=True, timeout=100)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
