@@ -59,7 +59,7 @@ constexpr int kWinItems = 4;  // item slots
 //   kSharp 2                            1 / 4    (6e-4)      141.6
 //   kSharp 4                            0 / 0    (7e-4 to go) 144.7
 //   kSharp 8                            0 / 0    (1.4e-3)    150.3
-//   always hi + lo                      0 / 0                165.5
+//   always hi + lo                      0 / 0    (2.0e-3)    164.2
 constexpr float kSharp = 4.f;
 
 // 16 bytes of an output row: one store, or, where the rows do not start on 16-byte
