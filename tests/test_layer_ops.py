@@ -877,3 +877,37 @@ def test_steps_captured_in_a_graph(gpu):
     root = os.path.dirname(os.path.dirname(mk.__file__))
     r = subprocess.run([sys.executable, "-c", CAPTURED_STEPS, root], capture_output=True, text=True, timeout=100)
     assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
+
+
+@pytest.mark.gpu
+def test_the_stride_of_an_extent_of_one_is_nothing(gpu):
+    """Producers leave any value there; no call reads it, or takes it for an alignment."""
+    import torch
+
+    g = torch.Generator(device="cuda").manual_seed(3)
+    half = lambda *s: torch.randn(s, generator=g, device="cuda", dtype=torch.float16)  # noqa: E731
+
+    def odd(t):
+        return torch.as_strided(t, t.shape, [3 if n == 1 else st for n, st in zip(t.shape, t.stride())])
+
+    q, k, v = half(1, 4, 64), half(1, 1, 64), half(1, 1, 64)
+    kc, vc, tk, tv = half(1, 1, 8, 16, 8), half(1, 1, 64, 16), half(1, 16, 1, 64), half(1, 16, 1, 64)
+    tables, lens = torch.zeros((1, 1), dtype=torch.int32, device="cuda"), torch.tensor([11], dtype=torch.int32, device="cuda")
+    ind, pos = torch.tensor([0, 1], dtype=torch.int32, device="cuda"), torch.tensor([10], dtype=torch.int32, device="cuda")
+    slot, cs = torch.tensor([10], device="cuda"), torch.randn((20, 64), generator=g, device="cuda")
+
+    def run(f):
+        a = (1, 0.125, 16, 16)
+        kc1, vc1, tk1, tv1 = (f(t.clone()) for t in (kc, vc, tk, tv))
+        mk.reshape_and_cache(f(k), f(v), kc1, vc1, f(slot))
+        mk.qk_norm_rope_append(f(q), f(k), f(v), f(pos), cs, tk1, tv1, f(slot), q_out=f(q.clone()))
+        outs = [kc1, vc1, tk1, tv1]
+        outs += [mk.paged_attention_v1(f(q), kc1, vc1, f(tables), f(lens), *a)]
+        outs += [mk.paged_attention_window(f(q), *c, f(tables), f(lens), *a, 5, 2) for c in ((kc1, vc1), (tk1, tv1))]
+        outs += [mk.paged_prefill_window(f(q), *c, f(tables), ind, f(lens), 1, 0.125, 16, 5, 2) for c in ((kc1, vc1), (tk1, tv1))]
+        mk.synchronize()
+        return [o.cpu().numpy() if hasattr(o, "cpu") else o.to_numpy() for o in outs]
+
+    for a, b in zip(run(odd), run(lambda t: t)):
+        np.testing.assert_array_equal(a.reshape(-1), b.reshape(-1))
+    assert _lib.get_status(0, clear=True) == 0
